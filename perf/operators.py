@@ -209,11 +209,11 @@ def run(state):
 # ------------------------------------------------------------------------------- the plain forms
 def _row_scales(x):
     top = x.abs().amax(-1, keepdim=True).clamp_min(TINY)
-    return top / E4M3_MAX, E4M3_MAX / top
+    return top * (1 / E4M3_MAX), E4M3_MAX * torch.reciprocal(top)
 
 
 def _quantise(x):
-    """(e4m3 values, scale of each row): scale = max |x| / 448, value = x * (448 / max |x|)."""
+    """(e4m3 values, scale of each row): scale = max |x| * (1 / 448), value = x * (448 * (1 / max))."""
     scale, inv = _row_scales(x)
     q = (x * inv).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return q, scale.squeeze(-1)
@@ -489,7 +489,7 @@ def _round_e4m3(x):
 def _levels(x):
     """e4m3 values (as 64-bit numbers) and scales of fp32 rows, the scales fp32 as they are kept."""
     top = torch.max(x.abs(), -1).values.clamp_min(TINY)
-    inv = torch.tensor(E4M3_MAX, device=x.device) / top
+    inv = torch.full_like(top, E4M3_MAX) * (torch.ones_like(top) / top)  # in fp32, as defined
     return _round_e4m3(x * inv[:, None]), (top.double() / E4M3_MAX).float().double()
 
 
