@@ -339,9 +339,11 @@ def _step(s):
 
 # --------------------------------------------------------------------------- the framework's calls
 class _Memory:
-    """A framework tensor's memory as torch reads it."""
+    """A framework tensor's memory as torch reads it; torch holds this object as long as a view of
+    it lives, and this object the tensor."""
 
     def __init__(self, t, typestr):
+        self.tensor = t
         self.__cuda_array_interface__ = {"shape": t.shape, "typestr": typestr, "version": 2,
                                          "data": (t.device_ptr, False), "strides": None}
 
