@@ -58,13 +58,18 @@ typedef enum mnn_status {
   MNN_ERR_TENSOR_NOT_FOUND = 15        /* tensorNotFound */
 } mnn_status;
 
-typedef enum mnn_dtype { MNN_F32 = 0, MNN_BF16 = 1 } mnn_dtype;
+/* I32: token positions, lengths and counts. E4M3: 8-bit floats (OCP e4m3: 4 exponent and 3 mantissa
+ * bits, largest value 448, no infinities), each row with a scale beside it. */
+typedef enum mnn_dtype { MNN_F32 = 0, MNN_BF16 = 1, MNN_I32 = 2, MNN_E4M3 = 3 } mnn_dtype;
 
 /* Compute precision of the matrix products (GEMM, implicit-GEMM conv, attention).
  * F32: fp32 operands on v_mfma_f32_*_f32. BF16: operands rounded to bf16 (RNE),
  * fp32 accumulation (precedent: HalfLinear, HalfPrecisionLinear.swift:60-212).
- * Norms, softmax and activations always run in fp32. */
-typedef enum mnn_precision { MNN_PRECISION_F32 = 0, MNN_PRECISION_BF16 = 1 } mnn_precision;
+ * E4M3 (Linear / FusedLinear only, other layers refuse it): 8-bit operands with a scale per row,
+ * fp32 accumulation. Norms, softmax and activations always run in fp32. */
+typedef enum mnn_precision {
+  MNN_PRECISION_F32 = 0, MNN_PRECISION_BF16 = 1, MNN_PRECISION_E4M3 = 2
+} mnn_precision;
 
 /* Fused activation codes. 0-4 are FusedConv1D's (Conv1D.swift:960-973); FusedLinear's sigmoid
  * and tanh (Linear.swift:630-639) get codes 5 and 6 here. Leaky ReLU's slope is 0.01 (the
@@ -203,6 +208,91 @@ mnn_status mnn_fused_linear_create(mnn_device dev, int in_features, int out_feat
                                    int use_bias, mnn_activation activation,
                                    float leaky_relu_alpha, mnn_precision precision,
                                    mnn_layer* out);
+
+/* A Linear of precision MNN_PRECISION_E4M3 on rows that are in 8 bits already, with the residual added
+ * in the epilogue: output = act(scales[i] * wscales[n] * sum_k input[i][k] w[n][k] + bias[n]) +
+ * residual. No counterpart in the reference. The weights are kept in 8 bits from loadWeights on, row
+ * n as w * (448 * (1 / max|w|)) rounded to nearest even, its scale max|w| * (1 / 448) (a row maximum
+ * below 2^-100 counts as 2^-100). input: MNN_E4M3 [.., in_features] with scales, an MNN_F32 tensor of
+ * one value per row (as mnn_rmsnorm_forward_residual writes them), or MNN_F32 / MNN_BF16 with scales
+ * NULL, rounded to 8 bits per row by the same rule in a launch before the product (as mnn_layer_forward
+ * of such a layer does, which writes f32). output: MNN_F32 or MNN_BF16, rounded once; residual: NULL or
+ * of the output's type and count, and it may be the output itself. Other layers, or a Linear of another
+ * precision, give MNN_ERR_INVALID_ARGUMENT. */
+mnn_status mnn_linear_forward_scaled(mnn_layer layer, mnn_tensor input, mnn_tensor scales,
+                                     mnn_tensor residual, mnn_tensor output, mnn_stream s);
+
+/* RMSNorm over the last dimension, beside LayerNorm (no counterpart in the reference): y = x *
+ * rsqrt(mean(x^2) + epsilon) * weight. Parameter "weight"/"gamma" [F], 1 until loaded. mnn_layer_forward
+ * takes f32 or bf16 input and writes f32. */
+mnn_status mnn_rmsnorm_create(mnn_device dev, int feature_size, float epsilon, mnn_layer* out);
+/* The same with the residual's addition before it and an output of 16 or 8 bits: h = input + residual
+ * (residual NULL: h = input), sum = h (sum may be NULL; it may be the input or the residual itself),
+ * output = RMSNorm of h as added in fp32, before sum's rounding. input, residual and sum share a type,
+ * MNN_F32 or MNN_BF16, and a count; output: MNN_F32 or MNN_BF16 with scales NULL, or MNN_E4M3 with
+ * scales, an MNN_F32 tensor of one value per row: value = y * (448 * (1 / max|y|)) rounded to nearest
+ * even, scale = max|y| * (1 / 448), a row maximum below 2^-100 counting as 2^-100. A row that holds a NaN
+ * or an infinity comes out as NaN values or with a scale that is not finite. */
+mnn_status mnn_rmsnorm_forward_residual(mnn_layer layer, mnn_tensor input, mnn_tensor residual,
+                                        mnn_tensor sum, mnn_tensor output, mnn_tensor scales,
+                                        mnn_stream s);
+
+#define MNN_ROTARY_MAX_AXES 4
+typedef struct mnn_rotary_desc {
+  int head_dim;
+  int num_axes;                         /* 1..4 */
+  int axis_dims[MNN_ROTARY_MAX_AXES];   /* dimensions that axis a turns: even, > 0, sum <= head_dim */
+  float base;                           /* of the angular rates, e.g. 10000 */
+  int interleaved;                      /* 1: pairs (2i, 2i + 1); 0: pairs (i, i + axis_dims[a] / 2) */
+} mnn_rotary_desc;
+/* Rotary positions over several axes (time frames and frequency bands of a spectrogram's tokens, for
+ * instance; no counterpart in the reference). The head's dimensions are taken in order, axis_dims[0]
+ * first; pair i of axis a turns by the angle position[a] * base^(-2i / axis_dims[a]): (u, v) -> (u cos -
+ * v sin, v cos + u sin). Dimensions behind the last axis pass unchanged. Angles are reduced in 64 bits,
+ * so far positions lose nothing. No weights. */
+mnn_status mnn_rotary_create(mnn_device dev, const mnn_rotary_desc* desc, mnn_layer* out);
+/* q [S, H * head_dim] or [B, S, H * head_dim] and k (NULL, or any number of heads on the same tokens),
+ * MNN_F32 or MNN_BF16; positions MNN_I32 [S, num_axes], shared by the batch, or [B, S, num_axes], any
+ * values. q_out / k_out have their input's type and count and may be the input itself. */
+mnn_status mnn_rotary_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor positions,
+                              mnn_tensor q_out, mnn_tensor k_out, mnn_stream s);
+
+typedef struct mnn_window_attention_desc {
+  int num_heads, num_kv_heads;  /* query heads h read key/value head h * num_kv_heads / num_heads */
+  int head_dim;                 /* a multiple of 8, <= 128 */
+  int window_left;              /* tokens before the query's own that it sees, >= 0 */
+  int window_right;             /* tokens behind it, >= 0 (0: causal) */
+  int sinks;                    /* first tokens that stay visible, >= 0 */
+  float scale;                  /* of the scores; 0: 1 / sqrt(head_dim) */
+} mnn_window_attention_desc;
+/* Attention over a sliding window with a few first tokens that stay visible (no counterpart in the
+ * reference). The query of token i sees the keys j <= i + window_right with j >= i - window_left or j <
+ * sinks. Softmax and sums run in fp32; f32 tensors keep fp32 products, bf16 ones take bf16 products with
+ * fp32 accumulation. No weights: q, k and v are projected (and turned) before. */
+mnn_status mnn_window_attention_create(mnn_device dev, const mnn_window_attention_desc* desc,
+                                       mnn_layer* out);
+/* Whole sequences: q and output [S, H * head_dim] or [B, S, H * head_dim], k and v the same of
+ * num_kv_heads, all MNN_F32 or all MNN_BF16. lengths: NULL, or MNN_I32 [B], the tokens of each padded
+ * sequence (values outside 0..S count as the nearer of the two): keys behind a sequence's end are seen by
+ * nobody, whatever they hold, and output rows behind it are left as they were. output may not be an
+ * input. */
+mnn_status mnn_window_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                        mnn_tensor lengths, mnn_tensor output, mnn_stream s);
+/* The next T tokens of each of B streams, on rolling caches. q and output [B, T, H * head_dim], k and v
+ * [B, T, num_kv_heads * head_dim], caches [B, C, num_kv_heads * head_dim], all of one type. positions:
+ * MNN_I32 [B], the tokens each stream has had before this call, which the caller keeps and moves on; steps:
+ * NULL (all T) or MNN_I32 [B], how many of the T rows are tokens of that stream (values outside 0..T count
+ * as the nearer of the two). A stream with none of the rows, or a position that is negative or above
+ * 2^31 - 1 - T, is left alone: neither its output nor its cache is touched; nor are output rows behind a
+ * stream's last. The call
+ * attends, with causal windows (window_right 0), to what the cache holds of the tokens before and to the
+ * new ones, and writes the new keys and values to their slots: token p to slot p for p < sinks, else to
+ * sinks + (p - sinks) % (C - sinks). C >= sinks + window_left + T, so that no new token takes the slot of
+ * one that is still seen; the same call again on the same caches gives the same result. output and
+ * caches may not be other arguments too. */
+mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                     mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
+                                     mnn_tensor v_cache, mnn_tensor output, mnn_stream s);
 
 /* MultiHeadAttention / CrossAttention (Attention.swift:15-1063), PyTorch packing:
  * "in_proj_weight" [3E, E] rows Q;K;V, "in_proj_bias" [3E], "out_proj_weight" [E, E],

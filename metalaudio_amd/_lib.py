@@ -33,7 +33,8 @@ STATUS = {
 
 ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "gelu": 3, "swish": 4, "sigmoid": 5, "tanh": 6}
 PAD = {"valid": 0, "same": 1, "explicit": 2, "reflect": 3}
-PRECISION = {"f32": 0, "bf16": 1}
+PRECISION = {"f32": 0, "bf16": 1, "e4m3": 2}
+DTYPE = {"f32": 0, "bf16": 1, "i32": 2, "e4m3": 3}
 
 
 class MNNError(RuntimeError):
@@ -96,6 +97,17 @@ class FreqBlockDesc(C.Structure):
         "stride_w", "num_groups")]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [("head_dim", C.c_int), ("num_axes", C.c_int), ("axis_dims", C.c_int * 4),
+                ("base", C.c_float), ("interleaved", C.c_int)]
+
+
+class WindowAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in (
+        "num_heads", "num_kv_heads", "head_dim", "window_left", "window_right", "sinks")] + [
+        ("scale", C.c_float)]
+
+
 class SeparatorDesc(C.Structure):
     _fields_ = [("input_channels", C.c_int), ("num_stems", C.c_int), ("levels", C.c_int),
                 ("channels", C.c_int * 8), ("kernel_size", C.c_int), ("stride", C.c_int),
@@ -146,6 +158,14 @@ SIGNATURES = {
     "mnn_linear_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, PP]),
     "mnn_fused_linear_create": (
         C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, PP]),
+    "mnn_linear_forward_scaled": (C.c_int, [P, P, P, P, P, P]),
+    "mnn_rmsnorm_create": (C.c_int, [P, C.c_int, C.c_float, PP]),
+    "mnn_rmsnorm_forward_residual": (C.c_int, [P, P, P, P, P, P, P]),
+    "mnn_rotary_create": (C.c_int, [P, C.POINTER(RotaryDesc), PP]),
+    "mnn_rotary_forward": (C.c_int, [P, P, P, P, P, P, P]),
+    "mnn_window_attention_create": (C.c_int, [P, C.POINTER(WindowAttentionDesc), PP]),
+    "mnn_window_attention_forward": (C.c_int, [P, P, P, P, P, P, P]),
+    "mnn_window_attention_step": (C.c_int, [P, P, P, P, P, P, P, P, P, P]),
     "mnn_mha_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, PP]),
     "mnn_feedforward_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, PP]),
     "mnn_encoder_block_create": (C.c_int, [P, C.POINTER(EncoderBlockDesc), PP]),

@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <thread>
 
 #include "layers.hpp"
@@ -9,6 +10,7 @@
 #include "safetensors.hpp"
 #include "stft.hpp"
 #include "separate.hpp"
+#include "token_layers.hpp"
 #include "weight_names.hpp"
 
 using namespace mnn;
@@ -88,6 +90,33 @@ Stream resolve_stream(Device* d, mnn_stream s) {
   }
   return Stream{d, d->default_stream, false};
 }
+
+// For layers whose products are not made in 8 bits.
+mnn_precision wide(mnn_precision p) {
+  MNN_REQUIRE(p == MNN_PRECISION_F32 || p == MNN_PRECISION_BF16, MNN_ERR_INVALID_CONFIGURATION,
+              "precision must be f32 or bf16");
+  return p;
+}
+
+std::unique_ptr<Layer> any_linear(Device* d, int in, int out, bool bias, int act, mnn_precision p,
+                                  float alpha = 0.01f) {
+  return p == MNN_PRECISION_E4M3 ? make_linear_e4m3(d, in, out, bias, act, alpha)
+                                 : make_linear(d, in, out, bias, act, wide(p), alpha);
+}
+
+// What the entry points with several tensors share: the layer's device is alive and owns each tensor
+// (NULL ones are left out); the device becomes current and the call's stream is returned.
+Stream enter(Layer* l, std::initializer_list<const Tensor*> tensors, mnn_stream st) {
+  Device* d = l->device();
+  d->check_alive();
+  for (const Tensor* t : tensors)
+    MNN_REQUIRE(!t || t->dev == d, MNN_ERR_INVALID_ARGUMENT,
+                "tensors and layer on different devices");
+  Stream s = resolve_stream(d, st);
+  d->make_current();
+  return s;
+}
+Tensor* opt(mnn_tensor t) { return t ? T(t) : nullptr; }
 
 mnn_layer wrap(std::unique_ptr<Layer> l) { return reinterpret_cast<mnn_layer>(l.release()); }
 
@@ -323,7 +352,8 @@ mnn_status mnn_tensor_create(mnn_device dev, mnn_dtype dtype, int rank, const in
     Device* d = D(dev);
     d->check_alive();
     MNN_REQUIRE(out, MNN_ERR_INVALID_ARGUMENT, "null output");
-    MNN_REQUIRE(dtype == MNN_F32 || dtype == MNN_BF16, MNN_ERR_INVALID_ARGUMENT, "bad dtype");
+    MNN_REQUIRE(dtype == MNN_F32 || dtype == MNN_BF16 || dtype == MNN_I32 || dtype == MNN_E4M3,
+                MNN_ERR_INVALID_ARGUMENT, "bad dtype");
     *out = reinterpret_cast<mnn_tensor>(tensor_create(d, dtype, to_shape(rank, dims)));
   });
 }
@@ -409,11 +439,11 @@ mnn_status mnn_tensor_device_ptr(mnn_tensor t, void** ptr) {
   })
 
 mnn_status mnn_conv1d_create(mnn_device dev, const mnn_conv1d_desc* desc, mnn_layer* out) {
-  MNN_CREATE(make_conv1d(d, need(desc)));
+  MNN_CREATE((wide(need(desc).precision), make_conv1d(d, *desc)));
 }
 mnn_status mnn_fused_conv1d_create(mnn_device dev, const mnn_conv1d_desc* desc,
                                    float leaky_relu_alpha, mnn_layer* out) {
-  MNN_CREATE(make_conv1d(d, need(desc), leaky_relu_alpha));
+  MNN_CREATE((wide(need(desc).precision), make_conv1d(d, *desc, leaky_relu_alpha)));
 }
 mnn_status mnn_conv1d_forward_residual(mnn_layer layer, mnn_tensor input, mnn_tensor residual,
                                        mnn_tensor output, mnn_stream st) {
@@ -464,25 +494,83 @@ mnn_status mnn_glu_create(mnn_device dev, int out_channels, mnn_layer* out) {
 }
 mnn_status mnn_linear_create(mnn_device dev, int in_features, int out_features, int use_bias,
                              mnn_activation act, mnn_precision prec, mnn_layer* out) {
-  MNN_CREATE(make_linear(d, in_features, out_features, use_bias != 0, act, prec));
+  MNN_CREATE(any_linear(d, in_features, out_features, use_bias != 0, act, prec));
 }
 mnn_status mnn_fused_linear_create(mnn_device dev, int in_features, int out_features,
                                    int use_bias, mnn_activation act, float leaky_relu_alpha,
                                    mnn_precision prec, mnn_layer* out) {
-  MNN_CREATE(make_linear(d, in_features, out_features, use_bias != 0, act, prec,
-                         leaky_relu_alpha));
+  MNN_CREATE(any_linear(d, in_features, out_features, use_bias != 0, act, prec, leaky_relu_alpha));
+}
+mnn_status mnn_linear_forward_scaled(mnn_layer layer, mnn_tensor input, mnn_tensor scales,
+                                     mnn_tensor residual, mnn_tensor output, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *in = T(input), *sc = opt(scales), *res = opt(residual), *out = T(output);
+    Stream s = enter(l, {in, sc, res, out}, st);
+    linear_forward_scaled(l, *in, sc, res, *out, s);
+  });
+}
+mnn_status mnn_rmsnorm_create(mnn_device dev, int feature_size, float epsilon, mnn_layer* out) {
+  MNN_CREATE(make_rmsnorm(d, feature_size, epsilon));
+}
+mnn_status mnn_rmsnorm_forward_residual(mnn_layer layer, mnn_tensor input, mnn_tensor residual,
+                                        mnn_tensor sum, mnn_tensor output, mnn_tensor scales,
+                                        mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *in = T(input), *res = opt(residual), *h = opt(sum), *out = T(output),
+           *sc = opt(scales);
+    Stream s = enter(l, {in, res, h, out, sc}, st);
+    rmsnorm_forward_residual(l, *in, res, h, *out, sc, s);
+  });
+}
+mnn_status mnn_rotary_create(mnn_device dev, const mnn_rotary_desc* desc, mnn_layer* out) {
+  MNN_CREATE(make_rotary(d, need(desc)));
+}
+mnn_status mnn_rotary_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor positions,
+                              mnn_tensor q_out, mnn_tensor k_out, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tq = T(q), *tk = opt(k), *pos = T(positions), *qo = T(q_out), *ko = opt(k_out);
+    Stream s = enter(l, {tq, tk, pos, qo, ko}, st);
+    rotary_forward(l, *tq, tk, *pos, *qo, ko, s);
+  });
+}
+mnn_status mnn_window_attention_create(mnn_device dev, const mnn_window_attention_desc* desc,
+                                       mnn_layer* out) {
+  MNN_CREATE(make_window_attention(d, need(desc)));
+}
+mnn_status mnn_window_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                        mnn_tensor lengths, mnn_tensor output, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tq = T(q), *tk = T(k), *tv = T(v), *len = opt(lengths), *out = T(output);
+    Stream s = enter(l, {tq, tk, tv, len, out}, st);
+    window_attention_forward(l, *tq, *tk, *tv, len, *out, s);
+  });
+}
+mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                     mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
+                                     mnn_tensor v_cache, mnn_tensor output, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tq = T(q), *tk = T(k), *tv = T(v), *pos = T(positions), *stp = opt(steps),
+           *kc = T(k_cache), *vc = T(v_cache), *out = T(output);
+    Stream s = enter(l, {tq, tk, tv, pos, stp, kc, vc, out}, st);
+    window_attention_step(l, *tq, *tk, *tv, *pos, stp, *kc, *vc, *out, s);
+  });
 }
 mnn_status mnn_mha_create(mnn_device dev, int embed_dim, int num_heads, int use_bias,
                           mnn_precision prec, mnn_layer* out) {
-  MNN_CREATE(make_mha(d, embed_dim, num_heads, use_bias != 0, prec));
+  MNN_CREATE(make_mha(d, embed_dim, num_heads, use_bias != 0, wide(prec)));
 }
 mnn_status mnn_feedforward_create(mnn_device dev, int input_dim, int hidden_dim,
                                   mnn_precision prec, mnn_layer* out) {
-  MNN_CREATE(make_feedforward(d, input_dim, hidden_dim, prec));
+  MNN_CREATE(make_feedforward(d, input_dim, hidden_dim, wide(prec)));
 }
 mnn_status mnn_encoder_block_create(mnn_device dev, const mnn_encoder_block_desc* desc,
                                     mnn_layer* out) {
-  MNN_CREATE(make_encoder_block(d, need(desc)));
+  MNN_CREATE((wide(need(desc).precision), make_encoder_block(d, *desc)));
 }
 mnn_status mnn_conv_transpose1d_create(mnn_device dev, const mnn_conv_transpose1d_desc* desc,
                                        mnn_layer* out) {
@@ -960,19 +1048,21 @@ mnn_status mnn_mtla_writer_destroy(mnn_mtla_writer w) {
 
 mnn_status mnn_transformer_layer_create(mnn_device dev, int embed_dim, int num_heads, int ffn_dim,
                                         float layer_scale, mnn_precision prec, mnn_layer* out) {
-  MNN_CREATE(make_transformer_layer(d, embed_dim, num_heads, ffn_dim, layer_scale, prec));
+  MNN_CREATE(make_transformer_layer(d, embed_dim, num_heads, ffn_dim, layer_scale, wide(prec)));
 }
 mnn_status mnn_cross_transformer_create(mnn_device dev, int embed_dim, int num_heads, int ffn_dim,
                                         int num_layers, float layer_scale, mnn_precision prec,
                                         mnn_layer* out) {
   MNN_CREATE(
-      make_cross_transformer(d, embed_dim, num_heads, ffn_dim, num_layers, layer_scale, prec));
+      make_cross_transformer(d, embed_dim, num_heads, ffn_dim, num_layers, layer_scale,
+                                    wide(prec)));
 }
 
 mnn_status mnn_cross_transformer_encoder_create(mnn_device dev, int embed_dim, int num_heads,
                                                 int ffn_dim, int num_layers, mnn_precision prec,
                                                 mnn_layer* out) {
-  MNN_CREATE(make_cross_transformer_encoder(d, embed_dim, num_heads, ffn_dim, num_layers, prec));
+  MNN_CREATE(make_cross_transformer_encoder(d, embed_dim, num_heads, ffn_dim, num_layers,
+                                            wide(prec)));
 }
 
 mnn_status mnn_layer_destroy(mnn_layer layer) {
@@ -1006,8 +1096,9 @@ mnn_status mnn_layer_forward(mnn_layer layer, mnn_tensor input, mnn_tensor outpu
     d->check_alive();
     MNN_REQUIRE(in->dev == d && o->dev == d, MNN_ERR_INVALID_ARGUMENT,
                 "tensors and layer on different devices");
-    MNN_REQUIRE(in->dtype == MNN_F32 || l->accepts_bf16(), MNN_ERR_INVALID_ARGUMENT,
-                l->kind() << ": input must be f32");
+    MNN_REQUIRE(in->dtype == MNN_F32 || (in->dtype == MNN_BF16 && l->accepts_bf16()),
+                MNN_ERR_INVALID_ARGUMENT, l->kind() << ": input must be f32"
+                                              << (l->accepts_bf16() ? " or bf16" : ""));
     Stream s = resolve_stream(d, st);
     d->make_current();
     l->forward(*in, *o, s);

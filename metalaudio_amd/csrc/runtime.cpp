@@ -6,7 +6,7 @@
 
 namespace mnn {
 
-size_t dtype_size(mnn_dtype t) { return t == MNN_BF16 ? 2 : 4; }
+size_t dtype_size(mnn_dtype t) { return t == MNN_E4M3 ? 1 : t == MNN_BF16 ? 2 : 4; }
 
 std::atomic<int64_t> g_device_allocations{0};
 
@@ -185,6 +185,8 @@ Tensor* Sequential::forward_locked(const Tensor& in, Stream& s) {
   MNN_REQUIRE(ok, MNN_ERR_INPUT_SHAPE_MISMATCH,
               "Model input shape mismatch: expected " << shape_str(expect) << ", got "
                                                       << shape_str(in.shape));
+  MNN_REQUIRE(in.dtype == MNN_F32 || (in.dtype == MNN_BF16 && layers_[0]->accepts_bf16()),
+              MNN_ERR_INVALID_ARGUMENT, layers_[0]->kind() << ": unsupported input type");
   Plan* p = plan_for(in.shape);
   last_plan_ = p;
   const Tensor* cur = &in;

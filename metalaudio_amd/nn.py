@@ -14,14 +14,14 @@ from typing import Iterable, Optional, Sequence
 import numpy as np
 
 from . import _lib
-from ._lib import (ACT, PAD, PRECISION, Conv1dDesc, Conv2dDesc, ConvTranspose1dDesc,
+from ._lib import (ACT, DTYPE, PAD, PRECISION, Conv1dDesc, Conv2dDesc, ConvTranspose1dDesc,
                    ConvTranspose2dDesc, DecoderBlockDesc, EncoderBlockDesc, FreqBlockDesc, MNNError,
-                   SeparatorDesc, check, dims, lib)
+                   RotaryDesc, SeparatorDesc, WindowAttentionDesc, check, dims, lib)
 
 __all__ = [
     "MNNError", "AudioDevice", "Stream", "Tensor", "Layer", "Conv1D", "DynamicConv1D",
-    "FusedConv1D", "GroupNorm", "LayerNorm", "GELU", "GLU", "Linear", "FusedLinear",
-    "MultiHeadAttention", "CrossAttention",
+    "FusedConv1D", "GroupNorm", "LayerNorm", "RMSNorm", "GELU", "GLU", "Linear", "FusedLinear",
+    "Rotary", "WindowAttention", "MultiHeadAttention", "CrossAttention",
     "FeedForward", "UNetEncoderBlock", "ConvTranspose1D", "DynamicConvTranspose1D",
     "UNetDecoderBlock", "unet_padding", "unet_bottleneck_length", "TransformerLayer",
     "CrossTransformerEncoder", "Sequential", "SafeTensors", "BinaryModelFile", "WeightNameMapper",
@@ -102,6 +102,10 @@ def _sh(stream: Optional[Stream]):
     return stream.handle if stream is not None else None
 
 
+def _th(tensor):
+    return tensor.handle if tensor is not None else None
+
+
 def bf16_bits(a) -> np.ndarray:
     """fp32 -> bf16 bit patterns (uint16), round to nearest even, NaN kept quiet."""
     u = _f32(a).view(np.uint32).astype(np.uint64)
@@ -110,10 +114,34 @@ def bf16_bits(a) -> np.ndarray:
     return np.where(nan, ((u >> 16) | 0x40).astype(np.uint16), r)
 
 
+def e4m3_bits(a) -> np.ndarray:
+    """fp32 -> e4m3 bit patterns (uint8), round to nearest even; NaN and what rounds beyond the
+    largest value, 448, become NaN (the type has no infinities)."""
+    x = _f32(a)
+    mag = np.abs(x).astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        exp = np.clip(np.frexp(mag)[1] - 1, -6, 8)
+        units = np.rint(np.ldexp(mag, 3 - exp))  # of 2^(exp - 3); 16 units are the next exponent's 8
+        value = np.where(units < 8, units, units + 8 * (exp + 6))
+        bits = np.where(value <= 0x7E, value, 0x7F)  # NaN compares false
+    return (bits.astype(np.uint8) | (np.signbit(x).astype(np.uint8) << 7)).reshape(x.shape)
+
+
+def _e4m3_values() -> np.ndarray:
+    b = np.arange(128)
+    e, m = b >> 3, b & 7
+    v = np.where(e > 0, np.ldexp(8.0 + m, e - 10), np.ldexp(m.astype(np.float64), -9))
+    v[127] = np.nan
+    return np.concatenate([v, -v]).astype(np.float32)
+
+
+E4M3_VALUES = _e4m3_values()  # the value of each of the 256 bit patterns
+
+
 class Tensor:
-    """Device tensor, contiguous row-major, zero-initialised (Tensor.swift:59-141); fp32 or bf16
-    (dtype "bf16": 16-bit values, host data rounded to nearest even on upload, widened to fp32
-    on download)."""
+    """Device tensor, contiguous row-major, zero-initialised (Tensor.swift:59-141); fp32, bf16 or
+    e4m3 (dtype "bf16" / "e4m3": 16- and 8-bit values, host data rounded to nearest even on
+    upload, widened to fp32 on download), or "i32" for positions and lengths."""
 
     def __init__(self, device: AudioDevice, shape: Sequence[int], _handle=None, _owned=True,
                  dtype: str = "f32"):
@@ -122,8 +150,8 @@ class Tensor:
         if _handle is None:
             h = C.c_void_p()
             shape = [int(s) for s in shape]
-            check(lib().mnn_tensor_create(device.handle, {"f32": 0, "bf16": 1}[dtype],
-                                          len(shape), dims(shape), C.byref(h)))
+            check(lib().mnn_tensor_create(device.handle, DTYPE[dtype], len(shape), dims(shape),
+                                          C.byref(h)))
             _handle = h
         self.handle = _handle
         self._owned = _owned
@@ -131,7 +159,7 @@ class Tensor:
     @classmethod
     def from_numpy(cls, device: AudioDevice, arr, stream: Optional[Stream] = None,
                    dtype: str = "f32") -> "Tensor":
-        a = _f32(arr)
+        a = np.asarray(arr) if dtype == "i32" else _f32(arr)
         t = cls(device, a.shape, dtype=dtype)
         t.copy_from(a, stream)
         return t
@@ -152,13 +180,23 @@ class Tensor:
 
     def copy_from(self, arr, stream: Optional[Stream] = None) -> None:
         """Tensor.copy(from:) — synchronous upload."""
-        a = _f32(arr)
+        if self.dtype == "i32":
+            a = np.ascontiguousarray(np.asarray(arr, dtype=np.int32))
+        else:
+            a = _f32(arr)
         if self.dtype == "bf16":
             a = np.ascontiguousarray(bf16_bits(a))
+        elif self.dtype == "e4m3":
+            a = np.ascontiguousarray(e4m3_bits(a))
         check(lib().mnn_tensor_upload(self.handle, a.ctypes.data, a.nbytes, _sh(stream)))
 
     def to_numpy(self, stream: Optional[Stream] = None) -> np.ndarray:
-        """toArray() — synchronous download, shaped like the tensor (fp32)."""
+        """toArray() — synchronous download, shaped like the tensor (fp32; int32 for "i32")."""
+        if self.dtype in ("i32", "e4m3"):
+            raw = np.empty(self.shape, dtype=np.int32 if self.dtype == "i32" else np.uint8)
+            check(lib().mnn_tensor_download(self.handle, raw.ctypes.data, raw.nbytes,
+                                            _sh(stream)))
+            return raw if self.dtype == "i32" else E4M3_VALUES[raw]
         if self.dtype == "bf16":
             raw = np.empty(self.shape, dtype=np.uint16)
             check(lib().mnn_tensor_download(self.handle, raw.ctypes.data, raw.nbytes,
@@ -325,6 +363,26 @@ class LayerNorm(Layer):
         self.load_weights_named("beta", beta)
 
 
+class RMSNorm(Layer):
+    """y = x * rsqrt(mean(x^2) + epsilon) * weight over the last dimension."""
+
+    def __init__(self, device, feature_size, epsilon=1e-5):
+        super().__init__(device, _create(lib().mnn_rmsnorm_create, device.handle, feature_size,
+                                         epsilon))
+
+    def load_parameters(self, weight) -> None:
+        self.load_weights_named("weight", weight)
+
+    def forward_residual(self, input: Tensor, residual: Optional[Tensor], output: Tensor,
+                         sum: Optional[Tensor] = None, scales: Optional[Tensor] = None,
+                         stream: Optional[Stream] = None) -> None:
+        """sum = input + residual; output = RMSNorm(sum), in 8 bits with `scales` per row where
+        the output is "e4m3"."""
+        check(lib().mnn_rmsnorm_forward_residual(self.handle, input.handle, _th(residual),
+                                                 _th(sum), output.handle, _th(scales),
+                                                 _sh(stream)))
+
+
 class GELU(Layer):
     def __init__(self, device, input_shape):
         super().__init__(device, _create(lib().mnn_gelu_create, device.handle, len(input_shape),
@@ -337,6 +395,9 @@ class GLU(Layer):
 
 
 class Linear(Layer):
+    """Linear (Linear.swift:27-460); precision "f32", "bf16", or "e4m3": weights and input in 8
+    bits with a scale per row."""
+
     def __init__(self, device, input_features, output_features, use_bias=True, activation="none",
                  precision="f32", leaky_relu_alpha=None):
         if leaky_relu_alpha is None:
@@ -355,6 +416,15 @@ class Linear(Layer):
             self.load_weights_named("bias", bias)
 
 
+    def forward_scaled(self, input: Tensor, scales: Optional[Tensor], output: Tensor,
+                       residual: Optional[Tensor] = None,
+                       stream: Optional[Stream] = None) -> None:
+        """Precision "e4m3": output = act(input W^T + bias) + residual, input "e4m3" with its row
+        scales, or "f32" / "bf16" without."""
+        check(lib().mnn_linear_forward_scaled(self.handle, input.handle, _th(scales),
+                                              _th(residual), output.handle, _sh(stream)))
+
+
 class FusedLinear(Linear):
     """FusedLinear (Linear.swift:475-672): activation (default relu) and leakyReluAlpha."""
 
@@ -362,6 +432,51 @@ class FusedLinear(Linear):
                  leaky_relu_alpha=0.01, precision="f32"):
         super().__init__(device, input_features, output_features, use_bias, activation,
                          precision, leaky_relu_alpha=leaky_relu_alpha)
+
+
+class Rotary(Layer):
+    """Rotary positions over one to four axes: `axis_dims` dimensions of each head turn with the
+    token's position on each axis, the rest pass."""
+
+    def __init__(self, device, head_dim, axis_dims, base=10000.0, interleaved=False):
+        axis_dims = [int(d) for d in axis_dims]
+        if len(axis_dims) > 4:
+            raise ValueError("Rotary: at most 4 axes")
+        d = RotaryDesc(head_dim, len(axis_dims), (C.c_int * 4)(*axis_dims), base,
+                       int(interleaved))
+        super().__init__(device, _create(lib().mnn_rotary_create, device.handle, C.byref(d)))
+
+    def forward(self, q: Tensor, k: Optional[Tensor], positions: Tensor,  # type: ignore[override]
+                q_out: Tensor, k_out: Optional[Tensor] = None,
+                stream: Optional[Stream] = None) -> None:
+        check(lib().mnn_rotary_forward(self.handle, q.handle, _th(k), positions.handle,
+                                       q_out.handle, _th(k_out), _sh(stream)))
+
+
+class WindowAttention(Layer):
+    """Attention of token i to the tokens i - window_left .. i + window_right and the first
+    `sinks` ones."""
+
+    def __init__(self, device, num_heads, head_dim, num_kv_heads=None, window_left=0,
+                 window_right=0, sinks=0, scale=0.0):
+        d = WindowAttentionDesc(num_heads, num_heads if num_kv_heads is None else num_kv_heads,
+                                head_dim, window_left, window_right, sinks, scale)
+        super().__init__(device, _create(lib().mnn_window_attention_create, device.handle,
+                                         C.byref(d)))
+
+    def forward(self, q: Tensor, k: Tensor, v: Tensor, output: Tensor,  # type: ignore[override]
+                lengths: Optional[Tensor] = None, stream: Optional[Stream] = None) -> None:
+        check(lib().mnn_window_attention_forward(self.handle, q.handle, k.handle, v.handle,
+                                                 _th(lengths), output.handle, _sh(stream)))
+
+    def step(self, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, k_cache: Tensor,
+             v_cache: Tensor, output: Tensor, steps: Optional[Tensor] = None,
+             stream: Optional[Stream] = None) -> None:
+        """The streams' next tokens on their rolling caches (causal); see
+        mnn_window_attention_step."""
+        check(lib().mnn_window_attention_step(self.handle, q.handle, k.handle, v.handle,
+                                              positions.handle, _th(steps), k_cache.handle,
+                                              v_cache.handle, output.handle, _sh(stream)))
 
 
 class MultiHeadAttention(Layer):
