@@ -1,7 +1,11 @@
 // Window attention over whole sequences: o_i = sum_j p_ij v_j, p_i = softmax of scale q_i k_j over the keys
 // j <= i + right with j >= i - left or j < sinks.
+#include "lds_dma.hpp"
 #include "token_ops.hpp"
 #include "window_row.hpp"
+#include "x3.hpp"
+
+#include <type_traits>
 
 namespace mnn {
 namespace k {
@@ -29,23 +33,335 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
   if (lane + 64 < a.hd) o[lane + 64] = from_f32<T>(o1);
 }
 
-// A wave per query.
-template <class T>
-__global__ __launch_bounds__(256) void window_any_kernel(WindowArgs a) {
-  const int b = blockIdx.z, h = blockIdx.y;
+// A workgroup is 4 waves of 32 queries of one head over blocks of keys that all four read from LDS. Each
+// wave computes the TRANSPOSED scores S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q):
+// keys 8 (v / 4) + 4 g + v % 4 of query q) is the B operand that O^T += V^T P^T needs when its k slots take
+// those keys, so P goes from the softmax straight into the second product. K and V lie in LDS row by row as
+// they come; V^T's fragments (4 keys of one dimension a lane) are transposed on the way out by
+// ds_read_b64_tr_b16. f32 values are three bf16 parts each and six partial products are kept (x3.hpp); the
+// workgroup splits a block of K and V as it stores it.
+//
+// Only the blocks that a query of the workgroup sees are visited, and of those a wave computes the ones
+// that its own queries see; the mask is applied where a block is not wholly visible to all 32. While one
+// block is computed the next one's rows are on their way to registers.
+//
+// Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
+//
+// A key that a query does not see has probability 0, but 0 times a value that is not finite is NaN, and
+// parts of tiny or overflowing f32 values are off: queries whose result is not finite (or, in f32, below
+// 2^-109) are computed again by window_query.
+template <class T, int KS>
+struct WindowCfg {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int PARTS = F32 ? 3 : 1;
+  static constexpr int BKV = F32 ? 32 : 64;   // keys per block
+  static constexpr int NT = BKV / 32;
+  static constexpr int DT = (KS + 1) / 2;     // 32-row tiles of O^T
+  // bytes from one key's row to the next in LDS: 8 rows of 16-byte reads on distinct banks
+  static constexpr int PITCH = KS * 32 + (KS % 2 ? 0 : 16);
+  static constexpr int PLANE = BKV * PITCH;
+  static constexpr int CHUNKS = BKV * KS * 2;  // of 8 values, in a block of K or V
+  static constexpr int PER = (CHUNKS + 255) / 256;
+};
+
+template <class T, int KS>
+__global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_kernel(WindowArgs a) {
+  using Cfg = WindowCfg<T, KS>;
+  constexpr int PARTS = Cfg::PARTS, BKV = Cfg::BKV, NT = Cfg::NT, DT = Cfg::DT, PITCH = Cfg::PITCH;
+  constexpr int PLANE = Cfg::PLANE, PER = Cfg::PER;
+  constexpr bool F32 = Cfg::F32;
+  // K planes, then V planes; V's fragments of the last 32 dimensions may reach 32 bytes past its rows
+  __shared__ __attribute__((aligned(16))) char smem[2 * PARTS * PLANE + 64];
+
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // consecutive units, the heads that share K and V first, run on one XCD and share its L2
+  const int nq = (a.S + 127) / 128, G = a.H / a.KV;
+  const int64_t units = (int64_t)nq * a.H * a.B;
+  int64_t unit = xcd_logical_tile((int)blockIdx.x, (int)units);
+  const int gi = (int)(unit % G);
+  unit /= G;
+  const int q0 = (int)(unit % nq) * 128;
+  unit /= nq;
+  const int kvh = (int)(unit % a.KV), b = (int)(unit / a.KV), h = kvh * G + gi;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < len; i += (int64_t)gridDim.x * 4)
-    window_query<T>(a, b, h, (int)i, len);
+  if (q0 >= len) return;
+  const int qw = q0 + 32 * wave;              // this wave's first query
+  const int qn = min(qw + 31, len - 1);       // and last
+  const int qi = qw + l32;                    // the lane's
+  const int kvw = a.KV * a.hd, qrow = a.H * a.hd;
+  const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.S * kvw + kvh * a.hd;
+  const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.S * kvw + kvh * a.hd;
+
+  // blocks: those of the sinks before the window's first, then the window's
+  const int last = min(q0 + 127, len - 1);
+  const int first_blk = max(0, q0 - a.left) / BKV;
+  const int last_blk = (int)min((int64_t)len - 1, (int64_t)last + a.right) / BKV;
+  const int sink_blks = (int)min((int64_t)first_blk, ((int64_t)a.sinks + BKV - 1) / BKV);
+  const int n = sink_blks + last_blk - first_blk + 1;
+  auto block_of = [&](int t) { return t < sink_blks ? t : first_blk + t - sink_blks; };
+
+  // one block of K and V on its way: 8 values a chunk
+  typedef float floatx8 __attribute__((ext_vector_type(8)));
+  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+  using Chunk = std::conditional_t<F32, floatx8, uintx4>;
+  Chunk ck[PER], cv[PER];
+  auto fetch = [&](int blk) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = tid + 256 * i, row = e / (2 * KS), c = e % (2 * KS);
+      if (e < Cfg::CHUNKS && 8 * c < a.hd) {
+        const int64_t at = (int64_t)min(blk * BKV + row, len - 1) * kvw + 8 * c;
+        ck[i] = *reinterpret_cast<const Chunk*>(kb + at);
+        cv[i] = *reinterpret_cast<const Chunk*>(vb + at);
+      }
+    }
+  };
+  auto parts_of = [&](Chunk x, float by) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e] * by;
+    return split8(y);
+  };
+  auto put = [&](Chunk x, char* to) {
+    if constexpr (F32) {
+      const Split8 s = parts_of(x, 1.f);
+      *reinterpret_cast<bf16x8*>(to) = s.h;
+      *reinterpret_cast<bf16x8*>(to + PLANE) = s.m;
+      *reinterpret_cast<bf16x8*>(to + 2 * PLANE) = s.l;
+    } else {
+      *reinterpret_cast<Chunk*>(to) = x;
+    }
+  };
+  auto store = [&] {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = tid + 256 * i, row = e / (2 * KS), c = e % (2 * KS);
+      if (e < Cfg::CHUNKS && 8 * c < a.hd) {
+        put(ck[i], smem + row * PITCH + 16 * c);
+        put(cv[i], smem + PARTS * PLANE + row * PITCH + 16 * c);
+      }
+    }
+  };
+  if (a.hd < 16 * KS) {  // columns behind the head's last stay zero
+    for (int e = tid; e < 2 * PARTS * BKV; e += 256)
+      for (int c = a.hd / 8; c < 2 * KS; ++c)
+        *reinterpret_cast<float4*>(smem + e * PITCH + 16 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  fetch(block_of(0));
+
+  // Q: B operand, query l32, dimensions 16 s + 8 g .. + 7. f32: times the scale in powers of two; bf16: as
+  // it is, up to the scale's sign, the scale in the exponent instead.
+  const float qs = a.scale * 1.4426950408889634f;
+  const float cs = F32 ? 1.f : fabsf(qs);
+  bf16x8 qf[KS][PARTS];
+  {
+    const T* p = static_cast<const T*>(a.q) + ((int64_t)b * a.S + min(qi, len - 1)) * qrow + h * a.hd + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Chunk x = 0;
+      if (16 * s + 8 * g < a.hd) x = *reinterpret_cast<const Chunk*>(p + 16 * s);
+      if constexpr (F32) {
+        const Split8 sp = parts_of(x, qs);
+        qf[s][0] = sp.h;
+        qf[s][1] = sp.m;
+        qf[s][2] = sp.l;
+      } else {
+        qf[s][0] = __builtin_bit_cast(bf16x8, x ^ (qs < 0.f ? 0x80008000u : 0u));
+      }
+    }
+  }
+
+  floatx16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
+  float ref = 0.f, lsum = 0.f;  // ref: in the scores' units
+  bool begun = false;           // whether the query has seen a key
+
+  const char* kf0 = smem + l32 * PITCH + 16 * g;
+  const char* vf0 = smem + PARTS * PLANE + (4 * g + ((lane & 15) >> 2)) * PITCH + 32 * ((lane >> 4) & 1) +
+                    8 * (lane & 3);
+  auto vfrag = [&](int part, int t, int ks) {  // dimensions 32 t + l32, keys 16 ks + 4 g + {0..3, 8..11}
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    const char* p = vf0 + part * PLANE + 16 * ks * PITCH + 64 * t;
+    union {
+      short4v s[2];
+      bf16x8 f;
+    } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
+    u.s[1] =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p + 8 * PITCH));
+    return u.f;
+  };
+
+  store();
+  for (int t = 0; t < n; ++t) {
+    lds_barrier();
+    const int k0 = block_of(t) * BKV, k1 = k0 + BKV - 1;
+    if (t + 1 < n) fetch(block_of(t + 1));
+    // seen by any query of the wave?
+    const bool any = qw <= qn && k0 <= (int64_t)qn + a.right && (k1 >= qw - a.left || k0 < a.sinks);
+    if (any) {
+      floatx16 st[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) st[j][v] = 0.f;
+        if constexpr (F32) {
+          floatx16 low;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) low[v] = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            Split8 kx, qx{qf[s][0], qf[s][1], qf[s][2]};
+            kx.h = *reinterpret_cast<const bf16x8*>(kf0 + 32 * s);
+            kx.m = *reinterpret_cast<const bf16x8*>(kf0 + PLANE + 32 * s);
+            kx.l = *reinterpret_cast<const bf16x8*>(kf0 + 2 * PLANE + 32 * s);
+#pragma unroll
+            for (int p = 0; p < 5; ++p) low = mfma_x3(kx, qx, low, p);
+            st[j] = mfma_x3(kx, qx, st[j], 5);
+          }
+#pragma unroll
+          for (int v = 0; v < 16; ++v) st[j][v] += low[v];
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+            st[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                *reinterpret_cast<const bf16x8*>(kf0 + 32 * j * PITCH + 32 * s), qf[s][0], st[j], 0, 0, 0);
+        }
+      }
+      const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= (int64_t)qw + a.right && k1 < len;
+      if (!whole) {
+        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right), lo = qi - a.left;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int key = k0 + 32 * j + 8 * (v / 4) + 4 * g + (v % 4);
+            if (!(key <= hi && (key >= lo || key < a.sinks))) st[j][v] = -INFINITY;
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, st[j][v]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const bool move = begun ? (mx - ref) * cs > 8.f : mx > -INFINITY;
+      if (__any(move)) {
+        // the first visible key has nothing to rescale
+        const float alpha = !move ? 1.f : begun ? __builtin_amdgcn_exp2f((ref - mx) * cs) : 0.f;
+        lsum *= alpha;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] *= alpha;
+        ref = move ? mx : ref;
+        begun |= move;
+      }
+      const float off = ref * cs;
+      // the block's probabilities are added up by themselves before they join the running sum
+      float ps = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2 * NT; ++ks) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(st[ks >> 1][8 * (ks & 1) + e], cs, -off));
+          ps += p[e];
+        }
+        if constexpr (F32) {
+          const Split8 px = split8(p);
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            const Split8 vx{vfrag(0, i, ks), vfrag(1, i, ks), vfrag(2, i, ks)};
+#pragma unroll
+            for (int m = 0; m < 6; ++m) o[i] = mfma_x3(vx, px, o[i], m);
+          }
+        } else {
+          // probabilities to bf16, to nearest: each is off by 2^-9 of itself at most, the sum keeps fp32
+          const bf16x8 px = __builtin_bit_cast(
+              bf16x8, uintx4{cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                             cvt_pk_bf16(p[6], p[7])});
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(0, i, ks), px, o[i], 0, 0, 0);
+        }
+      }
+      lsum += ps;
+    }
+    lds_barrier();
+    if (t + 1 < n) store();
+  }
+
+  const float l = lsum + __shfl_xor(lsum, 32, 64);
+  const float inv = 1.f / l;
+  float chk = l * 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int c = 0; c < 2 * KS; ++c)  // dimensions 8 c + 4 g .. + 3
+    if (8 * c < a.hd) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = o[c / 4][4 * (c % 4) + e];
+        chk = fmaf(x, 0.f, chk);
+        if (F32) bad |= (x != 0.f) & (fabsf(x) < l * 0x1p-109f);
+      }
+    }
+  unsigned long long again = __ballot(qi < len && (bad || !(chk == 0.f)));
+  again = (again | (again >> 32)) & 0xffffffffull;
+  if (qi < len && !((again >> l32) & 1)) {
+    T* out = static_cast<T*>(a.o) + ((int64_t)b * a.S + qi) * qrow + h * a.hd + 4 * g;
+#pragma unroll
+    for (int c = 0; c < 2 * KS; ++c)
+      if (8 * c < a.hd) {
+        const floatx16& ot = o[c / 4];
+        const int v = 4 * (c % 4);
+        if constexpr (F32)
+          *reinterpret_cast<float4*>(out + 8 * c) =
+              make_float4(ot[v] * inv, ot[v + 1] * inv, ot[v + 2] * inv, ot[v + 3] * inv);
+        else
+          *reinterpret_cast<uint2*>(out + 8 * c) =
+              make_uint2(cvt_pk_bf16(ot[v] * inv, ot[v + 1] * inv),
+                         cvt_pk_bf16(ot[v + 2] * inv, ot[v + 3] * inv));
+      }
+  }
+  while (again) {
+    const int j = __builtin_ctzll(again);
+    again &= again - 1;
+    window_query<T>(a, b, h, qw + j, len);
+  }
+}
+
+template <class T, int KS>
+void launch_window(const LaunchCtx& c, const WindowArgs& a) {
+  const int64_t units = (int64_t)((a.S + 127) / 128) * a.H * a.B;
+  MNN_REQUIRE(units < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
+              "WindowAttention: too many tokens in one call");
+  launch(c, sizeof(T) == 4 ? "window_f32" : "window_bf16", window_kernel<T, KS>, dim3((unsigned)units),
+         dim3(256), 0, a);
+}
+
+template <class T>
+void launch_window_t(const LaunchCtx& c, const WindowArgs& a) {
+  switch ((a.hd + 15) / 16) {
+    case 1:
+    case 2: return launch_window<T, 2>(c, a);
+    case 3: return launch_window<T, 3>(c, a);
+    case 4: return launch_window<T, 4>(c, a);
+    case 5: return launch_window<T, 5>(c, a);
+    case 6: return launch_window<T, 6>(c, a);
+    default: return launch_window<T, 8>(c, a);
+  }
 }
 
 }  // namespace
 
 void window_attention(const LaunchCtx& c, const WindowArgs& a) {
-  const dim3 grid((unsigned)std::min<int64_t>((a.S + 3) / 4, 1 << 15), a.H, a.B);
   if (a.type == MNN_F32)
-    launch(c, "window_any_f32", window_any_kernel<float>, grid, dim3(256), 0, a);
+    launch_window_t<float>(c, a);
   else
-    launch(c, "window_any_bf16", window_any_kernel<__bf16>, grid, dim3(256), 0, a);
+    launch_window_t<__bf16>(c, a);
 }
 
 }  // namespace k
