@@ -62,10 +62,12 @@ struct WindowCfg {
   static constexpr int PLANE = BKV * PITCH;
   static constexpr int CHUNKS = BKV * KS * 2;  // of 8 values, in a block of K or V
   static constexpr int PER = (CHUNKS + 255) / 256;
+  // workgroups a CU, as the registers allow without spilling
+  static constexpr int OCC = F32 ? (KS > 6 ? 1 : KS > 4 ? 2 : 3) : (KS > 6 ? 2 : KS > 4 ? 3 : 4);
 };
 
 template <class T, int KS>
-__global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_kernel(WindowArgs a) {
+__global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(WindowArgs a) {
   using Cfg = WindowCfg<T, KS>;
   constexpr int PARTS = Cfg::PARTS, BKV = Cfg::BKV, NT = Cfg::NT, DT = Cfg::DT, PITCH = Cfg::PITCH;
   constexpr int PLANE = Cfg::PLANE, PER = Cfg::PER;
@@ -234,21 +236,24 @@ __global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_
       }
       const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= (int64_t)qw + a.right && k1 < len;
       if (!whole) {
-        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right), lo = qi - a.left;
+        const int first = k0 + 4 * g;  // the lane's: key c below is first + c
+        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right) - first;
+        const int lo = qi - a.left - first, sk = a.sinks - first;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int key = k0 + 32 * j + 8 * (v / 4) + 4 * g + (v % 4);
-            if (!(key <= hi && (key >= lo || key < a.sinks))) st[j][v] = -INFINITY;
+            const int c = 32 * j + 8 * (v / 4) + v % 4;
+            st[j][v] = (c <= hi) & ((c >= lo) | (c < sk)) ? st[j][v] : -INFINITY;
           }
       }
+      // maximum keeps NaN, which costs no canonical forms; a NaN neither moves the reference nor passes
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, st[j][v]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        for (int v = 0; v < 16; v += 2) mx = max_nan(max_nan(mx, st[j][v]), st[j][v + 1]);
+      mx = other_half(mx, max_nan);
       const bool move = begun ? (mx - ref) * cs > 8.f : mx > -INFINITY;
       if (__any(move)) {
         // the first visible key has nothing to rescale
@@ -268,7 +273,7 @@ __global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = __builtin_amdgcn_exp2f(fmaf(st[ks >> 1][8 * (ks & 1) + e], cs, -off));
-          ps += p[e];
+          if (F32) ps += p[e];
         }
         if constexpr (F32) {
           const Split8 px = split8(p);
@@ -279,10 +284,13 @@ __global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_
             for (int m = 0; m < 6; ++m) o[i] = mfma_x3(vx, px, o[i], m);
           }
         } else {
-          // probabilities to bf16, to nearest: each is off by 2^-9 of itself at most, the sum keeps fp32
-          const bf16x8 px = __builtin_bit_cast(
-              bf16x8, uintx4{cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
-                             cvt_pk_bf16(p[6], p[7])});
+          // probabilities to bf16, to nearest (each is off by 2^-9 of itself at most), and the sum of
+          // those, two an instruction
+          const uintx4 pb{cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                          cvt_pk_bf16(p[6], p[7])};
+          const bf16x8 px = __builtin_bit_cast(bf16x8, pb);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ps = add_pair(pb[e], ps);
 #pragma unroll
           for (int i = 0; i < DT; ++i)
             o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(0, i, ks), px, o[i], 0, 0, 0);
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(256, KS > 6 && sizeof(T) == 4 ? 1 : 2) void window_
     if (t + 1 < n) store();
   }
 
-  const float l = lsum + __shfl_xor(lsum, 32, 64);
+  const float l = other_half(lsum, [](float x, float y) { return x + y; });
   const float inv = 1.f / l;
   float chk = l * 0.f;
   bool bad = false;

@@ -18,6 +18,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
 }
 
+// op of a lane's value and that of the lane 32 away.
+template <class F>
+__device__ __forceinline__ float other_half(float v, F op) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned x = r[0], y = r[1];  // as values: a bit cast of r[1] itself reads r[0]
+  return op(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+
+// c + the two bf16 values in x.
+__device__ __forceinline__ float add_pair(unsigned x, float c) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x),
+                                         __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
+}
+
 // Scale of an e4m3 row from its largest magnitude: a value is kept as x * inv. No clamp is needed behind
 // it: x * (448 * (1 / max)) is above 448 by three roundings at most, and all up to 464 round to 448.
 constexpr float kE4m3Max = 448.f;
