@@ -5,6 +5,7 @@
 #include "token_ops.hpp"
 #include "window_row.hpp"
 
+#include <algorithm>
 #include <climits>
 
 namespace mnn {
@@ -25,18 +26,42 @@ __device__ __forceinline__ int slot_of(const WindowStepArgs& a, int p) {
   return p < a.sinks ? p : a.sinks + (p - a.sinks) % (a.C - a.sinks);
 }
 
-// A wave per query and head; the first head of each group writes the token's key and value.
+// The rows of a call that one workgroup answers: R of the T * G queries (token t, head g of the group) that
+// read key/value head kvh of stream b, and the keys that any of them sees, numbered from 0: the sinks before
+// the window's first token, then the window.
+struct Rows {
+  int b, kvh, row0, pos, nt;  // nt: tokens of the stream in this call
+  int t0, t1;                 // first and last token among the rows
+  int lo, ns, n;              // the window's first token, sinks before it, keys in all
+  int ring, wrapped;          // wrapped: place in the ring of token max(lo, sinks)
+};
+template <int R>
+__device__ __forceinline__ bool rows_setup(const WindowStepArgs& a, int unit, int tiles, Rows& w) {
+  const int rt = unit % tiles, G = a.H / a.KV;
+  w.kvh = unit / tiles % a.KV;
+  w.b = unit / tiles / a.KV;
+  w.row0 = rt * R;
+  w.nt = rows_of(a, w.b, w.pos);
+  w.t0 = w.row0 / G;
+  if (w.t0 >= w.nt) return false;
+  w.t1 = min(w.nt - 1, (w.row0 + R - 1) / G);
+  w.lo = max(0, w.pos + w.t0 - a.left);
+  w.ns = min(a.sinks, w.lo);
+  w.n = w.ns + w.pos + w.t1 - w.lo + 1;
+  w.ring = a.C - a.sinks;
+  w.wrapped = (max(w.lo, a.sinks) - a.sinks) % w.ring;
+  return true;
+}
+
+// Query (t, h) of stream b by one wave, without the keys that it does not see.
 template <class T>
-__global__ __launch_bounds__(64) void window_step_any_kernel(WindowStepArgs a) {
-  const int lane = threadIdx.x, h = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-  int pos;
-  if (t >= rows_of(a, b, pos)) return;
-  const int group = a.H / a.KV, kvw = a.KV * a.hd, i = pos + t;
+__device__ __forceinline__ void step_query(const WindowStepArgs& a, int b, int h, int t, int pos) {
+  const int lane = threadIdx.x & 63, group = a.H / a.KV, kvw = a.KV * a.hd, i = pos + t;
   const int64_t col = (int64_t)(h / group) * a.hd;
   const T* kn = static_cast<const T*>(a.k) + (int64_t)b * a.T * kvw + col;
   const T* vn = static_cast<const T*>(a.v) + (int64_t)b * a.T * kvw + col;
-  T* kc = static_cast<T*>(a.kc) + (int64_t)b * a.C * kvw + col;
-  T* vc = static_cast<T*>(a.vc) + (int64_t)b * a.C * kvw + col;
+  const T* kc = static_cast<const T*>(a.kc) + (int64_t)b * a.C * kvw + col;
+  const T* vc = static_cast<const T*>(a.vc) + (int64_t)b * a.C * kvw + col;
   const int lo = max(0, i - a.left), ns = min(a.sinks, lo);
   auto row = [&](int64_t n, const T* cache, const T* fresh) {
     const int p = (int)(n < ns ? n : lo + (n - ns));
@@ -49,23 +74,348 @@ __global__ __launch_bounds__(64) void window_step_any_kernel(WindowStepArgs a) {
   T* o = static_cast<T*>(a.o) + at;
   if (lane < a.hd) o[lane] = from_f32<T>(o0);
   if (lane + 64 < a.hd) o[lane + 64] = from_f32<T>(o1);
-  if (h % group == 0) {
-    const int64_t to = (int64_t)slot_of(a, i) * kvw, from = (int64_t)t * kvw;
-    for (int d = lane; d < a.hd; d += 64) {
-      kc[to + d] = kn[from + d];
-      vc[to + d] = vn[from + d];
+}
+
+// A lane's eight dimensions of a row.
+template <class T>
+struct Eight {
+  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+  uintx4 x[sizeof(T) / 2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = uintx4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = reinterpret_cast<const uintx4*>(p)[i];
+  }
+  __device__ __forceinline__ float operator[](int e) const {
+    unsigned u;
+    if constexpr (sizeof(T) == 4)
+      u = x[e / 4][e % 4];
+    else
+      u = e & 1 ? x[0][e / 2] & 0xffff0000u : x[0][e / 2] << 16;
+    return __builtin_bit_cast(float, u);
+  }
+};
+// bf16: pairs of products an instruction, exact and added in fp32
+__device__ __forceinline__ float dot8(const Eight<__bf16>& x, const Eight<__bf16>& y) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned u = x.x[0][i], v = y.x[0][i];
+    s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, u), __builtin_bit_cast(bf16x2, v), s,
+                                        false);
+  }
+  return s;
+}
+__device__ __forceinline__ float dot8(const Eight<float>& x, const Eight<float>& y) {
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+  return s;
+}
+
+// v + that of the lane OFF away (xor), for OFF = 8, 16, 32 without LDS.
+template <int OFF>
+__device__ __forceinline__ float add_xor(float v) {
+  if constexpr (OFF == 32) {
+    return other_half(v, [](float x, float y) { return x + y; });
+  } else if constexpr (OFF == 16) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned x = r[0], y = r[1];
+    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
+  } else if constexpr (OFF == 8) {
+    return v + dpp_mov<0x128>(v);  // row_ror:8
+  } else {
+    return v + __shfl_xor(v, OFF, 64);
+  }
+}
+// Sum over aligned groups of L lanes, the same bits in each lane of a group.
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (L > 1) v += dpp_mov<0xB1>(v);
+  if constexpr (L > 2) v += dpp_mov<0x4E>(v);
+  if constexpr (L > 4) v += dpp_mov<0x141>(v);
+  if constexpr (L > 8) v += dpp_mov<0x140>(v);
+  return v;
+}
+// Sum over the lanes that hold the same dimensions: groups of L lanes, 64 / L of them.
+template <int L>
+__device__ __forceinline__ float across_groups(float v) {
+  if constexpr (L <= 1) v = add_xor<1>(v);
+  if constexpr (L <= 2) v = add_xor<2>(v);
+  if constexpr (L <= 4) v = add_xor<4>(v);
+  if constexpr (L <= 8) v = add_xor<8>(v);
+  v = add_xor<16>(v);
+  return add_xor<32>(v);
+}
+
+// W waves answer R rows. L lanes take a key, eight dimensions each (head dims that are no power of two leave
+// some idle), so a wave holds 64 / L keys at a time and U of those in flight; every group of L lanes keeps
+// running maxima, sums and outputs of its own, which are joined at the end, first in the wave, then in LDS,
+// then, if the keys are split over workgroups, by window_join_kernel. On the vector units: a key's row feeds
+// R dot products only, 4 bytes of cache an instruction at R = 1, and the matrix units would stand idle for the
+// loads just the same.
+template <class T, int L, int R, int W>
+__global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, int tiles, int nsplit,
+                                                             float* part) {
+  constexpr int KPW = 64 / L, U = sizeof(T) == 4 ? 2 : 4;
+  extern __shared__ float sh[];  // [W][R][hd + 2], [R]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % L, grp = lane / L;
+  const int sp = blockIdx.x % nsplit, unit = blockIdx.x / nsplit;
+  Rows w;
+  if (!rows_setup<R>(a, unit, tiles, w)) return;
+  const int G = a.H / a.KV, kvw = a.KV * a.hd, hd = a.hd;
+  const bool on = 8 * j < hd;
+  const int64_t col = (int64_t)w.kvh * hd + (on ? 8 * j : 0);
+  const T* kn = static_cast<const T*>(a.k) + (int64_t)w.b * a.T * kvw + col;
+  const T* vn = static_cast<const T*>(a.v) + (int64_t)w.b * a.T * kvw + col;
+  T* kc = static_cast<T*>(a.kc) + (int64_t)w.b * a.C * kvw + col;
+  T* vc = static_cast<T*>(a.vc) + (int64_t)w.b * a.C * kvw + col;
+
+  const float qs = a.scale * 1.4426950408889634f;
+  Eight<T> q[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = w.row0 + r, t = row / G, h = w.kvh * G + row % G;
+    q[r].clear();
+    if (on && t < w.nt)
+      q[r].load(static_cast<const T*>(a.q) + ((int64_t)w.b * a.T + t) * a.H * hd + (int64_t)h * hd + 8 * j);
+  }
+  float m[R], l[R], o[R][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
+  }
+  const int begin = (int)((int64_t)w.n * sp / nsplit), end = (int)((int64_t)w.n * (sp + 1) / nsplit);
+  const bool mixed = w.t0 != w.t1;  // rows of several tokens, which see different keys
+  for (int i = begin + wave * KPW * U; i < end; i += W * KPW * U) {
+    Eight<T> kx[U], vx[U];
+    int p[U];  // the lane's keys as positions
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int idx = i + u * KPW + grp;
+      p[u] = idx < w.ns ? idx : w.lo + idx - w.ns;
+      kx[u].clear();
+      vx[u].clear();
+      if (on && idx < end) {
+        int64_t at;
+        int slot = p[u];
+        if (slot >= a.sinks) {
+          slot = w.wrapped + (slot - max(w.lo, a.sinks));
+          slot = a.sinks + (slot >= w.ring ? slot - w.ring : slot);
+        }
+        const bool fresh = p[u] >= w.pos;
+        at = (int64_t)(fresh ? p[u] - w.pos : slot) * kvw;
+        kx[u].load((fresh ? kn : kc) + at);
+        vx[u].load((fresh ? vn : vc) + at);
+      }
+      if (idx >= end) p[u] = -1;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float s[U], top = m[r];
+      const int mine = w.pos + (w.row0 + r) / G;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = group_sum<L>(dot8(kx[u], q[r])) * qs;
+        const bool seen = p[u] >= 0 && (!mixed || (p[u] <= mine && (p[u] >= mine - a.left || p[u] < a.sinks)));
+        if (!seen) s[u] = -INFINITY;
+        top = max_nan(top, s[u]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float alpha = __builtin_amdgcn_exp2f(m[r] - ref);
+      m[r] = top;
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float pu = __builtin_amdgcn_exp2f(s[u] - ref);
+        l[r] += pu;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(pu, vx[u][e], o[r][e]);
+      }
     }
   }
+
+  // the new tokens' keys and values to their slots
+  if (w.row0 == 0 && sp == 0 && on) {
+    for (int t = threadIdx.x / L; t < w.nt; t += W * KPW) {
+      const int64_t to = (int64_t)slot_of(a, w.pos + t) * kvw, from = (int64_t)t * kvw;
+      Eight<T> x;
+      x.load(kn + from);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<typename Eight<T>::uintx4*>(kc + to)[i] = x.x[i];
+      x.load(vn + from);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<typename Eight<T>::uintx4*>(vc + to)[i] = x.x[i];
+    }
+  }
+
+  // the wave's groups, then the waves
+  const int ld = hd + 2;
+  float* again = sh + W * R * ld;  // rows to compute again
+  if (threadIdx.x < R) again[threadIdx.x] = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float top = m[r];
+#pragma unroll
+    for (int off = L; off < 64; off <<= 1) top = max_nan(top, __shfl_xor(top, off, 64));
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float by = __builtin_amdgcn_exp2f(m[r] - ref);
+    const float lr = across_groups<L>(l[r] * by);
+    float* to = sh + (wave * R + r) * ld;
+    if (lane == 0) {
+      to[hd] = top;
+      to[hd + 1] = lr;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = across_groups<L>(o[r][e] * by);
+      if (grp == 0 && on) to[8 * j + e] = x;
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * hd; e += W * 64) {
+    const int r = e / hd, d = e % hd, row = w.row0 + r, t = row / G;
+    if (t >= w.nt) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < W; ++v) top = max_nan(top, sh[(v * R + r) * ld + hd]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float lr = 0.f, x = 0.f;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const float* f = sh + (v * R + r) * ld;
+      const float by = __builtin_amdgcn_exp2f(f[hd] - ref);
+      lr = fmaf(f[hd + 1], by, lr);
+      x = fmaf(f[d], by, x);
+    }
+    if (nsplit > 1) {
+      float* f = part + ((int64_t)blockIdx.x * R + r) * ld;
+      f[d] = x;
+      if (d == 0) {
+        f[hd] = top;
+        f[hd + 1] = lr;
+      }
+    } else {
+      x /= lr;
+      static_cast<T*>(a.o)[((int64_t)w.b * a.T + t) * a.H * hd + (int64_t)(w.kvh * G + row % G) * hd + d] =
+          from_f32<T>(x);
+      // a key that this row does not see had weight 0 times a value that is not finite, perhaps
+      if (mixed && !(x * 0.f == 0.f)) again[r] = 1.f;
+    }
+  }
+  if (nsplit > 1 || !mixed) return;
+  __syncthreads();
+  for (int r = wave; r < R; r += W) {
+    const int row = w.row0 + r;
+    if (row / G < w.nt && again[r] == 1.f)
+      step_query<T>(a, w.b, w.kvh * G + row % G, row / G, w.pos);
+  }
+}
+
+// Joins the key ranges of split rows: a workgroup per unit, thread (row, dimension).
+template <class T, int R>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowStepArgs a, int tiles, int nsplit,
+                                                          const float* part) {
+  __shared__ int again[R];
+  Rows w;
+  if (!rows_setup<R>(a, blockIdx.x, tiles, w)) return;
+  const int G = a.H / a.KV, hd = a.hd, ld = hd + 2;
+  if (threadIdx.x < R) again[threadIdx.x] = 0;
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * hd; e += 256) {
+    const int r = e / hd, d = e % hd, row = w.row0 + r, t = row / G;
+    if (t >= w.nt) continue;
+    const float* f0 = part + ((int64_t)blockIdx.x * nsplit * R + r) * ld;
+    float top = -INFINITY;
+    for (int s = 0; s < nsplit; ++s) top = max_nan(top, f0[(int64_t)s * R * ld + hd]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float l = 0.f, x = 0.f;
+    for (int s = 0; s < nsplit; ++s) {
+      const float* f = f0 + (int64_t)s * R * ld;
+      const float by = __builtin_amdgcn_exp2f(f[hd] - ref);
+      l = fmaf(f[hd + 1], by, l);
+      x = fmaf(f[d], by, x);
+    }
+    x /= l;
+    static_cast<T*>(a.o)[((int64_t)w.b * a.T + t) * a.H * hd + (int64_t)(w.kvh * G + row % G) * hd + d] =
+        from_f32<T>(x);
+    if (!(x * 0.f == 0.f)) again[r] = 1;
+  }
+  if (w.t0 == w.t1) return;
+  __syncthreads();
+  for (int r = threadIdx.x >> 6; r < R; r += 4) {
+    const int row = w.row0 + r;
+    if (row / G < w.nt && again[r]) step_query<T>(a, w.b, w.kvh * G + row % G, row / G, w.pos);
+  }
+}
+
+// How a call is cut: rows a workgroup, its waves, and how many workgroups share a unit's keys.
+struct Plan {
+  int R, nsplit;
+  int64_t tiles;
+};
+constexpr int kWaves = 16;
+Plan plan_of(const WindowStepArgs& a, int cus) {
+  Plan p;
+  const int64_t rows = (int64_t)a.T * (a.H / a.KV);
+  p.R = rows >= 4 ? 4 : rows >= 2 ? 2 : 1;
+  p.tiles = (rows + p.R - 1) / p.R;
+  const int64_t units = (int64_t)a.B * a.KV * p.tiles;
+  const int64_t keys = std::min<int64_t>((int64_t)a.left + a.sinks + a.T, a.C);
+  // a split for every 512 keys while that leaves no more workgroups than compute units
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({keys / 512, cus / std::max<int64_t>(units, 1), 16}));
+  return p;
+}
+
+template <class T, int L, int R>
+void launch_step(const LaunchCtx& c, const WindowStepArgs& a, const Plan& p, float* part) {
+  const int64_t units = (int64_t)a.B * a.KV * p.tiles;
+  MNN_REQUIRE(units * p.nsplit < (1 << 22), MNN_ERR_INVALID_CONFIGURATION,
+              "WindowAttention: too many streams and tokens in one step");
+  const size_t lds = sizeof(float) * (kWaves * R * (a.hd + 2) + R);
+  launch(c, sizeof(T) == 4 ? "window_step_f32" : "window_step_bf16", window_step_kernel<T, L, R, kWaves>,
+         dim3((unsigned)(units * p.nsplit)), dim3(64 * kWaves), lds, a, (int)p.tiles, p.nsplit, part);
+  if (p.nsplit > 1)
+    launch(c, sizeof(T) == 4 ? "window_join_f32" : "window_join_bf16", window_join_kernel<T, R>,
+           dim3((unsigned)units), dim3(256), 0, a, (int)p.tiles, p.nsplit, (const float*)part);
+}
+template <class T, int L>
+void launch_step_r(const LaunchCtx& c, const WindowStepArgs& a, const Plan& p, float* part) {
+  if (p.R == 4) return launch_step<T, L, 4>(c, a, p, part);
+  if (p.R == 2) return launch_step<T, L, 2>(c, a, p, part);
+  launch_step<T, L, 1>(c, a, p, part);
+}
+template <class T>
+void launch_step_t(const LaunchCtx& c, const WindowStepArgs& a, const Plan& p, float* part) {
+  if (a.hd > 64) return launch_step_r<T, 16>(c, a, p, part);
+  if (a.hd > 32) return launch_step_r<T, 8>(c, a, p, part);
+  launch_step_r<T, 4>(c, a, p, part);
 }
 
 }  // namespace
 
-void window_step(const LaunchCtx& c, const WindowStepArgs& a) {
-  const dim3 grid(a.H, a.T, a.B);
+int64_t window_step_part_floats(const LaunchCtx& c, const WindowStepArgs& a) {
+  const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
+  return p.nsplit == 1 ? 0 : (int64_t)a.B * a.KV * p.tiles * p.nsplit * p.R * (a.hd + 2);
+}
+
+void window_step(const LaunchCtx& c, const WindowStepArgs& a, float* part) {
+  const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
+  MNN_REQUIRE(p.nsplit == 1 || part, MNN_ERR_INVALID_ARGUMENT, "window step: split keys need a workspace");
   if (a.type == MNN_F32)
-    launch(c, "window_step_any_f32", window_step_any_kernel<float>, grid, dim3(64), 0, a);
+    launch_step_t<float>(c, a, p, part);
   else
-    launch(c, "window_step_any_bf16", window_step_any_kernel<__bf16>, grid, dim3(64), 0, a);
+    launch_step_t<__bf16>(c, a, p, part);
 }
 
 }  // namespace k

@@ -457,7 +457,8 @@ class WindowAttentionLayer : public ManyInputLayer {
     a.left = d_.window_left;
     a.sinks = d_.sinks;
     a.scale = d_.scale;
-    k::window_step(ctx(s), a);
+    const int64_t part = k::window_step_part_floats(ctx(s), a);
+    k::window_step(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
   }
 
  private:
@@ -486,6 +487,7 @@ class WindowAttentionLayer : public ManyInputLayer {
                 "WindowAttention: output is an input");
   }
   mnn_window_attention_desc d_;
+  Scratch scratch_;
 };
 
 }  // namespace

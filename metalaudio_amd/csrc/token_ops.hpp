@@ -84,7 +84,9 @@ struct WindowStepArgs {
   int left = 0, sinks = 0;
   float scale = 1.f;
 };
-void window_step(const LaunchCtx& c, const WindowStepArgs& a);
+// floats of workspace that a call needs (0: none), the same on every call of the same sizes
+int64_t window_step_part_floats(const LaunchCtx& c, const WindowStepArgs& a);
+void window_step(const LaunchCtx& c, const WindowStepArgs& a, float* part);
 
 }  // namespace k
 }  // namespace mnn
