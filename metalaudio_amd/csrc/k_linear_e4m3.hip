@@ -7,8 +7,10 @@
 // times that (2^-9), is made with them. fp32 output is not: e4m3 values are bf16 values, so both operands
 // are widened (v_cvt_scalef32_pk_bf16_fp8, two values an instruction) and multiplied by the bf16
 // instructions (2.2 PFLOP/s), 9e-9 off on the same sums.
+#include "lds_dma.hpp"
 #include "token_ops.hpp"
 #include "token_utils.hpp"
+#include "x3.hpp"
 
 namespace mnn {
 namespace k {
@@ -18,6 +20,7 @@ using namespace dev;
 namespace {
 
 typedef int intx8 __attribute__((ext_vector_type(8)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
 
 // Eight e4m3 values to bf16, exactly.
 __device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
@@ -29,55 +32,257 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Lane (g, r) holds 32 bytes of row r of both operands: which k they are does not matter as long as both
-// sides agree. The result of (a rows, b rows): b row l % 16, a rows 4 (l / 16) + v.
+// 64 products a row: lane (g, r) holds 32 bytes of row r of both operands (which k they are does not matter
+// as long as both sides agree). The result: b's row l % 32, a's rows 8 (v / 4) + 4 (l / 32) + v % 4.
 template <class T>
-__device__ __forceinline__ floatx4 mfma_e4m3(intx8 a, intx8 b, floatx4 c) {
-  if constexpr (sizeof(T) == 2) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(a[i], a[i + 1]), widen8(b[i], b[i + 1]), c, 0, 0,
-                                                  0);
-    return c;
+struct Operand;  // 32 bytes of a row as the products of T's output take them
+template <>
+struct Operand<__bf16> {
+  intx8 x;
+  __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
+    x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
+};
+template <>
+struct Operand<float> {
+  bf16x8 x[4];
+  __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
+    x[0] = widen8(lo[0], lo[1]);
+    x[1] = widen8(lo[2], lo[3]);
+    x[2] = widen8(hi[0], hi[1]);
+    x[3] = widen8(hi[2], hi[3]);
+  }
+};
+__device__ __forceinline__ floatx16 mul(const Operand<__bf16>& a, const Operand<__bf16>& b, floatx16 c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.x, b.x, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mul(const Operand<float>& a, const Operand<float>& b, floatx16 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.x[i], b.x[i], c, 0, 0, 0);
+  return c;
 }
 
-__device__ __forceinline__ intx8 load32(const uint8_t* p) {
-  intx8 v;
-  reinterpret_cast<int4*>(&v)[0] = reinterpret_cast<const int4*>(p)[0];
-  reinterpret_cast<int4*>(&v)[1] = reinterpret_cast<const int4*>(p)[1];
-  return v;
-}
-
-// Four results of one row m, columns n .. n + 3.
-template <class T>
-__device__ __forceinline__ void store4(const LinearE4m3Args& a, int64_t m, int n, floatx4 acc) {
-  if (m >= a.M) return;
+// y[m][n .. n + CNT) from sums, CNT consecutive columns; `vec`: all of them are there and rows keep 16-byte
+// alignment.
+template <class T, int CNT>
+__device__ __forceinline__ void finish(const LinearE4m3Args& a, int64_t m, int n, const float* acc,
+                                       const float* ws, const float* bias, bool vec) {
   const float xs = a.xs[m];
+  const int64_t at = m * a.N + n;
+  T* y = static_cast<T*>(a.y) + at;
+  const T* r = a.r ? static_cast<const T*>(a.r) + at : nullptr;
+  float v[CNT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= a.N) return;
-    float v = acc[i] * xs * a.ws[n + i] + (a.bias ? a.bias[n + i] : 0.f);
-    v = apply_act(v, a.act, a.alpha);
-    const int64_t at = m * a.N + n + i;
-    if (a.r) v += to_f32(static_cast<const T*>(a.r)[at]);
-    static_cast<T*>(a.y)[at] = from_f32<T>(v);
+  for (int i = 0; i < CNT; ++i) v[i] = apply_act(fmaf(acc[i] * xs, ws[i], bias[i]), a.act, a.alpha);
+  if constexpr (CNT % 8 == 0) {
+    if (vec) {
+      typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+      constexpr int V = CNT * (int)sizeof(T) / 16;
+      if (r) {
+        uintx4 u[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[i] = reinterpret_cast<const uintx4*>(r)[i];
+#pragma unroll
+        for (int i = 0; i < CNT; ++i) {
+          unsigned w;
+          if constexpr (sizeof(T) == 4)
+            w = u[i / 4][i % 4];
+          else
+            w = i & 1 ? u[i / 8][i % 8 / 2] & 0xffff0000u : u[i / 8][i % 8 / 2] << 16;
+          v[i] += __builtin_bit_cast(float, w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        uintx4 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4)
+            u[e] = __builtin_bit_cast(unsigned, v[4 * i + e]);
+          else
+            u[e] = cvt_pk_bf16(v[8 * i + 2 * e], v[8 * i + 2 * e + 1]);
+        }
+        reinterpret_cast<uintx4*>(y)[i] = u;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < CNT; ++i)
+    if (n + i < a.N) y[i] = from_f32<T>(v[i] + (r ? to_f32(r[i]) : 0.f));
+}
+
+// Scales and biases of CNT consecutive columns (those behind the last column: 0).
+template <int CNT>
+__device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* ws, float* bias) {
+#pragma unroll
+  for (int i = 0; i < CNT; ++i) {
+    const int c = min(n + i, a.N - 1);
+    ws[i] = a.ws[c];
+    bias[i] = a.bias ? a.bias[c] : 0.f;
   }
 }
 
-// A wave per 16 x 16 results, operands straight from memory.
+// BM x BN results a workgroup, WM x WN a wave, the depth 128 at a time through a ring of S slots in LDS,
+// which global_load_lds fills: the rows of x, then those of w, 128 bytes each, 16-byte chunk c of row r in
+// place c ^ (r % 8), so that fragment reads of 32 rows spread over the banks. One barrier a step: behind it,
+// the step's slot is whole and the one before it free to be filled again.
+//
+// Rows behind the last are read as the last one; their results are not stored. The results go through LDS
+// once more (the ring is done with), so that scales, residual and output are read and written row by row.
+template <class T, int BM, int BN, int WM, int WN, int S>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
+  constexpr int NW = BM / WM * (BN / WN);
+  constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;
+  static_assert(SLOT % (1024 * NW) == 0, "whole loads a wave");
+  constexpr int FM = WM / 32, FN = WN / 32;
+  constexpr int OP = WN + 4;  // floats a row of the results in LDS
+  constexpr int BYTES = S * SLOT > NW * 32 * OP * 4 ? S * SLOT : NW * 32 * OP * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / (BN / WN), wn = wave % (BN / WN);
+  // tiles of neighbouring rows of w beside each other on one XCD
+  const int nt = (a.N + BN - 1) / BN;
+  const int tile = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
+  const int64_t m0 = (int64_t)(tile / nt) * BM;
+  const int n0 = tile % nt * BN;
+
+  // load i of this wave: rows 8 j .. + 7 of the slot, j = i NW + wave; the first BM rows are x's
+  const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
+  const char* src[LOADS];  // wave-uniform bases
+  unsigned off[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int row = 8 * (i * NW + wave);
+    const bool isx = row < BM;
+    const int64_t first = isx ? m0 + row : n0 + row - BM, last = isx ? a.M - 1 : a.N - 1;
+    const int64_t base = min(first, last);
+    src[i] = reinterpret_cast<const char*>((isx ? a.x : a.w) + base * a.K);
+    off[i] = (unsigned)min((int64_t)row_in, last - base) * (unsigned)a.K + 16u * chunk;
+  }
+  const unsigned lds0 = lds_address(smem);
+  auto issue = [&](int k, int slot) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      lds_dma16_s(reinterpret_cast<const float*>(src[i]), off[i] + 128u * k,
+                  __builtin_amdgcn_readfirstlane(lds0 + slot * SLOT + 1024u * (i * NW + wave)));
+  };
+
+  floatx16 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+
+  const int nk = a.K / 128;
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < nk) issue(s, s);
+  // chunk c of a row that is l32 modulo 32
+  auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 & 7)) << 4); };
+  const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
+  int slot = 0;
+  for (int k = 0; k < nk; ++k) {
+    wait_lgkmcnt0();
+    if (S > 2 && k + S - 2 < nk)
+      wait_vmcnt<(S - 2) * LOADS>();
+    else
+      wait_vmcnt<0>();
+    stage_barrier();
+    if (k + S - 1 < nk) issue(k + S - 1, slot == 0 ? S - 1 : slot - 1);
+    const char* p = smem + slot * SLOT;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int c0 = at(4 * s + 2 * g), c1 = at(4 * s + 2 * g + 1);
+      Operand<T> x[FM], w[FN];
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+        x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
+                 *reinterpret_cast<const intx4*>(p + xa + 4096 * j + c1));
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+        w[i].set(*reinterpret_cast<const intx4*>(p + wa + 4096 * i + c0),
+                 *reinterpret_cast<const intx4*>(p + wa + 4096 * i + c1));
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = mul(w[i], x[j], acc[i][j]);
+    }
+    slot = slot + 1 == S ? 0 : slot + 1;
+  }
+
+  // 32 rows of results at a time, through a part of LDS that is this wave's
+  __syncthreads();
+  float* out = reinterpret_cast<float*>(smem) + wave * 32 * OP;
+  constexpr int PER_ROW = WN / 8;  // lanes
+  const int cn = 8 * (lane % PER_ROW), n = n0 + wn * WN + cn;
+  float ws[8], bias[8];
+  columns<8>(a, n, ws, bias);
+  const bool vec = a.N % 8 == 0 && n < a.N;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<float4*>(out + l32 * OP + 32 * i + 8 * q + 4 * g) =
+            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+    wait_lgkmcnt0();
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 32 * PER_ROW / 64; ++r) {
+      const int row = r * (64 / PER_ROW) + lane / PER_ROW;
+      const int64_t m = m0 + wm * WM + 32 * j + row;
+      float v[8];
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(out + row * OP + cn);
+      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(out + row * OP + cn + 4);
+      if (m < a.M && n < a.N) finish<T, 8>(a, m, n, v, ws, bias, vec);
+    }
+    wait_lgkmcnt0();
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Few rows (up to 32): the weights are all the traffic. A workgroup takes 32 rows of w, its eight waves an
+// eighth of the depth each, operands straight from memory (a wave reads 64 bytes of 32 rows at a time, four
+// such steps in flight); their sums meet in LDS.
 template <class T>
-__global__ __launch_bounds__(256) void linear_e4m3_any_kernel(LinearE4m3Args a) {
-  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-  const int64_t nt = (a.N + 15) / 16, m0 = (blockIdx.x / nt * 4 + (threadIdx.x >> 6)) * 16;
-  const int n0 = (int)(blockIdx.x % nt) * 16;
-  const uint8_t* x = a.x + min(m0 + r, a.M - 1) * a.K + 32 * g;
-  const uint8_t* w = a.w + (int64_t)min(n0 + r, a.N - 1) * a.K + 32 * g;
-  floatx4 acc{0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < a.K; k += 128) acc = mfma_e4m3<T>(load32(w + k), load32(x + k), acc);
-  store4<T>(a, m0 + r, n0 + 4 * g, acc);
+__global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) {
+  __shared__ float sum[8][32][33];  // [wave][m][n]
+  const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = threadIdx.x >> 6;
+  const int n0 = blockIdx.x * 32;
+  const uint8_t* x = a.x + min((int64_t)l32, a.M - 1) * a.K + 32 * g;
+  const uint8_t* w = a.w + (int64_t)min(n0 + l32, a.N - 1) * a.K + 32 * g;
+  const int steps = a.K / 64, s0 = steps * wave / 8, s1 = steps * (wave + 1) / 8;
+  floatx16 acc;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+  auto load = [](const uint8_t* p, Operand<T>& o) {
+    const intx4* q = reinterpret_cast<const intx4*>(p);
+    o.set(q[0], q[1]);
+  };
+#pragma unroll 4
+  for (int s = s0; s < s1; ++s) {
+    Operand<T> xo, wo;
+    load(x + 64 * s, xo);
+    load(w + 64 * s, wo);
+    acc = mul(wo, xo, acc);
+  }
+#pragma unroll
+  for (int v = 0; v < 16; ++v) sum[wave][l32][8 * (v / 4) + 4 * g + v % 4] = acc[v];
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * a.M; e += 512) {
+    const int m = e / 32, n = n0 + e % 32;
+    if (n >= a.N) continue;
+    float v = 0.f, ws, bias;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sum[i][m][e % 32];
+    columns<1>(a, n, &ws, &bias);
+    finish<T, 1>(a, m, n, &v, &ws, &bias, false);
+  }
 }
 
 __global__ __launch_bounds__(256) void pad_rows_u8_kernel(const uint8_t* x, int64_t rows, int n,
@@ -97,14 +302,37 @@ void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint
   launch(c, "pad_rows_u8", pad_rows_u8_kernel, grid, dim3(256), 0, x, rows, n, y, ld);
 }
 
+namespace {
+template <class T, int BM, int BN, int WM, int WN, int S>
+void launch_tile(const LaunchCtx& c, const LinearE4m3Args& a, const char* name) {
+  const int64_t tiles = (a.M + BM - 1) / BM * ((a.N + BN - 1) / BN);
+  MNN_REQUIRE(tiles < (1 << 22), MNN_ERR_INVALID_CONFIGURATION, "Linear: too many rows in one call");
+  constexpr int threads = BM / WM * (BN / WN) * 64;
+  launch(c, name, linear_e4m3_kernel<T, BM, BN, WM, WN, S>, dim3((unsigned)tiles), dim3(threads), 0, a);
+}
+
+template <class T>
+void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
+  constexpr bool F32 = sizeof(T) == 4;
+  if (a.M <= 32)
+    return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
+                  dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
+  const int cus = c.dev->props.multiProcessorCount;
+  auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
+  if (tiles(256, 256) >= cus)
+    return launch_tile<T, 256, 256, 128, 64, 2>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
+  if (tiles(128, 128) >= cus / 2)
+    return launch_tile<T, 128, 128, 64, 64, 2>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
+  launch_tile<T, 64, 64, 32, 32, 4>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
+}
+}  // namespace
+
 void linear_e4m3(const LaunchCtx& c, const LinearE4m3Args& a) {
-  const int64_t wgs = (a.M + 63) / 64 * ((a.N + 15) / 16);
-  MNN_REQUIRE(wgs < (1 << 23), MNN_ERR_INVALID_CONFIGURATION, "Linear: too many rows in one call");
+  if (a.M <= 0) return;
   if (a.out == MNN_F32)
-    launch(c, "linear_e4m3_any_f32", linear_e4m3_any_kernel<float>, dim3((unsigned)wgs), dim3(256), 0, a);
+    linear_e4m3_t<float>(c, a);
   else
-    launch(c, "linear_e4m3_any_bf16", linear_e4m3_any_kernel<__bf16>, dim3((unsigned)wgs), dim3(256), 0,
-           a);
+    linear_e4m3_t<__bf16>(c, a);
 }
 
 }  // namespace k

@@ -231,7 +231,8 @@ def linear_case(dev, stream, M, K, N, act="none", residual=False, inp="e4m3", ou
     (129, 1536, 384, {"residual": True}), (257, 512, 513, {"act": "tanh"}), (700, 384, 1152, {}),
     (1344, 384, 1536, {"act": "gelu", "out": "bf16"}), (2688, 1536, 384, {"residual": True}),
     (200, 2048, 2048, {"act": "leaky_relu", "residual": True}), (130, 640, 130, {"act": "sigmoid"}),
-    (1000, 256, 260, {"bias": False, "residual": True, "out": "bf16"}), (511, 896, 1026, {"out": "bf16"})])
+    (1000, 256, 260, {"bias": False, "residual": True, "out": "bf16"}), (511, 896, 1026, {"out": "bf16"}),
+    (4099, 256, 4104, {"residual": True, "out": "bf16"}), (4097, 384, 4100, {"act": "relu"})])
 def test_linear_e4m3(dev, stream, M, K, N, kw):
     say(f"linear e4m3 {M}x{K}x{N} {kw}")
     linear_case(dev, stream, M, K, N, **kw)
