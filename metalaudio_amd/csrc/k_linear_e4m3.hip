@@ -12,6 +12,8 @@
 #include "token_utils.hpp"
 #include "x3.hpp"
 
+#include <type_traits>
+
 namespace mnn {
 namespace k {
 
@@ -62,55 +64,71 @@ __device__ __forceinline__ floatx16 mul(const Operand<float>& a, const Operand<f
   return c;
 }
 
-// y[m][n .. n + CNT) from sums, CNT consecutive columns; `vec`: all of them are there and rows keep 16-byte
-// alignment.
-template <class T, int CNT>
-__device__ __forceinline__ void finish(const LinearE4m3Args& a, int64_t m, int n, const float* acc,
-                                       const float* ws, const float* bias, bool vec) {
-  const float xs = a.xs[m];
-  const int64_t at = m * a.N + n;
-  T* y = static_cast<T*>(a.y) + at;
-  const T* r = a.r ? static_cast<const T*>(a.r) + at : nullptr;
-  float v[CNT];
+// The activation of CNT values; its choice is made once for all of them (a branch an element, the same for
+// every lane or not, took 32 us of a round of 256 x 256 results).
+template <int CNT>
+__device__ __forceinline__ void activate(float (&v)[CNT], int act, float alpha) {
+  auto all = [&](auto code) {
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) v[i] = apply_act(fmaf(acc[i] * xs, ws[i], bias[i]), a.act, a.alpha);
-  if constexpr (CNT % 8 == 0) {
+    for (int i = 0; i < CNT; ++i) v[i] = apply_act(v[i], decltype(code)::value, alpha);
+  };
+  switch (act) {
+    case 1: return all(std::integral_constant<int, 1>{});
+    case 2: return all(std::integral_constant<int, 2>{});
+    case 3: return all(std::integral_constant<int, 3>{});
+    case 4: return all(std::integral_constant<int, 4>{});
+    case 5: return all(std::integral_constant<int, 5>{});
+    case 6: return all(std::integral_constant<int, 6>{});
+    default: return;
+  }
+}
+
+// Eight consecutive values of a row as they lie in memory: 16-byte aligned, or `cnt` of them one by one.
+template <class T>
+struct Row8 {
+  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+  static constexpr int V = (int)sizeof(T) / 2;
+  uintx4 u[V];
+  __device__ __forceinline__ void load(const T* p, bool vec, int cnt) {
     if (vec) {
-      typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-      constexpr int V = CNT * (int)sizeof(T) / 16;
-      if (r) {
-        uintx4 u[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) u[i] = reinterpret_cast<const uintx4*>(r)[i];
+      for (int i = 0; i < V; ++i) u[i] = reinterpret_cast<const uintx4*>(p)[i];
+    } else {
+      T t[8];
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) {
-          unsigned w;
-          if constexpr (sizeof(T) == 4)
-            w = u[i / 4][i % 4];
-          else
-            w = i & 1 ? u[i / 8][i % 8 / 2] & 0xffff0000u : u[i / 8][i % 8 / 2] << 16;
-          v[i] += __builtin_bit_cast(float, w);
-        }
-      }
+      for (int i = 0; i < 8; ++i) t[i] = i < cnt ? p[i] : (T)0.f;
+      __builtin_memcpy(u, t, sizeof(u));
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    unsigned w;
+    if constexpr (sizeof(T) == 4)
+      w = u[i / 4][i % 4];
+    else
+      w = i & 1 ? u[0][i / 2] & 0xffff0000u : u[0][i / 2] << 16;
+    return __builtin_bit_cast(float, w);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8], bool vec, int cnt) {
+    if (vec) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        uintx4 u;
+        uintx4 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (sizeof(T) == 4)
-            u[e] = __builtin_bit_cast(unsigned, v[4 * i + e]);
+            w[e] = __builtin_bit_cast(unsigned, v[4 * i + e]);
           else
-            u[e] = cvt_pk_bf16(v[8 * i + 2 * e], v[8 * i + 2 * e + 1]);
+            w[e] = cvt_pk_bf16(v[2 * e], v[2 * e + 1]);
         }
-        reinterpret_cast<uintx4*>(y)[i] = u;
+        reinterpret_cast<uintx4*>(p)[i] = w;
       }
-      return;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < cnt) p[i] = from_f32<T>(v[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < CNT; ++i)
-    if (n + i < a.N) y[i] = from_f32<T>(v[i] + (r ? to_f32(r[i]) : 0.f));
-}
+};
 
 // Scales and biases of CNT consecutive columns (those behind the last column: 0).
 template <int CNT>
@@ -139,14 +157,20 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   constexpr int OP = WN + 4;  // floats a row of the results in LDS
   constexpr int BYTES = S * SLOT > NW * 32 * OP * 4 ? S * SLOT : NW * 32 * OP * 4;
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+  __shared__ float xs[BM];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / (BN / WN), wn = wave % (BN / WN);
   // tiles of neighbouring rows of w beside each other on one XCD
   const int nt = (a.N + BN - 1) / BN;
   const int tile = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
-  const int64_t m0 = (int64_t)(tile / nt) * BM;
-  const int n0 = tile % nt * BN;
+  // tiles run down GM rows of tiles, then to the next column of them: the workgroups of an XCD at one
+  // time share a block of x and of w in its L2
+  constexpr int GM = 8;
+  const int mt = (int)((a.M + BM - 1) / BM), grp = tile / (GM * nt), in = tile - grp * GM * nt;
+  const int gm = min(GM, mt - grp * GM);
+  const int64_t m0 = (int64_t)(grp * GM + in % gm) * BM;
+  const int n0 = in / gm * BN;
 
   // load i of this wave: rows 8 j .. + 7 of the slot, j = i NW + wave; the first BM rows are x's
   const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
@@ -181,6 +205,12 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
     if (s < nk) issue(s, s);
+  // what the results need besides: this lane's columns and the tile's row scales
+  constexpr int PER_ROW = WN / 8;  // lanes
+  const int cn = 8 * (lane % PER_ROW), n = n0 + wn * WN + cn;
+  float ws[8], bias[8];
+  columns<8>(a, n, ws, bias);
+  for (int i = threadIdx.x; i < BM; i += NW * 64) xs[i] = a.xs[min(m0 + i, a.M - 1)];
   // chunk c of a row that is l32 modulo 32
   auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
@@ -214,16 +244,23 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     slot = slot + 1 == S ? 0 : slot + 1;
   }
 
-  // 32 rows of results at a time, through a part of LDS that is this wave's
+  // 32 rows of results at a time, through a part of LDS that is this wave's; the residual's rows are on
+  // their way meanwhile (all of them are read before a row is written: they may be the output's)
   __syncthreads();
   float* out = reinterpret_cast<float*>(smem) + wave * 32 * OP;
-  constexpr int PER_ROW = WN / 8;  // lanes
-  const int cn = 8 * (lane % PER_ROW), n = n0 + wn * WN + cn;
-  float ws[8], bias[8];
-  columns<8>(a, n, ws, bias);
-  const bool vec = a.N % 8 == 0 && n < a.N;
+  const bool vec = a.N % 8 == 0;
+  const int cnt = a.N - n;  // columns that are there (<= 0: none)
+  constexpr int PASSES = 32 * PER_ROW / 64, ROWS = 64 / PER_ROW;
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
+    const int64_t mj = m0 + wm * WM + 32 * j + lane / PER_ROW;
+    Row8<T> res[PASSES];
+    if (a.r) {
+#pragma unroll
+      for (int r = 0; r < PASSES; ++r)
+        if (mj + r * ROWS < a.M && cnt > 0)
+          res[r].load(static_cast<const T*>(a.r) + (mj + r * ROWS) * a.N + n, vec, cnt);
+    }
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -233,13 +270,21 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int r = 0; r < 32 * PER_ROW / 64; ++r) {
-      const int row = r * (64 / PER_ROW) + lane / PER_ROW;
-      const int64_t m = m0 + wm * WM + 32 * j + row;
+    for (int r = 0; r < PASSES; ++r) {
+      const int row = r * ROWS + lane / PER_ROW;
+      const float by = xs[wm * WM + 32 * j + row];
       float v[8];
       *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(out + row * OP + cn);
       *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(out + row * OP + cn + 4);
-      if (m < a.M && n < a.N) finish<T, 8>(a, m, n, v, ws, bias, vec);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * by, ws[e], bias[e]);
+      activate(v, a.act, a.alpha);
+      if (a.r) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += res[r][e];
+      }
+      if (mj + r * ROWS < a.M && cnt > 0)
+        Row8<T>::store(static_cast<T*>(a.y) + (mj + r * ROWS) * a.N + n, v, vec, cnt);
     }
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();
@@ -277,11 +322,15 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
   for (int e = threadIdx.x; e < 32 * a.M; e += 512) {
     const int m = e / 32, n = n0 + e % 32;
     if (n >= a.N) continue;
-    float v = 0.f, ws, bias;
+    float v[1] = {0.f}, ws, bias;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += sum[i][m][e % 32];
+    for (int i = 0; i < 8; ++i) v[0] += sum[i][m][e % 32];
     columns<1>(a, n, &ws, &bias);
-    finish<T, 1>(a, m, n, &v, &ws, &bias, false);
+    v[0] = fmaf(v[0] * a.xs[m], ws, bias);
+    activate(v, a.act, a.alpha);
+    const int64_t at = (int64_t)m * a.N + n;
+    if (a.r) v[0] += to_f32(static_cast<const T*>(a.r)[at]);
+    static_cast<T*>(a.y)[at] = from_f32<T>(v[0]);
   }
 }
 
@@ -317,13 +366,16 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   if (a.M <= 32)
     return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
                   dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
+  // The largest tile that still gives most compute units one: us at (M, K, N), 256 / 128 / 64 square:
+  // 8192 x 4096 x 4096 bf16 132 / 147 / 208, 10752 x 384 x 1536 bf16 18.6 / 21.7 / 23.7, 10752 x 1536 x 384
+  // f32 42 / 22.0 / 21.6, 2688 x 384 x 1152 bf16 14.5 / 8.7 / 6.9, 200 x 1536 x 384 f32 37 / 16.6 / 8.0.
   const int cus = c.dev->props.multiProcessorCount;
-  auto tiles = [&](int bm, int bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
-  if (tiles(256, 256) >= cus)
+  auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
+  if (4 * tiles(256) >= 3 * cus)
     return launch_tile<T, 256, 256, 128, 64, 2>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
-  if (tiles(128, 128) >= cus / 2)
+  if (tiles(128) >= cus)
     return launch_tile<T, 128, 128, 64, 64, 2>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
-  launch_tile<T, 64, 64, 32, 32, 4>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
+  launch_tile<T, 64, 64, 32, 32, 2>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
 }
 }  // namespace
 
