@@ -83,52 +83,26 @@ __device__ __forceinline__ void activate(float (&v)[CNT], int act, float alpha) 
   }
 }
 
-// Eight consecutive values of a row as they lie in memory: 16-byte aligned, or `cnt` of them one by one.
+// Eight values of a row, or the first `cnt` of them one by one where the row is not aligned.
 template <class T>
-struct Row8 {
-  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-  static constexpr int V = (int)sizeof(T) / 2;
-  uintx4 u[V];
-  __device__ __forceinline__ void load(const T* p, bool vec, int cnt) {
-    if (vec) {
+__device__ __forceinline__ void load_some(Eight<T>& x, const T* p, bool vec, int cnt) {
+  if (vec) return x.load(p);
+  T t[8];
 #pragma unroll
-      for (int i = 0; i < V; ++i) u[i] = reinterpret_cast<const uintx4*>(p)[i];
-    } else {
-      T t[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = i < cnt ? p[i] : (T)0.f;
-      __builtin_memcpy(u, t, sizeof(u));
-    }
+  for (int i = 0; i < 8; ++i) t[i] = i < cnt ? p[i] : (T)0.f;
+  __builtin_memcpy(x.x, t, sizeof(x.x));
+}
+template <class T>
+__device__ __forceinline__ void store_some(T* p, const float* v, bool vec, int cnt) {
+  if (vec) {
+    Eight<T> x;
+    x.set(v);
+    return x.store(p);
   }
-  __device__ __forceinline__ float operator[](int i) const {
-    unsigned w;
-    if constexpr (sizeof(T) == 4)
-      w = u[i / 4][i % 4];
-    else
-      w = i & 1 ? u[0][i / 2] & 0xffff0000u : u[0][i / 2] << 16;
-    return __builtin_bit_cast(float, w);
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8], bool vec, int cnt) {
-    if (vec) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        uintx4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(T) == 4)
-            w[e] = __builtin_bit_cast(unsigned, v[4 * i + e]);
-          else
-            w[e] = cvt_pk_bf16(v[2 * e], v[2 * e + 1]);
-        }
-        reinterpret_cast<uintx4*>(p)[i] = w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < cnt) p[i] = from_f32<T>(v[i]);
-    }
-  }
-};
+  for (int i = 0; i < 8; ++i)
+    if (i < cnt) p[i] = from_f32<T>(v[i]);
+}
 
 // Scales and biases of CNT consecutive columns (those behind the last column: 0).
 template <int CNT>
@@ -254,12 +228,12 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int64_t mj = m0 + wm * WM + 32 * j + lane / PER_ROW;
-    Row8<T> res[PASSES];
+    Eight<T> res[PASSES];
     if (a.r) {
 #pragma unroll
       for (int r = 0; r < PASSES; ++r)
         if (mj + r * ROWS < a.M && cnt > 0)
-          res[r].load(static_cast<const T*>(a.r) + (mj + r * ROWS) * a.N + n, vec, cnt);
+          load_some(res[r], static_cast<const T*>(a.r) + (mj + r * ROWS) * a.N + n, vec, cnt);
     }
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -284,7 +258,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
         for (int e = 0; e < 8; ++e) v[e] += res[r][e];
       }
       if (mj + r * ROWS < a.M && cnt > 0)
-        Row8<T>::store(static_cast<T*>(a.y) + (mj + r * ROWS) * a.N + n, v, vec, cnt);
+        store_some(static_cast<T*>(a.y) + (mj + r * ROWS) * a.N + n, v, vec, cnt);
     }
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();

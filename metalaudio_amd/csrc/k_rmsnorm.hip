@@ -5,6 +5,9 @@
 #include "token_ops.hpp"
 #include "token_utils.hpp"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace mnn {
 namespace k {
 
@@ -65,15 +68,128 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
   }
 }
 
+// Rows of up to 4096 values, a multiple of 8: a wave a row, which stays in its registers from the first read
+// to the last write, lane l holding values 512 i + 8 l .. + 7; the weights too, over all of a wave's rows.
+// Bound by memory (two loads and two stores a value).
+template <class T, int NV, mnn_dtype OUT>
+__global__ __launch_bounds__(256) void rmsnorm_wave_kernel(RmsNormArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t step = (int64_t)gridDim.x * 4;
+  float w[NV][8];
+  bool on[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    on[i] = 512 * i + 8 * lane < a.F;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[i][e] = a.w && on[i] ? a.w[512 * i + 8 * lane + e] : 1.f;
+  }
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows; row += step) {
+    const int64_t at = row * a.F + 8 * lane;
+    Eight<T> x[NV], r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i].clear();
+      r[i].clear();
+      if (on[i]) {
+        x[i].load(static_cast<const T*>(a.x) + at + 512 * i);
+        if (a.r) r[i].load(static_cast<const T*>(a.r) + at + 512 * i);
+      }
+    }
+    float h[NV][8], ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[i][e] = a.r ? x[i][e] + r[i][e] : x[i][e];
+        ss = fmaf(h[i][e], h[i][e], ss);
+      }
+    if (a.sum) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (on[i]) {
+          Eight<T> o;
+          o.set(h[i]);
+          o.store(static_cast<T*>(a.sum) + at + 512 * i);
+        }
+    }
+    float top = 0.f;
+    if (a.w) {
+      const float norm = rsqrtf(group_reduce<64>(ss, Plus{}) / (float)a.F + a.eps);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * norm * w[i][e];
+    }
+    if constexpr (OUT == MNN_E4M3) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (on[i]) top = max_nan(top, fabsf(h[i][e]));
+      const RowScale rs = row_scale(group_reduce<64>(top, max_nan));
+      if (lane == 0) a.scales[row] = rs.scale;
+      uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy + 8 * lane;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float* v = h[i];
+        if (on[i])
+          *reinterpret_cast<uint2*>(y + 512 * i) =
+              make_uint2(pack_e4m3(v[0] * rs.inv, v[1] * rs.inv, v[2] * rs.inv, v[3] * rs.inv),
+                         pack_e4m3(v[4] * rs.inv, v[5] * rs.inv, v[6] * rs.inv, v[7] * rs.inv));
+        else if (512 * i + 8 * lane < a.ldy)
+          *reinterpret_cast<uint2*>(y + 512 * i) = make_uint2(0, 0);
+      }
+    } else {
+      using O = std::conditional_t<OUT == MNN_F32, float, __bf16>;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (on[i]) {
+          Eight<O> o;
+          o.set(h[i]);
+          o.store(static_cast<O*>(a.y) + row * a.ldy + 512 * i + 8 * lane);
+        }
+    }
+  }
+}
+
+template <class T, int NV>
+void launch_wave(const LaunchCtx& c, const RmsNormArgs& a) {
+  const char* name = sizeof(T) == 4 ? "rmsnorm_wave_f32" : "rmsnorm_wave_bf16";
+  // eight workgroups a compute unit keep their weights over several rows
+  const dim3 grid((unsigned)std::min<int64_t>((a.rows + 3) / 4, 8 * c.dev->props.multiProcessorCount));
+  if (a.out == MNN_E4M3)
+    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_E4M3>, grid, dim3(256), 0, a);
+  else if (a.out == MNN_BF16)
+    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_BF16>, grid, dim3(256), 0, a);
+  else
+    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_F32>, grid, dim3(256), 0, a);
+}
+
+template <class T>
+void rmsnorm_t(const LaunchCtx& c, const RmsNormArgs& a) {
+  if (a.F % 8 == 0 && a.ldy % 8 == 0 && a.ldy <= 4096) {
+    switch ((a.ldy + 511) / 512) {
+      case 1: return launch_wave<T, 1>(c, a);
+      case 2: return launch_wave<T, 2>(c, a);
+      case 3: return launch_wave<T, 3>(c, a);
+      case 4: return launch_wave<T, 4>(c, a);
+      case 5:
+      case 6: return launch_wave<T, 6>(c, a);
+      default: return launch_wave<T, 8>(c, a);
+    }
+  }
+  launch(c, sizeof(T) == 4 ? "rmsnorm_any_f32" : "rmsnorm_any_bf16", rmsnorm_any_kernel<T>,
+         dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)), dim3(256), 0, a);
+}
+
 }  // namespace
 
 void rmsnorm(const LaunchCtx& c, const RmsNormArgs& a) {
   if (a.rows <= 0 || a.F <= 0) return;
-  const dim3 grid((unsigned)std::min<int64_t>(a.rows, 1 << 20));
   if (a.in == MNN_F32)
-    launch(c, "rmsnorm_any_f32", rmsnorm_any_kernel<float>, grid, dim3(256), 0, a);
+    rmsnorm_t<float>(c, a);
   else
-    launch(c, "rmsnorm_any_bf16", rmsnorm_any_kernel<__bf16>, grid, dim3(256), 0, a);
+    rmsnorm_t<__bf16>(c, a);
 }
 
 }  // namespace k

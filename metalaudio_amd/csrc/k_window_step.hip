@@ -76,28 +76,6 @@ __device__ __forceinline__ void step_query(const WindowStepArgs& a, int b, int h
   if (lane + 64 < a.hd) o[lane + 64] = from_f32<T>(o1);
 }
 
-// A lane's eight dimensions of a row.
-template <class T>
-struct Eight {
-  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-  uintx4 x[sizeof(T) / 2];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = uintx4{0, 0, 0, 0};
-  }
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x[i] = reinterpret_cast<const uintx4*>(p)[i];
-  }
-  __device__ __forceinline__ float operator[](int e) const {
-    unsigned u;
-    if constexpr (sizeof(T) == 4)
-      u = x[e / 4][e % 4];
-    else
-      u = e & 1 ? x[0][e / 2] & 0xffff0000u : x[0][e / 2] << 16;
-    return __builtin_bit_cast(float, u);
-  }
-};
 // bf16: pairs of products an instruction, exact and added in fp32
 __device__ __forceinline__ float dot8(const Eight<__bf16>& x, const Eight<__bf16>& y) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -117,40 +95,12 @@ __device__ __forceinline__ float dot8(const Eight<float>& x, const Eight<float>&
   return s;
 }
 
-// v + that of the lane OFF away (xor), for OFF = 8, 16, 32 without LDS.
-template <int OFF>
-__device__ __forceinline__ float add_xor(float v) {
-  if constexpr (OFF == 32) {
-    return other_half(v, [](float x, float y) { return x + y; });
-  } else if constexpr (OFF == 16) {
-    const unsigned u = __builtin_bit_cast(unsigned, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const unsigned x = r[0], y = r[1];
-    return __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
-  } else if constexpr (OFF == 8) {
-    return v + dpp_mov<0x128>(v);  // row_ror:8
-  } else {
-    return v + __shfl_xor(v, OFF, 64);
-  }
-}
-// Sum over aligned groups of L lanes, the same bits in each lane of a group.
-template <int L>
-__device__ __forceinline__ float group_sum(float v) {
-  if constexpr (L > 1) v += dpp_mov<0xB1>(v);
-  if constexpr (L > 2) v += dpp_mov<0x4E>(v);
-  if constexpr (L > 4) v += dpp_mov<0x141>(v);
-  if constexpr (L > 8) v += dpp_mov<0x140>(v);
-  return v;
-}
-// Sum over the lanes that hold the same dimensions: groups of L lanes, 64 / L of them.
+// Sum over the lanes that hold the same dimensions: groups of L lanes (4, 8 or 16), 64 / L of them.
 template <int L>
 __device__ __forceinline__ float across_groups(float v) {
-  if constexpr (L <= 1) v = add_xor<1>(v);
-  if constexpr (L <= 2) v = add_xor<2>(v);
-  if constexpr (L <= 4) v = add_xor<4>(v);
-  if constexpr (L <= 8) v = add_xor<8>(v);
-  v = add_xor<16>(v);
-  return add_xor<32>(v);
+  if constexpr (L <= 4) v += __shfl_xor(v, 4, 64);
+  if constexpr (L <= 8) v += dpp_mov<0x128>(v);  // row_ror:8
+  return other_half(other_row(v, Plus{}), Plus{});
 }
 
 // W waves answer R rows. L lanes take a key, eight dimensions each (head dims that are no power of two leave
@@ -224,7 +174,7 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
       const int mine = w.pos + (w.row0 + r) / G;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        s[u] = group_sum<L>(dot8(kx[u], q[r])) * qs;
+        s[u] = group_reduce<L>(dot8(kx[u], q[r]), Plus{}) * qs;
         const bool seen = p[u] >= 0 && (!mixed || (p[u] <= mine && (p[u] >= mine - a.left || p[u] < a.sinks)));
         if (!seen) s[u] = -INFINITY;
         top = max_nan(top, s[u]);
@@ -251,11 +201,9 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
       const int64_t to = (int64_t)slot_of(a, w.pos + t) * kvw, from = (int64_t)t * kvw;
       Eight<T> x;
       x.load(kn + from);
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<typename Eight<T>::uintx4*>(kc + to)[i] = x.x[i];
+      x.store(kc + to);
       x.load(vn + from);
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<typename Eight<T>::uintx4*>(vc + to)[i] = x.x[i];
+      x.store(vc + to);
     }
   }
 
