@@ -239,7 +239,7 @@ mnn_status mnn_rmsnorm_forward_residual(mnn_layer layer, mnn_tensor input, mnn_t
 
 #define MNN_ROTARY_MAX_AXES 4
 typedef struct mnn_rotary_desc {
-  int head_dim;
+  int head_dim;                         /* <= 4096 */
   int num_axes;                         /* 1..4 */
   int axis_dims[MNN_ROTARY_MAX_AXES];   /* dimensions that axis a turns: even, > 0, sum <= head_dim */
   float base;                           /* of the angular rates, e.g. 10000 */

@@ -5,6 +5,8 @@
 #include "token_ops.hpp"
 #include "token_utils.hpp"
 
+#include <algorithm>
+
 namespace mnn {
 namespace k {
 
@@ -17,49 +19,135 @@ __device__ __forceinline__ void turn_of(int pos, double rate, float& cs, float& 
   sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
 }
 
-// A thread per token, tensor, head and dimension pair, or dimension behind the last axis.
-template <class T>
-__global__ __launch_bounds__(256) void rotary_any_kernel(RotaryArgs a) {
-  const int units = a.pairs + (a.hd - 2 * a.pairs);  // of one head
-  const int heads = a.heads[0] + a.heads[1];
-  const int64_t total = a.B * a.S * heads * units;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int u = (int)(i % units);
-    int h = (int)(i / units % heads);
-    const int64_t tok = i / units / heads;
-    const int which = h >= a.heads[0];
-    if (which) h -= a.heads[0];
-    const int64_t at = (tok * a.heads[which] + h) * a.hd;
-    const T* x = static_cast<const T*>(a.x[which]) + at;
-    T* y = static_cast<T*>(a.y[which]) + at;
-    if (u >= a.pairs) {
-      y[u + a.pairs] = x[u + a.pairs];
-      continue;
+// A workgroup takes `toks` tokens: first their sines and cosines, once for all heads of both tensors, into
+// LDS, then the rows. A thread's unit is VE pairs: VE values and their VE partners half an axis away, or 2 VE
+// values in a row where pairs are interleaved; 2 VE values (one, for VE = 1) behind the last axis pass. VE = 8
+// or 4 makes them 16-byte accesses of f32 and 16 or 8 of bf16, where every axis is a whole number of units.
+// Both partners are read before either is written, so the output may be the input. Bound by memory.
+template <class T, int VE, bool INTER>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int toks) {
+  extern __shared__ float2 turns[];  // [toks][pairs]
+  constexpr int RU = VE == 1 ? 1 : 2 * VE;
+  typedef T Part __attribute__((ext_vector_type(VE)));
+  const int turning = a.pairs / VE, units = turning + (a.hd - 2 * a.pairs) / RU;  // of one head
+  const int heads = a.heads[0] + a.heads[1], per_tok = units * heads;
+  const int64_t total = a.B * a.S;
+  for (int64_t tok0 = (int64_t)blockIdx.x * toks; tok0 < total; tok0 += (int64_t)gridDim.x * toks) {
+    const int n = (int)min((int64_t)toks, total - tok0);
+    for (int i = threadIdx.x; i < n * a.pairs; i += 256) {
+      const int u = i % a.pairs;
+      const int64_t tok = tok0 + i / a.pairs;
+      int axis = 0, j = u;
+      while (j >= a.dims[axis] / 2) j -= a.dims[axis++] / 2;  // ends: u is one of the axes' pairs
+      float2 t;
+      turn_of(a.pos[(a.shared ? tok % a.S : tok) * a.axes + axis], a.rate[u], t.x, t.y);
+      turns[i] = t;
     }
-    int axis = 0, first = 0, j = u;  // pair j of the axis, whose dimensions begin at `first`
-    while (j >= a.dims[axis] / 2) {
-      j -= a.dims[axis] / 2;
-      first += a.dims[axis++];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * per_tok; i += 256) {
+      const int ti = i / per_tok, rest = i - ti * per_tok;
+      int h = rest / units;
+      const int u = rest - h * units, which = h >= a.heads[0];
+      if (which) h -= a.heads[0];
+      const int64_t at = ((tok0 + ti) * (which ? a.heads[1] : a.heads[0]) + h) * a.hd;
+      const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + at;
+      T* y = static_cast<T*>(which ? a.y[1] : a.y[0]) + at;
+      if (u >= turning) {
+        const int d = 2 * a.pairs + (u - turning) * RU;
+        if constexpr (VE == 1) {
+          y[d] = x[d];
+        } else {
+          const Part p = *reinterpret_cast<const Part*>(x + d), q = *reinterpret_cast<const Part*>(x + d + VE);
+          *reinterpret_cast<Part*>(y + d) = p;
+          *reinterpret_cast<Part*>(y + d + VE) = q;
+        }
+        continue;
+      }
+      int j = u * VE, first = 0;  // pair j of the axis, whose dimensions begin at `first`
+      int half = a.dims[0] / 2;
+      if constexpr (!INTER) {
+#pragma unroll
+        for (int axis = 0; axis < 3; ++axis)
+          if (j >= half) {  // only while the axes before were passed too
+            j -= half;
+            first += 2 * half;
+            half = a.dims[axis + 1] / 2;
+          } else {
+            break;
+          }
+      }
+      const int d0 = INTER ? 2 * j : first + j, d1 = INTER ? d0 + VE : d0 + half;
+      const Part p = *reinterpret_cast<const Part*>(x + d0), q = *reinterpret_cast<const Part*>(x + d1);
+      float in[2 * VE], out[2 * VE];  // p then q
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        in[e] = to_f32((T)p[e]);
+        in[VE + e] = to_f32((T)q[e]);
+      }
+      const float2* t = turns + ti * a.pairs + u * VE;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float2 c = t[e];
+        if (INTER) {
+          out[2 * e] = in[2 * e] * c.x - in[2 * e + 1] * c.y;
+          out[2 * e + 1] = in[2 * e + 1] * c.x + in[2 * e] * c.y;
+        } else {
+          out[e] = in[e] * c.x - in[VE + e] * c.y;
+          out[VE + e] = in[VE + e] * c.x + in[e] * c.y;
+        }
+      }
+      Part po, qo;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        po[e] = from_f32<T>(out[e]);
+        qo[e] = from_f32<T>(out[VE + e]);
+      }
+      *reinterpret_cast<Part*>(y + d0) = po;
+      *reinterpret_cast<Part*>(y + d1) = qo;
     }
-    const int p0 = first + (a.interleaved ? 2 * j : j);
-    const int p1 = a.interleaved ? p0 + 1 : p0 + a.dims[axis] / 2;
-    float cs, sn;
-    turn_of(a.pos[(a.shared ? tok % a.S : tok) * a.axes + axis], a.rate[u], cs, sn);
-    const float v0 = to_f32(x[p0]), v1 = to_f32(x[p1]);
-    y[p0] = from_f32<T>(v0 * cs - v1 * sn);
-    y[p1] = from_f32<T>(v1 * cs + v0 * sn);
+    __syncthreads();
   }
+}
+
+// Whether units of VE pairs fill every axis, and what is behind them.
+bool whole_units(const RotaryArgs& a, int VE) {
+  bool ok = a.hd % VE == 0 && (a.hd - 2 * a.pairs) % (2 * VE) == 0 && a.pairs % VE == 0;
+  for (int i = 0; i < a.axes && !a.interleaved; ++i) ok = ok && a.dims[i] / 2 % VE == 0;
+  return ok;
+}
+
+template <class T, int VE>
+void launch_rotary(const LaunchCtx& c, const RotaryArgs& a) {
+  const int heads = a.heads[0] + a.heads[1];
+  const int64_t units = (int64_t)heads * (a.pairs / VE + (a.hd - 2 * a.pairs) / (VE == 1 ? 1 : 2 * VE));
+  // tokens a workgroup: four units a thread, as few as the compute units still have work for, and as the
+  // table of turns has room for (16 KB)
+  const int64_t tokens = a.B * a.S, cus = c.dev->props.multiProcessorCount;
+  int64_t toks = std::max<int64_t>(1, 1024 / units);
+  toks = std::min({toks, std::max<int64_t>(1, tokens / (2 * cus)), std::max<int64_t>(1, 2048 / a.pairs)});
+  const dim3 grid((unsigned)std::min<int64_t>((tokens + toks - 1) / toks, 1 << 20));
+  const char* name = sizeof(T) == 4 ? "rotary_f32" : "rotary_bf16";
+  const size_t lds = sizeof(float2) * toks * a.pairs;
+  if (a.interleaved)
+    launch(c, name, rotary_kernel<T, VE, true>, grid, dim3(256), lds, a, (int)toks);
+  else
+    launch(c, name, rotary_kernel<T, VE, false>, grid, dim3(256), lds, a, (int)toks);
+}
+template <class T>
+void rotary_t(const LaunchCtx& c, const RotaryArgs& a) {
+  if constexpr (sizeof(T) == 2)
+    if (whole_units(a, 8)) return launch_rotary<T, 8>(c, a);
+  if (whole_units(a, 4)) return launch_rotary<T, 4>(c, a);
+  launch_rotary<T, 1>(c, a);
 }
 
 }  // namespace
 
 void rotary(const LaunchCtx& c, const RotaryArgs& a) {
-  const int64_t total = a.B * a.S * (a.heads[0] + a.heads[1]) * (a.hd - a.pairs);
-  const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 1 << 20));
   if (a.type == MNN_F32)
-    launch(c, "rotary_any_f32", rotary_any_kernel<float>, grid, dim3(256), 0, a);
+    rotary_t<float>(c, a);
   else
-    launch(c, "rotary_any_bf16", rotary_any_kernel<__bf16>, grid, dim3(256), 0, a);
+    rotary_t<__bf16>(c, a);
 }
 
 }  // namespace k

@@ -265,7 +265,7 @@ class LinearE4m3Layer : public Layer {
 class RotaryLayer : public ManyInputLayer {
  public:
   RotaryLayer(Device* d, const mnn_rotary_desc& desc) : ManyInputLayer(d), d_(desc) {
-    MNN_REQUIRE(desc.head_dim > 0 && desc.head_dim <= (1 << 16), MNN_ERR_INVALID_CONFIGURATION,
+    MNN_REQUIRE(desc.head_dim > 0 && desc.head_dim <= 4096, MNN_ERR_INVALID_CONFIGURATION,
                 "Rotary: head dim " << desc.head_dim);
     MNN_REQUIRE(desc.num_axes >= 1 && desc.num_axes <= MNN_ROTARY_MAX_AXES,
                 MNN_ERR_INVALID_CONFIGURATION, "Rotary: " << desc.num_axes << " axes");
@@ -307,7 +307,7 @@ class RotaryLayer : public ManyInputLayer {
       split_heads("Rotary", in[i]->shape, d_.head_dim, B, S, n);
       MNN_REQUIRE(i == 0 || (B == a.B && S == a.S), MNN_ERR_SHAPE_MISMATCH,
                   "Rotary: k is " << shape_str(kt->shape) << " beside q " << shape_str(q.shape));
-      MNN_REQUIRE(n <= (1 << 16), MNN_ERR_INVALID_CONFIGURATION, "Rotary: " << n << " heads");
+      MNN_REQUIRE(n <= 65535, MNN_ERR_INVALID_CONFIGURATION, "Rotary: " << n << " heads");
       MNN_REQUIRE(out[i]->dtype == in[i]->dtype, MNN_ERR_INVALID_ARGUMENT,
                   "Rotary: an output has its input's type");
       MNN_REQUIRE(out[i]->count() == in[i]->count(), MNN_ERR_BUFFER_SIZE_MISMATCH,
