@@ -5,6 +5,7 @@
 #include "window_row.hpp"
 #include "x3.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mnn {
@@ -33,8 +34,10 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
   if (lane + 64 < a.hd) o[lane + 64] = from_f32<T>(o1);
 }
 
-// A workgroup is 4 waves of 32 queries of one head over blocks of keys that all four read from LDS. Each
-// wave computes the TRANSPOSED scores S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q):
+// A workgroup takes the keys that BQ queries of one head see, in blocks that lie in LDS, by NW waves: NW / KW
+// groups of 32 queries by KW groups of keys, which take every KW-th block and whose results are joined at the
+// end (KW > 1 for grids that would leave most of the GPU idle: then each of a few waves a
+// compute unit waits for its next block for longer than it computes). Each wave computes the TRANSPOSED scores S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q):
 // keys 8 (v / 4) + 4 g + v % 4 of query q) is the B operand that O^T += V^T P^T needs when its k slots take
 // those keys, so P goes from the softmax straight into the second product. K and V lie in LDS row by row as
 // they come; V^T's fragments (4 keys of one dimension a lane) are transposed on the way out by
@@ -50,7 +53,7 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // A key that a query does not see has probability 0, but 0 times a value that is not finite is NaN, and
 // parts of tiny or overflowing f32 values are off: queries whose result is not finite (or, in f32, below
 // 2^-109) are computed again by window_query.
-template <class T, int KS>
+template <class T, int KS, int KW>
 struct WindowCfg {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int PARTS = F32 ? 3 : 1;
@@ -61,34 +64,41 @@ struct WindowCfg {
   static constexpr int PITCH = KS * 32 + (KS % 2 ? 0 : 16);
   static constexpr int PLANE = BKV * PITCH;
   static constexpr int CHUNKS = BKV * KS * 2;  // of 8 values, in a block of K or V
-  static constexpr int PER = (CHUNKS + 255) / 256;
+  static constexpr int NW = KW == 1 ? 4 : 8, THREADS = 64 * NW, BQ = 32 * NW / KW;
+  static constexpr int PER = (KW * CHUNKS + THREADS - 1) / THREADS;
+  // K planes, then V planes, of KW blocks; V's fragments of the last 32 dimensions may reach 32 bytes past
+  // its rows. At the end, the other key groups' results: maximum, sum and O^T of each lane
+  static constexpr int SLOT = 2 * PARTS * PLANE;
+  static constexpr int JOIN = (KW - 1) * (NW / KW) * (16 * DT + 2) * 256;
+  static constexpr int LDS = KW * SLOT + 64 > JOIN ? KW * SLOT + 64 : JOIN;
   // workgroups a CU, as the registers allow without spilling
-  static constexpr int OCC = F32 ? (KS > 6 ? 1 : KS > 4 ? 2 : 3) : (KS > 6 ? 2 : KS > 4 ? 3 : 4);
+  static constexpr int OCC = KW > 1 ? 1
+                             : F32  ? (KS > 6 ? 1 : KS > 4 ? 2 : 3)
+                                    : (KS > 6 ? 2 : KS > 4 ? 3 : 4);
 };
 
-template <class T, int KS>
-__global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(WindowArgs a) {
-  using Cfg = WindowCfg<T, KS>;
+template <class T, int KS, int KW>
+__global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, KW>::OCC)) void window_kernel(WindowArgs a) {
+  using Cfg = WindowCfg<T, KS, KW>;
   constexpr int PARTS = Cfg::PARTS, BKV = Cfg::BKV, NT = Cfg::NT, DT = Cfg::DT, PITCH = Cfg::PITCH;
-  constexpr int PLANE = Cfg::PLANE, PER = Cfg::PER;
+  constexpr int PLANE = Cfg::PLANE, PER = Cfg::PER, SLOT = Cfg::SLOT, BQ = Cfg::BQ;
+  constexpr int THREADS = Cfg::THREADS;
   constexpr bool F32 = Cfg::F32;
-  // K planes, then V planes; V's fragments of the last 32 dimensions may reach 32 bytes past its rows
-  __shared__ __attribute__((aligned(16))) char smem[2 * PARTS * PLANE + 64];
+  __shared__ __attribute__((aligned(16))) char smem[Cfg::LDS];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qg = wave / KW, kg = wave % KW;
   // consecutive units, the heads that share K and V first, run on one XCD and share its L2
-  const int nq = (a.S + 127) / 128, G = a.H / a.KV;
-  const int64_t units = (int64_t)nq * a.H * a.B;
-  int64_t unit = xcd_logical_tile((int)blockIdx.x, (int)units);
-  const int gi = (int)(unit % G);
+  const int nq = (a.S + BQ - 1) / BQ, G = a.H / a.KV;
+  int unit = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
+  const int gi = unit % G;
   unit /= G;
-  const int q0 = (int)(unit % nq) * 128;
+  const int q0 = unit % nq * BQ;
   unit /= nq;
-  const int kvh = (int)(unit % a.KV), b = (int)(unit / a.KV), h = kvh * G + gi;
+  const int kvh = unit % a.KV, b = unit / a.KV, h = kvh * G + gi;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
   if (q0 >= len) return;
-  const int qw = q0 + 32 * wave;              // this wave's first query
+  const int qw = q0 + 32 * qg;                // this wave's first query
   const int qn = min(qw + 31, len - 1);       // and last
   const int qi = qw + l32;                    // the lane's
   const int kvw = a.KV * a.hd, qrow = a.H * a.hd;
@@ -96,28 +106,35 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.S * kvw + kvh * a.hd;
 
   // blocks: those of the sinks before the window's first, then the window's
-  const int last = min(q0 + 127, len - 1);
+  const int last = min(q0 + BQ - 1, len - 1);
   const int first_blk = max(0, q0 - a.left) / BKV;
   const int last_blk = (int)min((int64_t)len - 1, (int64_t)last + a.right) / BKV;
   const int sink_blks = (int)min((int64_t)first_blk, ((int64_t)a.sinks + BKV - 1) / BKV);
   const int n = sink_blks + last_blk - first_blk + 1;
   auto block_of = [&](int t) { return t < sink_blks ? t : first_blk + t - sink_blks; };
 
-  // one block of K and V on its way: 8 values a chunk
+  // KW blocks of K and V on their way: 8 values a chunk
   typedef float floatx8 __attribute__((ext_vector_type(8)));
   typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
   using Chunk = std::conditional_t<F32, floatx8, uintx4>;
   Chunk ck[PER], cv[PER];
-  auto fetch = [&](int blk) {
+  auto each = [&](auto f) {  // f(i, block of the KW, row, chunk) for each chunk of the thread's
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int e = tid + 256 * i, row = e / (2 * KS), c = e % (2 * KS);
-      if (e < Cfg::CHUNKS && 8 * c < a.hd) {
-        const int64_t at = (int64_t)min(blk * BKV + row, len - 1) * kvw + 8 * c;
-        ck[i] = *reinterpret_cast<const Chunk*>(kb + at);
-        cv[i] = *reinterpret_cast<const Chunk*>(vb + at);
-      }
+      const int e = tid + THREADS * i, j = KW == 1 ? 0 : e / Cfg::CHUNKS;
+      const int row = (KW == 1 ? e : e % Cfg::CHUNKS) / (2 * KS), c = e % (2 * KS);
+      if (e < KW * Cfg::CHUNKS && 8 * c < a.hd) f(i, j, row, c);
     }
+  };
+  // blocks past the last and rows past the last key: the last ones again (the former are not computed, the
+  // latter's scores masked)
+  auto fetch = [&](int t) {
+    each([&](int i, int j, int row, int c) {
+      const int blk = block_of(KW == 1 ? t : min(t * KW + j, n - 1));
+      const int64_t at = (int64_t)min(blk * BKV + row, len - 1) * kvw + 8 * c;
+      ck[i] = *reinterpret_cast<const Chunk*>(kb + at);
+      cv[i] = *reinterpret_cast<const Chunk*>(vb + at);
+    });
   };
   auto parts_of = [&](Chunk x, float by) {
     float y[8];
@@ -136,21 +153,18 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
     }
   };
   auto store = [&] {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = tid + 256 * i, row = e / (2 * KS), c = e % (2 * KS);
-      if (e < Cfg::CHUNKS && 8 * c < a.hd) {
-        put(ck[i], smem + row * PITCH + 16 * c);
-        put(cv[i], smem + PARTS * PLANE + row * PITCH + 16 * c);
-      }
-    }
+    each([&](int i, int j, int row, int c) {
+      char* at = smem + j * SLOT + row * PITCH + 16 * c;
+      put(ck[i], at);
+      put(cv[i], at + PARTS * PLANE);
+    });
   };
   if (a.hd < 16 * KS) {  // columns behind the head's last stay zero
-    for (int e = tid; e < 2 * PARTS * BKV; e += 256)
+    for (int e = tid; e < KW * 2 * PARTS * BKV; e += THREADS)
       for (int c = a.hd / 8; c < 2 * KS; ++c)
         *reinterpret_cast<float4*>(smem + e * PITCH + 16 * c) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  fetch(block_of(0));
+  fetch(0);
 
   // Q: B operand, query l32, dimensions 16 s + 8 g .. + 7. f32: times the scale in powers of two; bf16: as
   // it is, up to the scale's sign, the scale in the exponent instead.
@@ -182,8 +196,8 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
   float ref = 0.f, lsum = 0.f;  // ref: in the scores' units
   bool begun = false;           // whether the query has seen a key
 
-  const char* kf0 = smem + l32 * PITCH + 16 * g;
-  const char* vf0 = smem + PARTS * PLANE + (4 * g + ((lane & 15) >> 2)) * PITCH + 32 * ((lane >> 4) & 1) +
+  const char* kf0 = smem + kg * SLOT + l32 * PITCH + 16 * g;
+  const char* vf0 = smem + kg * SLOT + PARTS * PLANE + (4 * g + ((lane & 15) >> 2)) * PITCH + 32 * ((lane >> 4) & 1) +
                     8 * (lane & 3);
   auto vfrag = [&](int part, int t, int ks) {  // dimensions 32 t + l32, keys 16 ks + 4 g + {0..3, 8..11}
     typedef short short4v __attribute__((ext_vector_type(4)));
@@ -199,40 +213,41 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
   };
 
   store();
-  for (int t = 0; t < n; ++t) {
+  for (int t = 0; t * KW < n; ++t) {
     lds_barrier();
-    const int k0 = block_of(t) * BKV, k1 = k0 + BKV - 1;
-    if (t + 1 < n) fetch(block_of(t + 1));
+    const int k0 = block_of(t * KW + kg) * BKV, k1 = k0 + BKV - 1;
+    if ((t + 1) * KW < n) fetch(t + 1);
     // seen by any query of the wave?
-    const bool any = qw <= qn && k0 <= (int64_t)qn + a.right && (k1 >= qw - a.left || k0 < a.sinks);
+    const bool any = qw <= qn && t * KW + kg < n && k0 <= (int64_t)qn + a.right && (k1 >= qw - a.left || k0 < a.sinks);
     if (any) {
       floatx16 st[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v) st[j][v] = 0.f;
-        if constexpr (F32) {
-          floatx16 low;
+      if constexpr (F32) {
+        floatx16 low;  // the five smaller products, in an accumulator of their own (x3.hpp)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) low[v] = 0.f;
+        for (int v = 0; v < 16; ++v) low[v] = 0.f;
 #pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            Split8 kx, qx{qf[s][0], qf[s][1], qf[s][2]};
-            kx.h = *reinterpret_cast<const bf16x8*>(kf0 + 32 * s);
-            kx.m = *reinterpret_cast<const bf16x8*>(kf0 + PLANE + 32 * s);
-            kx.l = *reinterpret_cast<const bf16x8*>(kf0 + 2 * PLANE + 32 * s);
+        for (int s = 0; s < KS; ++s) {
+          Split8 kx, qx{qf[s][0], qf[s][1], qf[s][2]};
+          kx.h = *reinterpret_cast<const bf16x8*>(kf0 + 32 * s);
+          kx.m = *reinterpret_cast<const bf16x8*>(kf0 + PLANE + 32 * s);
+          kx.l = *reinterpret_cast<const bf16x8*>(kf0 + 2 * PLANE + 32 * s);
 #pragma unroll
-            for (int p = 0; p < 5; ++p) low = mfma_x3(kx, qx, low, p);
-            st[j] = mfma_x3(kx, qx, st[j], 5);
-          }
+          for (int p = 0; p < 5; ++p) low = mfma_x3(kx, qx, low, p);
+          st[0] = mfma_x3(kx, qx, st[0], 5);
+        }
 #pragma unroll
-          for (int v = 0; v < 16; ++v) st[j][v] += low[v];
-        } else {
+        for (int v = 0; v < 16; ++v) st[0][v] += low[v];
+      } else {
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
             st[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 *reinterpret_cast<const bf16x8*>(kf0 + 32 * j * PITCH + 32 * s), qf[s][0], st[j], 0, 0, 0);
-        }
       }
       const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= (int64_t)qw + a.right && k1 < len;
       if (!whole) {
@@ -299,7 +314,39 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
       lsum += ps;
     }
     lds_barrier();
-    if (t + 1 < n) store();
+    if ((t + 1) * KW < n) store();
+  }
+
+  if constexpr (KW > 1) {  // the other key groups' results to the first's waves
+    constexpr int PER_WAVE = (16 * DT + 2) * 64;
+    float* sh = reinterpret_cast<float*>(smem) + lane;
+    if (kg) {
+      float* to = sh + (qg * (KW - 1) + kg - 1) * PER_WAVE;
+      to[0] = begun ? ref : lsum == 0.f ? -INFINITY : 0.f;  // NaN scores leave ref at 0 and a sum of NaN
+      to[64] = lsum;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) to[64 * (2 + 16 * i + v)] = o[i][v];
+    }
+    __syncthreads();
+    if (kg) return;
+#pragma unroll 1
+    for (int j = 0; j < KW - 1; ++j) {
+      const float* from = sh + (qg * (KW - 1) + j) * PER_WAVE;
+      const float r = from[0];
+      if (r == -INFINITY) continue;  // it saw nothing of this query's
+      const float top = begun ? max_nan(ref, r) : r;
+      const float by0 = begun ? __builtin_amdgcn_exp2f((ref - top) * cs) : 0.f;
+      const float by1 = __builtin_amdgcn_exp2f((r - top) * cs);
+      lsum = lsum * by0 + from[64] * by1;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[i][v] = o[i][v] * by0 + from[64 * (2 + 16 * i + v)] * by1;
+      ref = top;
+      begun = true;
+    }
   }
 
   const float l = other_half(lsum, [](float x, float y) { return x + y; });
@@ -341,13 +388,32 @@ __global__ __launch_bounds__(256, (WindowCfg<T, KS>::OCC)) void window_kernel(Wi
   }
 }
 
-template <class T, int KS>
-void launch_window(const LaunchCtx& c, const WindowArgs& a) {
-  const int64_t units = (int64_t)((a.S + 127) / 128) * a.H * a.B;
+template <class T, int KS, int KW>
+void launch_window_kw(const LaunchCtx& c, const WindowArgs& a) {
+  using Cfg = WindowCfg<T, KS, KW>;
+  const int64_t units = (int64_t)cdiv(a.S, Cfg::BQ) * a.H * a.B;
   MNN_REQUIRE(units < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
               "WindowAttention: too many tokens in one call");
-  launch(c, sizeof(T) == 4 ? "window_f32" : "window_bf16", window_kernel<T, KS>, dim3((unsigned)units),
-         dim3(256), 0, a);
+  launch(c, sizeof(T) == 4 ? "window_f32" : "window_bf16", window_kernel<T, KS, KW>, dim3((unsigned)units),
+         dim3(Cfg::THREADS), 0, a);
+}
+
+template <class T, int KS>
+void launch_window(const LaunchCtx& c, const WindowArgs& a) {
+  // Key groups by how much of the GPU 128 queries a workgroup would fill. us for KW = 1 / 2 / 4, 8 heads:
+  // f32 hd 48 1344 tokens, 168 both ways (88 workgroups): 33 / 27 / 18; 2 x 1344, 511 both ways (176): 62 / 50 /
+  // 48; 4096, 2047 back (256): 111 / 88 / 98; 4 x 1344 (352): 45 / 49 / 50. bf16 hd 64 the same: 17 / 14 / 10,
+  // 26 / 21 / 25, 42 / 33 / 41, 21 / 20 / 27; 16384, 1023 back (1024): 58 / 61 / 116. f32 hd 128 has registers
+  // for one wave a SIMD with KW = 1: 16384, 1023 back 534 / 430.
+  const int64_t wgs = (int64_t)cdiv(a.S, 128) * a.H * a.B, cus = c.dev->props.multiProcessorCount;
+  const int64_t keys = std::min<int64_t>(a.S, (int64_t)128 + a.left + a.right + a.sinks);
+  constexpr bool F32 = sizeof(T) == 4, FOUR = KS <= 5 || !F32;  // four blocks fit in LDS
+  if (keys > 2 * WindowCfg<T, KS, 1>::BKV) {
+    if constexpr (FOUR)
+      if (2 * wgs < cus) return launch_window_kw<T, KS, 4>(c, a);
+    if (4 * wgs < 5 * cus || (F32 && KS > 6)) return launch_window_kw<T, KS, 2>(c, a);
+  }
+  launch_window_kw<T, KS, 1>(c, a);
 }
 
 template <class T>

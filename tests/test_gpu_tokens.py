@@ -442,6 +442,8 @@ def window_case(dev, stream, B, S, H, KV, hd, left, right, sinks, dtype, lengths
     (1, 64, 2, 1, 64, 63, 0, 0), (1, 65, 1, 1, 128, 1000, 1000, 70), (2, 130, 4, 2, 32, 16, 16, 4),
     (1, 257, 2, 2, 72, 100, 0, 33), (1, 300, 1, 1, 96, 0, 299, 3), (1, 200, 2, 1, 16, 7, 3, 0),
     (1, 400, 2, 2, 48, 168, 168, 4), (1, 513, 1, 1, 64, 64, 0, 65), (1, 700, 2, 1, 64, 300, 1, 129),
+    (5, 1030, 8, 8, 48, 70, 0, 3), (6, 901, 8, 2, 64, 200, 5, 70), (3, 1025, 16, 16, 128, 64, 64, 2),
+    (2, 1000, 8, 2, 64, 130, 0, 4), (2, 999, 8, 8, 80, 90, 33, 1), (1, 2500, 2, 2, 48, 1000, 0, 5),
     (1, 385, 1, 1, 128, 127, 0, 4), (3, 97, 5, 5, 24, 31, 31, 1), (1, 290, 1, 1, 104, 2 ** 30, 0, 2 ** 30)])
 def test_window_attention(dev, stream, B, S, H, KV, hd, left, right, sinks, dtype):
     say(f"window {B}x{S} heads {H}/{KV} hd {hd} left {left} right {right} sinks {sinks} {dtype}")
