@@ -112,14 +112,26 @@ __device__ __forceinline__ float across_groups(float v) {
 template <class T, int L, int R, int W>
 __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, int tiles, int nsplit,
                                                              float* part) {
-  constexpr int KPW = 64 / L, U = sizeof(T) == 4 ? 2 : 4;
+  constexpr int KPW = 64 / L, U = sizeof(T) == 4 ? 2 : R > 2 ? 4 : 8;
   extern __shared__ float sh[];  // [W][R][hd + 2], [R]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % L, grp = lane / L;
   const int sp = blockIdx.x % nsplit, unit = blockIdx.x / nsplit;
-  Rows w;
-  if (!rows_setup<R>(a, unit, tiles, w)) return;
   const int G = a.H / a.KV, kvw = a.KV * a.hd, hd = a.hd;
   const bool on = 8 * j < hd;
+  // the queries, before the stream's position has come: rows that are no tokens are not used
+  Eight<T> q[R];
+  {
+    const int row0 = unit % tiles * R, kvh = unit / tiles % a.KV, b = unit / tiles / a.KV;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int t = (row0 + r) / G, h = kvh * G + (row0 + r) % G;
+      q[r].clear();
+      if (on && t < a.T)
+        q[r].load(static_cast<const T*>(a.q) + ((int64_t)b * a.T + t) * a.H * hd + (int64_t)h * hd + 8 * j);
+    }
+  }
+  Rows w;
+  if (!rows_setup<R>(a, unit, tiles, w)) return;
   const int64_t col = (int64_t)w.kvh * hd + (on ? 8 * j : 0);
   const T* kn = static_cast<const T*>(a.k) + (int64_t)w.b * a.T * kvw + col;
   const T* vn = static_cast<const T*>(a.v) + (int64_t)w.b * a.T * kvw + col;
@@ -127,14 +139,6 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
   T* vc = static_cast<T*>(a.vc) + (int64_t)w.b * a.C * kvw + col;
 
   const float qs = a.scale * 1.4426950408889634f;
-  Eight<T> q[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = w.row0 + r, t = row / G, h = w.kvh * G + row % G;
-    q[r].clear();
-    if (on && t < w.nt)
-      q[r].load(static_cast<const T*>(a.q) + ((int64_t)w.b * a.T + t) * a.H * hd + (int64_t)h * hd + 8 * j);
-  }
   float m[R], l[R], o[R][8];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -270,38 +274,57 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
   }
 }
 
-// Joins the key ranges of split rows: a workgroup per unit, thread (row, dimension).
+// Joins the key ranges of split rows: a workgroup per unit, thread (row, dimension). The ranges' maxima and
+// sums come first, all at once, and become factors; the outputs are then read eight ranges at a time (one
+// after another, a range cost half a microsecond).
+constexpr int kMaxSplits = 32;
 template <class T, int R>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowStepArgs a, int tiles, int nsplit,
                                                           const float* part) {
+  __shared__ float by[R][kMaxSplits], inv[R];
   __shared__ int again[R];
+  const int G = a.H / a.KV, hd = a.hd, ld = hd + 2;
+  const float* unit0 = part + (int64_t)blockIdx.x * nsplit * R * ld;
   Rows w;
   if (!rows_setup<R>(a, blockIdx.x, tiles, w)) return;
-  const int G = a.H / a.KV, hd = a.hd, ld = hd + 2;
-  if (threadIdx.x < R) again[threadIdx.x] = 0;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (wave < R) {  // a wave a row, lane s the range s
+    const int r = wave;
+    float top = -INFINITY, l = 0.f;
+    if (lane < nsplit) {
+      top = unit0[((int64_t)lane * R + r) * ld + hd];
+      l = unit0[((int64_t)lane * R + r) * ld + hd + 1];
+    }
+    const float all = group_reduce<64>(top, max_nan), ref = all == -INFINITY ? 0.f : all;
+    const float f = __builtin_amdgcn_exp2f(top - ref);
+    const float sum = group_reduce<64>(l * f, Plus{});
+    if (lane < nsplit) by[r][lane] = f;
+    if (lane == 0) {
+      inv[r] = 1.f / sum;
+      again[r] = 0;
+    }
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < R * hd; e += 256) {
     const int r = e / hd, d = e % hd, row = w.row0 + r, t = row / G;
     if (t >= w.nt) continue;
-    const float* f0 = part + ((int64_t)blockIdx.x * nsplit * R + r) * ld;
-    float top = -INFINITY;
-    for (int s = 0; s < nsplit; ++s) top = max_nan(top, f0[(int64_t)s * R * ld + hd]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = 0.f, x = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-      const float* f = f0 + (int64_t)s * R * ld;
-      const float by = __builtin_amdgcn_exp2f(f[hd] - ref);
-      l = fmaf(f[hd + 1], by, l);
-      x = fmaf(f[d], by, x);
+    float x = 0.f;
+    for (int s0 = 0; s0 < nsplit; s0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = unit0[((int64_t)min(s0 + i, nsplit - 1) * R + r) * ld + d];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < nsplit) x = fmaf(v[i], by[r][s0 + i], x);
     }
-    x /= l;
+    x *= inv[r];
     static_cast<T*>(a.o)[((int64_t)w.b * a.T + t) * a.H * hd + (int64_t)(w.kvh * G + row % G) * hd + d] =
         from_f32<T>(x);
     if (!(x * 0.f == 0.f)) again[r] = 1;
   }
   if (w.t0 == w.t1) return;
   __syncthreads();
-  for (int r = threadIdx.x >> 6; r < R; r += 4) {
+  for (int r = wave; r < R; r += 4) {
     const int row = w.row0 + r;
     if (row / G < w.nt && again[r]) step_query<T>(a, w.b, w.kvh * G + row % G, row / G, w.pos);
   }
@@ -320,8 +343,13 @@ Plan plan_of(const WindowStepArgs& a, int cus) {
   p.tiles = (rows + p.R - 1) / p.R;
   const int64_t units = (int64_t)a.B * a.KV * p.tiles;
   const int64_t keys = std::min<int64_t>((int64_t)a.left + a.sinks + a.T, a.C);
-  // a split for every 512 keys while that leaves no more workgroups than compute units
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({keys / 512, cus / std::max<int64_t>(units, 1), 16}));
+  // A second launch costs about 2 us: keys are split only from 640 on, into ranges of 256, and while that
+  // leaves no more workgroups than compute units. us in one, ranges of 512 / 256 / 128: one stream, 4096 keys,
+  // 8 / 2 heads of 64, f32 - / 16.8 / 15.1 / 15.3; 8 heads of 128, bf16 - / 12.1 / 10.9 / 12.0; 8 streams, 1024
+  // keys, 8 heads of 64, f32 12.0 / 11.9 / 10.5 / 10.5; one stream, 516 keys, 8 heads of 48, f32 6.8 / - / 9.0 / 8.5.
+  p.nsplit = keys < 640 ? 1
+                        : (int)std::max<int64_t>(1, std::min<int64_t>({keys / 256, cus / std::max<int64_t>(units, 1),
+                                                                       kMaxSplits}));
   return p;
 }
 

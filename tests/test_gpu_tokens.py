@@ -1,6 +1,8 @@
 """The token operators through the C ABI against 64-bit references: RMS norm with residual and 8-bit
 output, the 8-bit linear layer, rotary positions, window attention and its step on rolling caches.
 Tolerances count roundings (token_refs.py) and were fixed before the first run."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -613,7 +615,8 @@ class Streams:
     (1, 1, 1, 8, 0, 0, 0, [1, 1, 1]), (1, 8, 8, 48, 11, 4, 0, [1] * 5 + [7, 1, 9, 1, 1, 1]),
     (3, 8, 2, 64, 100, 4, 3, [90, 1, 16, 1, 5, 1, 1]), (2, 4, 1, 128, 63, 0, 1, [64, 1, 1, 3, 1]),
     (2, 6, 3, 72, 5, 33, 0, [20, 1, 20, 1, 1]), (4, 5, 5, 32, 300, 1, 40, [257, 60, 1, 2]),
-    (1, 2, 1, 96, 1000, 2, 0, [1200, 1, 1]), (2, 16, 1, 64, 40, 2, 0, [30, 1, 4, 1])])
+    (1, 2, 1, 96, 1000, 2, 0, [1200, 1, 1]),
+    (2, 4, 2, 64, 2500, 5, 3, [2600, 1, 3, 1]), (1, 3, 3, 128, 900, 0, 7, [950, 2, 1]), (2, 16, 1, 64, 40, 2, 0, [30, 1, 4, 1])])
 def test_window_step(dev, stream, B, H, KV, hd, left, sinks, spare, chunks, dtype):
     say(f"step {B} streams heads {H}/{KV} hd {hd} left {left} sinks {sinks} chunks {chunks} {dtype}")
     s = Streams(dev, B, H, KV, hd, left, sinks, sinks + left + max(chunks) + spare, dtype)
@@ -682,3 +685,229 @@ def test_window_step_equals_whole_sequence(dev, stream):
     tol = attention_tolerance(spread, size, hd, S, "f32")
     check(whole.to_numpy()[0], want, tol, "whole")
     check(np.array(rows), want, tol, "steps")
+
+
+def test_window_step_slots_beyond_32_bit_offsets(dev, stream):
+    """A cache of 8.6 GB: the slots in use lie past 2^32 bytes and past 2^32 values."""
+    say("step far slots")
+    H, hd, left, slots = 32, 128, 6, (1 << 20) + 64
+    layer = nn.WindowAttention(dev, H, hd, H, left)
+    rng = np.random.default_rng(41)
+    kc, vc = (nn.Tensor(dev, (1, slots, H * hd), dtype="bf16") for _ in "kv")
+    hist, p0 = [], slots - 9
+    for i in range(12):  # runs over the ring's end
+        q, k, v = (rounded(rng.standard_normal((1, 1, H * hd)), "bf16") for _ in range(3))
+        hist.append((k[0, 0], v[0, 0]))
+        o = nn.Tensor(dev, q.shape, dtype="bf16")
+        layer.step(tensor(dev, q, "bf16"), tensor(dev, k, "bf16"), tensor(dev, v, "bf16"),
+                   tensor(dev, np.array([p0 + i]), "i32"), kc, vc, o, stream=stream)
+        if i < left:
+            continue  # the window still holds the cache's zeros
+        stream.sync(60000)
+        kk, vv = (np.array([h[c] for h in hist[-left - 1:]]) for c in (0, 1))
+        want, spread, size = attend(q[0], kk, vv, np.ones((1, left + 1), bool), H, H, hd ** -0.5)
+        check(o.to_numpy()[0], want, attention_tolerance(spread, size, hd, left + 1, "bf16"), f"token {i}")
+
+
+def test_rows_beyond_32_bit_offsets(dev, stream):
+    """Rows past 2^32 values: an 8-bit linear fills them with its bias, the norm reads them and its sum."""
+    say("far rows")
+    rows, F = (1 << 20) + 5, 4096
+    rng = np.random.default_rng(42)
+    bias = rounded(rng.standard_normal(F), "bf16")
+    lin = nn.Linear(dev, 8, F, precision="e4m3")
+    lin.load_weights(np.zeros((F, 8), np.float32), bias)
+    y = nn.Tensor(dev, (rows, F), dtype="bf16")
+    lin.forward_scaled(nn.Tensor(dev, (rows, 8), dtype="e4m3"), nn.Tensor(dev, (rows,)), y, stream=stream)
+    norm = nn.RMSNorm(dev, F)
+    total, scales, q = nn.Tensor(dev, (rows, F), dtype="bf16"), nn.Tensor(dev, (rows,)), nn.Tensor(
+        dev, (rows, F), dtype="e4m3")
+    norm.forward_residual(y, None, q, sum=total, scales=scales, stream=stream)
+    stream.sync(60000)
+    want = np.abs(rmsnorm(bias, np.ones(F), 1e-5)).max() / 448
+    first = scales.to_numpy()
+    check(first, np.full(rows, want), (F / 64 + 28) * EPS * want, "scales")
+    norm.forward_residual(total, None, q, scales=scales, stream=stream)
+    stream.sync(60000)
+    np.testing.assert_array_equal(scales.to_numpy(), first)
+
+
+# ------------------------------------------------------------------------ together, and captured
+class Block:
+    """Attention of a pre-norm transformer block on streams: norm with residual to 8 bits, q, k and v
+    in one product, rotary positions, the step on rolling caches, the output product with residual."""
+
+    def __init__(self, dev, B, E, heads, left, sinks, dtype, seed=0):
+        self.dev, self.B, self.E, self.H, self.hd, self.dtype = dev, B, E, heads, E // heads, dtype
+        rng = np.random.default_rng(seed)
+        self.w = {n: (rng.standard_normal((E, E)) / np.sqrt(E)).astype(np.float32) for n in "qkvo"}
+        self.b = {n: (0.1 * rng.standard_normal(E)).astype(np.float32) for n in "qkvo"}
+        self.g = (1 + 0.1 * rng.standard_normal(E)).astype(np.float32)
+        self.norm = nn.RMSNorm(dev, E)
+        self.norm.load_parameters(self.g)
+        self.lin = {}
+        for n in "qkvo":
+            self.lin[n] = nn.Linear(dev, E, E, precision="e4m3")
+            self.lin[n].load_weights(self.w[n], self.b[n])
+        self.dims = [self.hd // 2, self.hd // 4 * 2 - self.hd // 4 % 2 * 2]
+        self.rot = nn.Rotary(dev, self.hd, self.dims)
+        self.left, self.sinks, self.slots = left, sinks, sinks + left + 1
+        self.att = nn.WindowAttention(dev, heads, self.hd, window_left=left, sinks=sinks)
+        T = lambda dt, *shape: nn.Tensor(dev, shape, dtype=dt)  # noqa: E731
+        self.x, self.r = T(dtype, B, 1, E), T(dtype, B, 1, E)
+        self.h, self.n8, self.s = T(dtype, B, 1, E), T("e4m3", B, 1, E), T("f32", B)
+        self.t = {n: T(dtype, B, 1, E) for n in "qkvao"}
+        self.kc, self.vc = T(dtype, B, self.slots, E), T(dtype, B, self.slots, E)
+        self.pos, self.grid = T("i32", B), T("i32", B, 1, 2)
+
+    def run(self, stream):
+        t = self.t
+        self.norm.forward_residual(self.x, self.r, self.n8, sum=self.h, scales=self.s, stream=stream)
+        for n in "qkv":
+            self.lin[n].forward_scaled(self.n8, self.s, t[n], stream=stream)
+        self.rot.forward(t["q"], t["k"], self.grid, t["q"], t["k"], stream)
+        self.att.step(t["q"], t["k"], t["v"], self.pos, self.kc, self.vc, t["a"], stream=stream)
+        self.lin["o"].forward_scaled(t["a"], None, t["o"], residual=self.h, stream=stream)
+
+    def feed(self, x, r, pos):
+        self.x.copy_from(x)
+        self.r.copy_from(r)
+        self.pos.copy_from(np.array(pos))
+        self.grid.copy_from(np.array([[[p, p // 7]] for p in pos]))
+
+
+def linear_reference(x, xs, w, b, dtype):
+    wq, ws = quantise(w)
+    xd, wd = x.astype(np.float64) * xs[:, None], wq.astype(np.float64) * ws[:, None]
+    y = xd @ wd.T + b
+    mass = np.abs(xd) @ np.abs(wd).T
+    return y, (1.5 * x.shape[1] + 8) * EPS * (mass + np.abs(y) + 0.5) + HALF[dtype] * np.abs(y) * (dtype != "f32")
+
+
+@pytest.mark.parametrize("B,E,heads,dtype", [(3, 384, 8, "bf16"), (2, 96, 2, "f32")])
+def test_block_on_streams(dev, stream, B, E, heads, dtype):
+    """Every stage against its reference on what the GPU gave the stage before it."""
+    say(f"block {B} streams E {E} {dtype}")
+    m = Block(dev, B, E, heads, 9, 2, dtype)
+    rng = np.random.default_rng(51)
+    hist = [[] for _ in range(B)]
+    pos = [0, 3, 40][:B]  # the later streams' windows hold the caches' zeros at first
+    for b in range(B):
+        hist[b] = [(np.zeros(E), np.zeros(E))] * pos[b]
+    for _ in range(25):
+        x, r = (rounded(rng.standard_normal((B, 1, E)), dtype) for _ in range(2))
+        m.feed(x, r, pos)
+        m.run(stream)
+        stream.sync(60000)
+        h = m.h.to_numpy()
+        np.testing.assert_array_equal(h, rounded(x + r, dtype))
+        n8, s = m.n8.to_numpy()[:, 0], m.s.to_numpy()
+        y = rmsnorm((x + r)[:, 0], m.g, 1e-5)
+        unit = np.abs(y) / s[:, None]
+        check(n8 * s[:, None].astype(np.float64), y,
+              (np.maximum(unit * HALF["e4m3"], 2.0 ** -10) * (1 + 1e-5) + 448 * 80 * EPS) * s[:, None], "norm")
+        got = {n: t.to_numpy() for n, t in m.t.items()}
+        want, tol = linear_reference(n8, s, m.w["v"], m.b["v"], dtype)
+        check(got["v"][:, 0], want, tol, "v")
+        for n in "qk":
+            want, tol = linear_reference(n8, s, m.w[n], m.b[n], dtype)
+            grid = np.array([[[p, p // 7]] for p in pos])
+            turned = rotary(want[:, None], grid, heads, m.hd, m.dims)
+            size = np.abs(want).reshape(B, heads, m.hd).max(-1, keepdims=True).repeat(m.hd, -1).reshape(B, E)
+            slack = tol.reshape(B, heads, m.hd).max(-1, keepdims=True).repeat(m.hd, -1).reshape(B, E)
+            # a pair's errors add up to sqrt(2) of the larger one's, and one more rounding
+            check(got[n][:, 0], turned[:, 0], 1.5 * slack + size * (HALF[dtype] + 32 * EPS), n)
+        for b in range(B):
+            hist[b].append((got["k"][b, 0].astype(np.float64), got["v"][b, 0].astype(np.float64)))
+            keys = [i for i in range(pos[b] + 1) if i >= pos[b] - m.left or i < m.sinks]
+            kk, vv = (np.array([hist[b][i][c] for i in keys]) for c in (0, 1))
+            want, spread, size = attend(got["q"][b], kk, vv, np.ones((1, len(keys)), bool), heads, heads,
+                                        m.hd ** -0.5)
+            check(got["a"][b], want, attention_tolerance(spread, size, m.hd, len(keys), dtype), "attention")
+        aq, asc = quantise(got["a"][:, 0])
+        want, tol = linear_reference(aq, asc, m.w["o"], m.b["o"], dtype)
+        want = want + h[:, 0]
+        check(got["o"][:, 0], want, tol + (HALF[dtype] if dtype != "f32" else EPS) * np.abs(want), "out")
+        pos = [p + 1 for p in pos]
+
+
+class Graph:
+    """Calls on a stream, captured once and replayed."""
+
+    def __init__(self, stream, calls):
+        path = next(ln.split()[-1] for ln in open("/proc/self/maps") if "libamdhip64" in ln)
+        self.hip = C.CDLL(path)
+        self.s = C.c_void_p(C.cast(stream.handle, C.POINTER(C.c_void_p))[1])  # {device, hipStream_t, ..}
+        graph, self.exec = C.c_void_p(), C.c_void_p()
+        self.ok(self.hip.hipStreamBeginCapture(self.s, 2))
+        calls()
+        self.ok(self.hip.hipStreamEndCapture(self.s, C.byref(graph)))
+        self.ok(self.hip.hipGraphInstantiate(C.byref(self.exec), graph, None, None, C.c_size_t(0)))
+
+    def ok(self, status):
+        assert status == 0, f"hip status {status}"
+
+    def replay(self):
+        self.ok(self.hip.hipGraphLaunch(self.exec, self.s))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_block_captured_and_replayed(dev, dtype):
+    """The block in a graph, replayed with other inputs, positions and eager work of the same layers
+    between the replays (also larger calls, which grow their workspaces), equals the eager block."""
+    say(f"block captured {dtype}")
+    s, other = nn.Stream(dev), nn.Stream(dev)
+    B, E = 2, 192
+    eager, taken = (Block(dev, B, E, 4, 700, 2, dtype) for _ in range(2))  # split keys: a workspace
+    rng = np.random.default_rng(52)
+
+    def inputs():
+        return (rounded(rng.standard_normal((B, 1, E)), dtype) for _ in range(2))
+
+    x, r = inputs()
+    for m in (eager, taken):  # workspaces are made by a call outside the graph
+        m.feed(x, r, [0, 5])
+        m.run(s)
+    s.sync(60000)
+    graph = Graph(s, lambda: taken.run(s))
+    for i in range(6):
+        x, r = inputs()
+        pos = [3 * i, 1000 + i]
+        for m in (eager, taken):
+            m.feed(x, r, pos)
+        eager.run(other)
+        graph.replay()
+        s.sync(60000)
+        other.sync(60000)
+        for n in "qkvao":
+            np.testing.assert_array_equal(taken.t[n].to_numpy(), eager.t[n].to_numpy())
+        np.testing.assert_array_equal(taken.kc.to_numpy(), eager.kc.to_numpy())
+        # other calls of the captured layers, on their stream, larger than any before
+        big = tensor(dev, rng.standard_normal((40 + 30 * i, E)), dtype)
+        taken.lin["o"].forward_scaled(big, None, nn.Tensor(dev, (40 + 30 * i, E), dtype=dtype), stream=s)
+        n = 30 + 10 * i
+        qkv = [tensor(dev, rng.standard_normal((3, n, E)), dtype) for _ in range(3)]
+        caches = [nn.Tensor(dev, (3, 702 + n, E), dtype=dtype) for _ in range(2)]
+        taken.att.step(*qkv, tensor(dev, np.array([0, 9, 800]), "i32"), *caches,
+                       nn.Tensor(dev, (3, n, E), dtype=dtype), stream=s)
+        s.sync(60000)
+
+
+def test_calls_on_many_streams(dev):
+    """The same work on several streams at once, one layer a stream, and on the default stream."""
+    say("streams")
+    rng = np.random.default_rng(53)
+    S, H, hd = 300, 4, 48
+    x = [rng.standard_normal((1, S, H * hd)).astype(np.float32) for _ in range(3)]
+    want = None
+    jobs = []
+    for stream in [None] + [nn.Stream(dev) for _ in range(4)]:
+        layer = nn.WindowAttention(dev, H, hd, window_left=40, window_right=7, sinks=3)
+        out = nn.Tensor(dev, x[0].shape)
+        layer.forward(*(tensor(dev, v, "f32") for v in x), out, stream=stream)
+        jobs.append((layer, out))
+    dev.synchronize()
+    for _, out in jobs:
+        got = out.to_numpy()
+        want = got if want is None else want
+        np.testing.assert_array_equal(got, want)
