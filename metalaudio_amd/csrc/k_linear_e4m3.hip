@@ -267,29 +267,40 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 
 // Few rows (up to 32): the weights are all the traffic. A workgroup takes 32 rows of w, its eight waves an
 // eighth of the depth each, operands straight from memory (a wave reads 64 bytes of 32 rows at a time, four
-// such steps in flight); their sums meet in LDS.
+// such steps in flight); their sums meet in LDS. Rows of x may be of any length: what a lane would read past
+// a row's end is 0.
 template <class T>
 __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) {
   __shared__ float sum[8][32][33];  // [wave][m][n]
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = threadIdx.x >> 6;
   const int n0 = blockIdx.x * 32;
-  const uint8_t* x = a.x + min((int64_t)l32, a.M - 1) * a.K + 32 * g;
+  const uint8_t* x = a.x + min((int64_t)l32, a.M - 1) * a.ldx + 32 * g;
   const uint8_t* w = a.w + (int64_t)min(n0 + l32, a.N - 1) * a.K + 32 * g;
   const int steps = a.K / 64, s0 = steps * wave / 8, s1 = steps * (wave + 1) / 8;
   floatx16 acc;
 #pragma unroll
   for (int v = 0; v < 16; ++v) acc[v] = 0.f;
-  auto load = [](const uint8_t* p, Operand<T>& o) {
-    const intx4* q = reinterpret_cast<const intx4*>(p);
-    o.set(q[0], q[1]);
-  };
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
+  auto step = [&](int s, auto whole) {
+    const intx4* q = reinterpret_cast<const intx4*>(w + 64 * s);
     Operand<T> xo, wo;
-    load(x + 64 * s, xo);
-    load(w + 64 * s, wo);
+    wo.set(q[0], q[1]);
+    intx4 lo = 0, hi = 0;
+    if (decltype(whole)::value || 64 * s + 32 * g + 32 <= a.ldx) {
+      __builtin_memcpy(&lo, x + 64 * s, 16);
+      __builtin_memcpy(&hi, x + 64 * s + 16, 16);
+    } else {
+      for (int e = 0; e < a.ldx - 64 * s - 32 * g; ++e) {
+        intx4& part = e < 16 ? lo : hi;
+        part[e % 16 / 4] |= (int)x[64 * s + e] << 8 * (e % 4);
+      }
+    }
+    xo.set(lo, hi);
     acc = mul(wo, xo, acc);
-  }
+  };
+  const int whole = min(s1, a.ldx / 64);  // steps that end within a row
+#pragma unroll 4
+  for (int s = s0; s < whole; ++s) step(s, std::true_type{});
+  for (int s = max(s0, whole); s < s1; ++s) step(s, std::false_type{});
 #pragma unroll
   for (int v = 0; v < 16; ++v) sum[wave][l32][8 * (v / 4) + 4 * g + v % 4] = acc[v];
   __syncthreads();
@@ -337,7 +348,9 @@ void launch_tile(const LaunchCtx& c, const LinearE4m3Args& a, const char* name) 
 template <class T>
 void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   constexpr bool F32 = sizeof(T) == 4;
-  if (a.M <= 32)
+  MNN_REQUIRE(a.K % 128 == 0 && (a.ldx == a.K || a.M <= kLinearFew), MNN_ERR_INVALID_ARGUMENT,
+              "linear_e4m3: rows of x are not padded");
+  if (a.M <= kLinearFew)
     return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
                   dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
   // The largest tile that still gives most compute units one: us at (M, K, N), 256 / 128 / 64 square:

@@ -26,8 +26,8 @@ __device__ __forceinline__ float block_reduce(float v, float* sh, F op) {
   return op(op(sh[0], sh[1]), op(sh[2], sh[3]));
 }
 
-// Any row length and alignment: a workgroup per row in three passes over memory (the row's second and
-// third reads come from L2). Nothing is written before the last pass, so sum and y may be x or r.
+// Any row length: a workgroup per row in three passes over memory (the row's second and third reads come
+// from L2). Nothing is written before the last pass, so sum and y may be x or r.
 template <class T>
 __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
   __shared__ float sh[4];
@@ -68,115 +68,176 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
   }
 }
 
-// Rows of up to 4096 values, a multiple of 8: a wave a row, which stays in its registers from the first read
-// to the last write, lane l holding values 512 i + 8 l .. + 7; the weights too, over all of a wave's rows.
-// Bound by memory (two loads and two stores a value).
-template <class T, int NV, mnn_dtype OUT>
-__global__ __launch_bounds__(256) void rmsnorm_wave_kernel(RmsNormArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t step = (int64_t)gridDim.x * 4;
-  float w[NV][8];
+// Rows of whole chunks of 16 bytes that W waves hold in their registers from the first read to the last
+// write: NV chunks a lane, chunk i of lane l at (64 W i + l) VE, so that a load instruction covers 1 KB in a
+// row. The weights stay there too, over all the rows that a workgroup takes. Bound by memory (up to two loads
+// and two stores a value).
+template <class T, int NV, int W, mnn_dtype OUT>
+__global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
+  constexpr int VE = 16 / (int)sizeof(T);
+  typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+  __shared__ float sh[4][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = ((W == 1 ? 0 : wave * 64) + lane) * VE;
+  // over the W waves of a row. `at`, 0 or 1, keeps a row's two reductions apart and `parity` one row's from
+  // the next one's: a wave writes a place again only behind a barrier that is behind the others' reads of it
+  int parity = 0;
+  auto over_row = [&](float v, int at, auto op) {
+    v = group_reduce<64>(v, op);
+    if constexpr (W > 1) {
+      float* to = sh[2 * parity + at];
+      if (lane == 0) to[wave] = v;
+      __syncthreads();
+      v = op(op(to[0], to[1]), op(to[2], to[3]));
+    }
+    return v;
+  };
+  auto values = [](uintx4 x, float* v) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      unsigned u;
+      if constexpr (VE == 4)
+        u = x[e];
+      else
+        u = e & 1 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16;
+      v[e] = __builtin_bit_cast(float, u);
+    }
+  };
   bool on[NV];
+  float w[NV][VE];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    on[i] = 512 * i + 8 * lane < a.F;
+    on[i] = col + 64 * W * VE * i < a.F;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[i][e] = a.w && on[i] ? a.w[512 * i + 8 * lane + e] : 1.f;
+    for (int e = 0; e < VE; ++e) w[i][e] = a.w && on[i] ? a.w[col + 64 * W * VE * i + e] : 1.f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < a.rows; row += step) {
-    const int64_t at = row * a.F + 8 * lane;
-    Eight<T> x[NV], r[NV];
+  const int64_t first = W == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  for (int64_t row = first; row < a.rows; row += (int64_t)gridDim.x * (4 / W), parity ^= 1) {
+    const int64_t at = row * a.F + col;
+    uintx4 x[NV], r[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      x[i].clear();
-      r[i].clear();
+      x[i] = r[i] = uintx4{0, 0, 0, 0};
       if (on[i]) {
-        x[i].load(static_cast<const T*>(a.x) + at + 512 * i);
-        if (a.r) r[i].load(static_cast<const T*>(a.r) + at + 512 * i);
+        x[i] = *reinterpret_cast<const uintx4*>(static_cast<const T*>(a.x) + at + 64 * W * VE * i);
+        if (a.r) r[i] = *reinterpret_cast<const uintx4*>(static_cast<const T*>(a.r) + at + 64 * W * VE * i);
       }
     }
-    float h[NV][8], ss = 0.f;
+    float h[NV][VE], ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float add[VE];
+      values(x[i], h[i]);
+      values(r[i], add);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[i][e] = a.r ? x[i][e] + r[i][e] : x[i][e];
+      for (int e = 0; e < VE; ++e) {
+        if (a.r) h[i][e] += add[e];
         ss = fmaf(h[i][e], h[i][e], ss);
       }
+    }
     if (a.sum) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (on[i]) {
-          Eight<T> o;
-          o.set(h[i]);
-          o.store(static_cast<T*>(a.sum) + at + 512 * i);
+          uintx4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (VE == 4)
+              o[e] = __builtin_bit_cast(unsigned, h[i][e]);
+            else
+              o[e] = cvt_pk_bf16(h[i][2 * e], h[i][2 * e + 1]);
+          }
+          *reinterpret_cast<uintx4*>(static_cast<T*>(a.sum) + at + 64 * W * VE * i) = o;
         }
     }
-    float top = 0.f;
     if (a.w) {
-      const float norm = rsqrtf(group_reduce<64>(ss, Plus{}) / (float)a.F + a.eps);
+      const float norm = rsqrtf(over_row(ss, 0, Plus{}) / (float)a.F + a.eps);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * norm * w[i][e];
+        for (int e = 0; e < VE; ++e) h[i][e] = h[i][e] * norm * w[i][e];
     }
     if constexpr (OUT == MNN_E4M3) {
+      float top = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < VE; ++e)
           if (on[i]) top = max_nan(top, fabsf(h[i][e]));
-      const RowScale rs = row_scale(group_reduce<64>(top, max_nan));
-      if (lane == 0) a.scales[row] = rs.scale;
-      uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy + 8 * lane;
+      const RowScale rs = row_scale(over_row(top, 1, max_nan));
+      if (lane == 0 && (W == 1 || wave == 0)) a.scales[row] = rs.scale;
+      uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy + col;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const float* v = h[i];
-        if (on[i])
-          *reinterpret_cast<uint2*>(y + 512 * i) =
-              make_uint2(pack_e4m3(v[0] * rs.inv, v[1] * rs.inv, v[2] * rs.inv, v[3] * rs.inv),
-                         pack_e4m3(v[4] * rs.inv, v[5] * rs.inv, v[6] * rs.inv, v[7] * rs.inv));
-        else if (512 * i + 8 * lane < a.ldy)
-          *reinterpret_cast<uint2*>(y + 512 * i) = make_uint2(0, 0);
+        unsigned q[VE / 4];
+#pragma unroll
+        for (int e = 0; e < VE / 4; ++e)
+          q[e] = on[i] ? pack_e4m3(h[i][4 * e] * rs.inv, h[i][4 * e + 1] * rs.inv, h[i][4 * e + 2] * rs.inv,
+                                   h[i][4 * e + 3] * rs.inv)
+                       : 0u;
+        if (col + 64 * W * VE * i < a.ldy) {
+          if constexpr (VE == 4)
+            *reinterpret_cast<unsigned*>(y + 64 * W * VE * i) = q[0];
+          else
+            *reinterpret_cast<uint2*>(y + 64 * W * VE * i) = make_uint2(q[0], q[1]);
+        }
       }
     } else {
-      using O = std::conditional_t<OUT == MNN_F32, float, __bf16>;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (on[i]) {
-          Eight<O> o;
-          o.set(h[i]);
-          o.store(static_cast<O*>(a.y) + row * a.ldy + 512 * i + 8 * lane);
+      for (int i = 0; i < NV; ++i) {
+        if (!on[i]) continue;
+        const int64_t to = row * a.ldy + col + 64 * W * VE * i;
+        if constexpr (OUT == MNN_F32) {
+#pragma unroll
+          for (int e = 0; e < VE; e += 4)
+            *reinterpret_cast<float4*>(static_cast<float*>(a.y) + to + e) =
+                make_float4(h[i][e], h[i][e + 1], h[i][e + 2], h[i][e + 3]);
+        } else {
+          unsigned q[VE / 2];
+#pragma unroll
+          for (int e = 0; e < VE / 2; ++e) q[e] = cvt_pk_bf16(h[i][2 * e], h[i][2 * e + 1]);
+          if constexpr (VE == 4)
+            *reinterpret_cast<uint2*>(static_cast<__bf16*>(a.y) + to) = make_uint2(q[0], q[1]);
+          else
+            *reinterpret_cast<uint4*>(static_cast<__bf16*>(a.y) + to) = make_uint4(q[0], q[1], q[2], q[3]);
         }
+      }
     }
   }
 }
 
-template <class T, int NV>
-void launch_wave(const LaunchCtx& c, const RmsNormArgs& a) {
-  const char* name = sizeof(T) == 4 ? "rmsnorm_wave_f32" : "rmsnorm_wave_bf16";
+template <class T, int NV, int W>
+void launch_rows(const LaunchCtx& c, const RmsNormArgs& a) {
+  const char* name = sizeof(T) == 4 ? "rmsnorm_rows_f32" : "rmsnorm_rows_bf16";
   // eight workgroups a compute unit keep their weights over several rows
-  const dim3 grid((unsigned)std::min<int64_t>((a.rows + 3) / 4, 8 * c.dev->props.multiProcessorCount));
+  const int64_t wgs = W == 1 ? (a.rows + 3) / 4 : a.rows;
+  const dim3 grid((unsigned)std::min<int64_t>(wgs, 8 * c.dev->props.multiProcessorCount));
   if (a.out == MNN_E4M3)
-    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_E4M3>, grid, dim3(256), 0, a);
+    launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_E4M3>, grid, dim3(256), 0, a);
   else if (a.out == MNN_BF16)
-    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_BF16>, grid, dim3(256), 0, a);
+    launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_BF16>, grid, dim3(256), 0, a);
   else
-    launch(c, name, rmsnorm_wave_kernel<T, NV, MNN_F32>, grid, dim3(256), 0, a);
+    launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_F32>, grid, dim3(256), 0, a);
 }
 
+// A wave a row up to four chunks a lane; a workgroup a row for longer ones, and for rows so few that a wave
+// each would leave most of the GPU waiting for a handful of loads.
 template <class T>
 void rmsnorm_t(const LaunchCtx& c, const RmsNormArgs& a) {
-  if (a.F % 8 == 0 && a.ldy % 8 == 0 && a.ldy <= 4096) {
-    switch ((a.ldy + 511) / 512) {
-      case 1: return launch_wave<T, 1>(c, a);
-      case 2: return launch_wave<T, 2>(c, a);
-      case 3: return launch_wave<T, 3>(c, a);
-      case 4: return launch_wave<T, 4>(c, a);
-      case 5:
-      case 6: return launch_wave<T, 6>(c, a);
-      default: return launch_wave<T, 8>(c, a);
+  constexpr int VE = 16 / (int)sizeof(T);
+  if (a.F % VE == 0 && a.ldy % VE == 0 && a.ldy <= 8 * 256 * VE) {
+    const int n = (int)((a.ldy + 64 * VE - 1) / (64 * VE));  // chunks a lane of one wave
+    const bool few = a.rows < c.dev->props.multiProcessorCount;
+    if (n == 1) return launch_rows<T, 1, 1>(c, a);
+    if (n <= 4 && !few) {
+      if (n == 2) return launch_rows<T, 2, 1>(c, a);
+      if (n == 3) return launch_rows<T, 3, 1>(c, a);
+      return launch_rows<T, 4, 1>(c, a);
     }
+    if (n <= 4) return launch_rows<T, 1, 4>(c, a);
+    if (n <= 8) return launch_rows<T, 2, 4>(c, a);
+    if (n <= 16) return launch_rows<T, 4, 4>(c, a);
+    return launch_rows<T, 8, 4>(c, a);
   }
   launch(c, sizeof(T) == 4 ? "rmsnorm_any_f32" : "rmsnorm_any_bf16", rmsnorm_any_kernel<T>,
          dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)), dim3(256), 0, a);

@@ -148,7 +148,11 @@ class LinearE4m3Layer : public Layer {
                 "FusedLinear: leakyReluAlpha must be finite");
     if (bias) b_ = &add_param("bias", out);
     kp_ = (in + 127) / 128 * 128;
-    set_weights(std::vector<float>((size_t)in * out, 0.f).data());  // zero until loaded
+    dev_->make_current();
+    wq_.reserve((size_t)out * kp_);
+    ws_.reserve(sizeof(float) * out);
+    HIP_CHECK(hipMemset(wq_.ptr, 0, (size_t)out * kp_));  // zero until loaded
+    HIP_CHECK(hipMemset(ws_.ptr, 0, sizeof(float) * out));
   }
   const char* kind() const override { return "Linear"; }
   Shape input_shape() const override { return {in_}; }
@@ -166,7 +170,13 @@ class LinearE4m3Layer : public Layer {
     MNN_REQUIRE(n == (size_t)in_ * out_, MNN_ERR_BUFFER_SIZE_MISMATCH,
                 "Linear parameter 'weight': expected " << (size_t)in_ * out_ << " values, got " << n);
     MNN_REQUIRE(data, MNN_ERR_INVALID_ARGUMENT, "null data");
+    uint32_t bad = 0;  // all values at once, a loop that the compiler can vectorise
     for (size_t i = 0; i < n; ++i) {
+      uint32_t u;
+      std::memcpy(&u, data + i, 4);
+      bad |= (uint32_t)((u & 0x7f800000u) == 0x7f800000u);
+    }
+    for (size_t i = 0; bad && i < n; ++i) {
       MNN_REQUIRE(!std::isnan(data[i]), MNN_ERR_INVALID_CONFIGURATION,
                   name << " contain NaN values - model file may be corrupted");
       MNN_REQUIRE(!std::isinf(data[i]), MNN_ERR_INVALID_CONFIGURATION,
@@ -214,7 +224,7 @@ class LinearE4m3Layer : public Layer {
       k::rmsnorm(ctx(s), a);
       g.x = x;
       g.xs = xs;
-    } else if (kp_ != in_) {  // rows that do not fill the last depth step
+    } else if (kp_ != in_ && rows > k::kLinearFew) {  // rows that do not fill the last depth step
       uint8_t* x = static_cast<uint8_t*>(scratch_.get((size_t)rows * kp_));
       k::pad_rows_u8(ctx(s), g.x, rows, in_, x, kp_);
       g.x = x;
@@ -228,6 +238,7 @@ class LinearE4m3Layer : public Layer {
     g.M = rows;
     g.N = out_;
     g.K = kp_;
+    g.ldx = g.x == in.data ? in_ : kp_;
     g.act = act_;
     g.alpha = alpha_;
     k::linear_e4m3(ctx(s), g);
@@ -239,8 +250,6 @@ class LinearE4m3Layer : public Layer {
     DevBuf w;  // the fp32 rows, only while they are rounded
     w.reserve(sizeof(float) * in_ * out_);
     HIP_CHECK(hipMemcpy(w.ptr, data, sizeof(float) * in_ * out_, hipMemcpyHostToDevice));
-    wq_.reserve((size_t)out_ * kp_);
-    ws_.reserve(sizeof(float) * out_);
     k::RmsNormArgs a;
     a.x = w.ptr;
     a.in = MNN_F32;

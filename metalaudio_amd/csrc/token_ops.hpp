@@ -25,19 +25,20 @@ struct RmsNormArgs {
 void rmsnorm(const LaunchCtx& c, const RmsNormArgs& a);
 
 struct LinearE4m3Args {
-  const uint8_t* x = nullptr;  // [M][ldx]
+  const uint8_t* x = nullptr;  // [M][ldx], ldx = K or, up to kLinearFew rows, in_features
   const float* xs = nullptr;   // [M]
-  const uint8_t* w = nullptr;  // [N][ldw]
+  const uint8_t* w = nullptr;  // [N][K]
   const float* ws = nullptr;   // [N]
   const float* bias = nullptr; // [N] or null
   const void* r = nullptr;     // [M][N] of the output's type, or null; may be y
   void* y = nullptr;           // [M][N]
   mnn_dtype out = MNN_F32;     // f32 or bf16
   int64_t M = 0;
-  int N = 0, K = 0;            // K: a multiple of 128, the rows' zeros behind in_features included
+  int N = 0, K = 0, ldx = 0;   // K: a multiple of 128, the weights' zeros behind in_features included
   int act = 0;
   float alpha = 0.01f;
 };
+constexpr int kLinearFew = 32;
 void linear_e4m3(const LaunchCtx& c, const LinearE4m3Args& a);
 // rows of `n` bytes copied to rows of `ld` >= n, the rest zero
 void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint8_t* y, int ld);
