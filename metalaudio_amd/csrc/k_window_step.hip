@@ -104,15 +104,19 @@ __device__ __forceinline__ float across_groups(float v) {
 }
 
 // W waves answer R rows. L lanes take a key, eight dimensions each (head dims that are no power of two leave
-// some idle), so a wave holds 64 / L keys at a time and U of those in flight; every group of L lanes keeps
-// running maxima, sums and outputs of its own, which are joined at the end, first in the wave, then in LDS,
-// then, if the keys are split over workgroups, by window_join_kernel. On the vector units: a key's row feeds
-// R dot products only, 4 bytes of cache an instruction at R = 1, and the matrix units would stand idle for the
-// loads just the same.
+// some idle), so a wave holds 64 / L keys at a time, U of those computed while the next U are on their way;
+// every group of L lanes keeps running maxima, sums and outputs of its own, which are joined at the end, first
+// in the wave, then in LDS, then, if the keys are split over workgroups, by window_join_kernel. On the vector
+// units: a key's row feeds R dot products only, 4 bytes of cache an instruction at R = 1, and the matrix units
+// would stand idle for the loads just the same. One row of f32 at 64 streams, 8 heads of 128, 1024 keys runs
+// at 5.7 TB/s; four rows of bf16 (64 streams, 16 / 4 heads of 64, 2048 keys) at 3.7 TB/s, bound by the vector
+// units. Waves: 8, or 12 with half the keys in flight where four rows of bf16 leave them no more registers
+// (us at 16 without / 8 with / 12 with the next keys in flight: the latter case 30.6 / 31.9 / 30.1, one stream of
+// 8 heads of 48 in f32 6.9 / 6.5 / -).
 template <class T, int L, int R, int W>
 __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, int tiles, int nsplit,
                                                              float* part) {
-  constexpr int KPW = 64 / L, U = sizeof(T) == 4 ? 2 : R > 2 ? 4 : 8;
+  constexpr int KPW = 64 / L, U = sizeof(T) == 4 ? 2 : R > 2 ? 2 : 4;
   extern __shared__ float sh[];  // [W][R][hd + 2], [R]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane % L, grp = lane / L;
   const int sp = blockIdx.x % nsplit, unit = blockIdx.x / nsplit;
@@ -149,38 +153,43 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
   }
   const int begin = (int)((int64_t)w.n * sp / nsplit), end = (int)((int64_t)w.n * (sp + 1) / nsplit);
   const bool mixed = w.t0 != w.t1;  // rows of several tokens, which see different keys
-  for (int i = begin + wave * KPW * U; i < end; i += W * KPW * U) {
-    Eight<T> kx[U], vx[U];
-    int p[U];  // the lane's keys as positions
+  // U keys a group at a time; the next ones are on their way while these are computed
+  struct Keys {
+    Eight<T> k[U], v[U];
+    int p[U];  // the lane's keys as positions, -1: none
+  };
+  auto fetch = [&](int i, Keys& x) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int idx = i + u * KPW + grp;
-      p[u] = idx < w.ns ? idx : w.lo + idx - w.ns;
-      kx[u].clear();
-      vx[u].clear();
+      x.p[u] = idx >= end ? -1 : idx < w.ns ? idx : w.lo + idx - w.ns;
+      x.k[u].clear();
+      x.v[u].clear();
       if (on && idx < end) {
-        int64_t at;
-        int slot = p[u];
+        int slot = x.p[u];
         if (slot >= a.sinks) {
           slot = w.wrapped + (slot - max(w.lo, a.sinks));
           slot = a.sinks + (slot >= w.ring ? slot - w.ring : slot);
         }
-        const bool fresh = p[u] >= w.pos;
-        at = (int64_t)(fresh ? p[u] - w.pos : slot) * kvw;
-        kx[u].load((fresh ? kn : kc) + at);
-        vx[u].load((fresh ? vn : vc) + at);
+        const bool fresh = x.p[u] >= w.pos;
+        const int64_t at = (int64_t)(fresh ? x.p[u] - w.pos : slot) * kvw;
+        x.k[u].load((fresh ? kn : kc) + at);
+        x.v[u].load((fresh ? vn : vc) + at);
       }
-      if (idx >= end) p[u] = -1;
     }
+  };
+  auto compute = [&](const Keys& x) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float s[U], top = m[r];
       const int mine = w.pos + (w.row0 + r) / G;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        s[u] = group_reduce<L>(dot8(kx[u], q[r]), Plus{}) * qs;
-        const bool seen = p[u] >= 0 && (!mixed || (p[u] <= mine && (p[u] >= mine - a.left || p[u] < a.sinks)));
-        if (!seen) s[u] = -INFINITY;
+        s[u] = group_reduce<L>(dot8(x.k[u], q[r]), Plus{}) * qs;
+        const int p = x.p[u];
+        // without short circuits, which become branches (16 tokens, 8 heads of 48: 13.3 -> 12.0 us)
+        const bool seen = (p >= 0) & (!mixed | ((p <= mine) & ((p >= mine - a.left) | (p < a.sinks))));
+        s[u] = seen ? s[u] : -INFINITY;
         top = max_nan(top, s[u]);
       }
       const float ref = top == -INFINITY ? 0.f : top;
@@ -194,9 +203,20 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
         const float pu = __builtin_amdgcn_exp2f(s[u] - ref);
         l[r] += pu;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(pu, vx[u][e], o[r][e]);
+        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(pu, x.v[u][e], o[r][e]);
       }
     }
+  };
+  constexpr int STEP = W * KPW * U;
+  Keys x[2];
+  int i = begin + wave * KPW * U;
+  if (i < end) fetch(i, x[0]);
+  for (; i < end; i += 2 * STEP) {
+    if (i + STEP < end) fetch(i + STEP, x[1]);
+    compute(x[0]);
+    if (i + STEP >= end) break;
+    if (i + 2 * STEP < end) fetch(i + 2 * STEP, x[0]);
+    compute(x[1]);
   }
 
   // the new tokens' keys and values to their slots
@@ -335,7 +355,8 @@ struct Plan {
   int R, nsplit;
   int64_t tiles;
 };
-constexpr int kWaves = 16;
+template <class T, int R>
+constexpr int kWaves = sizeof(T) == 2 && R == 4 ? 12 : 8;
 Plan plan_of(const WindowStepArgs& a, int cus) {
   Plan p;
   const int64_t rows = (int64_t)a.T * (a.H / a.KV);
@@ -355,12 +376,13 @@ Plan plan_of(const WindowStepArgs& a, int cus) {
 
 template <class T, int L, int R>
 void launch_step(const LaunchCtx& c, const WindowStepArgs& a, const Plan& p, float* part) {
+  constexpr int W = kWaves<T, R>;
   const int64_t units = (int64_t)a.B * a.KV * p.tiles;
   MNN_REQUIRE(units * p.nsplit < (1 << 22), MNN_ERR_INVALID_CONFIGURATION,
               "WindowAttention: too many streams and tokens in one step");
-  const size_t lds = sizeof(float) * (kWaves * R * (a.hd + 2) + R);
-  launch(c, sizeof(T) == 4 ? "window_step_f32" : "window_step_bf16", window_step_kernel<T, L, R, kWaves>,
-         dim3((unsigned)(units * p.nsplit)), dim3(64 * kWaves), lds, a, (int)p.tiles, p.nsplit, part);
+  const size_t lds = sizeof(float) * (W * R * (a.hd + 2) + R);
+  launch(c, sizeof(T) == 4 ? "window_step_f32" : "window_step_bf16", window_step_kernel<T, L, R, W>,
+         dim3((unsigned)(units * p.nsplit)), dim3(64 * W), lds, a, (int)p.tiles, p.nsplit, part);
   if (p.nsplit > 1)
     launch(c, sizeof(T) == 4 ? "window_join_f32" : "window_join_bf16", window_join_kernel<T, R>,
            dim3((unsigned)units), dim3(256), 0, a, (int)p.tiles, p.nsplit, (const float*)part);

@@ -153,6 +153,7 @@ class LinearE4m3Layer : public Layer {
     ws_.reserve(sizeof(float) * out);
     HIP_CHECK(hipMemset(wq_.ptr, 0, (size_t)out * kp_));  // zero until loaded
     HIP_CHECK(hipMemset(ws_.ptr, 0, sizeof(float) * out));
+    HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream read them
   }
   const char* kind() const override { return "Linear"; }
   Shape input_shape() const override { return {in_}; }
