@@ -279,6 +279,8 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
         ref = move ? mx : ref;
         begun |= move;
       }
+      // ahead of the waves that are at their scores: this part feeds both pipes (57.4 -> 55.5 us at 16384 keys)
+      __builtin_amdgcn_s_setprio(1);
       const float off = ref * cs;
       // the block's probabilities are added up by themselves before they join the running sum
       float ps = 0.f;
@@ -311,6 +313,7 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
             o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(0, i, ks), px, o[i], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       lsum += ps;
     }
     lds_barrier();
