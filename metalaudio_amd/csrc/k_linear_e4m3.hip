@@ -122,6 +122,10 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 //
 // Rows behind the last are read as the last one; their results are not stored. The results go through LDS
 // once more (the ring is done with), so that scales, residual and output are read and written row by row.
+//
+// Bound by the matrix instructions and, in a grid of one or two rounds, by each round's first loads and results
+// (about 18 us at 256 x 256, 1.39 us a step of 128): 8192 x 4096 x 4096 to bf16 125 us (2.2 PFLOP/s), 10752 x 1536 x 384 to
+// f32 with residual 20 us.
 template <class T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);

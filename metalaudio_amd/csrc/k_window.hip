@@ -48,6 +48,9 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // that its own queries see; the mask is applied where a block is not wholly visible to all 32. While one
 // block is computed the next one's rows are on their way to registers.
 //
+// Bound by the vector units' issue beside the matrix instructions: 16384 tokens, 1023 back, 8 / 2 heads of 64 in bf16
+// 55.5 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 26.7 us (split of K, V and P).
+//
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
 // A key that a query does not see has probability 0, but 0 times a value that is not finite is NaN, and
