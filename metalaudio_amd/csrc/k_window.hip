@@ -49,7 +49,7 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // block is computed the next one's rows are on their way to registers.
 //
 // Bound by the vector units' issue beside the matrix instructions: 16384 tokens, 1023 back, 8 / 2 heads of 64 in bf16
-// 55.5 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 26.7 us (split of K, V and P).
+// 54 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 24.7 us (split of K, V and P).
 //
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
@@ -254,16 +254,22 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
       }
       const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= (int64_t)qw + a.right && k1 < len;
       if (!whole) {
+        // a bit a key: keys below hi, and not below lo or below the sinks' end; then two instructions a score
+        // that need no lane masks (three comparisons a score: 55.5 -> 54 us; 16384 keys)
         const int first = k0 + 4 * g;  // the lane's: key c below is first + c
-        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right) - first;
+        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right) + 1 - first;
         const int lo = qi - a.left - first, sk = a.sinks - first;
+        auto below = [](int n) { return (unsigned)((1ull << min(max(n, 0), 32)) - 1); };  // the first n of 32
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j) {
+          const int seen = (int)(below(hi - 32 * j) & (~below(lo - 32 * j) | below(sk - 32 * j)));
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int c = 32 * j + 8 * (v / 4) + v % 4;
-            st[j][v] = (c <= hi) & ((c >= lo) | (c < sk)) ? st[j][v] : -INFINITY;
+            const unsigned m = (unsigned)__builtin_amdgcn_sbfe(seen, 8 * (v / 4) + v % 4, 1);
+            const float x = st[j][v];
+            st[j][v] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & m) | (0xff800000u & ~m));
           }
+        }
       }
       // maximum keeps NaN, which costs no canonical forms; a NaN neither moves the reference nor passes
       float mx = -INFINITY;
@@ -271,9 +277,10 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int v = 0; v < 16; v += 2) mx = max_nan(max_nan(mx, st[j][v]), st[j][v + 1]);
-      mx = other_half(mx, max_nan);
-      const bool move = begun ? (mx - ref) * cs > 8.f : mx > -INFINITY;
-      if (__any(move)) {
+      const auto far = [&] { return begun ? (mx - ref) * cs > 8.f : mx > -INFINITY; };
+      if (__any(far())) {
+        mx = other_half(mx, max_nan);  // the query's other keys
+        const bool move = far();
         // the first visible key has nothing to rescale
         const float alpha = !move ? 1.f : begun ? __builtin_amdgcn_exp2f((ref - mx) * cs) : 0.f;
         lsum *= alpha;
