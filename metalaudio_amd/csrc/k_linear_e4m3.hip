@@ -229,7 +229,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   const bool vec = a.N % 8 == 0;
   const int cnt = a.N - n;  // columns that are there (<= 0: none)
   constexpr int PASSES = 32 * PER_ROW / 64, ROWS = 64 / PER_ROW;
-#pragma unroll
+#pragma unroll 1
   for (int j = 0; j < FM; ++j) {
     const int64_t mj = m0 + wm * WM + 32 * j + lane / PER_ROW;
     Eight<T> res[PASSES];
@@ -240,29 +240,38 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
           load_some(res[r], static_cast<const T*>(a.r) + (mj + r * ROWS) * a.N + n, vec, cnt);
     }
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+    for (int jj = 0; jj < FM; ++jj)
+      if (jj == j) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<float4*>(out + l32 * OP + 32 * i + 8 * q + 4 * g) =
-            make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(out + l32 * OP + 32 * i + 8 * q + 4 * g) =
+                make_float4(acc[i][jj][4 * q], acc[i][jj][4 * q + 1], acc[i][jj][4 * q + 2], acc[i][jj][4 * q + 3]);
+      }
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();
+    float v[8 * PASSES];
 #pragma unroll
     for (int r = 0; r < PASSES; ++r) {
       const int row = r * ROWS + lane / PER_ROW;
       const float by = xs[wm * WM + 32 * j + row];
-      float v[8];
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(out + row * OP + cn);
-      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(out + row * OP + cn + 4);
+      float* u = v + 8 * r;
+      *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(out + row * OP + cn);
+      *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(out + row * OP + cn + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaf(v[e] * by, ws[e], bias[e]);
-      activate(v, a.act, a.alpha);
+      for (int e = 0; e < 8; ++e) u[e] = fmaf(u[e] * by, ws[e], bias[e]);
+    }
+    activate(v, a.act, a.alpha);
+#pragma unroll
+    for (int r = 0; r < PASSES; ++r) {
+      float* u = v + 8 * r;
       if (a.r) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += res[r][e];
+        for (int e = 0; e < 8; ++e) u[e] += res[r][e];
       }
       if (mj + r * ROWS < a.M && cnt > 0)
-        store_some(static_cast<T*>(a.y) + (mj + r * ROWS) * a.N + n, v, vec, cnt);
+        store_some(static_cast<T*>(a.y) + (mj + r * ROWS) * a.N + n, u, vec, cnt);
     }
     wait_lgkmcnt0();
     __builtin_amdgcn_wave_barrier();
