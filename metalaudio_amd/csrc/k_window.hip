@@ -49,7 +49,7 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // block is computed the next one's rows are on their way to registers.
 //
 // Bound by the vector units' issue beside the matrix instructions: 16384 tokens, 1023 back, 8 / 2 heads of 64 in bf16
-// 54 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 24.7 us (split of K, V and P).
+// 53 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 24.4 us (split of K, V and P).
 //
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
@@ -108,10 +108,13 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
   const T* kb = static_cast<const T*>(a.k) + (int64_t)b * a.S * kvw + kvh * a.hd;
   const T* vb = static_cast<const T*>(a.v) + (int64_t)b * a.S * kvw + kvh * a.hd;
 
+  // last key that query i sees
+  auto behind = [&](int i) { return (int)min((unsigned)i + (unsigned)a.right, (unsigned)len - 1); };
+
   // blocks: those of the sinks before the window's first, then the window's
   const int last = min(q0 + BQ - 1, len - 1);
   const int first_blk = max(0, q0 - a.left) / BKV;
-  const int last_blk = (int)min((int64_t)len - 1, (int64_t)last + a.right) / BKV;
+  const int last_blk = behind(last) / BKV;
   const int sink_blks = (int)min((int64_t)first_blk, ((int64_t)a.sinks + BKV - 1) / BKV);
   const int n = sink_blks + last_blk - first_blk + 1;
   auto block_of = [&](int t) { return t < sink_blks ? t : first_blk + t - sink_blks; };
@@ -130,13 +133,25 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
     }
   };
   // blocks past the last and rows past the last key: the last ones again (the former are not computed, the
-  // latter's scores masked)
+  // latter's scores masked). One block is read from a scalar base at 32-bit offsets (64-bit addresses of each
+  // row: 54.6 -> 53.2 us at 16384 tokens)
+  const unsigned row_bytes = (unsigned)(kvw * sizeof(T));  // BKV of them: below 2^31
   auto fetch = [&](int t) {
+    const int blk0 = block_of(t * KW);
+    const unsigned end = min(BKV, len - 1 - blk0 * BKV) * row_bytes;  // of KW = 1: where the last row begins
+    const char* kt = reinterpret_cast<const char*>(kb + (int64_t)blk0 * BKV * kvw);
+    const char* vt = reinterpret_cast<const char*>(vb + (int64_t)blk0 * BKV * kvw);
     each([&](int i, int j, int row, int c) {
-      const int blk = block_of(KW == 1 ? t : min(t * KW + j, n - 1));
-      const int64_t at = (int64_t)min(blk * BKV + row, len - 1) * kvw + 8 * c;
-      ck[i] = *reinterpret_cast<const Chunk*>(kb + at);
-      cv[i] = *reinterpret_cast<const Chunk*>(vb + at);
+      if constexpr (KW == 1) {
+        const unsigned col = 8 * sizeof(T) * c, at = min(row * row_bytes, end) + col;
+        ck[i] = *reinterpret_cast<const Chunk*>(kt + at);
+        cv[i] = *reinterpret_cast<const Chunk*>(vt + at);
+      } else {
+        const int blk = block_of(min(t * KW + j, n - 1));
+        const int64_t at = (int64_t)min(blk * BKV + row, len - 1) * kvw + 8 * c;
+        ck[i] = *reinterpret_cast<const Chunk*>(kb + at);
+        cv[i] = *reinterpret_cast<const Chunk*>(vb + at);
+      }
     });
   };
   auto parts_of = [&](Chunk x, float by) {
@@ -215,13 +230,14 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
     return u.f;
   };
 
+  const int last_n = behind(qn), last_w = behind(qw);  // of the wave's last and first query
   store();
   for (int t = 0; t * KW < n; ++t) {
     lds_barrier();
     const int k0 = block_of(t * KW + kg) * BKV, k1 = k0 + BKV - 1;
     if ((t + 1) * KW < n) fetch(t + 1);
     // seen by any query of the wave?
-    const bool any = qw <= qn && t * KW + kg < n && k0 <= (int64_t)qn + a.right && (k1 >= qw - a.left || k0 < a.sinks);
+    const bool any = qw <= qn && t * KW + kg < n && k0 <= last_n && (k1 >= qw - a.left || k0 < a.sinks);
     if (any) {
       floatx16 st[NT];
 #pragma unroll
@@ -252,12 +268,12 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
             st[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                 *reinterpret_cast<const bf16x8*>(kf0 + 32 * j * PITCH + 32 * s), qf[s][0], st[j], 0, 0, 0);
       }
-      const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= (int64_t)qw + a.right && k1 < len;
+      const bool whole = (k0 >= qn - a.left || k1 < a.sinks) && k1 <= last_w;
       if (!whole) {
         // a bit a key: keys below hi, and not below lo or below the sinks' end; then two instructions a score
         // that need no lane masks (three comparisons a score: 55.5 -> 54 us; 16384 keys)
         const int first = k0 + 4 * g;  // the lane's: key c below is first + c
-        const int hi = (int)min((int64_t)len - 1, (int64_t)qi + a.right) + 1 - first;
+        const int hi = behind(qi) + 1 - first;
         const int lo = qi - a.left - first, sk = a.sinks - first;
         auto below = [](int n) { return (unsigned)((1ull << min(max(n, 0), 32)) - 1); };  // the first n of 32
 #pragma unroll
