@@ -36,10 +36,11 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 
 // A workgroup takes the keys that BQ queries of one head see, in blocks that lie in LDS, by NW waves: NW / KW
 // groups of 32 queries by KW groups of keys, which take every KW-th block and whose results are joined at the
-// end (KW > 1 for grids that would leave most of the GPU idle: then each of a few waves a
-// compute unit waits for its next block for longer than it computes). Each wave computes the TRANSPOSED scores S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q):
-// keys 8 (v / 4) + 4 g + v % 4 of query q) is the B operand that O^T += V^T P^T needs when its k slots take
-// those keys, so P goes from the softmax straight into the second product. K and V lie in LDS row by row as
+// end (KW > 1 for grids that would leave most of the GPU idle: then each of a few waves a compute unit waits for
+// its next block for longer than it computes). Each wave computes the TRANSPOSED scores S^T = K Q^T on
+// v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q): keys 8 (v / 4) + 4 g + v % 4 of query q) is the B operand
+// that O^T += V^T P^T needs when its k slots take those keys, so P goes from the softmax straight into the second
+// product. K and V lie in LDS row by row as
 // they come; V^T's fragments (4 keys of one dimension a lane) are transposed on the way out by
 // ds_read_b64_tr_b16. f32 values are three bf16 parts each and six partial products are kept (x3.hpp); the
 // workgroup splits a block of K and V as it stores it.
@@ -49,14 +50,14 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // block is computed the next one's rows are on their way to registers.
 //
 // Bound by the vector units' issue beside the matrix instructions: 16384 tokens, 1023 back, 8 / 2 heads of 64 in bf16
-// 53 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 24.4 us (split of K, V and P).
+// 52 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 19.9 us (split of K, V and P).
 //
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
 // A key that a query does not see has probability 0, but 0 times a value that is not finite is NaN, and
 // parts of tiny or overflowing f32 values are off: queries whose result is not finite (or, in f32, below
 // 2^-109) are computed again by window_query.
-template <class T, int KS, int KW>
+template <class T, int KS, int KW, int NW>
 struct WindowCfg {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int PARTS = F32 ? 3 : 1;
@@ -67,7 +68,7 @@ struct WindowCfg {
   static constexpr int PITCH = KS * 32 + (KS % 2 ? 0 : 16);
   static constexpr int PLANE = BKV * PITCH;
   static constexpr int CHUNKS = BKV * KS * 2;  // of 8 values, in a block of K or V
-  static constexpr int NW = KW == 1 ? 4 : 8, THREADS = 64 * NW, BQ = 32 * NW / KW;
+  static constexpr int THREADS = 64 * NW, BQ = 32 * NW / KW;
   static constexpr int PER = (KW * CHUNKS + THREADS - 1) / THREADS;
   // K planes, then V planes, of KW blocks; V's fragments of the last 32 dimensions may reach 32 bytes past
   // its rows. At the end, the other key groups' results: maximum, sum and O^T of each lane
@@ -80,9 +81,9 @@ struct WindowCfg {
                                     : (KS > 6 ? 2 : KS > 4 ? 3 : 4);
 };
 
-template <class T, int KS, int KW>
-__global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, KW>::OCC)) void window_kernel(WindowArgs a) {
-  using Cfg = WindowCfg<T, KS, KW>;
+template <class T, int KS, int KW, int NW>
+__global__ __launch_bounds__((WindowCfg<T, KS, KW, NW>::THREADS), (WindowCfg<T, KS, KW, NW>::OCC)) void window_kernel(WindowArgs a) {
+  using Cfg = WindowCfg<T, KS, KW, NW>;
   constexpr int PARTS = Cfg::PARTS, BKV = Cfg::BKV, NT = Cfg::NT, DT = Cfg::DT, PITCH = Cfg::PITCH;
   constexpr int PLANE = Cfg::PLANE, PER = Cfg::PER, SLOT = Cfg::SLOT, BQ = Cfg::BQ;
   constexpr int THREADS = Cfg::THREADS;
@@ -417,13 +418,13 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW>::THREADS), (WindowCfg<T, KS, 
   }
 }
 
-template <class T, int KS, int KW>
+template <class T, int KS, int KW, int NW>
 void launch_window_kw(const LaunchCtx& c, const WindowArgs& a) {
-  using Cfg = WindowCfg<T, KS, KW>;
+  using Cfg = WindowCfg<T, KS, KW, NW>;
   const int64_t units = (int64_t)cdiv(a.S, Cfg::BQ) * a.H * a.B;
   MNN_REQUIRE(units < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
               "WindowAttention: too many tokens in one call");
-  launch(c, sizeof(T) == 4 ? "window_f32" : "window_bf16", window_kernel<T, KS, KW>, dim3((unsigned)units),
+  launch(c, sizeof(T) == 4 ? "window_f32" : "window_bf16", window_kernel<T, KS, KW, NW>, dim3((unsigned)units),
          dim3(Cfg::THREADS), 0, a);
 }
 
@@ -434,15 +435,20 @@ void launch_window(const LaunchCtx& c, const WindowArgs& a) {
   // 48; 4096, 2047 back (256): 111 / 88 / 98; 4 x 1344 (352): 45 / 49 / 50. bf16 hd 64 the same: 17 / 14 / 10,
   // 26 / 21 / 25, 42 / 33 / 41, 21 / 20 / 27; 16384, 1023 back (1024): 58 / 61 / 116. f32 hd 128 has registers
   // for one wave a SIMD with KW = 1: 16384, 1023 back 534 / 430.
+  // Where workgroups of 96 queries, 4 key groups, 12 waves fit the compute units at once, each has a quarter less to do and a
+  // third wave a SIMD: 2 x 1344, 168 both ways, f32 hd 48 24.7 -> 20.8, hd 64 28.2 -> 24.5; 3008, 2047 back, f32 hd 64
+  // 88 -> 70, bf16 31.6 -> 25.5 (2 x 1344, 168 both ways 13.0 -> 13.1); in two rounds they lose (bf16 hd 64, 4 x 1344 17 -> 25).
   const int64_t wgs = (int64_t)cdiv(a.S, 128) * a.H * a.B, cus = c.dev->props.multiProcessorCount;
   const int64_t keys = std::min<int64_t>(a.S, (int64_t)128 + a.left + a.right + a.sinks);
   constexpr bool F32 = sizeof(T) == 4, FOUR = KS <= 5 || !F32;  // four blocks fit in LDS
-  if (keys > 2 * WindowCfg<T, KS, 1>::BKV) {
+  if (keys > 2 * WindowCfg<T, KS, 1, 4>::BKV) {
     if constexpr (FOUR)
-      if (2 * wgs < cus) return launch_window_kw<T, KS, 4>(c, a);
-    if (4 * wgs < 5 * cus || (F32 && KS > 6)) return launch_window_kw<T, KS, 2>(c, a);
+      if (2 * wgs < cus) return launch_window_kw<T, KS, 4, 8>(c, a);
+    if constexpr (KS <= 4)
+      if ((int64_t)cdiv(a.S, 96) * a.H * a.B <= cus) return launch_window_kw<T, KS, 4, 12>(c, a);
+    if (4 * wgs < 5 * cus || (F32 && KS > 6)) return launch_window_kw<T, KS, 2, 8>(c, a);
   }
-  launch_window_kw<T, KS, 1>(c, a);
+  launch_window_kw<T, KS, 1, 4>(c, a);
 }
 
 template <class T>

@@ -467,6 +467,21 @@ def test_window_attention_padded_batch(dev, stream, lengths, S, left, right, sin
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("S,H,KV,hd,left,right,sinks,lengths", [
+    (1345, 8, 8, 48, 168, 168, 4, [1345, 700]), (1101, 10, 5, 32, 300, 0, 45, [33, 1100]),
+    (1057, 8, 2, 64, 500, 2, 97, [1057, 961]), (1025, 9, 3, 40, 31, 64, 1, [1024, 0])])
+def test_window_attention_in_one_round(dev, stream, S, H, KV, hd, left, right, sinks, lengths, dtype):
+    """Two ragged sequences whose workgroups of 96 queries just fit the compute units, NaN behind their ends."""
+    say(f"window in one round {S} heads {H}/{KV} hd {hd} {dtype}")
+    rng = np.random.default_rng(25)
+    q, k, v = (rng.standard_normal((2, S, w * hd)).astype(np.float32) for w in (H, KV, KV))
+    for b, n in enumerate(lengths):
+        for x in (q, k, v):
+            x[b, n:] = np.nan
+    window_case(dev, stream, 2, S, H, KV, hd, left, right, sinks, dtype, lengths, q=q, k=k, v=v)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("what", ["k", "v"])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, 3e38])
 def test_window_attention_values_out_of_sight(dev, stream, what, bad, dtype):
