@@ -19,25 +19,35 @@ __device__ __forceinline__ void turn_of(int pos, double rate, float& cs, float& 
   sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
 }
 
+// i / d with by = floor(2^32 / d): the high product is the quotient or one less, for any i below 2^32.
+struct Divisor {
+  unsigned d, by;
+};
+__device__ __forceinline__ int quotient(int i, Divisor v) {
+  const unsigned q = __umulhi((unsigned)i, v.by);
+  return (int)(q + ((unsigned)i - q * v.d >= v.d));
+}
+
 // A workgroup takes `toks` tokens: first their sines and cosines, once for all heads of both tensors, into
 // LDS, then the rows. A thread's unit is VE pairs: VE values and their VE partners half an axis away, or 2 VE
 // values in a row where pairs are interleaved; 2 VE values (one, for VE = 1) behind the last axis pass. VE = 8
 // or 4 makes them 16-byte accesses of f32 and 16 or 8 of bf16, where every axis is a whole number of units.
 // Both partners are read before either is written, so the output may be the input. Bound by memory: 4 x 2688 tokens
-// of 8 + 8 heads of 48 in bf16 (33 MB) 9.4 us (20 us with the sines taken again for each head).
+// of 8 + 8 heads of 48 in bf16 (33 MB) 8.3 us (9.4 with divisions in place of quotient(), 20 with the sines taken again for
+// each head; four units a thread read ahead of the sines are no faster).
 template <class T, int VE, bool INTER>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int toks) {
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int toks, Divisor tok_units,
+                                                     Divisor head_units, Divisor tok_pairs) {
   extern __shared__ float2 turns[];  // [toks][pairs]
   constexpr int RU = VE == 1 ? 1 : 2 * VE;
   typedef T Part __attribute__((ext_vector_type(VE)));
-  const int turning = a.pairs / VE, units = turning + (a.hd - 2 * a.pairs) / RU;  // of one head
-  const int heads = a.heads[0] + a.heads[1], per_tok = units * heads;
+  const int turning = a.pairs / VE, units = (int)head_units.d, per_tok = (int)tok_units.d;  // of a head, a token
   const int64_t total = a.B * a.S;
   for (int64_t tok0 = (int64_t)blockIdx.x * toks; tok0 < total; tok0 += (int64_t)gridDim.x * toks) {
     const int n = (int)min((int64_t)toks, total - tok0);
     for (int i = threadIdx.x; i < n * a.pairs; i += 256) {
-      const int u = i % a.pairs;
-      const int64_t tok = tok0 + i / a.pairs;
+      const int ti = quotient(i, tok_pairs), u = i - ti * a.pairs;
+      const int64_t tok = tok0 + ti;
       int axis = 0, j = u;
       while (j >= a.dims[axis] / 2) j -= a.dims[axis++] / 2;  // ends: u is one of the axes' pairs
       float2 t;
@@ -46,8 +56,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int toks) {
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n * per_tok; i += 256) {
-      const int ti = i / per_tok, rest = i - ti * per_tok;
-      int h = rest / units;
+      const int ti = quotient(i, tok_units), rest = i - ti * per_tok;
+      int h = quotient(rest, head_units);
       const int u = rest - h * units, which = h >= a.heads[0];
       if (which) h -= a.heads[0];
       const int64_t at = ((tok0 + ti) * (which ? a.heads[1] : a.heads[0]) + h) * a.hd;
@@ -119,8 +129,8 @@ bool whole_units(const RotaryArgs& a, int VE) {
 
 template <class T, int VE>
 void launch_rotary(const LaunchCtx& c, const RotaryArgs& a) {
-  const int heads = a.heads[0] + a.heads[1];
-  const int64_t units = (int64_t)heads * (a.pairs / VE + (a.hd - 2 * a.pairs) / (VE == 1 ? 1 : 2 * VE));
+  const int heads = a.heads[0] + a.heads[1], of_head = a.pairs / VE + (a.hd - 2 * a.pairs) / (VE == 1 ? 1 : 2 * VE);
+  const int64_t units = (int64_t)heads * of_head;
   // tokens a workgroup: four units a thread, as few as the compute units still have work for, and as the
   // table of turns has room for (16 KB)
   const int64_t tokens = a.B * a.S, cus = c.dev->props.multiProcessorCount;
@@ -129,10 +139,11 @@ void launch_rotary(const LaunchCtx& c, const RotaryArgs& a) {
   const dim3 grid((unsigned)std::min<int64_t>((tokens + toks - 1) / toks, 1 << 20));
   const char* name = sizeof(T) == 4 ? "rotary_f32" : "rotary_bf16";
   const size_t lds = sizeof(float2) * toks * a.pairs;
+  auto by = [](int64_t d) { return Divisor{(unsigned)d, d == 1 ? ~0u : (unsigned)((1ull << 32) / d)}; };
   if (a.interleaved)
-    launch(c, name, rotary_kernel<T, VE, true>, grid, dim3(256), lds, a, (int)toks);
+    launch(c, name, rotary_kernel<T, VE, true>, grid, dim3(256), lds, a, (int)toks, by(units), by(of_head), by(a.pairs));
   else
-    launch(c, name, rotary_kernel<T, VE, false>, grid, dim3(256), lds, a, (int)toks);
+    launch(c, name, rotary_kernel<T, VE, false>, grid, dim3(256), lds, a, (int)toks, by(units), by(of_head), by(a.pairs));
 }
 template <class T>
 void rotary_t(const LaunchCtx& c, const RotaryArgs& a) {
