@@ -223,7 +223,7 @@ mnn_status mnn_linear_forward_scaled(mnn_layer layer, mnn_tensor input, mnn_tens
                                      mnn_tensor residual, mnn_tensor output, mnn_stream s);
 
 /* RMSNorm over the last dimension, beside LayerNorm (no counterpart in the reference): y = x *
- * rsqrt(mean(x^2) + epsilon) * weight. Parameter "weight"/"gamma" [F], 1 until loaded. mnn_layer_forward
+ * rsqrt(mean(x^2) + epsilon) * weight. Parameter "weight"/"gamma" [F], F <= 2^30, 1 until loaded. mnn_layer_forward
  * takes f32 or bf16 input and writes f32. */
 mnn_status mnn_rmsnorm_create(mnn_device dev, int feature_size, float epsilon, mnn_layer* out);
 /* The same with the residual's addition before it and an output of 16 or 8 bits: h = input + residual

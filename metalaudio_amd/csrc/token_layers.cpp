@@ -70,7 +70,8 @@ void split_heads(const char* what, const Shape& s, int64_t hd, int64_t& B, int64
 class RMSNormLayer : public Layer {
  public:
   RMSNormLayer(Device* d, int features, float eps) : Layer(d), F_(features), eps_(eps) {
-    MNN_REQUIRE(features > 0, MNN_ERR_INVALID_CONFIGURATION, "RMSNorm: featureSize <= 0");
+    MNN_REQUIRE(features > 0 && features <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
+                "RMSNorm: featureSize must be 1..2^30");
     MNN_REQUIRE(std::isfinite(eps) && eps >= 0.f, MNN_ERR_INVALID_CONFIGURATION,
                 "RMSNorm: epsilon must be finite and not negative");
     w_ = &add_param("weight", features, 1.f);

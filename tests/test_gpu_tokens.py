@@ -333,6 +333,12 @@ def test_linear_e4m3_refusals(dev, stream):
     f(T((0, 64), "e4m3"), T((0,)), T((0, 32)), stream=stream)
 
 
+def test_rmsnorm_refuses_more_features_than_its_indices_hold(dev):
+    say("rmsnorm features")
+    for n in (2 ** 30 + 1, 2 ** 31 - 1, -1):
+        refuses("MNN_ERR_INVALID_CONFIGURATION", lambda: nn.RMSNorm(dev, n))
+
+
 # ------------------------------------------------------------------------------ rotary positions
 @pytest.mark.parametrize("B,S,H,KV,hd,dims,inter,dtype", [
     (1, 1, 1, 1, 2, (2,), False, "f32"), (8, 1, 8, 8, 64, (32, 16), False, "f32"),
@@ -366,6 +372,24 @@ def test_rotary(dev, stream, B, S, H, KV, hd, dims, inter, dtype, in_place):
         check(got.to_numpy(), want, tol + HALF[dtype] * np.abs(want) * (dtype != "f32"), "turned")
         rest = sum(dims)  # passes unchanged
         np.testing.assert_array_equal(got.to_numpy().reshape(-1, hd)[:, rest:], x.reshape(-1, hd)[:, rest:])
+
+
+@pytest.mark.parametrize("H,hd,dims,inter,dtype", [
+    (9, 4096, (4096,), False, "f32"), (33, 4096, (2048, 2, 6), True, "bf16"), (1001, 6, (2, 2), False, "bf16"),
+    (700, 64, (16, 48), False, "f32")])
+def test_rotary_wide_tokens(dev, stream, H, hd, dims, inter, dtype):
+    """More units a token than a workgroup takes at a time."""
+    say(f"rotary {H} heads of {hd} {dims} {dtype}")
+    rng = np.random.default_rng(H)
+    q = rounded(rng.standard_normal((1, 5, H * hd)), dtype)
+    pos = rng.integers(0, 900, (5, len(dims))).astype(np.int32)
+    layer = nn.Rotary(dev, hd, dims, interleaved=inter)
+    qo = nn.Tensor(dev, q.shape, dtype=dtype)
+    layer.forward(tensor(dev, q, dtype), None, tensor(dev, pos, "i32"), qo, None, stream)
+    stream.sync(60000)
+    want = rotary(q, pos, H, hd, dims, 10000.0, inter)
+    big = np.abs(q.reshape(1, 5, H, hd)).max(-1, keepdims=True).repeat(hd, -1).reshape(q.shape)
+    check(qo.to_numpy(), want, big * 32 * EPS + HALF[dtype] * np.abs(want) * (dtype != "f32"), "turned")
 
 
 def test_rotary_q_alone_and_scores_of_shifted_tokens(dev, stream):
