@@ -240,6 +240,14 @@ def test_linear_e4m3(dev, stream, M, K, N, kw):
     linear_case(dev, stream, M, K, N, **kw)
 
 
+@pytest.mark.parametrize("M,K,N", [(3001, 256, 1240), (3007, 640, 1237), (2100, 256, 2056), (2099, 130, 2055)])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_linear_e4m3_middle_sizes(dev, stream, M, K, N, out):
+    """Between the square tiles' sizes, rows and columns that no tile divides, the residual in place."""
+    say(f"linear e4m3 middle {M}x{K}x{N} {out}")
+    linear_case(dev, stream, M, K, N, act="swish", residual=True, out=out, in_place=True)
+
+
 @pytest.mark.parametrize("M,K,N,inp,out", [(1, 384, 96, "f32", "f32"), (9, 257, 64, "bf16", "bf16"),
                                            (300, 512, 300, "bf16", "f32"), (45, 1000, 33, "f32", "bf16")])
 def test_linear_e4m3_rounds_wider_input(dev, stream, M, K, N, inp, out):
