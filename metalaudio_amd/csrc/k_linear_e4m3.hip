@@ -117,15 +117,16 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 
 // BM x BN results a workgroup, WM x WN a wave, the depth 128 at a time through a ring of S slots in LDS,
 // which global_load_lds fills: the rows of x, then those of w, 128 bytes each, 16-byte chunk c of row r in
-// place c ^ (r % 8), so that fragment reads of 32 rows spread over the banks. One barrier a step: behind it,
+// place c ^ (r / 2 % 8), so that 16 rows' reads are spread over all 64 banks (c ^ (r % 8) for rows 8 apart in the same
+// ones). One barrier a step: behind it,
 // the step's slot is whole and the one before it free to be filled again.
 //
 // Rows behind the last are read as the last one; their results are not stored. The results go through LDS
 // once more (the ring is done with), so that scales, residual and output are read and written row by row.
 //
 // Bound by the matrix instructions and, in a grid of one or two rounds, by each round's first loads and results
-// (about 18 us at 256 x 256, 1.39 us a step of 128): 8192 x 4096 x 4096 to bf16 125 us (2.2 PFLOP/s), 10752 x 1536 x 384 to
-// f32 with residual 20 us.
+// (about 18 us at 256 x 256): 8192 x 4096 x 4096 to bf16 118 us (2.3 PFLOP/s), 8192 x 8192 x 8192 423 us (2.6), 10752 x
+// 1536 x 384 to f32 with residual 19 us. w's fragments straight to registers instead, a step ahead, are no faster.
 template <class T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
@@ -151,7 +152,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   const int n0 = in / gm * BN;
 
   // load i of this wave: rows 8 j .. + 7 of the slot, j = i NW + wave; the first BM rows are x's
-  const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
+  static_assert(NW % 2 == 0, "j is odd for odd waves");
+  const int row_in = lane >> 3, chunk = (lane & 7) ^ (4 * (wave & 1) + (row_in >> 1));
   const char* src[LOADS];  // wave-uniform bases
   unsigned off[LOADS];
 #pragma unroll
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   columns<8>(a, n, ws, bias);
   for (int i = threadIdx.x; i < BM; i += NW * 64) xs[i] = a.xs[min(m0 + i, a.M - 1)];
   // chunk c of a row that is l32 modulo 32
-  auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 & 7)) << 4); };
+  auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 >> 1 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
   int slot = 0;
   for (int k = 0; k < nk; ++k) {
@@ -366,7 +368,7 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   if (a.M <= kLinearFew)
     return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
                   dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
-  // The largest tile that still gives most compute units one: us at (M, K, N), 256 / 128 / 64 square:
+  // The largest tile that still gives most compute units one: us at (M, K, N), 256 / 128 / 64 square as first built:
   // 8192 x 4096 x 4096 bf16 132 / 147 / 208, 10752 x 384 x 1536 bf16 18.6 / 21.7 / 23.7, 10752 x 1536 x 384
   // f32 42 / 22.0 / 21.6, 2688 x 384 x 1152 bf16 14.5 / 8.7 / 6.9, 200 x 1536 x 384 f32 37 / 16.6 / 8.0.
   const int cus = c.dev->props.multiProcessorCount;
