@@ -502,9 +502,9 @@ def test_window_attention_padded_batch(dev, stream, lengths, S, left, right, sin
 @pytest.mark.parametrize("S,H,KV,hd,left,right,sinks,lengths", [
     (1345, 8, 8, 48, 168, 168, 4, [1345, 700]), (1101, 10, 5, 32, 300, 0, 45, [33, 1100]),
     (1057, 8, 2, 64, 500, 2, 97, [1057, 961]), (1025, 9, 3, 40, 31, 64, 1, [1024, 0])])
-def test_window_attention_in_one_round(dev, stream, S, H, KV, hd, left, right, sinks, lengths, dtype):
+def test_window_attention_groups_of_96(dev, stream, S, H, KV, hd, left, right, sinks, lengths, dtype):
     """Two ragged sequences whose workgroups of 96 queries just fit the compute units, NaN behind their ends."""
-    say(f"window in one round {S} heads {H}/{KV} hd {hd} {dtype}")
+    say(f"window groups of 96 {S} heads {H}/{KV} hd {hd} {dtype}")
     rng = np.random.default_rng(25)
     q, k, v = (rng.standard_normal((2, S, w * hd)).astype(np.float32) for w in (H, KV, KV))
     for b, n in enumerate(lengths):
