@@ -1,12 +1,11 @@
 // The 8-bit linear product: y[m][n] = act(xs[m] ws[n] sum_k x[m][k] w[n][k] + bias[n]) + r[m][n], x and w
 // in e4m3.
 //
-// Which matrix instructions: those on 8-bit operands (v_mfma_f32_*_f8f6f4, 4.2 PFLOP/s here) add the
-// products of a group of lanes' bytes to about 14 bits below the largest one: a sum of 128 random
-// products is 1.3e-5 off (2-norm), whichever of them is taken. bf16 output, whose rounding is a hundred
-// times that (2^-9), is made with them. fp32 output is not: e4m3 values are bf16 values, so both operands
-// are widened (v_cvt_scalef32_pk_bf16_fp8, two values an instruction) and multiplied by the bf16
-// instructions (2.2 PFLOP/s), 9e-9 off on the same sums.
+// Which matrix instructions: e4m3 values are bf16 values, so both operands are widened
+// (v_cvt_scalef32_pk_bf16_fp8, two values an instruction) and multiplied by the bf16 instructions (2.2 PFLOP/s), whose
+// sums are fp32 sums: 9e-9 off (2-norm) over 128 random products. Those on 8-bit operands (v_mfma_f32_*_f8f6f4, 4.2
+// PFLOP/s here) add a group's products to about 14 bits below the largest one, 1.3e-5 off on the same sums, and lose
+// whatever is smaller where large products cancel: no rounding of the result hides that.
 #include "lds_dma.hpp"
 #include "token_ops.hpp"
 #include "token_utils.hpp"
@@ -21,7 +20,6 @@ using namespace dev;
 
 namespace {
 
-typedef int intx8 __attribute__((ext_vector_type(8)));
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
 // Eight e4m3 values to bf16, exactly.
@@ -36,17 +34,7 @@ __device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
 
 // 64 products a row: lane (g, r) holds 32 bytes of row r of both operands (which k they are does not matter
 // as long as both sides agree). The result: b's row l % 32, a's rows 8 (v / 4) + 4 (l / 32) + v % 4.
-template <class T>
-struct Operand;  // 32 bytes of a row as the products of T's output take them
-template <>
-struct Operand<__bf16> {
-  intx8 x;
-  __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
-    x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-};
-template <>
-struct Operand<float> {
+struct Operand {
   bf16x8 x[4];
   __device__ __forceinline__ void set(intx4 lo, intx4 hi) {
     x[0] = widen8(lo[0], lo[1]);
@@ -55,10 +43,7 @@ struct Operand<float> {
     x[3] = widen8(hi[2], hi[3]);
   }
 };
-__device__ __forceinline__ floatx16 mul(const Operand<__bf16>& a, const Operand<__bf16>& b, floatx16 c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.x, b.x, c, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ floatx16 mul(const Operand<float>& a, const Operand<float>& b, floatx16 c) {
+__device__ __forceinline__ floatx16 mul(const Operand& a, const Operand& b, floatx16 c) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.x[i], b.x[i], c, 0, 0, 0);
   return c;
@@ -124,9 +109,10 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 // Rows behind the last are read as the last one; their results are not stored. The results go through LDS
 // once more (the ring is done with), so that scales, residual and output are read and written row by row.
 //
-// Bound by the matrix instructions and, in a grid of one or two rounds, by each round's first loads and results
-// (about 18 us at 256 x 256): 8192 x 4096 x 4096 to bf16 118 us (2.3 PFLOP/s), 8192 x 8192 x 8192 423 us (2.6), 10752 x
-// 1536 x 384 to f32 with residual 19 us. w's fragments straight to registers instead, a step ahead, are no faster.
+// Bound by the matrix instructions beside the widening and, in a grid of one or two rounds, by each round's first
+// loads and results: 8192 x 4096 x 4096 to bf16 200 us (1.4 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
+// 1536 x 384 to f32 with residual 19 us. The widening spread between the products by hand changes nothing, nor do
+// waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
 template <class T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
@@ -207,7 +193,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int c0 = at(4 * s + 2 * g), c1 = at(4 * s + 2 * g + 1);
-      Operand<T> x[FM], w[FN];
+      Operand x[FM], w[FN];
 #pragma unroll
       for (int j = 0; j < FM; ++j)
         x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
@@ -297,7 +283,7 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
   for (int v = 0; v < 16; ++v) acc[v] = 0.f;
   auto step = [&](int s, auto whole) {
     const intx4* q = reinterpret_cast<const intx4*>(w + 64 * s);
-    Operand<T> xo, wo;
+    Operand xo, wo;
     wo.set(q[0], q[1]);
     intx4 lo = 0, hi = 0;
     if (decltype(whole)::value || 64 * s + 32 * g + 32 <= a.ldx) {
@@ -368,19 +354,18 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   if (a.M <= kLinearFew)
     return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
                   dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
-  // The largest tile that still gives most compute units one: us at (M, K, N), 256 / 128 / 64 square as first built:
-  // 8192 x 4096 x 4096 bf16 132 / 147 / 208, 10752 x 384 x 1536 bf16 18.6 / 21.7 / 23.7, 10752 x 1536 x 384
-  // f32 42 / 22.0 / 21.6, 2688 x 384 x 1152 bf16 14.5 / 8.7 / 6.9, 200 x 1536 x 384 f32 37 / 16.6 / 8.0.
-  const int cus = c.dev->props.multiProcessorCount;
+  // 256 square where the rounds of one tile a compute unit are 7/8 full: a third less widening a product, but one
+  // workgroup a compute unit, whose last round costs a whole one. us at (M, K, N), 256 / 128 / 64 square: 8192 x 4096 x
+  // 4096 bf16 203 / 227 / 281, f32 215 / 235 / 285; 10752 x 384 x 1536 bf16 (252 tiles) 19.2 / 20.2 / 23.6; 8192 x
+  // 1024 x 1536 bf16 (192 tiles) 32 / 29 / 35; 12800 x 1024 x 1536 bf16 (300 tiles) 58 / 44 / 52.
+  const int64_t cus = c.dev->props.multiProcessorCount;
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
-  if (4 * tiles(256) >= 3 * cus)
+  if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
     return launch_tile<T, 256, 256, 128, 64, 2>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
-  if (tiles(128) >= cus)
-    return launch_tile<T, 128, 128, 64, 64, 2>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
-  // 128 x 64 once nearly two a compute unit run: 10752 x 1536 x 384 f32 21.9 -> 20.4, bf16 16.5 -> 14.1; at one and a half they
-  // lose, 2688 x 384 x 1152 bf16 6.7 -> 7.4
-  if (4 * ((a.M + 127) / 128 * ((a.N + 63) / 64)) >= 7 * cus)
-    return launch_tile<T, 128, 64, 64, 32, 2>(c, a, F32 ? "linear_e4m3_128x64_f32" : "linear_e4m3_128x64_bf16");
+  // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
+  // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9
+  if (4 * tiles(128) >= 3 * cus)
+    return launch_tile<T, 128, 128, 64, 32, 2>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
   launch_tile<T, 64, 64, 32, 32, 2>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
 }
 }  // namespace
