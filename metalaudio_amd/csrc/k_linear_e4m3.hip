@@ -100,27 +100,27 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
   }
 }
 
-// BM x BN results a workgroup, WM x WN a wave, the depth 128 at a time through a ring of S slots in LDS,
+// BM x BN results a workgroup, WM x WN a wave, the depth 128 at a time through two slots in LDS,
 // which global_load_lds fills: the rows of x, then those of w, 128 bytes each, 16-byte chunk c of row r in
 // place c ^ (r / 2 % 8), so that 16 rows' reads are spread over all 64 banks (c ^ (r % 8) for rows 8 apart in the same
 // ones). One barrier a step: behind it,
-// the step's slot is whole and the one before it free to be filled again.
+// the step's slot is whole and the other one free to be filled again.
 //
 // Rows behind the last are read as the last one; their results are not stored. The results go through LDS
-// once more (the ring is done with), so that scales, residual and output are read and written row by row.
+// once more (the slots are done with), so that scales, residual and output are read and written row by row.
 //
 // Bound by the matrix instructions beside the widening and, in a grid of one or two rounds, by each round's first
 // loads and results: 8192 x 4096 x 4096 to bf16 200 us (1.4 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
 // 1536 x 384 to f32 with residual 19 us. The widening spread between the products by hand changes nothing, nor do
 // waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
-template <class T, int BM, int BN, int WM, int WN, int S>
+template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
   constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;
   static_assert(SLOT % (1024 * NW) == 0, "whole loads a wave");
   constexpr int FM = WM / 32, FN = WN / 32;
   constexpr int OP = WN + 4;  // floats a row of the results in LDS
-  constexpr int BYTES = S * SLOT > NW * 32 * OP * 4 ? S * SLOT : NW * 32 * OP * 4;
+  constexpr int BYTES = 2 * SLOT > NW * 32 * OP * 4 ? 2 * SLOT : NW * 32 * OP * 4;
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
   __shared__ float xs[BM];
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31;
@@ -168,9 +168,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
 
   const int nk = a.K / 128;
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s)
-    if (s < nk) issue(s, s);
+  issue(0, 0);
   // what the results need besides: this lane's columns and the tile's row scales
   constexpr int PER_ROW = WN / 8;  // lanes
   const int cn = 8 * (lane % PER_ROW), n = n0 + wn * WN + cn;
@@ -181,14 +179,11 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 >> 1 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
   int slot = 0;
-  for (int k = 0; k < nk; ++k) {
+  for (int k = 0; k < nk; ++k, slot ^= 1) {
     wait_lgkmcnt0();
-    if (S > 2 && k + S - 2 < nk)
-      wait_vmcnt<(S - 2) * LOADS>();
-    else
-      wait_vmcnt<0>();
+    wait_vmcnt<0>();
     stage_barrier();
-    if (k + S - 1 < nk) issue(k + S - 1, slot == 0 ? S - 1 : slot - 1);
+    if (k + 1 < nk) issue(k + 1, slot ^ 1);
     const char* p = smem + slot * SLOT;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -207,7 +202,6 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = mul(w[i], x[j], acc[i][j]);
     }
-    slot = slot + 1 == S ? 0 : slot + 1;
   }
 
   // 32 rows of results at a time, through a part of LDS that is this wave's; the residual's rows are on
@@ -338,12 +332,12 @@ void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint
 }
 
 namespace {
-template <class T, int BM, int BN, int WM, int WN, int S>
+template <class T, int BM, int BN, int WM, int WN>
 void launch_tile(const LaunchCtx& c, const LinearE4m3Args& a, const char* name) {
   const int64_t tiles = (a.M + BM - 1) / BM * ((a.N + BN - 1) / BN);
   MNN_REQUIRE(tiles < (1 << 22), MNN_ERR_INVALID_CONFIGURATION, "Linear: too many rows in one call");
   constexpr int threads = BM / WM * (BN / WN) * 64;
-  launch(c, name, linear_e4m3_kernel<T, BM, BN, WM, WN, S>, dim3((unsigned)tiles), dim3(threads), 0, a);
+  launch(c, name, linear_e4m3_kernel<T, BM, BN, WM, WN>, dim3((unsigned)tiles), dim3(threads), 0, a);
 }
 
 template <class T>
@@ -361,12 +355,12 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   const int64_t cus = c.dev->props.multiProcessorCount;
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
-    return launch_tile<T, 256, 256, 128, 64, 2>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
+    return launch_tile<T, 256, 256, 128, 64>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
   // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
   // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9
   if (4 * tiles(128) >= 3 * cus)
-    return launch_tile<T, 128, 128, 64, 32, 2>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
-  launch_tile<T, 64, 64, 32, 32, 2>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
+    return launch_tile<T, 128, 128, 64, 32>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
+  launch_tile<T, 64, 64, 32, 32>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
 }
 }  // namespace
 
