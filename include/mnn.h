@@ -224,7 +224,8 @@ mnn_status mnn_linear_forward_scaled(mnn_layer layer, mnn_tensor input, mnn_tens
 
 /* RMSNorm over the last dimension, beside LayerNorm (no counterpart in the reference): y = x *
  * rsqrt(mean(x^2) + epsilon) * weight. Parameter "weight"/"gamma" [F], F <= 2^30, 1 until loaded. mnn_layer_forward
- * takes f32 or bf16 input and writes f32. */
+ * takes f32 or bf16 input and writes f32. Finite rows keep their norm whatever their size, also where a
+ * square overflows fp32 or underflows; of a row of zeros with epsilon 0 there is none (NaN). */
 mnn_status mnn_rmsnorm_create(mnn_device dev, int feature_size, float epsilon, mnn_layer* out);
 /* The same with the residual's addition before it and an output of 16 or 8 bits: h = input + residual
  * (residual NULL: h = input), sum = h (sum may be NULL; it may be the input or the residual itself),

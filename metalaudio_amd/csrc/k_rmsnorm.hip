@@ -15,6 +15,15 @@ using namespace dev;
 
 namespace {
 
+// mean(h^2) + eps is used as it came where no square that counts has left fp32's range. Otherwise (finite
+// values above 1.8e19, or, with a small eps, tiny ones) the row's norm is taken of h times a power of two that
+// brings the larger of max|h| and sqrt(eps) to about 1: norm(h) = norm of s h with eps s^2.
+__device__ __forceinline__ bool mean_in_range(float v) { return v > 0x1p-80f && v < INFINITY; }
+__device__ __forceinline__ float unit_scale(float top, float eps) {
+  const int e = __builtin_amdgcn_frexp_expf(fmaxf(top, sqrtf(eps)));
+  return ldexpf(1.f, min(max(-e, -126), 127));
+}
+
 // One value of a row over the whole workgroup of 256.
 template <class F>
 __device__ __forceinline__ float block_reduce(float v, float* sh, F op) {
@@ -37,14 +46,29 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t at = row * a.F;
     auto h = [&](int i) { return to_f32(x[at + i]) + (r ? to_f32(r[at + i]) : 0.f); };
-    float norm = 1.f;
+    float norm = 1.f, s = 1.f;  // s: what h is taken times, see mean_in_range
     if (a.w) {
-      float ss = 0.f;
-      for (int i = threadIdx.x; i < a.F; i += 256) ss = fmaf(h(i), h(i), ss);
-      ss = block_reduce(ss, sh, [](float p, float q) { return p + q; });
-      norm = rsqrtf(ss / (float)a.F + a.eps);
+      auto mean = [&] {
+        float ss = 0.f;
+        for (int i = threadIdx.x; i < a.F; i += 256) {
+          const float hv = h(i) * s;
+          ss = fmaf(hv, hv, ss);
+        }
+        return block_reduce(ss, sh, Plus{}) / (float)a.F + a.eps * s * s;
+      };
+      float m = mean();
+      if (!mean_in_range(m)) {
+        float top = 0.f;
+        for (int i = threadIdx.x; i < a.F; i += 256) top = max_nan(top, fabsf(h(i)));
+        top = block_reduce(top, sh, max_nan);
+        if (top < INFINITY) {
+          s = unit_scale(top, a.eps);
+          m = mean();
+        }
+      }
+      norm = rsqrtf(m);
     }
-    auto y = [&](int i, float hv) { return a.w ? hv * norm * a.w[i] : hv; };
+    auto y = [&](int i, float hv) { return a.w ? hv * s * norm * a.w[i] : hv; };
     RowScale rs{1.f, 1.f};
     if (a.out == MNN_E4M3) {
       float top = 0.f;
@@ -77,16 +101,16 @@ template <class T, int NV, int W, mnn_dtype OUT>
 __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
   constexpr int VE = 16 / (int)sizeof(T);
   typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
-  __shared__ float sh[4][4];
+  __shared__ float sh[8][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = ((W == 1 ? 0 : wave * 64) + lane) * VE;
-  // over the W waves of a row. `at`, 0 or 1, keeps a row's two reductions apart and `parity` one row's from
+  // over the W waves of a row. `at`, 0 to 3, keeps a row's reductions apart and `parity` one row's from
   // the next one's: a wave writes a place again only behind a barrier that is behind the others' reads of it
   int parity = 0;
   auto over_row = [&](float v, int at, auto op) {
     v = group_reduce<64>(v, op);
     if constexpr (W > 1) {
-      float* to = sh[2 * parity + at];
+      float* to = sh[4 * parity + at];
       if (lane == 0) to[wave] = v;
       __syncthreads();
       v = op(op(to[0], to[1]), op(to[2], to[3]));
@@ -152,7 +176,28 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
         }
     }
     if (a.w) {
-      const float norm = rsqrtf(over_row(ss, 0, Plus{}) / (float)a.F + a.eps);
+      float mean = over_row(ss, 0, Plus{}) / (float)a.F + a.eps;
+      if (!mean_in_range(mean)) {  // the same for every lane of the row
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) top = max_nan(top, fabsf(h[i][e]));
+        top = over_row(top, 2, max_nan);
+        if (top < INFINITY) {
+          const float s = unit_scale(top, a.eps);
+          ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              h[i][e] *= s;
+              ss = fmaf(h[i][e], h[i][e], ss);
+            }
+          mean = over_row(ss, 3, Plus{}) / (float)a.F + a.eps * s * s;
+        }
+      }
+      const float norm = rsqrtf(mean);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll

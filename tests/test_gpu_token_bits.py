@@ -6,7 +6,7 @@ import pytest
 
 from metalaudio_amd import nn
 from tests.test_gpu_tokens import linear_case
-from tests.token_refs import EPS, HALF, quantise, rounded
+from tests.token_refs import EPS, HALF, TINY, quantise, rmsnorm, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,58 @@ def test_linear_e4m3_full_rounds(dev, stream, M, K, N, out):
     """Grids that fill the compute units with the largest tile, odd rows and columns, the residual in place."""
     say(f"linear full rounds {M}x{K}x{N} {out}")
     linear_case(dev, stream, M, K, N, act="swish", residual=True, out=out, in_place=True)
+
+
+# ------------------------------------------------------------------------------------- RMS norm
+@pytest.mark.parametrize("F", [8, 384, 1001, 1536, 5000])  # a wave a row, three passes, a workgroup a row
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("eps", [1e-5, 0.0, 1e-30])
+def test_rmsnorm_sizes_whose_squares_leave_fp32(dev, stream, F, dtype, eps):
+    """Finite rows whose squares overflow or underflow, ordinary ones between them."""
+    say(f"rmsnorm sizes {F} {dtype} epsilon {eps}")
+    rng = np.random.default_rng(F)
+    sizes = [1.0, 1e25, 3e37, 1e-25, 1e19, 1e-20, 2.0 ** -120, 1.0, 1e-12, 1e-40]
+    x = rng.standard_normal((len(sizes) + 2, F)).clip(-3, 3)
+    x[:len(sizes)] *= np.array(sizes)[:, None]
+    x[len(sizes)] *= 1e-3
+    x[len(sizes), F // 2] = 1e30  # one large value takes all of the norm
+    x[len(sizes) + 1] *= np.exp2(rng.integers(-60, 60, F))
+    x = rounded(x, dtype)
+    if dtype == "bf16":
+        x[9] = 1  # bf16 rounds the smallest row to few bits, or to zeros
+    w = (1 + 0.2 * rng.standard_normal(F)).astype(np.float32)
+    layer = nn.RMSNorm(dev, F, eps)
+    layer.load_parameters(w)
+    rows = x.shape[0]
+    y32, y8, s8 = nn.Tensor(dev, (rows, F)), nn.Tensor(dev, (rows, F), dtype="e4m3"), nn.Tensor(dev, (rows,))
+    total = nn.Tensor(dev, (rows, F), dtype=dtype)
+    layer.forward_residual(tensor(dev, x, dtype), None, y32, sum=total, stream=stream)
+    layer.forward_residual(tensor(dev, x, dtype), None, y8, scales=s8, stream=stream)
+    stream.sync(60000)
+    np.testing.assert_array_equal(total.to_numpy(), x)
+    want = rmsnorm(x, w, float(np.float32(eps)))
+    # as in test_rmsnorm_residual; a power of two in between rounds nothing
+    rel = (F / 64 + 24) * EPS
+    got = y32.to_numpy().astype(np.float64)
+    err = np.abs(got - want)
+    bad = ~(err <= rel * np.abs(want) + 1.5e-45)  # the smallest results have a step of 2^-149
+    assert not bad.any(), f"rows {sorted(set(np.argwhere(bad)[:, 0]))}: {got[bad][:3]} for {want[bad][:3]}"
+    top = np.maximum(np.abs(want).max(-1), TINY)
+    scales = s8.to_numpy().astype(np.float64)
+    assert (np.abs(scales - top / 448) <= (rel + 4 * EPS) * top / 448).all()
+    unit = np.abs(want) / scales[:, None]
+    step = np.maximum(unit * HALF["e4m3"], 2.0 ** -10) * (1 + 1e-5) + 448 * 2 * rel + unit * 8 * EPS
+    assert (np.abs(y8.to_numpy() * scales[:, None] - want) <= step * scales[:, None]).all()
+
+
+def test_rmsnorm_of_zeros_without_epsilon(dev, stream):
+    """0 / 0, and only in its row."""
+    say("rmsnorm zeros")
+    for F in (96, 1001):
+        x = np.ones((3, F), np.float32)
+        x[1] = 0
+        y = nn.Tensor(dev, (3, F))
+        nn.RMSNorm(dev, F, 0.0).forward_residual(tensor(dev, x, "f32"), None, y, stream=stream)
+        stream.sync(60000)
+        y = y.to_numpy()
+        assert np.isnan(y[1]).all() and (y[[0, 2]] == 1).all()
