@@ -26,6 +26,15 @@ __device__ __forceinline__ int slot_of(const WindowStepArgs& a, int p) {
   return p < a.sinks ? p : a.sinks + (p - a.sinks) % (a.C - a.sinks);
 }
 
+// Keys that tokens pos + t0 .. pos + t1 see, and the position of key `idx` of them: ns sinks, then the tokens from
+// lo on. Positions reach 2^31 - 1, so no sum on the way may pass them: as constant expressions, one that did would
+// not compile.
+constexpr int keys_of(int ns, int pos, int t0, int t1, int lo) { return ns + (pos + t0 - lo) + (t1 - t0) + 1; }
+constexpr int key_at(int ns, int lo, int idx) { return idx < ns ? idx : lo + (idx - ns); }
+static_assert(keys_of(33, INT_MAX - 16, 0, 15, INT_MAX - 616) == 33 + 600 + 16 &&
+                  key_at(33, INT_MAX - 616, 33 + 600 + 15) == INT_MAX - 1,
+              "the farthest call of 16 tokens, 600 back, 33 sinks");
+
 // The rows of a call that one workgroup answers: R of the T * G queries (token t, head g of the group) that
 // read key/value head kvh of stream b, and the keys that any of them sees, numbered from 0: the sinks before
 // the window's first token, then the window.
@@ -47,7 +56,7 @@ __device__ __forceinline__ bool rows_setup(const WindowStepArgs& a, int unit, in
   w.t1 = min(w.nt - 1, (w.row0 + R - 1) / G);
   w.lo = max(0, w.pos + w.t0 - a.left);
   w.ns = min(a.sinks, w.lo);
-  w.n = w.ns + w.pos + w.t1 - w.lo + 1;
+  w.n = keys_of(w.ns, w.pos, w.t0, w.t1, w.lo);
   w.ring = a.C - a.sinks;
   w.wrapped = (max(w.lo, a.sinks) - a.sinks) % w.ring;
   return true;
@@ -162,7 +171,7 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int idx = i + u * KPW + grp;
-      x.p[u] = idx >= end ? -1 : idx < w.ns ? idx : w.lo + idx - w.ns;
+      x.p[u] = idx >= end ? -1 : key_at(w.ns, w.lo, idx);
       x.k[u].clear();
       x.v[u].clear();
       if (on && idx < end) {
@@ -182,7 +191,7 @@ __global__ __launch_bounds__(W * 64) void window_step_kernel(WindowStepArgs a, i
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float s[U], top = m[r];
-      const int mine = w.pos + (w.row0 + r) / G;
+      const int mine = (int)((unsigned)w.pos + (unsigned)((w.row0 + r) / G));  // rows past the call's last wrap, unused
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         s[u] = group_reduce<L>(dot8(x.k[u], q[r]), Plus{}) * qs;

@@ -6,7 +6,8 @@ import pytest
 
 from metalaudio_amd import nn
 from tests.test_gpu_tokens import linear_case
-from tests.token_refs import EPS, HALF, TINY, quantise, rmsnorm, rounded
+from tests.token_refs import (EPS, HALF, TINY, attend, attention_tolerance, quantise, rmsnorm, rounded,
+                              slot_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +153,37 @@ def test_rmsnorm_of_zeros_without_epsilon(dev, stream):
         stream.sync(60000)
         y = y.to_numpy()
         assert np.isnan(y[1]).all() and (y[[0, 2]] == 1).all()
+
+
+# ------------------------------------------------------------------ window step at far positions
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H,KV,T,left,sinks,back", [(2, 2, 5, 30, 20, 0), (4, 2, 16, 900, 33, 0),
+                                                    (1, 1, 9, 700, 65, 3)])
+def test_window_step_farthest_positions(dev, stream, H, KV, T, left, sinks, back, dtype):
+    """Several new tokens up to position 2^31 - 2, sinks in sight, the keys over one workgroup and split."""
+    say(f"step farthest {T} tokens {left} back {sinks} sinks {dtype}")
+    hd, slots, p = 48, sinks + left + T + 2, 2 ** 31 - 1 - T - back
+    layer = nn.WindowAttention(dev, H, hd, KV, left, 0, sinks)
+    rng = np.random.default_rng(T)
+    w = KV * hd
+    kc, vc = (rounded(rng.standard_normal((1, slots, w)), dtype) for _ in "kv")
+    q = rounded(rng.standard_normal((1, T, H * hd)), dtype)
+    k, v = (rounded(rng.standard_normal((1, T, w)), dtype) for _ in "kv")
+    kt, vt = tensor(dev, kc, dtype), tensor(dev, vc, dtype)
+    out = nn.Tensor(dev, q.shape, dtype=dtype)
+    layer.step(tensor(dev, q, dtype), tensor(dev, k, dtype), tensor(dev, v, dtype),
+               tensor(dev, np.array([p]), "i32"), kt, vt, out, stream=stream)
+    stream.sync(60000)
+    tokens = list(range(sinks)) + list(range(p - left, p))
+    at = [slot_of(i, sinks, slots) for i in tokens]
+    kk, vv = np.concatenate([kc[0, at], k[0]]), np.concatenate([vc[0, at], v[0]])
+    key = np.array(tokens + list(range(p, p + T)))[None]
+    mine = np.arange(p, p + T)[:, None]
+    seen = (key <= mine) & ((key >= mine - left) | (key < sinks))
+    want, spread, size = attend(q[0], kk, vv, seen, H, KV, hd ** -0.5)
+    err = np.abs(out.to_numpy()[0] - want)
+    assert (err <= attention_tolerance(spread, size, hd, left + 1 + sinks, dtype)).all()
+    for i in range(T):
+        kc[0, slot_of(p + i, sinks, slots)], vc[0, slot_of(p + i, sinks, slots)] = k[0, i], v[0, i]
+    np.testing.assert_array_equal(kt.to_numpy(), kc)
+    np.testing.assert_array_equal(vt.to_numpy(), vc)
