@@ -1,7 +1,8 @@
 // Rotary positions over several axes: pair (u, v) of axis a and rate f turns by the angle pos_a * f,
 // (u cos - v sin, v cos + u sin). The angle is kept in turns: pos * (f / 2 pi) is one product in 64 bits,
-// whose fraction is what is left of it, exact to 2^-53 of the whole (2e-7 turns at position 2^31), and the
-// sine and cosine of that fraction are taken in fp32.
+// whose fraction is what is left of it, exact to 2^-53 of the whole (2e-7 turns at position 2^31). The sine and
+// cosine are taken in fp32 of the fraction rounded to fp32; what that rounding left out (up to 9e-8 of an angle,
+// more than the rounding of the results) is turned by as well, to first order.
 #include "token_ops.hpp"
 #include "token_utils.hpp"
 
@@ -15,8 +16,12 @@ using namespace dev;
 namespace {
 
 __device__ __forceinline__ void turn_of(int pos, double rate, float& cs, float& sn) {
-  const double t = (double)pos * rate;
-  sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
+  const double t = (double)pos * rate, f = t - rint(t);
+  const float h = (float)f, rest = (float)(f - (double)h) * 6.2831853f;
+  float c, s;
+  sincospif(2.f * h, &s, &c);
+  cs = fmaf(-s, rest, c);
+  sn = fmaf(c, rest, s);
 }
 
 // i / d with by = floor(2^32 / d): the high product is the quotient or one less, for any i below 2^32.

@@ -6,8 +6,8 @@ import pytest
 
 from metalaudio_amd import nn
 from tests.test_gpu_tokens import linear_case
-from tests.token_refs import (EPS, HALF, TINY, attend, attention_tolerance, quantise, rmsnorm, rounded,
-                              slot_of)
+from tests.token_refs import (EPS, HALF, TINY, attend, attention_tolerance, quantise, rmsnorm, rotary,
+                              rounded, slot_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +187,26 @@ def test_window_step_farthest_positions(dev, stream, H, KV, T, left, sinks, back
         kc[0, slot_of(p + i, sinks, slots)], vc[0, slot_of(p + i, sinks, slots)] = k[0, i], v[0, i]
     np.testing.assert_array_equal(kt.to_numpy(), kc)
     np.testing.assert_array_equal(vt.to_numpy(), vc)
+
+
+# ------------------------------------------------------------------------------ rotary positions
+@pytest.mark.parametrize("hd,inter", [(64, False), (64, True), (6, False)])
+@pytest.mark.parametrize("origin", [0, 900001])
+def test_rotary_angles_keep_their_bits(dev, stream, hd, inter, origin):
+    """Pairs (1, 0) turn into their cosine and sine: two roundings each (the function's, the remainder's
+    term), about 0.42 half steps rms of values of all sizes or 2.5e-8, together 3.5e-8, and a fifth more
+    for a function that is off by somewhat above half a step. An angle rounded to fp32 adds 4.1e-8."""
+    say(f"rotary bits hd {hd} interleaved {inter} from {origin}")
+    S, base = 4000, 3.0  # rates of all the pairs turn far
+    x = np.zeros((S, hd), np.float32)
+    x[:, 0::2] = 1 if inter else 0
+    x[:, :hd // 2] = x[:, :hd // 2] if inter else 1
+    pos = (origin + np.arange(S))[:, None]
+    y = nn.Tensor(dev, (S, hd))
+    nn.Rotary(dev, hd, [hd], base=base, interleaved=inter).forward(
+        tensor(dev, x, "f32"), None, tensor(dev, pos, "i32"), y, stream=stream)
+    stream.sync(60000)
+    want = rotary(x[None], pos, 1, hd, [hd], base, inter)[0]
+    off = np.linalg.norm(y.to_numpy() - want) / np.linalg.norm(want)
+    print(f"distance {off:.3g}")
+    assert off <= 4.2e-8
