@@ -55,8 +55,9 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
 // A key that a query does not see has probability 0, but 0 times a value that is not finite is NaN, and
-// parts of tiny or overflowing f32 values are off: queries whose result is not finite (or, in f32, below
-// 2^-109) are computed again by window_query.
+// parts of tiny or overflowing f32 values are off; and in bf16 c ref, rounded, of scores past 2^31 is so far from c times
+// the largest score that all probabilities may come out as 0 (their sum is about 1 or more otherwise). Queries whose
+// result is not finite, whose sum is small or, in f32, whose result is below 2^-109 are computed again by window_query.
 template <class T, int KS, int KW, int NW>
 struct WindowCfg {
   static constexpr bool F32 = sizeof(T) == 4;
@@ -382,7 +383,7 @@ __global__ __launch_bounds__((WindowCfg<T, KS, KW, NW>::THREADS), (WindowCfg<T, 
   const float l = other_half(lsum, [](float x, float y) { return x + y; });
   const float inv = 1.f / l;
   float chk = l * 0.f;
-  bool bad = false;
+  bool bad = !F32 && l < 0x1p-60f;
 #pragma unroll
   for (int c = 0; c < 2 * KS; ++c)  // dimensions 8 c + 4 g .. + 3
     if (8 * c < a.hd) {

@@ -7,7 +7,7 @@ import pytest
 from metalaudio_amd import nn
 from tests.test_gpu_tokens import linear_case
 from tests.token_refs import (EPS, HALF, TINY, attend, attention_tolerance, quantise, rmsnorm, rotary,
-                              rounded, slot_of)
+                              rounded, slot_of, window_seen)
 
 pytestmark = pytest.mark.gpu
 
@@ -210,3 +210,75 @@ def test_rotary_angles_keep_their_bits(dev, stream, hd, inter, origin):
     off = np.linalg.norm(y.to_numpy() - want) / np.linalg.norm(want)
     print(f"distance {off:.3g}")
     assert off <= 4.2e-8
+
+
+# -------------------------------------------------------------------------------------- attention
+BAD = [("k", np.inf), ("k", -np.inf), ("k", 3e38), ("k", -3e38), ("v", np.inf), ("v", 3e38), ("v", np.nan)]
+
+
+def sighted(got, want, tol, what):
+    """Infinities and NaN where the formula has them, the rest within the tolerance."""
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=what)
+    np.testing.assert_array_equal(got[np.isinf(want)], want[np.isinf(want)], err_msg=what)
+    fine = np.isfinite(want)
+    assert (np.abs(got[fine] - want[fine]) <= tol[fine]).all(), what
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("what,bad", BAD)
+@pytest.mark.parametrize("B,H", [(1, 1), (6, 8)])  # one or four key groups a workgroup
+def test_window_attention_of_a_value_in_sight(dev, stream, B, H, what, bad, dtype):
+    """The queries that see a key (or value) with an infinite, NaN or huge entry: a score of -infinity
+    has weight 0, one of +infinity or NaN leaves NaN, a huge one takes all or nothing. The queries' entry
+    beside the huge one is below 1, so that no sum of products leaves fp32."""
+    say(f"window in sight of {what} {bad} {dtype} {B} x {H}")
+    S, hd, left, sinks, at = 700, 48, 150, 2, 301
+    rng = np.random.default_rng(61)
+    q = rng.standard_normal((B, S, H * hd))
+    q[..., 5::hd] = rng.uniform(0.05, 0.9, (B, S, H)) * rng.choice([-1, 1], (B, S, H))
+    q, k, v = (rounded(x, dtype) for x in (q, *(rng.standard_normal((2, B, S, H * hd)))))
+    {"k": k, "v": v}[what][:, at, 5::hd] = rounded(np.float32(bad), dtype)
+    o = nn.Tensor(dev, q.shape, dtype=dtype)
+    nn.WindowAttention(dev, H, hd, window_left=left, sinks=sinks).forward(
+        *(tensor(dev, x, dtype) for x in (q, k, v)), o, stream=stream)
+    stream.sync(60000)
+    got = o.to_numpy()
+    rows = slice(at - 20, at + left + 20)
+    seen = window_seen(S, left, 0, sinks)[rows]
+    with np.errstate(invalid="ignore"):
+        for b in (0, B - 1):
+            want, spread, size = attend(q[b, rows], k[b], v[b], seen, H, H, hd ** -0.5)
+            # a huge score takes all: its own size is no error of the others
+            spread = np.where(np.isfinite(spread) & (spread < 1e3), spread, 0) + 10
+            sighted(got[b, rows], want, attention_tolerance(spread, np.abs(size), hd, S, dtype), f"sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("what,bad", BAD)
+@pytest.mark.parametrize("left", [150, 1000])  # one workgroup a head, or its keys split
+def test_window_step_of_a_value_in_sight(dev, stream, what, bad, left, dtype):
+    say(f"step in sight of {what} {bad} {dtype} {left} back")
+    hd, H, T, sinks = 48, 2, 6, 2
+    slots, p = sinks + left + T, 5 * left
+    at = p - left + 3  # seen by the first four of the six tokens
+    rng = np.random.default_rng(62)
+    q = rng.standard_normal((1, T, H * hd))
+    q[..., 5::hd] = rng.uniform(0.05, 0.9, (1, T, H)) * rng.choice([-1, 1], (1, T, H))
+    q = rounded(q, dtype)
+    kc, vc, k, v = (rounded(rng.standard_normal((1, n, H * hd)), dtype) for n in (slots, slots, T, T))
+    {"k": kc, "v": vc}[what][0, slot_of(at, sinks, slots), 5::hd] = rounded(np.float32(bad), dtype)
+    o = nn.Tensor(dev, q.shape, dtype=dtype)
+    nn.WindowAttention(dev, H, hd, window_left=left, sinks=sinks).step(
+        *(tensor(dev, x, dtype) for x in (q, k, v)), tensor(dev, np.array([p]), "i32"),
+        tensor(dev, kc, dtype), tensor(dev, vc, dtype), o, stream=stream)
+    stream.sync(60000)
+    tokens = list(range(sinks)) + list(range(p - left, p))
+    slot = [slot_of(i, sinks, slots) for i in tokens]
+    key = np.array(tokens + list(range(p, p + T)))[None]
+    mine = np.arange(p, p + T)[:, None]
+    seen = (key <= mine) & ((key >= mine - left) | (key < sinks))
+    with np.errstate(invalid="ignore"):
+        want, spread, size = attend(q[0], np.concatenate([kc[0, slot], k[0]]), np.concatenate([vc[0, slot], v[0]]),
+                                    seen, H, H, hd ** -0.5)
+    spread = np.where(np.isfinite(spread) & (spread < 1e3), spread, 0) + 10
+    sighted(o.to_numpy()[0], want, attention_tolerance(spread, np.abs(size), hd, left + 3, dtype), "step")
