@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from metalaudio_amd import nn
+from tests import token_bits as bits
 from tests.test_gpu_tokens import linear_case
 from tests.token_refs import (EPS, HALF, TINY, attend, attention_tolerance, quantise, rmsnorm, rotary,
                               rounded, slot_of, window_seen)
@@ -213,6 +214,56 @@ def test_rotary_angles_keep_their_bits(dev, stream, hd, inter, origin):
 
 
 # -------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,S,H,KV,hd,left,right,sinks", [
+    (2, 1345, 8, 8, 48, 168, 168, 4), (1, 700, 2, 1, 64, 300, 1, 129), (5, 1030, 8, 8, 48, 70, 0, 3),
+    (3, 1025, 16, 16, 128, 64, 64, 2), (1, 2500, 2, 2, 48, 1000, 0, 5), (2, 130, 4, 2, 32, 16, 16, 4),
+    (6, 901, 8, 2, 64, 200, 5, 70)])
+def test_window_attention_distance(dev, stream, B, S, H, KV, hd, left, right, sinks, dtype):
+    """The largest distance of a sequence from 64 bits, in every way that a call is cut."""
+    say(f"window distance {B}x{S} heads {H}/{KV} hd {hd} {dtype}")
+    rng = np.random.default_rng(S)
+    q, k = (rounded(rng.standard_normal((B, S, n * hd)) * 1.3, dtype) for n in (H, KV))
+    v = rounded(rng.standard_normal((B, S, KV * hd)), dtype)
+    o = nn.Tensor(dev, q.shape, dtype=dtype)
+    nn.WindowAttention(dev, H, hd, KV, left, right, sinks).forward(
+        *(tensor(dev, x, dtype) for x in (q, k, v)), o, stream=stream)
+    stream.sync(60000)
+    got, seen = o.to_numpy(), window_seen(S, left, right, sinks)
+    off = max(bits.distance(got[b], attend(q[b], k[b], v[b], seen, H, KV, hd ** -0.5)[0]) for b in range(B))
+    print(f"distance {off:.3g}")
+    assert off <= (bits.ATTENTION_F32 if dtype == "f32" else bits.ATTENTION_BF16)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T,H,KV,hd,left,sinks", [(3, 1, 8, 8, 48, 511, 4), (1, 5, 8, 2, 64, 900, 4),
+                                                    (2, 16, 4, 4, 128, 100, 33)])
+def test_window_step_distance(dev, stream, B, T, H, KV, hd, left, sinks, dtype):
+    """Steps keep their probabilities in fp32 whatever the tensors' type."""
+    say(f"step distance {B}x{T} heads {H}/{KV} hd {hd} {dtype}")
+    rng = np.random.default_rng(hd)
+    slots, p = sinks + left + T, 3000
+    kc, vc, k, v = (rounded(rng.standard_normal((B, n, KV * hd)) * s, dtype)
+                    for n, s in ((slots, 1.3), (slots, 1), (T, 1.3), (T, 1)))
+    q = rounded(rng.standard_normal((B, T, H * hd)) * 1.3, dtype)
+    o = nn.Tensor(dev, q.shape, dtype=dtype)
+    nn.WindowAttention(dev, H, hd, KV, left, 0, sinks).step(
+        *(tensor(dev, x, dtype) for x in (q, k, v)), tensor(dev, np.full(B, p), "i32"),
+        tensor(dev, kc, dtype), tensor(dev, vc, dtype), o, stream=stream)
+    stream.sync(60000)
+    tokens = list(range(sinks)) + list(range(p - left, p))
+    at = [slot_of(i, sinks, slots) for i in tokens]
+    key = np.array(tokens + list(range(p, p + T)))[None]
+    mine = np.arange(p, p + T)[:, None]
+    seen = (key <= mine) & ((key >= mine - left) | (key < sinks))
+    got = o.to_numpy()
+    off = max(bits.distance(got[b], attend(q[b], np.concatenate([kc[b, at], k[b]]),
+                                           np.concatenate([vc[b, at], v[b]]), seen, H, KV, hd ** -0.5)[0])
+              for b in range(B))
+    print(f"distance {off:.3g}")
+    assert off <= (bits.ATTENTION_F32 if dtype == "f32" else bits.STEP_BF16)
+
+
 BAD = [("k", np.inf), ("k", -np.inf), ("k", 3e38), ("k", -3e38), ("v", np.inf), ("v", 3e38), ("v", np.nan)]
 
 
