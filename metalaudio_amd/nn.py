@@ -106,6 +106,16 @@ def _th(tensor):
     return tensor.handle if tensor is not None else None
 
 
+def i32_values(a) -> np.ndarray:
+    """Values for an "i32" tensor; those that are no 32-bit integers are refused (numpy would wrap them)."""
+    x = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        y = np.ascontiguousarray(x.astype(np.int32)).reshape(x.shape)
+    if not np.array_equal(x, y):
+        raise ValueError("values of an i32 tensor must be integers from -2^31 to 2^31 - 1")
+    return y
+
+
 def bf16_bits(a) -> np.ndarray:
     """fp32 -> bf16 bit patterns (uint16), round to nearest even, NaN kept quiet."""
     u = _f32(a).view(np.uint32).astype(np.uint64)
@@ -180,10 +190,7 @@ class Tensor:
 
     def copy_from(self, arr, stream: Optional[Stream] = None) -> None:
         """Tensor.copy(from:) — synchronous upload."""
-        if self.dtype == "i32":
-            a = np.ascontiguousarray(np.asarray(arr, dtype=np.int32))
-        else:
-            a = _f32(arr)
+        a = i32_values(arr) if self.dtype == "i32" else _f32(arr)
         if self.dtype == "bf16":
             a = np.ascontiguousarray(bf16_bits(a))
         elif self.dtype == "e4m3":
