@@ -269,7 +269,8 @@ typedef struct mnn_window_attention_desc {
 /* Attention over a sliding window with a few first tokens that stay visible (no counterpart in the
  * reference). The query of token i sees the keys j <= i + window_right with j >= i - window_left or j <
  * sinks. Softmax and sums run in fp32; f32 tensors keep fp32 products, bf16 ones take bf16 products with
- * fp32 accumulation. No weights: q, k and v are projected (and turned) before. */
+ * fp32 accumulation: over whole sequences the probabilities are rounded to bf16 for theirs, in steps they
+ * stay in fp32. No weights: q, k and v are projected (and turned) before. */
 mnn_status mnn_window_attention_create(mnn_device dev, const mnn_window_attention_desc* desc,
                                        mnn_layer* out);
 /* Whole sequences: q and output [S, H * head_dim] or [B, S, H * head_dim], k and v the same of

@@ -110,7 +110,7 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 // once more (the slots are done with), so that scales, residual and output are read and written row by row.
 //
 // Bound by the matrix instructions beside the widening and, in a grid of one or two rounds, by each round's first
-// loads and results: 8192 x 4096 x 4096 to bf16 200 us (1.4 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
+// loads and results: 8192 x 4096 x 4096 to bf16 200 to 214 us (1.3 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
 // 1536 x 384 to f32 with residual 19 us. The widening spread between the products by hand changes nothing, nor do
 // waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
 template <class T, int BM, int BN, int WM, int WN>

@@ -95,8 +95,8 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
 // Rows of whole chunks of 16 bytes that W waves hold in their registers from the first read to the last
 // write: NV chunks a lane, chunk i of lane l at (64 W i + l) VE, so that a load instruction covers 1 KB in a
 // row. The weights stay there too, over all the rows that a workgroup takes. Bound by memory (up to two loads
-// and two stores a value): 65537 x 2048 bf16 with residual, sum and e4m3 output 174 us, 5.4 TB/s; 6436 x 2048 f32
-// 32 us; 10752 x 384 bf16 9.5 us.
+// and two stores a value): 65537 x 2048 bf16 with residual, sum and e4m3 output 175 us, 5.4 TB/s; 6436 x 2048 f32
+// 32 us; 10752 x 384 bf16 9.7 us.
 template <class T, int NV, int W, mnn_dtype OUT>
 __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
   constexpr int VE = 16 / (int)sizeof(T);

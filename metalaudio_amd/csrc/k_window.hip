@@ -50,7 +50,7 @@ __device__ __forceinline__ void window_query(const WindowArgs& a, int b, int h, 
 // block is computed the next one's rows are on their way to registers.
 //
 // Bound by the vector units' issue beside the matrix instructions: 16384 tokens, 1023 back, 8 / 2 heads of 64 in bf16
-// 52 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 19.9 us (split of K, V and P).
+// 52 us (0.6 PFLOP/s); f32, 2 x 1345 ragged tokens, 168 both ways, 8 heads of 48 20.4 us (split of K, V and P).
 //
 // Softmax: p = exp2(c s - ref) with a reference that moves only when a block's maximum exceeds it by 2^8.
 //
