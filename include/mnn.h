@@ -59,16 +59,18 @@ typedef enum mnn_status {
 } mnn_status;
 
 /* I32: token positions, lengths and counts. E4M3: 8-bit floats (OCP e4m3: 4 exponent and 3 mantissa
- * bits, largest value 448, no infinities), each row with a scale beside it. */
+ * bits, largest value 448, no infinities), each row, or each block of one, with a scale beside it. */
 typedef enum mnn_dtype { MNN_F32 = 0, MNN_BF16 = 1, MNN_I32 = 2, MNN_E4M3 = 3 } mnn_dtype;
 
 /* Compute precision of the matrix products (GEMM, implicit-GEMM conv, attention).
  * F32: fp32 operands on v_mfma_f32_*_f32. BF16: operands rounded to bf16 (RNE),
  * fp32 accumulation (precedent: HalfLinear, HalfPrecisionLinear.swift:60-212).
  * E4M3 (Linear / FusedLinear only, other layers refuse it): 8-bit operands with a scale per row,
- * fp32 accumulation. Norms, softmax and activations always run in fp32. */
+ * fp32 accumulation. E4M3_BLOCK (the same layers): 8-bit operands with a scale for each block of 128,
+ * so that a few large values cost the others no bits. Norms, softmax and activations always run in
+ * fp32. */
 typedef enum mnn_precision {
-  MNN_PRECISION_F32 = 0, MNN_PRECISION_BF16 = 1, MNN_PRECISION_E4M3 = 2
+  MNN_PRECISION_F32 = 0, MNN_PRECISION_BF16 = 1, MNN_PRECISION_E4M3 = 2, MNN_PRECISION_E4M3_BLOCK = 3
 } mnn_precision;
 
 /* Fused activation codes. 0-4 are FusedConv1D's (Conv1D.swift:960-973); FusedLinear's sigmoid
@@ -218,7 +220,11 @@ mnn_status mnn_fused_linear_create(mnn_device dev, int in_features, int out_feat
  * NULL, rounded to 8 bits per row by the same rule in a launch before the product (as mnn_layer_forward
  * of such a layer does, which writes f32). output: MNN_F32 or MNN_BF16, rounded once; residual: NULL or
  * of the output's type and count, and it may be the output itself. Other layers, or a Linear of another
- * precision, give MNN_ERR_INVALID_ARGUMENT. */
+ * precision, give MNN_ERR_INVALID_ARGUMENT.
+ * Precision MNN_PRECISION_E4M3_BLOCK: the weights have a scale for each 128 x 128 (the last rows and
+ * columns in smaller ones), scales is [.., ceil(in_features / 128)], one value for each 128 inputs of a
+ * row, and output = act(sum over blocks j of scales[i][j] * wscales[n / 128][j] * sum_k in j of
+ * input[i][k] w[n][k] + bias[n]) + residual; rows that come in f32 or bf16 are rounded block by block. */
 mnn_status mnn_linear_forward_scaled(mnn_layer layer, mnn_tensor input, mnn_tensor scales,
                                      mnn_tensor residual, mnn_tensor output, mnn_stream s);
 
@@ -233,7 +239,9 @@ mnn_status mnn_rmsnorm_create(mnn_device dev, int feature_size, float epsilon, m
  * MNN_F32 or MNN_BF16, and a count; output: MNN_F32 or MNN_BF16 with scales NULL, or MNN_E4M3 with
  * scales, an MNN_F32 tensor of one value per row: value = y * (448 * (1 / max|y|)) rounded to nearest
  * even, scale = max|y| * (1 / 448), a row maximum below 2^-100 counting as 2^-100. A row that holds a NaN
- * or an infinity comes out as NaN values or with a scale that is not finite. */
+ * or an infinity comes out as NaN values or with a scale that is not finite. scales of rows *
+ * ceil(feature_size / 128) values (where that is more than one a row): a maximum and a scale for each 128
+ * values of a row, the last block the shorter, as a Linear of MNN_PRECISION_E4M3_BLOCK reads them. */
 mnn_status mnn_rmsnorm_forward_residual(mnn_layer layer, mnn_tensor input, mnn_tensor residual,
                                         mnn_tensor sum, mnn_tensor output, mnn_tensor scales,
                                         mnn_stream s);
@@ -295,6 +303,62 @@ mnn_status mnn_window_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tenso
 mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
                                      mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
                                      mnn_tensor v_cache, mnn_tensor output, mnn_stream s);
+
+/* The same on caches in 8 bits, as mnn_kv_cache_write keeps them: k_cache and v_cache MNN_E4M3 [B, C,
+ * num_kv_heads * head_dim], k_scales and v_scales MNN_F32 [B, C, num_kv_heads]; q, k, v and output
+ * MNN_F32 or MNN_BF16. Every key is seen as the cache holds it, the call's own among them, so that T
+ * tokens in one call and one after the other see the same keys. With f32 the products are exact in the 8-bit values and
+ * take fp32 queries and probabilities; with bf16 the probabilities (times the value's scale) are rounded to bf16. */
+mnn_status mnn_window_attention_step_e4m3(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                          mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
+                                          mnn_tensor k_scales, mnn_tensor v_cache, mnn_tensor v_scales,
+                                          mnn_tensor output, mnn_stream s);
+
+/* Rolling caches of keys and values as rows of whole sequences are written to them and read back (no
+ * counterpart in the reference): token p of a stream lives in slot p for p < sinks, else in sinks +
+ * (p - sinks) % (C - sinks), as the window attention's step has it; with sinks 0 and no more tokens than
+ * slots that is slot p, as mnn_memory_attention_forward reads states. head_dim: a multiple of 8, <= 128.
+ * No weights. */
+mnn_status mnn_kv_cache_create(mnn_device dev, int num_kv_heads, int head_dim, int sinks,
+                               mnn_layer* out);
+/* Writes the next T tokens of each of B streams. k and v [B, T, num_kv_heads * head_dim], MNN_F32 or
+ * MNN_BF16; k_cache and v_cache [B, C, num_kv_heads * head_dim], C > sinks, of the type of k with k_scales
+ * and v_scales NULL, or MNN_E4M3 with MNN_F32 scales [B, C, num_kv_heads], one for each head's row: value =
+ * x * (448 * (1 / max|x|)) rounded to nearest even, scale = max|x| * (1 / 448), a maximum below 2^-100
+ * counting as 2^-100 (a row that holds a NaN or an infinity is read back as NaN or infinities). positions
+ * and steps (may be NULL) as for mnn_window_attention_step; T may be larger than the cache: of tokens that
+ * share a slot the last one stays. Other slots keep what they hold. No tensor may be two arguments. */
+mnn_status mnn_kv_cache_write(mnn_layer layer, mnn_tensor k, mnn_tensor v, mnn_tensor positions,
+                              mnn_tensor steps, mnn_tensor k_cache, mnn_tensor k_scales,
+                              mnn_tensor v_cache, mnn_tensor v_scales, mnn_stream s);
+/* Reads the slots of tokens positions[b] .. positions[b] + steps[b] - 1 (steps NULL: T of them) to the
+ * first rows of k and v, 8-bit values as value * scale, rounded once; tensors as above. Rows behind them
+ * are left as they were. What a slot holds is read whatever token wrote it. */
+mnn_status mnn_kv_cache_read(mnn_layer layer, mnn_tensor k_cache, mnn_tensor k_scales,
+                             mnn_tensor v_cache, mnn_tensor v_scales, mnn_tensor positions,
+                             mnn_tensor steps, mnn_tensor k, mnn_tensor v, mnn_stream s);
+
+typedef struct mnn_memory_attention_desc {
+  int num_heads, num_kv_heads;  /* query heads h read key/value head h * num_kv_heads / num_heads */
+  int head_dim;                 /* a multiple of 8, <= 128 */
+  float scale;                  /* of the scores; 0: 1 / sqrt(head_dim) */
+} mnn_memory_attention_desc;
+/* Attention of a decoder's tokens to an encoder's states, a sequence of another length whose keys and
+ * values are kept from call to call: the core of MultiHeadAttention's mnn_layer_forward_cross without its
+ * projections, with grouped heads and ragged lengths (no counterpart in the reference). */
+mnn_status mnn_memory_attention_create(mnn_device dev, const mnn_memory_attention_desc* desc,
+                                       mnn_layer* out);
+/* q and output [T, H * head_dim] or [B, T, H * head_dim], MNN_F32 or MNN_BF16; k and v [S, num_kv_heads *
+ * head_dim] or [B, S, num_kv_heads * head_dim] of that type with scales NULL, or MNN_E4M3 with MNN_F32
+ * k_scales and v_scales [B, S, num_kv_heads] (mnn_kv_cache_write's). query_lengths, lengths: NULL, or
+ * MNN_I32 [B], the tokens and states of each padded sequence (values outside 0..T and 0..S count as the
+ * nearer of the two): states behind a sequence's end are not read, output rows behind its last token are
+ * left as they were. Tokens of a sequence without states get zeros. Softmax and sums run in fp32; f32
+ * tensors keep fp32 products (8-bit values are exact in them), with bf16 ones the probabilities are rounded
+ * to bf16. output may not be an input. */
+mnn_status mnn_memory_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor k_scales,
+                                        mnn_tensor v, mnn_tensor v_scales, mnn_tensor query_lengths,
+                                        mnn_tensor lengths, mnn_tensor output, mnn_stream s);
 
 /* MultiHeadAttention / CrossAttention (Attention.swift:15-1063), PyTorch packing:
  * "in_proj_weight" [3E, E] rows Q;K;V, "in_proj_bias" [3E], "out_proj_weight" [E, E],

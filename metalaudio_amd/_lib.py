@@ -33,7 +33,7 @@ STATUS = {
 
 ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "gelu": 3, "swish": 4, "sigmoid": 5, "tanh": 6}
 PAD = {"valid": 0, "same": 1, "explicit": 2, "reflect": 3}
-PRECISION = {"f32": 0, "bf16": 1, "e4m3": 2}
+PRECISION = {"f32": 0, "bf16": 1, "e4m3": 2, "e4m3_block": 3}
 DTYPE = {"f32": 0, "bf16": 1, "i32": 2, "e4m3": 3}
 
 
@@ -108,6 +108,11 @@ class WindowAttentionDesc(C.Structure):
         ("scale", C.c_float)]
 
 
+class MemoryAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("num_heads", "num_kv_heads", "head_dim")] + [
+        ("scale", C.c_float)]
+
+
 class SeparatorDesc(C.Structure):
     _fields_ = [("input_channels", C.c_int), ("num_stems", C.c_int), ("levels", C.c_int),
                 ("channels", C.c_int * 8), ("kernel_size", C.c_int), ("stride", C.c_int),
@@ -166,6 +171,12 @@ SIGNATURES = {
     "mnn_window_attention_create": (C.c_int, [P, C.POINTER(WindowAttentionDesc), PP]),
     "mnn_window_attention_forward": (C.c_int, [P, P, P, P, P, P, P]),
     "mnn_window_attention_step": (C.c_int, [P, P, P, P, P, P, P, P, P, P]),
+    "mnn_window_attention_step_e4m3": (C.c_int, [P] * 12),
+    "mnn_kv_cache_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, PP]),
+    "mnn_kv_cache_write": (C.c_int, [P] * 10),
+    "mnn_kv_cache_read": (C.c_int, [P] * 10),
+    "mnn_memory_attention_create": (C.c_int, [P, C.POINTER(MemoryAttentionDesc), PP]),
+    "mnn_memory_attention_forward": (C.c_int, [P] * 10),
     "mnn_mha_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, PP]),
     "mnn_feedforward_create": (C.c_int, [P, C.c_int, C.c_int, C.c_int, PP]),
     "mnn_encoder_block_create": (C.c_int, [P, C.POINTER(EncoderBlockDesc), PP]),

@@ -100,8 +100,9 @@ mnn_precision wide(mnn_precision p) {
 
 std::unique_ptr<Layer> any_linear(Device* d, int in, int out, bool bias, int act, mnn_precision p,
                                   float alpha = 0.01f) {
-  return p == MNN_PRECISION_E4M3 ? make_linear_e4m3(d, in, out, bias, act, alpha)
-                                 : make_linear(d, in, out, bias, act, wide(p), alpha);
+  return p == MNN_PRECISION_E4M3 || p == MNN_PRECISION_E4M3_BLOCK
+             ? make_linear_e4m3(d, in, out, bias, act, alpha, p == MNN_PRECISION_E4M3_BLOCK)
+             : make_linear(d, in, out, bias, act, wide(p), alpha);
 }
 
 // What the entry points with several tensors share: the layer's device is alive and owns each tensor
@@ -558,6 +559,59 @@ mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k
            *kc = T(k_cache), *vc = T(v_cache), *out = T(output);
     Stream s = enter(l, {tq, tk, tv, pos, stp, kc, vc, out}, st);
     window_attention_step(l, *tq, *tk, *tv, *pos, stp, *kc, *vc, *out, s);
+  });
+}
+mnn_status mnn_window_attention_step_e4m3(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
+                                          mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
+                                          mnn_tensor k_scales, mnn_tensor v_cache, mnn_tensor v_scales,
+                                          mnn_tensor output, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tq = T(q), *tk = T(k), *tv = T(v), *pos = T(positions), *stp = opt(steps),
+           *kc = T(k_cache), *ks = T(k_scales), *vc = T(v_cache), *vs = T(v_scales), *out = T(output);
+    Stream s = enter(l, {tq, tk, tv, pos, stp, kc, ks, vc, vs, out}, st);
+    window_attention_step_e4m3(l, *tq, *tk, *tv, *pos, stp, *kc, *ks, *vc, *vs, *out, s);
+  });
+}
+mnn_status mnn_kv_cache_create(mnn_device dev, int num_kv_heads, int head_dim, int sinks,
+                               mnn_layer* out) {
+  MNN_CREATE(make_kv_cache(d, num_kv_heads, head_dim, sinks));
+}
+mnn_status mnn_kv_cache_write(mnn_layer layer, mnn_tensor k, mnn_tensor v, mnn_tensor positions,
+                              mnn_tensor steps, mnn_tensor k_cache, mnn_tensor k_scales,
+                              mnn_tensor v_cache, mnn_tensor v_scales, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tk = T(k), *tv = T(v), *pos = T(positions), *stp = opt(steps), *kc = T(k_cache),
+           *ks = opt(k_scales), *vc = T(v_cache), *vs = opt(v_scales);
+    Stream s = enter(l, {tk, tv, pos, stp, kc, ks, vc, vs}, st);
+    kv_cache_write(l, *tk, *tv, *pos, stp, *kc, ks, *vc, vs, s);
+  });
+}
+mnn_status mnn_kv_cache_read(mnn_layer layer, mnn_tensor k_cache, mnn_tensor k_scales,
+                             mnn_tensor v_cache, mnn_tensor v_scales, mnn_tensor positions,
+                             mnn_tensor steps, mnn_tensor k, mnn_tensor v, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *kc = T(k_cache), *ks = opt(k_scales), *vc = T(v_cache), *vs = opt(v_scales),
+           *pos = T(positions), *stp = opt(steps), *tk = T(k), *tv = T(v);
+    Stream s = enter(l, {kc, ks, vc, vs, pos, stp, tk, tv}, st);
+    kv_cache_read(l, *kc, ks, *vc, vs, *pos, stp, *tk, *tv, s);
+  });
+}
+mnn_status mnn_memory_attention_create(mnn_device dev, const mnn_memory_attention_desc* desc,
+                                       mnn_layer* out) {
+  MNN_CREATE(make_memory_attention(d, need(desc)));
+}
+mnn_status mnn_memory_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor k_scales,
+                                        mnn_tensor v, mnn_tensor v_scales, mnn_tensor query_lengths,
+                                        mnn_tensor lengths, mnn_tensor output, mnn_stream st) {
+  return guard([&] {
+    Layer* l = L(layer);
+    Tensor *tq = T(q), *tk = T(k), *ks = opt(k_scales), *tv = T(v), *vs = opt(v_scales),
+           *ql = opt(query_lengths), *len = opt(lengths), *out = T(output);
+    Stream s = enter(l, {tq, tk, ks, tv, vs, ql, len, out}, st);
+    memory_attention_forward(l, *tq, *tk, ks, *tv, vs, ql, len, *out, s);
   });
 }
 mnn_status mnn_mha_create(mnn_device dev, int embed_dim, int num_heads, int use_bias,

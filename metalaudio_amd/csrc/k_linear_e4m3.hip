@@ -1,5 +1,6 @@
 // The 8-bit linear product: y[m][n] = act(xs[m] ws[n] sum_k x[m][k] w[n][k] + bias[n]) + r[m][n], x and w
-// in e4m3.
+// in e4m3, or with scales for blocks of 128: act(sum_j xs[m][j] ws[n / 128][j] sum_{k in block j} x[m][k] w[n][k]
+// + bias[n]) + r[m][n].
 //
 // Which matrix instructions: e4m3 values are bf16 values, so both operands are widened
 // (v_cvt_scalef32_pk_bf16_fp8, two values an instruction) and multiplied by the bf16 instructions (2.2 PFLOP/s), whose
@@ -49,6 +50,16 @@ __device__ __forceinline__ floatx16 mul(const Operand& a, const Operand& b, floa
   return c;
 }
 
+// Blocks: a product of 64 of them begins at 0, and joins the running sums times its two scales.
+__device__ __forceinline__ void mul_scaled(const Operand& a, const Operand& b, float by, floatx16& c) {
+  floatx16 t;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) t[v] = 0.f;
+  t = mul(a, b, t);
+#pragma unroll
+  for (int v = 0; v < 16; ++v) c[v] = fmaf(t[v], by, c[v]);
+}
+
 // The activation of CNT values; its choice is made once for all of them (a branch an element, the same for
 // every lane or not, took 32 us of a round of 256 x 256 results).
 template <int CNT>
@@ -89,13 +100,15 @@ __device__ __forceinline__ void store_some(T* p, const float* v, bool vec, int c
     if (i < cnt) p[i] = from_f32<T>(v[i]);
 }
 
-// Scales and biases of CNT consecutive columns (those behind the last column: 0).
-template <int CNT>
+// Scales and biases of CNT consecutive columns, those behind the last column as the last; the scales of
+// blocks are in the sums already, but for their unit: the weights' scales are kept as 1 at most, or in units of the
+// largest, so that their products with those of x overflow only where results do.
+template <int CNT, bool BLK>
 __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* ws, float* bias) {
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
     const int c = min(n + i, a.N - 1);
-    ws[i] = a.ws[c];
+    ws[i] = BLK ? a.unit : a.ws[c];
     bias[i] = a.bias ? a.bias[c] : 0.f;
   }
 }
@@ -113,7 +126,7 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 // loads and results: 8192 x 4096 x 4096 to bf16 200 to 214 us (1.3 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
 // 1536 x 384 to f32 with residual 19 us. The widening spread between the products by hand changes nothing, nor do
 // waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, bool BLK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
   constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;
@@ -173,8 +186,25 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   constexpr int PER_ROW = WN / 8;  // lanes
   const int cn = 8 * (lane % PER_ROW), n = n0 + wn * WN + cn;
   float ws[8], bias[8];
-  columns<8>(a, n, ws, bias);
-  for (int i = threadIdx.x; i < BM; i += NW * 64) xs[i] = a.xs[min(m0 + i, a.M - 1)];
+  columns<8, BLK>(a, n, ws, bias);
+  if constexpr (!BLK)
+    for (int i = threadIdx.x; i < BM; i += NW * 64) xs[i] = a.xs[min(m0 + i, a.M - 1)];
+  // blocks: the scales of a depth step's products, one a lane for 32 rows of x (this wave's rows of w are of one
+  // block), on their way a step ahead
+  static_assert(kScaleBlock == 128 && kScaleBlock % WN == 0, "a block a depth step and a wave");
+  const float *xsp[FM], *wsp = nullptr;
+  float by[FM], xnext[FM], wnext = 0.f;
+  auto next_scales = [&](int k) {
+    wnext = wsp[k];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) xnext[j] = xsp[j][k];
+  };
+  if constexpr (BLK) {
+    wsp = a.ws + (int64_t)(min(n0 + wn * WN, a.N - 1) / kScaleBlock) * nk;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) xsp[j] = a.xs + min(m0 + wm * WM + 32 * j + l32, a.M - 1) * nk;
+    next_scales(0);
+  }
   // chunk c of a row that is l32 modulo 32
   auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 >> 1 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
@@ -183,12 +213,31 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     wait_lgkmcnt0();
     wait_vmcnt<0>();
     stage_barrier();
+    if constexpr (BLK) {
+#pragma unroll
+      for (int j = 0; j < FM; ++j) by[j] = xnext[j] * wnext;
+      if (k + 1 < nk) next_scales(k + 1);
+    }
     if (k + 1 < nk) issue(k + 1, slot ^ 1);
     const char* p = smem + slot * SLOT;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int c0 = at(4 * s + 2 * g), c1 = at(4 * s + 2 * g + 1);
       Operand x[FM], w[FN];
+      if constexpr (BLK) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+          w[i].set(*reinterpret_cast<const intx4*>(p + wa + 4096 * i + c0),
+                   *reinterpret_cast<const intx4*>(p + wa + 4096 * i + c1));
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
+                   *reinterpret_cast<const intx4*>(p + xa + 4096 * j + c1));
+#pragma unroll
+          for (int i = 0; i < FN; ++i) mul_scaled(w[i], x[j], by[j], acc[i][j]);
+        }
+        continue;
+      }
 #pragma unroll
       for (int j = 0; j < FM; ++j)
         x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
@@ -237,7 +286,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
     for (int r = 0; r < PASSES; ++r) {
       const int row = r * ROWS + lane / PER_ROW;
-      const float by = xs[wm * WM + 32 * j + row];
+      const float by = BLK ? 1.f : xs[wm * WM + 32 * j + row];
       float* u = v + 8 * r;
       *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(out + row * OP + cn);
       *reinterpret_cast<float4*>(u + 4) = *reinterpret_cast<const float4*>(out + row * OP + cn + 4);
@@ -264,7 +313,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 // eighth of the depth each, operands straight from memory (a wave reads 64 bytes of 32 rows at a time, four
 // such steps in flight); their sums meet in LDS. Rows of x may be of any length: what a lane would read past
 // a row's end is 0.
-template <class T>
+template <class T, bool BLK>
 __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) {
   __shared__ float sum[8][32][33];  // [wave][m][n]
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = threadIdx.x >> 6;
@@ -275,6 +324,9 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
   floatx16 acc;
 #pragma unroll
   for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+  const int nk = a.K / kScaleBlock;
+  const float* xsp = a.xs + (BLK ? min((int64_t)l32, a.M - 1) * nk : 0);
+  const float* wsp = a.ws + (BLK ? (int64_t)(n0 / kScaleBlock) * nk : 0);
   auto step = [&](int s, auto whole) {
     const intx4* q = reinterpret_cast<const intx4*>(w + 64 * s);
     Operand xo, wo;
@@ -290,7 +342,10 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
       }
     }
     xo.set(lo, hi);
-    acc = mul(wo, xo, acc);
+    if constexpr (BLK)
+      mul_scaled(wo, xo, xsp[s / 2] * wsp[s / 2], acc);
+    else
+      acc = mul(wo, xo, acc);
   };
   const int whole = min(s1, a.ldx / 64);  // steps that end within a row
 #pragma unroll 4
@@ -305,8 +360,8 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
     float v[1] = {0.f}, ws, bias;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[0] += sum[i][m][e % 32];
-    columns<1>(a, n, &ws, &bias);
-    v[0] = fmaf(v[0] * a.xs[m], ws, bias);
+    columns<1, BLK>(a, n, &ws, &bias);
+    v[0] = fmaf(v[0] * (BLK ? 1.f : a.xs[m]), ws, bias);
     activate(v, a.act, a.alpha);
     const int64_t at = (int64_t)m * a.N + n;
     if (a.r) v[0] += to_f32(static_cast<const T*>(a.r)[at]);
@@ -324,7 +379,41 @@ __global__ __launch_bounds__(256) void pad_rows_u8_kernel(const uint8_t* x, int6
   }
 }
 
+// Weights in blocks of 128 square: a workgroup a block, a row a wave's pass, two values a lane.
+__global__ __launch_bounds__(256) void quantise_tiles_kernel(const float* w, int N, int n, uint8_t* y, int ld,
+                                                             float* scales, float inv_unit) {
+  __shared__ float sh[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r0 = blockIdx.y * kScaleBlock, c0 = blockIdx.x * kScaleBlock;
+  const int r1 = min(r0 + kScaleBlock, N);
+  auto at = [&](int r, int c) { return c < n ? w[(int64_t)r * n + c] : 0.f; };
+  float top = 0.f;
+  for (int r = r0 + wave; r < r1; r += 4)
+    top = max_nan(top, max_nan(fabsf(at(r, c0 + lane)), fabsf(at(r, c0 + 64 + lane))));
+  top = group_reduce<64>(top, max_nan);
+  if (lane == 0) sh[wave] = top;
+  __syncthreads();
+  const RowScale rs = row_scale(max_nan(max_nan(sh[0], sh[1]), max_nan(sh[2], sh[3])));
+  for (int r = r0 + wave; r < r1; r += 4)
+#pragma unroll
+    for (int c = c0 + lane; c < c0 + kScaleBlock; c += 64)
+      y[(int64_t)r * ld + c] = (uint8_t)pack_e4m3(at(r, c) * rs.inv, 0.f, 0.f, 0.f);
+  if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = rs.scale * inv_unit;
+}
+
 }  // namespace
+
+void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y, int ld, float* scales,
+                    float unit) {
+  MNN_REQUIRE(ld == scale_blocks(n) * kScaleBlock, MNN_ERR_INVALID_ARGUMENT, "quantise_tiles: rows of whole blocks");
+  // up to 2^17 rows of blocks (N <= 2^24), 2^13 in a launch's y
+  for (int r0 = 0; r0 < N; r0 += kScaleBlock << 13) {
+    const int rows = std::min(N - r0, kScaleBlock << 13);
+    const dim3 grid((unsigned)scale_blocks(n), (unsigned)scale_blocks(rows));
+    launch(c, "quantise_tiles", quantise_tiles_kernel, grid, dim3(256), 0, w + (int64_t)r0 * n, rows, n,
+           y + (int64_t)r0 * ld, ld, scales + (int64_t)(r0 / kScaleBlock) * scale_blocks(n), 1.f / unit);
+  }
+}
 
 void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint8_t* y, int ld) {
   const dim3 grid((unsigned)std::min<int64_t>((rows * ld + 255) / 256, 1 << 20));
@@ -332,21 +421,31 @@ void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint
 }
 
 namespace {
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, bool BLK, int BM, int BN, int WM, int WN>
 void launch_tile(const LaunchCtx& c, const LinearE4m3Args& a, const char* name) {
   const int64_t tiles = (a.M + BM - 1) / BM * ((a.N + BN - 1) / BN);
   MNN_REQUIRE(tiles < (1 << 22), MNN_ERR_INVALID_CONFIGURATION, "Linear: too many rows in one call");
   constexpr int threads = BM / WM * (BN / WN) * 64;
-  launch(c, name, linear_e4m3_kernel<T, BM, BN, WM, WN>, dim3((unsigned)tiles), dim3(threads), 0, a);
+  launch(c, name, linear_e4m3_kernel<T, BLK, BM, BN, WM, WN>, dim3((unsigned)tiles), dim3(threads), 0, a);
 }
 
-template <class T>
+// The kernel's name in timings and traces.
+const char* tile_name(bool blocks, int tile, bool f32) {
+  static const char* const names[2][4][2] = {
+      {{"linear_e4m3_few_bf16", "linear_e4m3_few_f32"}, {"linear_e4m3_64_bf16", "linear_e4m3_64_f32"},
+       {"linear_e4m3_128_bf16", "linear_e4m3_128_f32"}, {"linear_e4m3_256_bf16", "linear_e4m3_256_f32"}},
+      {{"linear_blocks_few_bf16", "linear_blocks_few_f32"}, {"linear_blocks_64_bf16", "linear_blocks_64_f32"},
+       {"linear_blocks_128_bf16", "linear_blocks_128_f32"}, {"linear_blocks_256_bf16", "linear_blocks_256_f32"}}};
+  return names[blocks][tile][f32];
+}
+
+template <class T, bool BLK>
 void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   constexpr bool F32 = sizeof(T) == 4;
   MNN_REQUIRE(a.K % 128 == 0 && (a.ldx == a.K || a.M <= kLinearFew), MNN_ERR_INVALID_ARGUMENT,
               "linear_e4m3: rows of x are not padded");
   if (a.M <= kLinearFew)
-    return launch(c, F32 ? "linear_e4m3_few_f32" : "linear_e4m3_few_bf16", linear_e4m3_few_kernel<T>,
+    return launch(c, tile_name(BLK, 0, F32), linear_e4m3_few_kernel<T, BLK>,
                   dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
   // 256 square where the rounds of one tile a compute unit are 7/8 full: a third less widening a product, but one
   // workgroup a compute unit, whose last round costs a whole one. us at (M, K, N), 256 / 128 / 64 square: 8192 x 4096 x
@@ -355,21 +454,23 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   const int64_t cus = c.dev->props.multiProcessorCount;
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
-    return launch_tile<T, 256, 256, 128, 64>(c, a, F32 ? "linear_e4m3_256_f32" : "linear_e4m3_256_bf16");
+    return launch_tile<T, BLK, 256, 256, 128, 64>(c, a, tile_name(BLK, 3, F32));
   // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
   // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9
   if (4 * tiles(128) >= 3 * cus)
-    return launch_tile<T, 128, 128, 64, 32>(c, a, F32 ? "linear_e4m3_128_f32" : "linear_e4m3_128_bf16");
-  launch_tile<T, 64, 64, 32, 32>(c, a, F32 ? "linear_e4m3_64_f32" : "linear_e4m3_64_bf16");
+    return launch_tile<T, BLK, 128, 128, 64, 32>(c, a, tile_name(BLK, 2, F32));
+  launch_tile<T, BLK, 64, 64, 32, 32>(c, a, tile_name(BLK, 1, F32));
 }
 }  // namespace
 
 void linear_e4m3(const LaunchCtx& c, const LinearE4m3Args& a) {
   if (a.M <= 0) return;
+  if (a.blocks)
+    return a.out == MNN_F32 ? linear_e4m3_t<float, true>(c, a) : linear_e4m3_t<__bf16, true>(c, a);
   if (a.out == MNN_F32)
-    linear_e4m3_t<float>(c, a);
+    linear_e4m3_t<float, false>(c, a);
   else
-    linear_e4m3_t<__bf16>(c, a);
+    linear_e4m3_t<__bf16, false>(c, a);
 }
 
 }  // namespace k

@@ -1,6 +1,7 @@
 // RMS norm with the residual's addition before it and an output of 32, 16 or 8 bits:
 // h = x + r, y = h * rsqrt(mean(h^2) + eps) * w, and for 8 bits q = e4m3(y * (448 * (1 / max|y|))) with
-// the row's scale max|y| * (1 / 448). Without weights, the rows of x are rounded to 8 bits as they are.
+// the row's scale max|y| * (1 / 448), or such a maximum and scale for each block of 128 values. Without
+// weights, the rows of x are rounded to 8 bits as they are.
 // h, its sum of squares and y stay in fp32; the norm is taken of h before it is rounded to the sum's type.
 #include "token_ops.hpp"
 #include "token_utils.hpp"
@@ -70,12 +71,35 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
     }
     auto y = [&](int i, float hv) { return a.w ? hv * s * norm * a.w[i] : hv; };
     RowScale rs{1.f, 1.f};
-    if (a.out == MNN_E4M3) {
+    if (a.out == MNN_E4M3 && !a.blocks) {
       float top = 0.f;
       for (int i = threadIdx.x; i < a.F; i += 256) top = max_nan(top, fabsf(y(i, h(i))));
       rs = row_scale(block_reduce(top, sh, max_nan));
     }
     __syncthreads();  // every read of the row's other passes is done
+    if (a.blocks) {  // a wave a block, two values a lane
+      const int nb = scale_blocks(a.F), lane = threadIdx.x & 63;
+      for (int64_t i0 = (threadIdx.x >> 6) * kScaleBlock; i0 < a.ldy; i0 += 4 * kScaleBlock) {
+        float hv[2], v[2], top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t i = i0 + lane + 64 * e;
+          hv[e] = i < a.F ? h((int)i) : 0.f;
+          v[e] = i < a.F ? y((int)i, hv[e]) : 0.f;
+          top = max_nan(top, fabsf(v[e]));
+        }
+        const RowScale bs = row_scale(group_reduce<64>(top, max_nan));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t i = i0 + lane + 64 * e;
+          if (sum && i < a.F) sum[at + i] = from_f32<T>(hv[e]);
+          if (i < a.ldy)
+            static_cast<uint8_t*>(a.y)[row * a.ldy + i] = (uint8_t)pack_e4m3(v[e] * bs.inv, 0.f, 0.f, 0.f);
+        }
+        if (lane == 0 && i0 < a.F) a.scales[row * nb + i0 / kScaleBlock] = bs.scale;
+      }
+      continue;
+    }
     for (int64_t i = threadIdx.x; i < a.ldy; i += 256) {
       const float hv = i < a.F ? h((int)i) : 0.f;
       const float v = i < a.F ? y((int)i, hv) : 0.f;
@@ -97,7 +121,9 @@ __global__ __launch_bounds__(256) void rmsnorm_any_kernel(RmsNormArgs a) {
 // row. The weights stay there too, over all the rows that a workgroup takes. Bound by memory (up to two loads
 // and two stores a value): 65537 x 2048 bf16 with residual, sum and e4m3 output 175 us, 5.4 TB/s; 6436 x 2048 f32
 // 32 us; 10752 x 384 bf16 9.7 us.
-template <class T, int NV, int W, mnn_dtype OUT>
+//
+// BLK: scales of blocks, whose 128 values lie in neighbouring lanes of one chunk.
+template <class T, int NV, int W, mnn_dtype OUT, bool BLK = false>
 __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
   constexpr int VE = 16 / (int)sizeof(T);
   typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
@@ -204,22 +230,40 @@ __global__ __launch_bounds__(256) void rmsnorm_rows_kernel(RmsNormArgs a) {
         for (int e = 0; e < VE; ++e) h[i][e] = h[i][e] * norm * w[i][e];
     }
     if constexpr (OUT == MNN_E4M3) {
-      float top = 0.f;
+      float inv[NV];
+      if constexpr (BLK) {
+        constexpr int L = kScaleBlock / VE;  // lanes a block
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+          float top = 0.f;
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (on[i]) top = max_nan(top, fabsf(h[i][e]));
-      const RowScale rs = row_scale(over_row(top, 1, max_nan));
-      if (lane == 0 && (W == 1 || wave == 0)) a.scales[row] = rs.scale;
+          for (int e = 0; e < VE; ++e)
+            if (on[i]) top = max_nan(top, fabsf(h[i][e]));
+          const RowScale rs = row_scale(group_reduce<L>(top, max_nan));
+          inv[i] = rs.inv;
+          const int first = col + 64 * W * VE * i;
+          if (lane % L == 0 && first < a.F) a.scales[row * scale_blocks(a.F) + first / kScaleBlock] = rs.scale;
+        }
+      } else {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if (on[i]) top = max_nan(top, fabsf(h[i][e]));
+        const RowScale rs = row_scale(over_row(top, 1, max_nan));
+        if (lane == 0 && (W == 1 || wave == 0)) a.scales[row] = rs.scale;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) inv[i] = rs.inv;
+      }
       uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy + col;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         unsigned q[VE / 4];
 #pragma unroll
         for (int e = 0; e < VE / 4; ++e)
-          q[e] = on[i] ? pack_e4m3(h[i][4 * e] * rs.inv, h[i][4 * e + 1] * rs.inv, h[i][4 * e + 2] * rs.inv,
-                                   h[i][4 * e + 3] * rs.inv)
+          q[e] = on[i] ? pack_e4m3(h[i][4 * e] * inv[i], h[i][4 * e + 1] * inv[i], h[i][4 * e + 2] * inv[i],
+                                   h[i][4 * e + 3] * inv[i])
                        : 0u;
         if (col + 64 * W * VE * i < a.ldy) {
           if constexpr (VE == 4)
@@ -258,7 +302,9 @@ void launch_rows(const LaunchCtx& c, const RmsNormArgs& a) {
   // eight workgroups a compute unit keep their weights over several rows
   const int64_t wgs = W == 1 ? (a.rows + 3) / 4 : a.rows;
   const dim3 grid((unsigned)std::min<int64_t>(wgs, 8 * c.dev->props.multiProcessorCount));
-  if (a.out == MNN_E4M3)
+  if (a.out == MNN_E4M3 && a.blocks)
+    launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_E4M3, true>, grid, dim3(256), 0, a);
+  else if (a.out == MNN_E4M3)
     launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_E4M3>, grid, dim3(256), 0, a);
   else if (a.out == MNN_BF16)
     launch(c, name, rmsnorm_rows_kernel<T, NV, W, MNN_BF16>, grid, dim3(256), 0, a);

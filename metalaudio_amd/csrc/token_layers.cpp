@@ -1,5 +1,6 @@
 // Argument checks and launch planning of the token layers; the arithmetic is in k_rmsnorm.hip,
-// k_linear_e4m3.hip, k_rotary.hip, k_window.hip and k_window_step.hip.
+// k_linear_e4m3.hip, k_rotary.hip, k_window.hip, k_window_step.hip, k_kv_cache.hip, k_memory.hip and
+// k_rows.hip.
 #include "token_layers.hpp"
 
 #include <algorithm>
@@ -66,6 +67,36 @@ void split_heads(const char* what, const Shape& s, int64_t hd, int64_t& B, int64
   n = s.back() / hd;
 }
 
+// What a call writes is no input of it, and no two of its outputs are one tensor.
+void check_apart(const char* what, std::initializer_list<const Tensor*> inputs,
+                 std::initializer_list<const Tensor*> written) {
+  for (auto w = written.begin(); w != written.end(); ++w) {
+    for (const Tensor* t : inputs)
+      MNN_REQUIRE(!same(*w, t), MNN_ERR_INVALID_ARGUMENT, what << ": an output or cache is an input");
+    for (auto u = written.begin(); u != w; ++u)
+      MNN_REQUIRE(!same(*w, *u), MNN_ERR_INVALID_ARGUMENT,
+                  what << ": outputs, caches and scales must be tensors of their own");
+  }
+}
+
+// Scales [.., n, heads] of 8-bit rows [.., n, heads * hd].
+void check_scales(const char* what, const Tensor& scales, const Tensor& rows, int heads) {
+  MNN_REQUIRE(scales.dtype == MNN_F32, MNN_ERR_INVALID_ARGUMENT, what << ": scales must be f32");
+  Shape want = rows.shape;
+  want.back() = heads;
+  MNN_REQUIRE(scales.shape == want, MNN_ERR_SHAPE_MISMATCH,
+              what << ": scales " << shape_str(scales.shape) << ", expected " << shape_str(want));
+}
+
+// An i32 tensor of one value for each of B streams, where given.
+void check_counts(const char* what, const Tensor* t, int64_t B, const char* names) {
+  if (!t) return;
+  MNN_REQUIRE(t->dtype == MNN_I32, MNN_ERR_INVALID_ARGUMENT, what << ": " << names << " must be i32");
+  MNN_REQUIRE(t->count() == B, MNN_ERR_BUFFER_SIZE_MISMATCH,
+              what << ": " << t->count() << " " << names << " for a batch of " << B);
+}
+const int* i32(const Tensor* t) { return t ? static_cast<const int*>(t->data) : nullptr; }
+
 // ------------------------------------------------------------------ RMSNorm
 class RMSNormLayer : public Layer {
  public:
@@ -105,8 +136,11 @@ class RMSNormLayer : public Layer {
     for (const Tensor* t : {res, (const Tensor*)sum, (const Tensor*)&out})
       MNN_REQUIRE(!t || t->count() == in.count(), MNN_ERR_BUFFER_SIZE_MISMATCH,
                   "RMSNorm: " << shape_str(t->shape) << " beside an input of " << shape_str(in.shape));
-    MNN_REQUIRE(!scales || scales->count() == rows, MNN_ERR_BUFFER_SIZE_MISMATCH,
-                "RMSNorm: " << scales->count() << " scales for " << rows << " rows");
+    const int64_t blocks = k::scale_blocks(F_);
+    MNN_REQUIRE(!scales || scales->count() == rows || scales->count() == rows * blocks,
+                MNN_ERR_BUFFER_SIZE_MISMATCH,
+                "RMSNorm: " << scales->count() << " scales for " << rows << " rows of " << blocks
+                            << " blocks");
     MNN_REQUIRE(!same(sum, &out), MNN_ERR_INVALID_ARGUMENT, "RMSNorm: sum and output are one tensor");
     for (const Tensor* t : {&in, res, (const Tensor*)sum, (const Tensor*)&out})
       MNN_REQUIRE(!same(scales, t), MNN_ERR_INVALID_ARGUMENT,
@@ -122,6 +156,7 @@ class RMSNormLayer : public Layer {
     a.y = out.data;
     a.out = out.dtype;
     a.scales = scales ? scales->f32() : nullptr;
+    a.blocks = scales && scales->count() != rows;  // of rows of one block, the two are the same
     a.rows = rows;
     a.F = F_;
     a.ldy = F_;
@@ -137,11 +172,11 @@ class RMSNormLayer : public Layer {
 
 // ------------------------------------------------------------------ Linear in 8 bits
 // Weights are kept as e4m3 rows, padded with zeros to a multiple of the product's depth step, beside one
-// scale a row; no fp32 copy stays on the device.
+// scale a row or, in blocks, one for each 128 x 128; no fp32 copy stays on the device.
 class LinearE4m3Layer : public Layer {
  public:
-  LinearE4m3Layer(Device* d, int in, int out, bool bias, int act, float alpha)
-      : Layer(d), in_(in), out_(out), act_(act), alpha_(alpha) {
+  LinearE4m3Layer(Device* d, int in, int out, bool bias, int act, float alpha, bool blocks)
+      : Layer(d), in_(in), out_(out), act_(act), alpha_(alpha), blocks_(blocks), kb_(blocks ? k::scale_blocks(in) : 1) {
     MNN_REQUIRE(in > 0 && out > 0, MNN_ERR_INVALID_CONFIGURATION, "Linear: sizes must be > 0");
     MNN_REQUIRE(in <= (1 << 20) && out <= (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
                 "Linear: more than 2^20 inputs or 2^24 outputs in 8 bits");
@@ -151,9 +186,10 @@ class LinearE4m3Layer : public Layer {
     kp_ = (in + 127) / 128 * 128;
     dev_->make_current();
     wq_.reserve((size_t)out * kp_);
-    ws_.reserve(sizeof(float) * out);
+    const size_t scales = blocks ? (size_t)k::scale_blocks(out) * kb_ : out;
+    ws_.reserve(sizeof(float) * scales);
     HIP_CHECK(hipMemset(wq_.ptr, 0, (size_t)out * kp_));  // zero until loaded
-    HIP_CHECK(hipMemset(ws_.ptr, 0, sizeof(float) * out));
+    HIP_CHECK(hipMemset(ws_.ptr, 0, sizeof(float) * scales));
     HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream read them
   }
   const char* kind() const override { return "Linear"; }
@@ -202,17 +238,20 @@ class LinearE4m3Layer : public Layer {
     for (const Tensor* t : {res, (const Tensor*)&out})
       MNN_REQUIRE(!t || t->count() == rows * out_, MNN_ERR_BUFFER_SIZE_MISMATCH,
                   "Linear: " << shape_str(t->shape) << " for " << rows << " rows of " << out_);
-    MNN_REQUIRE(!scales || scales->count() == rows, MNN_ERR_BUFFER_SIZE_MISMATCH,
-                "Linear: " << scales->count() << " scales for " << rows << " rows");
+    MNN_REQUIRE(!scales || scales->count() == rows * kb_, MNN_ERR_BUFFER_SIZE_MISMATCH,
+                "Linear: " << scales->count() << " scales for " << rows << " rows of " << kb_
+                           << (blocks_ ? " blocks" : ""));
     MNN_REQUIRE(!same(&in, &out) && !same(scales, &out), MNN_ERR_INVALID_ARGUMENT,
                 "Linear: output is the input or its scales");
     if (rows == 0) return;
     k::LinearE4m3Args g;
+    g.blocks = blocks_;
+    g.unit = unit_;
     g.x = static_cast<const uint8_t*>(in.data);
     g.xs = scales ? scales->f32() : nullptr;
     if (!scales) {  // rows rounded to 8 bits first, their scales behind them
       const size_t bytes = (size_t)rows * kp_;
-      uint8_t* x = static_cast<uint8_t*>(scratch_.get(bytes + sizeof(float) * rows));
+      uint8_t* x = static_cast<uint8_t*>(scratch_.get(bytes + sizeof(float) * rows * kb_));
       float* xs = reinterpret_cast<float*>(x + bytes);
       k::RmsNormArgs a;
       a.x = in.data;
@@ -220,6 +259,7 @@ class LinearE4m3Layer : public Layer {
       a.y = x;
       a.out = MNN_E4M3;
       a.scales = xs;
+      a.blocks = blocks_;
       a.rows = rows;
       a.F = in_;
       a.ldy = kp_;
@@ -252,6 +292,15 @@ class LinearE4m3Layer : public Layer {
     DevBuf w;  // the fp32 rows, only while they are rounded
     w.reserve(sizeof(float) * in_ * out_);
     HIP_CHECK(hipMemcpy(w.ptr, data, sizeof(float) * in_ * out_, hipMemcpyHostToDevice));
+    const LaunchCtx c{dev_, dev_->default_stream};
+    if (blocks_) {
+      float top = 512.f;
+      for (size_t i = 0; i < (size_t)in_ * out_; ++i) top = std::max(top, std::fabs(data[i]));
+      unit_ = std::ldexp(1.f, std::ilogb(top) - 9);  // about the largest scale, where that is above 1
+      k::quantise_tiles(c, w.f32(), out_, in_, wq_.as<uint8_t>(), kp_, ws_.f32(), unit_);
+      HIP_CHECK(hipStreamSynchronize(c.stream));
+      return;
+    }
     k::RmsNormArgs a;
     a.x = w.ptr;
     a.in = MNN_F32;
@@ -261,12 +310,14 @@ class LinearE4m3Layer : public Layer {
     a.rows = out_;
     a.F = in_;
     a.ldy = kp_;
-    const LaunchCtx c{dev_, dev_->default_stream};
     k::rmsnorm(c, a);
     HIP_CHECK(hipStreamSynchronize(c.stream));
   }
   int in_, out_, act_, kp_ = 0;
   float alpha_;
+  bool blocks_;
+  int kb_;  // scales a row of the input
+  float unit_ = 1.f;
   Param* b_ = nullptr;
   DevBuf wq_, ws_;
   Scratch scratch_;
@@ -411,7 +462,7 @@ class WindowAttentionLayer : public ManyInputLayer {
     k::window_attention(ctx(s), a);
   }
   void step(const Tensor& q, const Tensor& kt, const Tensor& v, const Tensor& pos, const Tensor* steps,
-            Tensor& kc, Tensor& vc, Tensor& out, Stream& s) {
+            Tensor& kc, Tensor* ks, Tensor& vc, Tensor* vs, Tensor& out, Stream& s) {
     MNN_REQUIRE(d_.window_right == 0, MNN_ERR_INVALID_CONFIGURATION,
                 "WindowAttention: a step has no tokens to come (window_right "
                     << d_.window_right << ")");
@@ -421,8 +472,8 @@ class WindowAttentionLayer : public ManyInputLayer {
                 "WindowAttention: " << T << " new tokens in one step, at most 65535");
     const int64_t kvw = (int64_t)d_.num_kv_heads * d_.head_dim;
     for (const Tensor* c : {&kc, &vc}) {
-      MNN_REQUIRE(c->dtype == q.dtype, MNN_ERR_INVALID_ARGUMENT,
-                  "WindowAttention: the caches have the type of q");
+      MNN_REQUIRE(c->dtype == (ks ? MNN_E4M3 : q.dtype), MNN_ERR_INVALID_ARGUMENT,
+                  "WindowAttention: the caches " << (ks ? "with scales are e4m3" : "have the type of q"));
       MNN_REQUIRE(c->shape.size() == 3 && c->shape[0] == B && c->shape[2] == kvw &&
                       c->shape == kc.shape,
                   MNN_ERR_SHAPE_MISMATCH, "WindowAttention: cache " << shape_str(c->shape)
@@ -439,17 +490,11 @@ class WindowAttentionLayer : public ManyInputLayer {
         MNN_REQUIRE(t->count() == B, MNN_ERR_BUFFER_SIZE_MISMATCH,
                     "WindowAttention: " << t->count() << " positions or steps for a batch of " << B);
       }
-    const Tensor* written[3] = {&kc, &vc, &out};
-    for (int i = 0; i < 3; ++i) {
-      for (const Tensor* t : {&q, &kt, &v, &pos, steps})
-        MNN_REQUIRE(!same(written[i], t), MNN_ERR_INVALID_ARGUMENT,
-                    "WindowAttention: an output or cache is an input");
-      for (int j = 0; j < i; ++j)
-        MNN_REQUIRE(!same(written[i], written[j]), MNN_ERR_INVALID_ARGUMENT,
-                    "WindowAttention: output and caches must be three tensors");
-    }
+    for (const Tensor* c : {ks, vs})
+      if (c) check_scales("WindowAttention", *c, kc, d_.num_kv_heads);
+    check_apart("WindowAttention", {&q, &kt, &v, &pos, steps}, {&kc, &vc, &out, ks, vs});
     if (B * T == 0) return;
-    k::WindowStepArgs a;
+    k::WindowStepHeldArgs a;
     a.q = q.data;
     a.k = kt.data;
     a.v = v.data;
@@ -468,6 +513,13 @@ class WindowAttentionLayer : public ManyInputLayer {
     a.left = d_.window_left;
     a.sinks = d_.sinks;
     a.scale = d_.scale;
+    if (ks) {
+      a.ks = ks->f32();
+      a.vs = vs->f32();
+      const int64_t part = k::window_step_e4m3_part_floats(ctx(s), a);
+      return k::window_step_e4m3(ctx(s), a,
+                                 part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
+    }
     const int64_t part = k::window_step_part_floats(ctx(s), a);
     k::window_step(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
   }
@@ -501,6 +553,151 @@ class WindowAttentionLayer : public ManyInputLayer {
   Scratch scratch_;
 };
 
+// ------------------------------------------------------------------ rolling caches
+class KVCacheLayer : public ManyInputLayer {
+ public:
+  KVCacheLayer(Device* d, int kv_heads, int hd, int sinks)
+      : ManyInputLayer(d), KV_(kv_heads), hd_(hd), sinks_(sinks) {
+    MNN_REQUIRE(kv_heads > 0 && kv_heads <= 65535, MNN_ERR_INVALID_CONFIGURATION,
+                "KVCache: " << kv_heads << " heads");
+    MNN_REQUIRE(hd > 0 && hd % 8 == 0 && hd <= 128, MNN_ERR_INVALID_CONFIGURATION,
+                "KVCache: head dim " << hd << " is no multiple of 8 up to 128");
+    MNN_REQUIRE(sinks >= 0 && sinks <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
+                "KVCache: sinks must be 0..2^30");
+  }
+  const char* kind() const override { return "KVCache"; }
+  Shape input_shape() const override { return {0, (int64_t)KV_ * hd_}; }
+  Shape output_shape() const override { return input_shape(); }
+  // rows to the caches, or back
+  void run(const Tensor& kt, const Tensor& v, const Tensor& pos, const Tensor* steps, const Tensor& kc,
+           const Tensor* ks, const Tensor& vc, const Tensor* vs, bool write, Stream& s) {
+    const char* const what = "KVCache";
+    const int64_t kvw = (int64_t)KV_ * hd_;
+    MNN_REQUIRE(is_float(kt) && v.dtype == kt.dtype, MNN_ERR_INVALID_ARGUMENT,
+                "KVCache: k and v must both be f32 or both bf16");
+    MNN_REQUIRE(kt.shape.size() == 3 && kt.shape[2] == kvw && v.shape == kt.shape,
+                MNN_ERR_SHAPE_MISMATCH, "KVCache: k " << shape_str(kt.shape) << " and v "
+                                            << shape_str(v.shape) << ", expected [B, T, " << kvw << "]");
+    const int64_t B = kt.shape[0], T = kt.shape[1];
+    MNN_REQUIRE(B <= 65535 && T <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
+                "KVCache: batch " << B << " or " << T << " tokens too large");
+    MNN_REQUIRE(kc.dtype == vc.dtype && (kc.dtype == kt.dtype || kc.dtype == MNN_E4M3),
+                MNN_ERR_INVALID_ARGUMENT, "KVCache: the caches have the type of k or are e4m3");
+    MNN_REQUIRE((kc.dtype == MNN_E4M3) == (ks != nullptr) && (ks != nullptr) == (vs != nullptr),
+                MNN_ERR_INVALID_ARGUMENT, "KVCache: scales go with e4m3 caches");
+    MNN_REQUIRE(kc.shape.size() == 3 && kc.shape[0] == B && kc.shape[2] == kvw && vc.shape == kc.shape,
+                MNN_ERR_SHAPE_MISMATCH,
+                "KVCache: caches " << shape_str(kc.shape) << " and " << shape_str(vc.shape)
+                                   << ", expected [" << B << ", slots, " << kvw << "]");
+    MNN_REQUIRE(kc.shape[1] > sinks_ && kc.shape[1] <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
+                "KVCache: " << kc.shape[1] << " slots beside " << sinks_ << " sinks, at most 2^30");
+    for (const Tensor* c : {ks, vs})
+      if (c) check_scales(what, *c, kc, KV_);
+    check_counts(what, &pos, B, "positions");
+    check_counts(what, steps, B, "steps");
+    if (write)
+      check_apart(what, {&kt, &v, &pos, steps}, {&kc, &vc, ks, vs});
+    else
+      check_apart(what, {&kc, &vc, ks, vs, &pos, steps}, {&kt, &v});
+    if (B * T == 0) return;
+    k::KVCacheArgs a;
+    a.rows[0] = kt.data;
+    a.rows[1] = v.data;
+    a.cache[0] = kc.data;
+    a.cache[1] = vc.data;
+    a.scales[0] = ks ? ks->f32() : nullptr;
+    a.scales[1] = vs ? vs->f32() : nullptr;
+    a.type = kt.dtype;
+    a.pos = i32(&pos);
+    a.steps = i32(steps);
+    a.B = (int)B;
+    a.T = (int)T;
+    a.C = (int)kc.shape[1];
+    a.KV = KV_;
+    a.hd = hd_;
+    a.sinks = sinks_;
+    if (write)
+      k::kv_cache_write(ctx(s), a);
+    else
+      k::kv_cache_read(ctx(s), a);
+  }
+
+ private:
+  int KV_, hd_, sinks_;
+};
+
+// ------------------------------------------------------------------ attention to an encoder's states
+class MemoryAttentionLayer : public ManyInputLayer {
+ public:
+  MemoryAttentionLayer(Device* d, const mnn_memory_attention_desc& desc) : ManyInputLayer(d), d_(desc) {
+    MNN_REQUIRE(desc.num_heads > 0 && desc.num_kv_heads > 0 && desc.num_heads <= 65535 &&
+                    desc.num_heads % desc.num_kv_heads == 0,
+                MNN_ERR_INVALID_CONFIGURATION,
+                "MemoryAttention: " << desc.num_heads << " heads on " << desc.num_kv_heads);
+    MNN_REQUIRE(desc.head_dim > 0 && desc.head_dim % 8 == 0 && desc.head_dim <= 128,
+                MNN_ERR_INVALID_CONFIGURATION,
+                "MemoryAttention: head dim " << desc.head_dim << " is no multiple of 8 up to 128");
+    MNN_REQUIRE(std::isfinite(desc.scale), MNN_ERR_INVALID_CONFIGURATION,
+                "MemoryAttention: scale must be finite");
+    if (d_.scale == 0.f) d_.scale = 1.f / std::sqrt((float)desc.head_dim);
+  }
+  const char* kind() const override { return "MemoryAttention"; }
+  Shape input_shape() const override { return {0, (int64_t)d_.num_heads * d_.head_dim}; }
+  Shape output_shape() const override { return input_shape(); }
+  void run(const Tensor& q, const Tensor& kt, const Tensor* ks, const Tensor& v, const Tensor* vs,
+           const Tensor* qlen, const Tensor* len, Tensor& out, Stream& s) {
+    const char* const what = "MemoryAttention";
+    int64_t B, T, b, S, n;
+    split_heads(what, q.shape, d_.head_dim, B, T, n);
+    MNN_REQUIRE(n == d_.num_heads, MNN_ERR_SHAPE_MISMATCH,
+                "MemoryAttention: q " << shape_str(q.shape) << " has " << n << " heads, expected "
+                                      << d_.num_heads);
+    split_heads(what, kt.shape, d_.head_dim, b, S, n);
+    MNN_REQUIRE(b == B && n == d_.num_kv_heads && v.shape == kt.shape, MNN_ERR_SHAPE_MISMATCH,
+                "MemoryAttention: k " << shape_str(kt.shape) << " and v " << shape_str(v.shape)
+                                      << " beside q " << shape_str(q.shape));
+    MNN_REQUIRE(is_float(q) && out.dtype == q.dtype, MNN_ERR_INVALID_ARGUMENT,
+                "MemoryAttention: q and output must both be f32 or both bf16");
+    MNN_REQUIRE(kt.dtype == v.dtype && (kt.dtype == q.dtype || kt.dtype == MNN_E4M3),
+                MNN_ERR_INVALID_ARGUMENT, "MemoryAttention: k and v have the type of q or are e4m3");
+    MNN_REQUIRE((kt.dtype == MNN_E4M3) == (ks != nullptr) && (ks != nullptr) == (vs != nullptr),
+                MNN_ERR_INVALID_ARGUMENT, "MemoryAttention: scales go with e4m3 states");
+    for (const Tensor* c : {ks, vs})
+      if (c) check_scales(what, *c, kt, d_.num_kv_heads);
+    MNN_REQUIRE(out.count() == q.count(), MNN_ERR_BUFFER_SIZE_MISMATCH,
+                "MemoryAttention: output " << shape_str(out.shape) << " for q " << shape_str(q.shape));
+    MNN_REQUIRE(B <= 65535 && T <= (1 << 24) && S <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
+                "MemoryAttention: batch " << B << ", " << T << " tokens or " << S << " states too large");
+    check_counts(what, qlen, B, "query lengths");
+    check_counts(what, len, B, "lengths");
+    check_apart(what, {&q, &kt, ks, &v, vs, qlen, len}, {&out});
+    if (B * T == 0) return;
+    k::MemoryArgs a;
+    a.q = q.data;
+    a.k = kt.data;
+    a.v = v.data;
+    a.ks = ks ? ks->f32() : nullptr;
+    a.vs = vs ? vs->f32() : nullptr;
+    a.o = out.data;
+    a.type = q.dtype;
+    a.qlen = i32(qlen);
+    a.len = i32(len);
+    a.B = (int)B;
+    a.T = (int)T;
+    a.S = (int)S;
+    a.H = d_.num_heads;
+    a.KV = d_.num_kv_heads;
+    a.hd = d_.head_dim;
+    a.scale = d_.scale;
+    const int64_t part = k::memory_part_floats(ctx(s), a);
+    k::memory_attention(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
+  }
+
+ private:
+  mnn_memory_attention_desc d_;
+  Scratch scratch_;
+};
+
 }  // namespace
 
 std::unique_ptr<Layer> make_rmsnorm(Device* d, int features, float eps) {
@@ -512,12 +709,12 @@ void rmsnorm_forward_residual(Layer* l, const Tensor& in, const Tensor* res, Ten
 }
 
 std::unique_ptr<Layer> make_linear_e4m3(Device* d, int in, int out, bool bias, int act,
-                                        float leaky_alpha) {
-  return std::make_unique<LinearE4m3Layer>(d, in, out, bias, act, leaky_alpha);
+                                        float leaky_alpha, bool blocks) {
+  return std::make_unique<LinearE4m3Layer>(d, in, out, bias, act, leaky_alpha, blocks);
 }
 void linear_forward_scaled(Layer* l, const Tensor& in, const Tensor* scales, const Tensor* res,
                            Tensor& out, Stream& s) {
-  as<LinearE4m3Layer>(l, "mnn_linear_forward_scaled (precision e4m3)").run(in, scales, res, out, s);
+  as<LinearE4m3Layer>(l, "mnn_linear_forward_scaled (precision e4m3 or e4m3_block)").run(in, scales, res, out, s);
 }
 
 std::unique_ptr<Layer> make_rotary(Device* d, const mnn_rotary_desc& desc) {
@@ -539,7 +736,38 @@ void window_attention_step(Layer* l, const Tensor& q, const Tensor& kt, const Te
                            const Tensor& pos, const Tensor* steps, Tensor& k_cache, Tensor& v_cache,
                            Tensor& out, Stream& s) {
   as<WindowAttentionLayer>(l, "mnn_window_attention_step")
-      .step(q, kt, v, pos, steps, k_cache, v_cache, out, s);
+      .step(q, kt, v, pos, steps, k_cache, nullptr, v_cache, nullptr, out, s);
+}
+void window_attention_step_e4m3(Layer* l, const Tensor& q, const Tensor& kt, const Tensor& v,
+                                const Tensor& pos, const Tensor* steps, Tensor& k_cache, Tensor& k_scales,
+                                Tensor& v_cache, Tensor& v_scales, Tensor& out, Stream& s) {
+  as<WindowAttentionLayer>(l, "mnn_window_attention_step_e4m3")
+      .step(q, kt, v, pos, steps, k_cache, &k_scales, v_cache, &v_scales, out, s);
+}
+
+std::unique_ptr<Layer> make_kv_cache(Device* d, int kv_heads, int head_dim, int sinks) {
+  return std::make_unique<KVCacheLayer>(d, kv_heads, head_dim, sinks);
+}
+void kv_cache_write(Layer* l, const Tensor& kt, const Tensor& v, const Tensor& pos, const Tensor* steps,
+                    Tensor& k_cache, Tensor* k_scales, Tensor& v_cache, Tensor* v_scales, Stream& s) {
+  as<KVCacheLayer>(l, "mnn_kv_cache_write")
+      .run(kt, v, pos, steps, k_cache, k_scales, v_cache, v_scales, true, s);
+}
+void kv_cache_read(Layer* l, const Tensor& k_cache, const Tensor* k_scales, const Tensor& v_cache,
+                   const Tensor* v_scales, const Tensor& pos, const Tensor* steps, Tensor& kt, Tensor& v,
+                   Stream& s) {
+  as<KVCacheLayer>(l, "mnn_kv_cache_read")
+      .run(kt, v, pos, steps, k_cache, k_scales, v_cache, v_scales, false, s);
+}
+
+std::unique_ptr<Layer> make_memory_attention(Device* d, const mnn_memory_attention_desc& desc) {
+  return std::make_unique<MemoryAttentionLayer>(d, desc);
+}
+void memory_attention_forward(Layer* l, const Tensor& q, const Tensor& kt, const Tensor* k_scales,
+                              const Tensor& v, const Tensor* v_scales, const Tensor* query_lengths,
+                              const Tensor* lengths, Tensor& out, Stream& s) {
+  as<MemoryAttentionLayer>(l, "mnn_memory_attention_forward")
+      .run(q, kt, k_scales, v, v_scales, query_lengths, lengths, out, s);
 }
 
 }  // namespace mnn

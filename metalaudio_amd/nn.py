@@ -15,13 +15,13 @@ import numpy as np
 
 from . import _lib
 from ._lib import (ACT, DTYPE, PAD, PRECISION, Conv1dDesc, Conv2dDesc, ConvTranspose1dDesc,
-                   ConvTranspose2dDesc, DecoderBlockDesc, EncoderBlockDesc, FreqBlockDesc, MNNError,
-                   RotaryDesc, SeparatorDesc, WindowAttentionDesc, check, dims, lib)
+                   ConvTranspose2dDesc, DecoderBlockDesc, EncoderBlockDesc, FreqBlockDesc,
+                   MemoryAttentionDesc, MNNError, RotaryDesc, SeparatorDesc, WindowAttentionDesc, check, dims, lib)
 
 __all__ = [
     "MNNError", "AudioDevice", "Stream", "Tensor", "Layer", "Conv1D", "DynamicConv1D",
     "FusedConv1D", "GroupNorm", "LayerNorm", "RMSNorm", "GELU", "GLU", "Linear", "FusedLinear",
-    "Rotary", "WindowAttention", "MultiHeadAttention", "CrossAttention",
+    "Rotary", "WindowAttention", "KVCache", "MemoryAttention", "MultiHeadAttention", "CrossAttention",
     "FeedForward", "UNetEncoderBlock", "ConvTranspose1D", "DynamicConvTranspose1D",
     "UNetDecoderBlock", "unet_padding", "unet_bottleneck_length", "TransformerLayer",
     "CrossTransformerEncoder", "Sequential", "SafeTensors", "BinaryModelFile", "WeightNameMapper",
@@ -383,8 +383,8 @@ class RMSNorm(Layer):
     def forward_residual(self, input: Tensor, residual: Optional[Tensor], output: Tensor,
                          sum: Optional[Tensor] = None, scales: Optional[Tensor] = None,
                          stream: Optional[Stream] = None) -> None:
-        """sum = input + residual; output = RMSNorm(sum), in 8 bits with `scales` per row where
-        the output is "e4m3"."""
+        """sum = input + residual; output = RMSNorm(sum), in 8 bits with `scales` per row, or per
+        128 values of one, where the output is "e4m3"."""
         check(lib().mnn_rmsnorm_forward_residual(self.handle, input.handle, _th(residual),
                                                  _th(sum), output.handle, _th(scales),
                                                  _sh(stream)))
@@ -402,8 +402,8 @@ class GLU(Layer):
 
 
 class Linear(Layer):
-    """Linear (Linear.swift:27-460); precision "f32", "bf16", or "e4m3": weights and input in 8
-    bits with a scale per row."""
+    """Linear (Linear.swift:27-460); precision "f32", "bf16", or weights and input in 8 bits, with
+    a scale per row ("e4m3") or per block of 128 ("e4m3_block")."""
 
     def __init__(self, device, input_features, output_features, use_bias=True, activation="none",
                  precision="f32", leaky_relu_alpha=None):
@@ -426,8 +426,8 @@ class Linear(Layer):
     def forward_scaled(self, input: Tensor, scales: Optional[Tensor], output: Tensor,
                        residual: Optional[Tensor] = None,
                        stream: Optional[Stream] = None) -> None:
-        """Precision "e4m3": output = act(input W^T + bias) + residual, input "e4m3" with its row
-        scales, or "f32" / "bf16" without."""
+        """Precision "e4m3" or "e4m3_block": output = act(input W^T + bias) + residual, input "e4m3"
+        with its scales, per row or per 128 values of one, or "f32" / "bf16" without."""
         check(lib().mnn_linear_forward_scaled(self.handle, input.handle, _th(scales),
                                               _th(residual), output.handle, _sh(stream)))
 
@@ -478,12 +478,60 @@ class WindowAttention(Layer):
 
     def step(self, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, k_cache: Tensor,
              v_cache: Tensor, output: Tensor, steps: Optional[Tensor] = None,
-             stream: Optional[Stream] = None) -> None:
+             stream: Optional[Stream] = None, k_scales: Optional[Tensor] = None,
+             v_scales: Optional[Tensor] = None) -> None:
         """The streams' next tokens on their rolling caches (causal); see
-        mnn_window_attention_step."""
-        check(lib().mnn_window_attention_step(self.handle, q.handle, k.handle, v.handle,
-                                              positions.handle, _th(steps), k_cache.handle,
-                                              v_cache.handle, output.handle, _sh(stream)))
+        mnn_window_attention_step, and with scales mnn_window_attention_step_e4m3."""
+        if k_scales is None and v_scales is None:
+            check(lib().mnn_window_attention_step(self.handle, q.handle, k.handle, v.handle,
+                                                  positions.handle, _th(steps), k_cache.handle,
+                                                  v_cache.handle, output.handle, _sh(stream)))
+        else:
+            check(lib().mnn_window_attention_step_e4m3(
+                self.handle, q.handle, k.handle, v.handle, positions.handle, _th(steps),
+                k_cache.handle, _th(k_scales), v_cache.handle, _th(v_scales), output.handle,
+                _sh(stream)))
+
+
+class KVCache(Layer):
+    """Keys and values of whole sequences into rolling caches and back, in the type they come in or
+    in 8 bits with a scale for each head's row."""
+
+    def __init__(self, device, num_kv_heads, head_dim, sinks=0):
+        super().__init__(device, _create(lib().mnn_kv_cache_create, device.handle, num_kv_heads,
+                                         head_dim, sinks))
+
+    def write(self, k: Tensor, v: Tensor, positions: Tensor, k_cache: Tensor, v_cache: Tensor,
+              k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None,
+              steps: Optional[Tensor] = None, stream: Optional[Stream] = None) -> None:
+        check(lib().mnn_kv_cache_write(self.handle, k.handle, v.handle, positions.handle,
+                                       _th(steps), k_cache.handle, _th(k_scales), v_cache.handle,
+                                       _th(v_scales), _sh(stream)))
+
+    def read(self, k_cache: Tensor, v_cache: Tensor, positions: Tensor, k: Tensor, v: Tensor,
+             k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None,
+             steps: Optional[Tensor] = None, stream: Optional[Stream] = None) -> None:
+        check(lib().mnn_kv_cache_read(self.handle, k_cache.handle, _th(k_scales), v_cache.handle,
+                                      _th(v_scales), positions.handle, _th(steps), k.handle,
+                                      v.handle, _sh(stream)))
+
+
+class MemoryAttention(Layer):
+    """Attention of a decoder's tokens to an encoder's states, a sequence of another length."""
+
+    def __init__(self, device, num_heads, head_dim, num_kv_heads=None, scale=0.0):
+        d = MemoryAttentionDesc(num_heads, num_heads if num_kv_heads is None else num_kv_heads,
+                                head_dim, scale)
+        super().__init__(device, _create(lib().mnn_memory_attention_create, device.handle,
+                                         C.byref(d)))
+
+    def forward(self, q: Tensor, k: Tensor, v: Tensor, output: Tensor,  # type: ignore[override]
+                query_lengths: Optional[Tensor] = None, lengths: Optional[Tensor] = None,
+                k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None,
+                stream: Optional[Stream] = None) -> None:
+        check(lib().mnn_memory_attention_forward(self.handle, q.handle, k.handle, _th(k_scales),
+                                                 v.handle, _th(v_scales), _th(query_lengths),
+                                                 _th(lengths), output.handle, _sh(stream)))
 
 
 class MultiHeadAttention(Layer):
