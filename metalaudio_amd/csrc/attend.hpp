@@ -1,0 +1,329 @@
+// Softmax attention of 32 queries to blocks of 32 keys by one wave on the bf16 matrix cores, for keys and values
+// in f32, bf16 or e4m3.
+//
+// The scores are computed TRANSPOSED, S^T = K Q^T on v_mfma_f32_32x32x16_bf16: the accumulator (lane (g, q): keys
+// 8 (v / 4) + 4 g + v % 4 of query q) is the B operand that O^T += V^T P^T needs when its k slots take those keys, so
+// P goes from the softmax straight into the second product. V lies in LDS row by row, in bf16; V^T's fragments
+// (4 keys of one dimension a lane) are transposed on the way out by ds_read_b64_tr_b16.
+//
+// f32 operands are three bf16 parts each and six partial products are kept (x3.hpp). e4m3 values are bf16 values, so
+// they take one part, and three products with f32 queries and probabilities; their rows' scales multiply the scores,
+// and the probabilities before these are rounded or split.
+//
+// Softmax: p = exp2(s - ref), s in powers of two, with a reference that moves only when a block's maximum exceeds
+// it by 2^8. Differences are taken before the exponential, in fp32, so that no score is too large for it.
+//
+// Results that are not finite (a value of 2^120 or more times p <= 2^8, or parts of values that are not finite) or,
+// in f32, so small that parts of them have left bf16's range are computed again by attend_row.
+#pragma once
+
+#include "kv_slots.hpp"
+#include "token_utils.hpp"
+#include "x3.hpp"
+
+namespace mnn {
+namespace dev {
+
+struct E4m3 {
+  uint8_t x;
+};
+
+// Eight e4m3 values to bf16, exactly.
+__device__ __forceinline__ bf16x8 widen8(uint2 q) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Eight values of a row as they come: split in three for f32, else one part.
+template <class M>
+struct Parts {
+  static constexpr int N = sizeof(M) == 4 ? 3 : 1;
+  bf16x8 p[N];
+};
+template <class M>
+__device__ __forceinline__ Parts<M> parts_of(const Eight<M>& x) {
+  Parts<M> r;
+  if constexpr (sizeof(M) == 4) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = x[e];
+    const Split8 s = split8(v);
+    r.p[0] = s.h;
+    r.p[1] = s.m;
+    r.p[2] = s.l;
+  } else {
+    r.p[0] = __builtin_bit_cast(bf16x8, x.x[0]);
+  }
+  return r;
+}
+template <>
+struct Eight<E4m3> {
+  uint2 x;
+  __device__ __forceinline__ void clear() { x = make_uint2(0, 0); }
+  __device__ __forceinline__ void load(const E4m3* p) { x = *reinterpret_cast<const uint2*>(p); }
+};
+__device__ __forceinline__ Parts<E4m3> parts_of(const Eight<E4m3>& x) {
+  Parts<E4m3> r;
+  r.p[0] = widen8(x.x);
+  return r;
+}
+
+template <class T, class M, int KS>  // T: of queries and output, M: of keys and values, head dims up to 16 KS
+struct Attend {
+  static constexpr bool F32 = sizeof(T) == 4, HELD = sizeof(M) == 1;
+  static constexpr int PQ = F32 ? 3 : 1, PM = Parts<M>::N;
+  static constexpr int DT = (KS + 1) / 2;  // 32-row tiles of O^T
+  // bytes from one key's row to the next in LDS: 8 rows of 16-byte reads on distinct banks
+  static constexpr int PITCH = KS * 32 + (KS % 2 ? 0 : 16);
+  static constexpr int PLANE = 32 * PITCH;
+  // a result below this may miss bits of its operands' parts (x3.hpp): those below 2^-110 of f32 values, or of
+  // probabilities times a scale, with values up to 448 of them
+  static constexpr float TINY_RESULT = HELD ? 0x1p-96f : 0x1p-109f;
+
+  bf16x8 q[KS][PQ];
+  floatx16 o[DT];
+  float ref, sum;  // the query's; the sum of the lane's keys
+  bool begun;      // whether the query has a score above -infinity
+
+  // The dimensions of chunk s of lane half g: 8 of them. Rows of e4m3 are read 16 bytes a lane, two chunks.
+  static __device__ __forceinline__ int dim_of(int s, int g) {
+    if (HELD && !(KS % 2 && s == KS - 1)) return 32 * (s / 2) + 16 * g + 8 * (s % 2);
+    return 16 * s + 8 * g;
+  }
+  // Whether a chunk may lie behind a head's last dimension (head dims are multiples of 8, and of 16 KS - 8 or
+  // more but for the smallest and largest KS).
+  static constexpr bool may_end(int s) {
+    return KS == 2 ? true : KS == 8 ? s >= 6 : HELD && KS % 2 == 0 ? s == KS - 1 : s == KS - 1;
+  }
+
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[t][v] = 0.f;
+    ref = 0.f;
+    sum = 0.f;
+    begun = false;
+  }
+
+  // Q as B operand; f32 times the scale in powers of two, bf16 as it is (cs: what is left to multiply scores by)
+  __device__ __forceinline__ void load_q(const T* p, bool on, int hd, float scale, float& cs) {
+    const int g = (threadIdx.x & 63) >> 5;
+    const float qs = scale * 1.4426950408889634f;
+    cs = F32 ? 1.f : qs;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = dim_of(s, g);
+      Eight<T> x;
+      x.clear();
+      if (on && d < hd) x.load(p + d);
+      if constexpr (F32) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = x[e] * qs;
+        const Split8 sp = split8(v);
+        q[s][0] = sp.h;
+        q[s][1] = sp.m;
+        q[s][2] = sp.l;
+      } else {
+        q[s][0] = __builtin_bit_cast(bf16x8, x.x[0]);
+      }
+    }
+  }
+
+  // Scores of 32 keys, k(s): chunk s of the lane's key.
+  template <class K>
+  __device__ __forceinline__ floatx16 scores(K k) const {
+    floatx16 st, low;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) st[v] = low[v] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const Parts<M> x = k(s);
+      if constexpr (PM == 3) {  // the five smaller products in an accumulator of their own (x3.hpp)
+        const Split8 kx{x.p[0], x.p[1], x.p[2]}, qx{q[s][0], q[s][1], q[s][2]};
+#pragma unroll
+        for (int p = 0; p < 5; ++p) low = mfma_x3(kx, qx, low, p);
+        st = mfma_x3(kx, qx, st, 5);
+      } else if constexpr (PQ == 3) {
+        low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.p[0], q[s][2], low, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.p[0], q[s][1], low, 0, 0, 0);
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.p[0], q[s][0], st, 0, 0, 0);
+      } else {
+        st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x.p[0], q[s][0], st, 0, 0, 0);
+      }
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) st[v] += low[v];
+    }
+    return st;
+  }
+
+  // Scores of keys that the query does not see, as bits of `seen`, become -infinity: two instructions a score that
+  // need no lane masks.
+  static __device__ __forceinline__ void mask(floatx16& st, int seen) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const unsigned m = (unsigned)__builtin_amdgcn_sbfe(seen, 8 * (v / 4) + v % 4, 1);
+      const float x = st[v];
+      st[v] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, x) & m) | (0xff800000u & ~m));
+    }
+  }
+  // The first n of 32 keys.
+  static __device__ __forceinline__ unsigned below(int n) { return (unsigned)((1ull << min(max(n, 0), 32)) - 1); }
+
+  // Moves the reference for scores st (in powers of two) where it has to.
+  __device__ __forceinline__ void refer(const floatx16& st) {
+    float mx = -INFINITY;  // keeps NaN, which neither moves the reference nor passes
+#pragma unroll
+    for (int v = 0; v < 16; v += 2) mx = max_nan(max_nan(mx, st[v]), st[v + 1]);
+    refer_to(mx);
+  }
+  __device__ __forceinline__ void refer_to(float mx) {
+    const auto far = [&] { return begun ? mx - ref > 8.f : mx > -INFINITY; };
+    if (__any(far())) {
+      mx = other_half(mx, max_nan);  // the query's other keys
+      const bool move = far();
+      // the first visible key has nothing to rescale
+      const float alpha = !move ? 1.f : begun ? __builtin_amdgcn_exp2f(ref - mx) : 0.f;
+      sum *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[i] *= alpha;
+      ref = move ? mx : ref;
+      begun |= move;
+    }
+  }
+
+  // Probabilities of 32 keys and the second product; v: fragments of V^T, vs: the values' scales (e4m3) of the
+  // lane's keys.
+  template <class V, class S>
+  __device__ __forceinline__ void add(const floatx16& st, V v, S vs) {
+    typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+    float ps = 0.f;  // added up by themselves before they join the running sum
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(st[8 * ks + e] - ref);
+        if (F32 || HELD) ps += p[e];
+        if (HELD) p[e] *= vs(8 * ks + e);
+      }
+      if constexpr (F32) {
+        const Split8 px = split8(p);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          if constexpr (PM == 3) {
+            const Split8 vx{v(0, i, ks), v(1, i, ks), v(2, i, ks)};
+#pragma unroll
+            for (int m = 0; m < 6; ++m) o[i] = mfma_x3(vx, px, o[i], m);
+          } else {
+            const bf16x8 vx = v(0, i, ks);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx, px.l, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx, px.m, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vx, px.h, o[i], 0, 0, 0);
+          }
+        }
+      } else {
+        // probabilities to bf16, to nearest (each is off by 2^-9 of itself at most): what the second product takes.
+        // Without scales the sum is that of the rounded ones, two an instruction
+        const uintx4 pb{cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]),
+                        cvt_pk_bf16(p[6], p[7])};
+        const bf16x8 px = __builtin_bit_cast(bf16x8, pb);
+        if (!HELD) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ps = add_pair(pb[e], ps);
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v(0, i, ks), px, o[i], 0, 0, 0);
+      }
+    }
+    sum += ps;
+  }
+
+  // Where the lane's fragments of V^T begin in a block of V in LDS, and fragment (part, dimensions 32 t + l32, keys
+  // 16 ks + 4 g + {0..3, 8..11}).
+  static __device__ __forceinline__ const char* v_first(const char* block) {
+    const int lane = threadIdx.x & 63, g = lane >> 5;
+    return block + (4 * g + ((lane & 15) >> 2)) * PITCH + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  }
+  static __device__ __forceinline__ bf16x8 v_frag(const char* first, int plane_bytes, int part, int t, int ks) {
+    typedef short short4v __attribute__((ext_vector_type(4)));
+    const char* p = first + part * plane_bytes + 16 * ks * PITCH + 64 * t;
+    union {
+      short4v s[2];
+      bf16x8 f;
+    } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p + 8 * PITCH));
+    return u.f;
+  }
+
+  // Whether a result (of a sum l) has to be computed again.
+  static __device__ __forceinline__ bool doubtful(float x) {
+    return !(x * 0.f == 0.f) || (F32 && x != 0.f && fabsf(x) < TINY_RESULT);
+  }
+};
+
+// One query by one wave, on the vector units in fp32, in two passes: the scores' maximum and their sum, then the
+// outputs of dimensions lane and lane + 64, each value times its own probability. The keys that the query sees are
+// taken 64 at a time, lane j scoring key j; others are not read. key_at(t) / value_at(t): rows of the t-th of n
+// visible keys.
+template <class T, class K, class V>
+__device__ __forceinline__ void attend_row(const T* __restrict__ q, int hd, float scale, int64_t n, K key_at, V value_at,
+                                           float& o0, float& o1) {
+  const int lane = threadIdx.x & 63;
+  const float qs = scale * 1.4426950408889634f;
+  auto score = [&](int64_t t) {
+    if (t >= n) return -INFINITY;
+    const auto kp = key_at(t);
+    float dot = 0.f;
+    for (int d = 0; d < hd; ++d) dot = fmaf(to_f32(q[d]) * qs, to_f32(kp[d]), dot);
+    return dot;
+  };
+  float m = -INFINITY, l = 0.f;
+  for (int64_t t0 = 0; t0 < n; t0 += 64) {
+    const float s = score(t0 + lane), mn = max_nan(m, group_reduce<64>(s, max_nan));
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    l = l * __builtin_amdgcn_exp2f(m - ref) + group_reduce<64>(t0 + lane < n ? __builtin_amdgcn_exp2f(s - ref) : 0.f, Plus{});
+    m = mn;
+  }
+  const float ref = m == -INFINITY ? 0.f : m, inv = 1.f / l;
+  o0 = o1 = 0.f;
+  for (int64_t t0 = 0; t0 < n; t0 += 64) {
+    const int cnt = (int)(n - t0 < 64 ? n - t0 : 64);
+    const float p = lane < cnt ? __builtin_amdgcn_exp2f(score(t0 + lane) - ref) * inv : 0.f;
+    for (int j = 0; j < cnt; ++j) {
+      const float pj = __shfl(p, j, 64);
+      const auto vp = value_at(t0 + j);
+      if (lane < hd) o0 = fmaf(pj, to_f32(vp[lane]), o0);
+      if (lane + 64 < hd) o1 = fmaf(pj, to_f32(vp[lane + 64]), o1);
+    }
+  }
+}
+
+// A row of 8-bit values and its scale, or a row that is still to be rounded to them, read as what they stand for.
+template <class T>
+struct HeldRow {
+  const uint8_t* p;
+  const T* fresh;  // not null: the row as it came
+  float scale, inv;
+  __device__ __forceinline__ float operator[](int d) const {
+    const int q = fresh ? (int)pack_e4m3(to_f32(fresh[d]) * inv, 0.f, 0.f, 0.f) : (int)p[d];
+    return __builtin_amdgcn_cvt_f32_fp8(q, 0) * scale;
+  }
+  static __device__ __forceinline__ HeldRow rounding(const T* x, int hd) {
+    float top = 0.f;
+    for (int d = 0; d < hd; ++d) top = max_nan(top, fabsf(to_f32(x[d])));
+    const RowScale rs = row_scale(top);
+    return {nullptr, x, rs.scale, rs.inv};
+  }
+};
+
+}  // namespace dev
+}  // namespace mnn

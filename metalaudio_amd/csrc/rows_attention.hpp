@@ -1,0 +1,15 @@
+// Attention of a few rows (tokens x the query heads of one key/value head) of each sequence to many keys: a decoder's
+// next tokens on an encoder's states, or on a rolling cache in 8 bits.
+#pragma once
+
+#include "token_ops.hpp"
+
+namespace mnn {
+namespace k {
+
+// floats of workspace that a call needs (0: none), the same on every call of the same sizes
+int64_t memory_rows_part_floats(const LaunchCtx& c, const MemoryArgs& a);
+void memory_rows(const LaunchCtx& c, const MemoryArgs& a, float* part);
+
+}  // namespace k
+}  // namespace mnn
