@@ -11,7 +11,9 @@
 // and the probabilities before these are rounded or split.
 //
 // Softmax: p = exp2(s - ref), s in powers of two, with a reference that moves only when a block's maximum exceeds
-// it by 2^8. Differences are taken before the exponential, in fp32, so that no score is too large for it.
+// it by 2^8. Where many queries share keys in LDS (STAGED) bf16 scores stay as the products give them and p is exp2(c s
+// - c ref) in one fused step: c ref is rounded, by the same amount for all keys of a reference, but of scores past 2^31
+// all probabilities may come out as 0 then (their sum is about 1 or more otherwise): such rows are computed again, too.
 //
 // Results that are not finite (a value of 2^120 or more times p <= 2^8, or parts of values that are not finite) or,
 // in f32, so small that parts of them have left bf16's range are computed again by attend_row.
@@ -72,9 +74,11 @@ __device__ __forceinline__ Parts<E4m3> parts_of(const Eight<E4m3>& x) {
   return r;
 }
 
-template <class T, class M, int KS>  // T: of queries and output, M: of keys and values, head dims up to 16 KS
+// T: of queries and output, M: of keys and values, head dims up to 16 KS; STAGED: keys come from LDS, in bf16 parts
+template <class T, class M, int KS, bool STAGED>
 struct Attend {
   static constexpr bool F32 = sizeof(T) == 4, HELD = sizeof(M) == 1;
+  static constexpr bool RAW = STAGED && !F32 && !HELD;  // scores are multiplied by cs in the exponent
   static constexpr int PQ = F32 ? 3 : 1, PM = Parts<M>::N;
   static constexpr int DT = (KS + 1) / 2;  // 32-row tiles of O^T
   // bytes from one key's row to the next in LDS: 8 rows of 16-byte reads on distinct banks
@@ -88,10 +92,11 @@ struct Attend {
   floatx16 o[DT];
   float ref, sum;  // the query's; the sum of the lane's keys
   bool begun;      // whether the query has a score above -infinity
+  float cs;        // what is left to multiply scores by
 
-  // The dimensions of chunk s of lane half g: 8 of them. Rows of e4m3 are read 16 bytes a lane, two chunks.
+  // The dimensions of chunk s of lane half g: 8 of them. Rows of e4m3 are read from memory 16 bytes a lane, two chunks.
   static __device__ __forceinline__ int dim_of(int s, int g) {
-    if (HELD && !(KS % 2 && s == KS - 1)) return 32 * (s / 2) + 16 * g + 8 * (s % 2);
+    if (HELD && !STAGED && !(KS % 2 && s == KS - 1)) return 32 * (s / 2) + 16 * g + 8 * (s % 2);
     return 16 * s + 8 * g;
   }
   // Whether a chunk may lie behind a head's last dimension (head dims are multiples of 8, and of 16 KS - 8 or
@@ -110,11 +115,12 @@ struct Attend {
     begun = false;
   }
 
-  // Q as B operand; f32 times the scale in powers of two, bf16 as it is (cs: what is left to multiply scores by)
-  __device__ __forceinline__ void load_q(const T* p, bool on, int hd, float scale, float& cs) {
+  // Q as B operand; f32 times the scale in powers of two, bf16 as it is, up to the scale's sign
+  __device__ __forceinline__ void load_q(const T* p, bool on, int hd, float scale) {
     const int g = (threadIdx.x & 63) >> 5;
     const float qs = scale * 1.4426950408889634f;
-    cs = F32 ? 1.f : qs;
+    cs = F32 ? 1.f : fabsf(qs);
+    const unsigned sign = qs < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = dim_of(s, g);
@@ -130,7 +136,7 @@ struct Attend {
         q[s][1] = sp.m;
         q[s][2] = sp.l;
       } else {
-        q[s][0] = __builtin_bit_cast(bf16x8, x.x[0]);
+        q[s][0] = __builtin_bit_cast(bf16x8, x.x[0] ^ sign);
       }
     }
   }
@@ -177,20 +183,21 @@ struct Attend {
   // The first n of 32 keys.
   static __device__ __forceinline__ unsigned below(int n) { return (unsigned)((1ull << min(max(n, 0), 32)) - 1); }
 
-  // Moves the reference for scores st (in powers of two) where it has to.
-  __device__ __forceinline__ void refer(const floatx16& st) {
-    float mx = -INFINITY;  // keeps NaN, which neither moves the reference nor passes
+  // The larger of mx and scores st; keeps NaN, which neither moves the reference nor passes.
+  static __device__ __forceinline__ float largest(const floatx16& st, float mx) {
 #pragma unroll
     for (int v = 0; v < 16; v += 2) mx = max_nan(max_nan(mx, st[v]), st[v + 1]);
-    refer_to(mx);
+    return mx;
   }
-  __device__ __forceinline__ void refer_to(float mx) {
-    const auto far = [&] { return begun ? mx - ref > 8.f : mx > -INFINITY; };
+  // Moves the reference for scores up to mx where it has to.
+  __device__ __forceinline__ void refer(float mx) {
+    const float unit = RAW ? cs : 1.f;
+    const auto far = [&] { return begun ? (mx - ref) * unit > 8.f : mx > -INFINITY; };
     if (__any(far())) {
       mx = other_half(mx, max_nan);  // the query's other keys
       const bool move = far();
       // the first visible key has nothing to rescale
-      const float alpha = !move ? 1.f : begun ? __builtin_amdgcn_exp2f(ref - mx) : 0.f;
+      const float alpha = !move ? 1.f : begun ? __builtin_amdgcn_exp2f((ref - mx) * unit) : 0.f;
       sum *= alpha;
 #pragma unroll
       for (int i = 0; i < DT; ++i) o[i] *= alpha;
@@ -205,12 +212,14 @@ struct Attend {
   __device__ __forceinline__ void add(const floatx16& st, V v, S vs) {
     typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
     float ps = 0.f;  // added up by themselves before they join the running sum
+    const float off = ref * cs;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(st[8 * ks + e] - ref);
+        const float s = st[8 * ks + e];
+        p[e] = __builtin_amdgcn_exp2f(RAW ? fmaf(s, cs, -off) : s - ref);
         if (F32 || HELD) ps += p[e];
         if (HELD) p[e] *= vs(8 * ks + e);
       }

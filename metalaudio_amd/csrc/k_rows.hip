@@ -113,7 +113,7 @@ __device__ void row_again(const RowsArgs& a, const Rows& w, int r) {
 
 template <class T, class M, int KS>
 struct RowsCfg {
-  using A = Attend<T, M, KS>;
+  using A = Attend<T, M, KS, false>;
   // waves: 4 where their registers do not fit in two waves a SIMD
   static constexpr int W = KS > (sizeof(M) == 4 ? 3 : A::F32 ? 4 : 6) ? 4 : 8;
   static constexpr int WAVE = A::PM * A::PLANE + 64 + (A::HELD ? 256 : 0);  // V's block, and the scales
@@ -126,7 +126,7 @@ template <class T, class M, int KS, bool STEP>
 __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsArgs a, int tiles, int nsplit,
                                                                            int slots, float* part) {
   using Cfg = RowsCfg<T, M, KS>;
-  using A = Attend<T, M, KS>;
+  using A = Attend<T, M, KS, false>;
   constexpr int W = Cfg::W, PM = A::PM, PLANE = A::PLANE;
   constexpr bool HELD = A::HELD;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -140,10 +140,9 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
 
   A at;
   at.begin();
-  float cs;
   const int row = w.row0 + l32, t = row / G;
   at.load_q(static_cast<const T*>(a.q) + (((int64_t)w.b * a.T + t) * a.H + w.kvh * G + row % G) * hd, l32 < w.rows, hd,
-            a.scale, cs);
+            a.scale);
   // the query's keys by number: below hi, and not below first or below the sinks' end
   int hi = w.n, first = 0, first_last = 0, hi_least = w.n;
   if constexpr (STEP) {
@@ -243,7 +242,7 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
       for (int i = 0; i < PM; ++i)
         *reinterpret_cast<bf16x8*>(mem + i * PLANE + l32 * A::PITCH + 2 * A::dim_of(s, g)) = p.p[i];
     }
-    if constexpr (HELD) scl[lane] = g ? x.scale : x.scale * cs;
+    if constexpr (HELD) scl[lane] = g ? x.scale : x.scale * at.cs;
     __builtin_amdgcn_wave_barrier();
     floatx16 st = at.scores([&](int s) {
       if (A::may_end(s) && A::dim_of(s, g) >= hd) x.k[s].clear();
@@ -260,14 +259,14 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
       }
     } else if constexpr (!A::F32) {
 #pragma unroll
-      for (int v = 0; v < 16; ++v) st[v] *= cs;
+      for (int v = 0; v < 16; ++v) st[v] *= at.cs;
     }
     const bool whole = k0 + 32 <= hi_least && (k0 >= first_last || k0 + 32 <= a.sinks);
     if (!whole) {
       const int c = k0 + 4 * g;  // the lane's: key i below is c + i
       A::mask(st, (int)(A::below(hi - c) & (STEP ? ~A::below(first - c) | A::below(a.sinks - c) : ~0u)));
     }
-    at.refer(st);
+    at.refer(A::largest(st, -INFINITY));
     float4 f[4];
     if constexpr (HELD) {
 #pragma unroll
@@ -408,7 +407,7 @@ __global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a, int tiles, i
     y = w.n ? y * inv[r] : 0.f;
     const int rr = w.row0 + r;
     static_cast<T*>(a.o)[(((int64_t)w.b * a.T + rr / G) * a.H + w.kvh * G + rr % G) * hd + d] = from_f32<T>(y);
-    if (Attend<T, M, 8>::doubtful(y)) again[r] = 1;
+    if (Attend<T, M, 8, false>::doubtful(y)) again[r] = 1;
   }
   __syncthreads();
   for (int r = wave; r < w.rows; r += 4)
