@@ -4,7 +4,8 @@
 // A workgroup takes 32 NW rows (row = token * G + head of the group: all heads that read one key/value head share its
 // states) and the keys of a sequence, or a range of them, in blocks that lie in LDS in bf16 parts, two slots, so that
 // one barrier a block is enough: behind it the next block's rows are fetched to registers, this one is computed
-// (attend.hpp), and the next one is split or widened and stored to the other slot.
+// (attend.hpp), and the next one is split or widened and stored to the other slot. Of workgroups that share out the keys
+// of the same rows the last one to finish joins the results of all of them.
 //
 // Bound by the vector units' issue beside the matrix instructions in bf16 (a quarter of it, 256 of 470 cycles for 32 x 32
 // scores, are exponentials), by the six products' matrix instructions in f32.
@@ -24,7 +25,7 @@ namespace {
 
 template <class T, class M, int KS, int NW>
 struct MemoryCfg {
-  using A = Attend<T, M, KS, true>;
+  using A = AttendMany<T, M, KS>;
   static constexpr int BKV = sizeof(M) == 4 ? 32 : 64, NT = BKV / 32;
   static constexpr int THREADS = 64 * NW, BQ = 32 * NW;
   static constexpr int PLANE = BKV * A::PITCH;
@@ -80,7 +81,7 @@ __device__ __forceinline__ void memory_row_again(const MemoryArgs& a, const Unit
 
 template <class T, class M, int KS, int NW>
 __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M, KS, NW>::OCC)) void memory_kernel(
-    MemoryArgs a, int tiles, int nsplit, float* part) {
+    MemoryArgs a, int tiles, int nsplit, float* part, int* counts) {
   using Cfg = MemoryCfg<T, M, KS, NW>;
   using A = typename Cfg::A;
   constexpr int BKV = Cfg::BKV, NT = Cfg::NT, PM = A::PM, PLANE = Cfg::PLANE, SLOT = Cfg::SLOT, PER = Cfg::PER;
@@ -187,7 +188,7 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
       const int left = u.n - blk * BKV;
       if (left < BKV) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) A::mask(st[j], (int)A::below(left - 32 * j - 4 * g));
+        for (int j = 0; j < NT; ++j) A::mask(st[j], (int)keys_below(left - 32 * j - 4 * g));
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) mx = A::largest(st[j], mx);
@@ -209,26 +210,42 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
     }
     if (blk + 1 < b1) store(slot ^ 1);
   }
-  if (!any) return;
 
-  const float l = other_half(at.sum, Plus{});
-  if (nsplit > 1) {  // O^T, reference and sum to the workspace
-    if (!mine) return;
-    const int ld = hd + 4;
-    float* to = part + ((int64_t)id * Cfg::BQ + 32 * wave + l32) * ld;
+  float l = other_half(at.sum, Plus{});
+  if (nsplit > 1) {
+    // O^T, reference and sum to the workspace, a register of all lanes beside each other; the last of the unit's
+    // workgroups joins them, in the keys' order
+    constexpr int REGS = 16 * A::DT + 2;
+    const int64_t step = (int64_t)tiles * NW * REGS * 64;  // from one range to the next
+    float* first = part + ((int64_t)(id - u.sp * tiles) * NW + wave) * REGS * 64 + lane;
+    float* to = first + u.sp * step;
+    if (any) {
 #pragma unroll
-    for (int c = 0; c < 2 * KS; ++c)
-      if (8 * c < hd) {
-        const floatx16& ot = at.o[c / 4];
-        const int v = 4 * (c % 4);
-        *reinterpret_cast<float4*>(to + 8 * c + 4 * g) = make_float4(ot[v], ot[v + 1], ot[v + 2], ot[v + 3]);
-      }
-    if (g == 0) {  // the reference in powers of two; NaN scores leave it at 0 and a sum of NaN
-      to[hd] = at.begun || !(l == 0.f) ? at.ref * (A::RAW ? at.cs : 1.f) : -INFINITY;
-      to[hd + 1] = l;
+      for (int i = 0; i < A::DT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) put_shared(to + 64 * (16 * i + v), at.o[i][v]);
+      // the reference in powers of two; NaN scores leave it at 0 and a sum of NaN
+      put_shared(to + 64 * (REGS - 2), at.begun || !(l == 0.f) ? at.ref * (A::RAW ? at.cs : 1.f) : -INFINITY);
+      put_shared(to + 64 * (REGS - 1), l);
     }
-    return;
+    const int unit = (u.b * a.KV + u.kvh) * tiles + u.row0 / Cfg::BQ;
+    if (!last_of(counts + unit, nsplit, reinterpret_cast<int*>(smem)) || !any) return;
+    float top = -INFINITY;
+    for (int s = 0; s < nsplit; ++s) top = max_nan(top, get_shared(first + s * step + 64 * (REGS - 2)));
+    const float ref = top == -INFINITY ? 0.f : top;
+    l = 0.f;
+    at.begin();
+    for (int s = 0; s < nsplit; ++s) {
+      const float* p = first + s * step;
+      const float by = __builtin_amdgcn_exp2f(get_shared(p + 64 * (REGS - 2)) - ref);
+      l = fmaf(get_shared(p + 64 * (REGS - 1)), by, l);
+#pragma unroll
+      for (int i = 0; i < A::DT; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) at.o[i][v] = fmaf(get_shared(p + 64 * (16 * i + v)), by, at.o[i][v]);
+    }
   }
+  if (!any) return;
   const float inv = u.n ? 1.f / l : 0.f;
   bool bad = A::RAW && l < 0x1p-60f && u.n;
 #pragma unroll
@@ -261,45 +278,7 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
   }
 }
 
-// Joins the key ranges of split rows: a wave a row.
 constexpr int kMaxSplits = 16;
-template <class T, class M>
-__global__ __launch_bounds__(256) void memory_join_kernel(MemoryArgs a, int tiles, int nsplit, int bq, const float* part) {
-  const int lane = threadIdx.x & 63, hd = a.hd, ld = hd + 4;
-  const int rows = a.T * (a.H / a.KV);  // of a sequence's head group, all of them
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int r = (int)(w % rows), head = (int)(w / rows);
-  if (head >= a.B * a.KV) return;
-  const int id0 = head * nsplit * tiles + r / bq;
-  const Unit u = unit_of(a, id0, tiles, nsplit, bq);
-  if (r >= u.rows) return;
-  const float* p = part + ((int64_t)id0 * bq + r % bq) * ld;
-  const int64_t step = (int64_t)tiles * bq * ld;  // to the next range
-  float top = -INFINITY, l = 0.f;
-  if (lane < nsplit) {
-    top = p[lane * step + hd];
-    l = p[lane * step + hd + 1];
-  }
-  const float all = group_reduce<16>(top, max_nan), ref = all == -INFINITY ? 0.f : all;
-  const float by = __builtin_amdgcn_exp2f(top - ref);
-  const float sum = group_reduce<16>(l * by, Plus{});
-  const float inv = u.n ? 1.f / __shfl(sum, 0, 64) : 0.f;
-  float y0 = 0.f, y1 = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float f = __shfl(by, s, 64);
-    if (lane < hd) y0 = fmaf(p[s * step + lane], f, y0);
-    if (lane + 64 < hd) y1 = fmaf(p[s * step + lane + 64], f, y1);
-  }
-  y0 *= inv;
-  y1 *= inv;
-  using A = Attend<T, M, 8, true>;
-  const bool bad = (A::RAW && u.n && __shfl(sum, 0, 64) < 0x1p-60f) || A::doubtful(y0) || A::doubtful(y1);
-  if (__any(bad)) return memory_row_again<T, M>(a, u, r);
-  T* o = static_cast<T*>(a.o) + row_at(a, u, r);
-  if (lane < hd) o[lane] = from_f32<T>(y0);
-  if (lane + 64 < hd) o[lane + 64] = from_f32<T>(y1);
-}
-
 constexpr int kWaves = 4;
 struct Plan {
   bool few;  // rows so few that the other kernel takes them
@@ -318,28 +297,24 @@ Plan plan_of(const MemoryArgs& a, int cus) {
 }
 
 template <class T, class M, int KS>
-void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, float* part) {
+void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
   launch(c, "memory", memory_kernel<T, M, KS, kWaves>, dim3((unsigned)(p.units * p.nsplit)), dim3(64 * kWaves), 0, a, p.tiles,
-         p.nsplit, part);
+         p.nsplit, join.part, join.counts);
 }
 template <class T, class M>
-void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, float* part) {
-  MNN_REQUIRE(p.units * p.nsplit < (1 << 24) && (int64_t)a.B * a.KV * a.T * (a.H / a.KV) < (1 << 26),
-              MNN_ERR_INVALID_CONFIGURATION, "MemoryAttention: too many tokens in one call");
-  MNN_REQUIRE(p.nsplit == 1 || part, MNN_ERR_INVALID_ARGUMENT, "memory attention: split keys need a workspace");
+void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
+  MNN_REQUIRE(p.units * p.nsplit < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
+              "MemoryAttention: too many tokens in one call");
+  MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,
+              "memory attention: split keys need a workspace");
   switch ((a.hd + 15) / 16) {
     case 1:
-    case 2: launch_ks<T, M, 2>(c, a, p, part); break;
-    case 3: launch_ks<T, M, 3>(c, a, p, part); break;
-    case 4: launch_ks<T, M, 4>(c, a, p, part); break;
-    case 5: launch_ks<T, M, 5>(c, a, p, part); break;
-    case 6: launch_ks<T, M, 6>(c, a, p, part); break;
-    default: launch_ks<T, M, 8>(c, a, p, part);
-  }
-  if (p.nsplit > 1) {
-    const int64_t rows = (int64_t)a.B * a.KV * a.T * (a.H / a.KV);
-    launch(c, "memory_join", memory_join_kernel<T, M>, dim3(cdiv(rows, 4)), dim3(256), 0, a, p.tiles, p.nsplit, 32 * kWaves,
-           (const float*)part);
+    case 2: launch_ks<T, M, 2>(c, a, p, join); break;
+    case 3: launch_ks<T, M, 3>(c, a, p, join); break;
+    case 4: launch_ks<T, M, 4>(c, a, p, join); break;
+    case 5: launch_ks<T, M, 5>(c, a, p, join); break;
+    case 6: launch_ks<T, M, 6>(c, a, p, join); break;
+    default: launch_ks<T, M, 8>(c, a, p, join);
   }
 }
 
@@ -348,15 +323,16 @@ void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, float* pa
 int64_t memory_part_floats(const LaunchCtx& c, const MemoryArgs& a) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
   if (p.few) return memory_rows_part_floats(c, a);
-  return p.nsplit == 1 ? 0 : p.units * p.nsplit * 32 * kWaves * (a.hd + 4);
+  const int dt = a.hd > 96 ? 4 : (a.hd + 31) / 32;  // 32-row tiles of O^T, as AttendMany has them
+  return p.nsplit == 1 ? 0 : p.units * p.nsplit * kWaves * (16 * dt + 2) * 64;
 }
-void memory_attention(const LaunchCtx& c, const MemoryArgs& a, float* part) {
+void memory_attention(const LaunchCtx& c, const MemoryArgs& a, const Join& join) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
-  if (p.few) return memory_rows(c, a, part);
+  if (p.few) return memory_rows(c, a, join);
   if (a.type == MNN_F32)
-    a.ks ? memory_tm<float, E4m3>(c, a, p, part) : memory_tm<float, float>(c, a, p, part);
+    a.ks ? memory_tm<float, E4m3>(c, a, p, join) : memory_tm<float, float>(c, a, p, join);
   else
-    a.ks ? memory_tm<__bf16, E4m3>(c, a, p, part) : memory_tm<__bf16, __bf16>(c, a, p, part);
+    a.ks ? memory_tm<__bf16, E4m3>(c, a, p, join) : memory_tm<__bf16, __bf16>(c, a, p, join);
 }
 
 }  // namespace k

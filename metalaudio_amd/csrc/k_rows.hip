@@ -1,15 +1,15 @@
 // Attention of a few rows of each sequence to many keys (rows_attention.hpp), and the window attention's step on
 // rolling caches in 8 bits.
 //
-// The rows that read one key/value head, tokens x heads of its group, are taken 32 at a time by a workgroup, or by
-// several that share out the keys. Each wave computes its own blocks of 32 keys for all 32 rows on the matrix cores
+// The rows that read one key/value head, tokens x heads of its group, are taken 16 at a time by a workgroup, or by
+// several that share out the keys. Each wave computes its own blocks of 32 keys for all 16 rows on the matrix cores
 // (attend.hpp): K goes from memory to registers as the A operand, V through a part of LDS that is the wave's, so that
 // no wave waits for another one before the end, where their results are joined. The next block is on its way while
-// one is computed.
+// one is computed. Of workgroups that share out the keys of the same rows the last one to finish joins the results of
+// all of them, in the order of their keys.
 //
-// The matrix cores and the softmax run at 32 rows whatever there are: a block of 32 keys, 4 KB of e4m3 at heads of 64,
-// takes a SIMD some 700 cycles, 14 TB/s over the GPU; rows on the vector units, eight lanes a key, cost those as much
-// for each row.
+// The matrix cores and the softmax run at 16 rows whatever there are (32 rows: twice the softmax, and registers for two
+// waves a SIMD instead of four); rows on the vector units, eight lanes a key, cost as much for each.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,34 +36,31 @@ struct RowsArgs {
   float scale;
 };
 
-// What a workgroup answers: rows row0 .. row0 + 31 (row = token * G + head of the group) of sequence b, and the keys
+// What a workgroup answers: rows row0 .. row0 + 15 (row = token * G + head of the group) of sequence b, and the keys
 // that any of them sees, numbered from 0. A step's: the sinks before the window's first token, then the window;
 // so a key is a sink if its number is below `sinks`, whichever the window's first token is.
 struct Rows {
-  int b, kvh, row0, rows;      // rows: of the tile's 32
+  int b, kvh, row0, rows;      // rows: of the tile's 16
   int n;                       // keys
-  int pos, nt, t0, lo, ns, ring, wrapped;  // of a step; wrapped: place in the ring of token max(lo, sinks)
+  int pos, nt, t0, t1, lo, ns, ring, wrapped;  // of a step; wrapped: place in the ring of token max(lo, sinks)
 };
+__device__ __forceinline__ int over(int x, int by) { return by == 1 ? x : (int)((unsigned)x / (unsigned)by); }
 template <bool STEP>
-__device__ __forceinline__ bool rows_of(const RowsArgs& a, int unit, int tiles, Rows& w) {
-  const int G = a.H / a.KV;
-  w.row0 = unit % tiles * 32;
-  w.kvh = unit / tiles % a.KV;
-  w.b = unit / tiles / a.KV;
+__device__ __forceinline__ bool rows_of(const RowsArgs& a, int G, Rows& w) {
   if constexpr (STEP)
     w.nt = kv_rows(a.c0, a.c1, w.b, a.T, w.pos);
   else
     w.nt = a.c0 ? min(max(a.c0[w.b], 0), a.T) : a.T;
-  w.rows = min(32, w.nt * G - w.row0);
+  w.rows = min(16, w.nt * G - w.row0);
   if (w.rows <= 0) return false;
   if constexpr (STEP) {
-    w.t0 = w.row0 / G;
-    const int t1 = (w.row0 + w.rows - 1) / G;
+    w.t0 = over(w.row0, G);
+    w.t1 = over(w.row0 + w.rows - 1, G);
     w.lo = max(0, w.pos + w.t0 - a.left);
     w.ns = min(a.sinks, w.lo);
-    w.n = w.ns + (w.pos + w.t0 - w.lo) + (t1 - w.t0) + 1;
+    w.n = w.ns + (w.pos + w.t0 - w.lo) + (w.t1 - w.t0) + 1;
     w.ring = a.S - a.sinks;
-    w.wrapped = (max(w.lo, a.sinks) - a.sinks) % w.ring;
+    w.wrapped = (int)((unsigned)(max(w.lo, a.sinks) - a.sinks) % (unsigned)w.ring);
   } else {
     w.n = a.c1 ? min(max(a.c1[w.b], 0), a.S) : a.S;
   }
@@ -113,55 +110,66 @@ __device__ void row_again(const RowsArgs& a, const Rows& w, int r) {
 
 template <class T, class M, int KS>
 struct RowsCfg {
-  using A = Attend<T, M, KS, false>;
-  // waves: 4 where their registers do not fit in two waves a SIMD
-  static constexpr int W = KS > (sizeof(M) == 4 ? 3 : A::F32 ? 4 : 6) ? 4 : 8;
-  static constexpr int WAVE = A::PM * A::PLANE + 64 + (A::HELD ? 256 : 0);  // V's block, and the scales
-  static constexpr int REGS = 16 * A::DT + 1;
+  using A = AttendFew<T, M, KS>;
+  static constexpr int W = A::PM == 3 && KS > 2 ? 4 : 8;               // waves
+  static constexpr int WAVE = A::PM * A::PLANE + (A::HELD ? 256 : 0);  // V's block, and the scales
+  static constexpr int REGS = 4 * A::OT + 1;
+  // waves a SIMD, as the registers allow
+  static constexpr int OCC = KS == 1   ? (A::PM == 3 ? 3 : 4)
+                             : A::PM == 3 ? (KS == 2 ? 2 : 1)
+                             : KS == 2    ? (A::HELD && !A::F32 ? 4 : 3)
+                                          : (KS == 3 && A::HELD && !A::F32 ? 3 : 2);
   // bytes: the waves' blocks, or at the end their results (lanes of rows that there are), references and sums
-  static int lds(int rows) { return std::max(W * WAVE, W * 4 * (REGS * 2 * rows + rows)) + 4 * 32; }
+  static int lds(int slots) { return std::max(W * WAVE, W * 4 * (REGS * 4 * slots + slots)) + 4 * 17; }
 };
 
 template <class T, class M, int KS, bool STEP>
-__global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsArgs a, int tiles, int nsplit,
-                                                                           int slots, float* part) {
+__global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OCC)) void rows_kernel(
+    RowsArgs a, int G, int tiles, int nsplit, int slots, float* part, int* counts) {
   using Cfg = RowsCfg<T, M, KS>;
-  using A = Attend<T, M, KS, false>;
+  using A = typename Cfg::A;
   constexpr int W = Cfg::W, PM = A::PM, PLANE = A::PLANE;
   constexpr bool HELD = A::HELD;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // consecutive units, the tiles and key ranges of one head first, run on one XCD and share its L2
-  const int id = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
-  const int unit = id / nsplit, sp = id % nsplit, G = a.H / a.KV, hd = a.hd;
+  // heads, key ranges, tiles, sequences: the heads of a sequence, whose rows share cache lines, run on one XCD at one time
+  const int hd = a.hd, id = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
   Rows w;
-  if (!rows_of<STEP>(a, unit, tiles, w)) return;
+  int rest = over(id, a.KV);
+  w.kvh = id - rest * a.KV;
+  const int sp = rest - over(rest, nsplit) * nsplit;
+  rest = over(rest, nsplit);
+  w.b = over(rest, tiles);
+  const int tile = rest - w.b * tiles;
+  w.row0 = 16 * tile;
+  // the queries' loads go out before the sequence's lengths have come; rows that are no tokens are not used
+  const int row = w.row0 + l16, t = over(row, G);
+  Eight<T> q[KS];
+  A::fetch_q(static_cast<const T*>(a.q) + (((int64_t)w.b * a.T + t) * a.H + w.kvh * G + (row - t * G)) * hd, t < a.T, hd, q);
+  if (!rows_of<STEP>(a, G, w)) return;
 
   A at;
   at.begin();
-  const int row = w.row0 + l32, t = row / G;
-  at.load_q(static_cast<const T*>(a.q) + (((int64_t)w.b * a.T + t) * a.H + w.kvh * G + row % G) * hd, l32 < w.rows, hd,
-            a.scale);
   // the query's keys by number: below hi, and not below first or below the sinks' end
   int hi = w.n, first = 0, first_last = 0, hi_least = w.n;
   if constexpr (STEP) {
-    const int i = w.pos + min(t, (w.row0 + w.rows - 1) / G);
+    const int i = w.pos + min(t, w.t1);
     hi = w.ns + (i - w.lo) + 1;
     first = w.ns + (max(0, i - a.left) - w.lo);
     hi_least = w.ns + (w.pos + w.t0 - w.lo) + 1;
-    first_last = w.ns + (max(0, w.pos + (w.row0 + w.rows - 1) / G - a.left) - w.lo);
+    first_last = w.ns + (max(0, w.pos + w.t1 - a.left) - w.lo);
   }
 
-  const int nb = (w.n + 31) / 32, b0 = (int)((int64_t)nb * sp / nsplit), b1 = (int)((int64_t)nb * (sp + 1) / nsplit);
+  const int nb = (w.n + 31) / 32, each = over(nb + nsplit - 1, nsplit), b0 = sp * each, b1 = min(nb, b0 + each);
   struct Block {
-    Eight<M> k[KS], v[KS];
-    float scale;  // of lane half 0: the key's, of half 1: the value's
+    Eight<M> k[2][KS], v[2][KS];  // of keys l16 and 16 + l16
+    float scale;                  // of lanes below 32: the scale of key lane, of the others: of value lane - 32
   };
   const int64_t seq = (int64_t)w.b * a.S * a.KV + w.kvh;
   const M* kb = static_cast<const M*>(a.k) + seq * hd;
   const M* vb = static_cast<const M*>(a.v) + seq * hd;
-  const float* sb = HELD ? (g ? a.vs : a.ks) + seq : nullptr;
+  const float* sb = HELD ? (lane < 32 ? a.ks : a.vs) + seq : nullptr;
   const bool wide = hd % 16 == 0;
   auto load = [&](const M* row, Eight<M>(&x)[KS]) {
 #pragma unroll
@@ -174,112 +182,134 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
           x[s + 1].x = make_uint2(two.z, two.w);
           continue;
         }
-        if (s % 2 == 1 && wide && s < KS) continue;
+        if (s % 2 == 1 && wide) continue;
       }
       x[s].load(row + (A::may_end(s) ? min(d, hd - 8) : d));
     }
   };
-  // keys behind the last: the last one again (their scores are masked, their values cleared); a step's own keys,
-  // which the cache does not hold yet: the slot that they will have
-  auto fetch = [&](int blk, Block& x) {
-    const int idx = min(blk * 32 + l32, w.n - 1);
-    const int64_t slot = STEP ? slot_of(a, w, token_of(w, idx)) : idx;
-    load(kb + slot * a.KV * hd, x.k);
-    load(vb + slot * a.KV * hd, x.v);
-    if constexpr (HELD) x.scale = sb[slot * a.KV];
-  };
   // a step's own keys and values, rounded as the cache will hold them
-  auto own_rows = [&](int idx, Block& x) {
-    const int p = token_of(w, min(idx, w.n - 1));
-    const bool mine = p >= w.pos;
-    const int64_t from = (((int64_t)w.b * a.T + (mine ? p - w.pos : 0)) * a.KV + w.kvh) * hd;
+  auto own_rows = [&](const int (&idx)[2], Block& x) {
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const T* src = static_cast<const T*>(kv ? a.vn : a.kn) + from;
-      Eight<T> e[KS];
-      float top = 0.f;
+    for (int j = 0; j < 2; ++j) {
+      const int p = token_of(w, idx[j]);
+      const bool mine = p >= w.pos;
+      const int64_t from = (((int64_t)w.b * a.T + (mine ? p - w.pos : 0)) * a.KV + w.kvh) * hd;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int d = A::dim_of(s, g);
-        e[s].clear();
-        if (mine && d < hd) e[s].load(src + d);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(e[s][i]));
-      }
-      const RowScale rs = row_scale(other_half(top, max_nan));
-      if constexpr (HELD) {
+      for (int kv = 0; kv < 2; ++kv) {
+        const T* src = static_cast<const T*>(kv ? a.vn : a.kn) + from;
+        Eight<T> e[KS];
+        float top = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const uint2 q = make_uint2(
-              pack_e4m3(e[s][0] * rs.inv, e[s][1] * rs.inv, e[s][2] * rs.inv, e[s][3] * rs.inv),
-              pack_e4m3(e[s][4] * rs.inv, e[s][5] * rs.inv, e[s][6] * rs.inv, e[s][7] * rs.inv));
-          if (mine) (kv ? x.v[s] : x.k[s]).x = q;
+          const int d = A::dim_of(s, g);
+          e[s].clear();
+          if (mine && d < hd) e[s].load(src + d);
         }
-        if (mine && g == kv) x.scale = rs.scale;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(e[s][i]));
+        const RowScale rs = row_scale(other_half(other_row(top, max_nan), max_nan));
+        if constexpr (HELD) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const uint2 r = make_uint2(
+                pack_e4m3(e[s][0] * rs.inv, e[s][1] * rs.inv, e[s][2] * rs.inv, e[s][3] * rs.inv),
+                pack_e4m3(e[s][4] * rs.inv, e[s][5] * rs.inv, e[s][6] * rs.inv, e[s][7] * rs.inv));
+            if (mine) (kv ? x.v[j][s] : x.k[j][s]).x = r;
+          }
+          if (mine && g == 2 * kv + j) x.scale = rs.scale;
+        }
       }
     }
+  };
+  // keys behind the last: the last one again (their scores are masked, their values cleared); a step's own keys,
+  // which the cache does not hold yet: the slot that they will have first, then the rows themselves
+  auto fetch = [&](int blk, Block& x) {
+    int idx[2];
+    int64_t slot[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      idx[j] = min(blk * 32 + 16 * j + l16, w.n - 1);
+      slot[j] = (int64_t)(STEP ? slot_of(a, w, token_of(w, idx[j])) : idx[j]) * a.KV;
+      load(kb + slot[j] * hd, x.k[j]);
+      load(vb + slot[j] * hd, x.v[j]);
+    }
+    if constexpr (HELD) x.scale = sb[g & 1 ? slot[1] : slot[0]];
+    if constexpr (STEP)
+      if (token_of(w, min(blk * 32 + 31, w.n - 1)) >= w.pos) own_rows(idx, x);
   };
 
   char* mem = smem + wave * Cfg::WAVE;
-  float* scl = reinterpret_cast<float*>(mem + PM * PLANE + 64);
+  float* scl = reinterpret_cast<float*>(mem + PM * PLANE);
   const char* v0 = A::v_first(mem);
   auto compute = [&](int blk, Block& x) {
     const int k0 = blk * 32;
-    if constexpr (STEP)
-      if (token_of(w, min(k0 + 31, w.n - 1)) >= w.pos) own_rows(k0 + l32, x);
     if (k0 + 32 > w.n) {
-      const bool there = k0 + l32 < w.n;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        if (!there) x.v[s].clear();
-      if (!there) x.scale = 0.f;
+      for (int j = 0; j < 2; ++j)
+        if (k0 + 16 * j + l16 >= w.n) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) x.v[j][s].clear();
+          if ((g & 1) == j) x.scale = 0.f;
+        }
     }
+    if constexpr (HELD) scl[lane] = lane < 32 ? x.scale * at.cs : x.scale;
+    floatx4 st[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      st[j] = at.scores([&](int s) {
+        if (A::may_end(s) && A::dim_of(s, g) >= hd) x.k[j][s].clear();
+        return parts_of(x.k[j][s]);
+      });
     // V to the wave's LDS: its reads below wait for these writes, and the next block's writes come behind them
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const Parts<M> p = parts_of(x.v[s]);
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < PM; ++i)
-        *reinterpret_cast<bf16x8*>(mem + i * PLANE + l32 * A::PITCH + 2 * A::dim_of(s, g)) = p.p[i];
-    }
-    if constexpr (HELD) scl[lane] = g ? x.scale : x.scale * at.cs;
+      for (int s = 0; s < KS; ++s) {
+        const Parts<M> p = parts_of(x.v[j][s]);
+#pragma unroll
+        for (int i = 0; i < PM; ++i)
+          *reinterpret_cast<bf16x8*>(mem + i * PLANE + (16 * j + l16) * A::PITCH + 2 * A::dim_of(s, g)) = p.p[i];
+      }
     __builtin_amdgcn_wave_barrier();
-    floatx16 st = at.scores([&](int s) {
-      if (A::may_end(s) && A::dim_of(s, g) >= hd) x.k[s].clear();
-      return parts_of(x.k[s]);
-    });
+    float vs[8];
     if constexpr (HELD) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 f = *reinterpret_cast<const float4*>(scl + 8 * j + 4 * g);
-        st[4 * j] *= f.x;
-        st[4 * j + 1] *= f.y;
-        st[4 * j + 2] *= f.z;
-        st[4 * j + 3] *= f.w;
+      for (int j = 0; j < 2; ++j) {
+        const float4 f = *reinterpret_cast<const float4*>(scl + 16 * j + 4 * g);
+        const float4 h = *reinterpret_cast<const float4*>(scl + 32 + 16 * j + 4 * g);
+        st[j] *= floatx4{f.x, f.y, f.z, f.w};
+        vs[4 * j] = h.x;
+        vs[4 * j + 1] = h.y;
+        vs[4 * j + 2] = h.z;
+        vs[4 * j + 3] = h.w;
       }
     } else if constexpr (!A::F32) {
 #pragma unroll
-      for (int v = 0; v < 16; ++v) st[v] *= at.cs;
+      for (int j = 0; j < 2; ++j) st[j] *= at.cs;
     }
     const bool whole = k0 + 32 <= hi_least && (k0 >= first_last || k0 + 32 <= a.sinks);
     if (!whole) {
       const int c = k0 + 4 * g;  // the lane's: key i below is c + i
-      A::mask(st, (int)(A::below(hi - c) & (STEP ? ~A::below(first - c) | A::below(a.sinks - c) : ~0u)));
-    }
-    at.refer(A::largest(st, -INFINITY));
-    float4 f[4];
-    if constexpr (HELD) {
+      const int seen = (int)(keys_below(hi - c) & (STEP ? ~keys_below(first - c) | keys_below(a.sinks - c) : ~0u));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float4*>(scl + 32 + 8 * j + 4 * g);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) st[j][v] = masked_score(st[j][v], seen, 16 * j + v);
     }
-    at.add(st, [&](int part, int t, int ks) { return A::v_frag(v0, PLANE, part, t, ks); },
-           [&](int v) { return v % 4 == 0 ? f[v / 4].x : v % 4 == 1 ? f[v / 4].y : v % 4 == 2 ? f[v / 4].z : f[v / 4].w; });
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) mx = max_nan(max_nan(max_nan(mx, st[j][0]), st[j][1]), max_nan(st[j][2], st[j][3]));
+    at.refer(mx);
+    at.add(st, [&](int part, int t) { return A::v_frag(v0, part, t); }, vs);
     __builtin_amdgcn_wave_barrier();
   };
 
   Block x[2];
   int blk = b0 + wave;
   if (blk < b1) fetch(blk, x[0]);
+  at.take_q(q, a.scale);
   for (; blk < b1; blk += 2 * W) {
     if (blk + W < b1) fetch(blk + W, x[1]);
     compute(blk, x[0]);
@@ -314,26 +344,34 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
   // the waves' results through LDS, only the rows' lanes
   const int nr = w.rows;
   constexpr int REGS = Cfg::REGS;
-  float* res = reinterpret_cast<float*>(smem);              // [W][REGS][2][slots]
-  float* refs = res + W * REGS * 2 * slots;                 // [W][slots]
-  int* again = reinterpret_cast<int*>(refs + W * slots);    // [32]
+  float* res = reinterpret_cast<float*>(smem);              // [W][REGS][4][slots]
+  float* refs = res + W * REGS * 4 * slots;                 // [W][slots]
+  int* again = reinterpret_cast<int*>(refs + W * slots);    // [16], and one for last_of
   __syncthreads();
-  if (l32 < nr) {
-    float* to = res + wave * REGS * 2 * slots + g * slots + l32;
+  if (l16 < nr) {
+    float* to = res + wave * REGS * 4 * slots + g * slots + l16;
 #pragma unroll
-    for (int i = 0; i < A::DT; ++i)
+    for (int i = 0; i < A::OT; ++i)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) to[(16 * i + v) * 2 * slots] = at.o[i][v];
-    to[16 * A::DT * 2 * slots] = at.sum;
+      for (int v = 0; v < 4; ++v) to[(4 * i + v) * 4 * slots] = at.o[i][v];
+    to[4 * A::OT * 4 * slots] = at.sum;
     // NaN scores leave the reference at 0 and a sum of NaN
-    if (g == 0) refs[wave * slots + l32] = at.begun || !(at.sum == 0.f) ? at.ref : -INFINITY;
+    if (g == 0) refs[wave * slots + l16] = at.begun ? at.ref : -INFINITY;
   }
-  if (tid < 32) again[tid] = 0;
+  if (tid < 16) again[tid] = 0;
   __syncthreads();
-  const int ld = hd + 2;
+  // joins n results of a row: references, sums and the output's value of each
+  auto finish = [&](int r, int d, float y, float l) {
+    y = w.n ? y / l : 0.f;
+    const int rr = w.row0 + r, t = over(rr, G);
+    static_cast<T*>(a.o)[(((int64_t)w.b * a.T + t) * a.H + w.kvh * G + (rr - t * G)) * hd + d] = from_f32<T>(y);
+    if (A::doubtful(y)) again[r] = 1;
+  };
+  const int ld = hd + 2, unit = (w.b * a.KV + w.kvh) * tiles + tile;
+  float* mine = part + ((int64_t)unit * nsplit + sp) * slots * ld;
   for (int e = tid; e < nr * hd; e += W * 64) {
     const int r = e / hd, d = e % hd;
-    const int reg = 16 * (d / 32) + 4 * (d % 32 / 8) + d % 4, half = d / 4 & 1;
+    const int at0 = ((4 * (d / 16) + d % 4) * 4 + d % 16 / 4) * slots;  // register, lane group
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < W; ++i) top = max_nan(top, refs[i * slots + r]);
@@ -342,118 +380,96 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64)) void rows_kernel(RowsA
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const float by = __builtin_amdgcn_exp2f(refs[i * slots + r] - from);
-      const float* f = res + i * REGS * 2 * slots + r;
-      l = fmaf(f[16 * A::DT * 2 * slots] + f[16 * A::DT * 2 * slots + slots], by, l);
-      y = fmaf(f[(reg * 2 + half) * slots], by, y);
+      const float* f = res + i * REGS * 4 * slots + r;
+      const float* sums = f + 4 * A::OT * 4 * slots;
+      l = fmaf((sums[0] + sums[slots]) + (sums[2 * slots] + sums[3 * slots]), by, l);
+      y = fmaf(f[at0], by, y);
     }
     if (nsplit > 1) {
-      float* f = part + ((int64_t)id * 32 + r) * ld;
-      f[d] = y;
+      put_shared(mine + r * ld + d, y);
       if (d == 0) {
-        f[hd] = top;
-        f[hd + 1] = l;
+        put_shared(mine + r * ld + hd, top);
+        put_shared(mine + r * ld + hd + 1, l);
       }
     } else {
-      y = w.n ? y / l : 0.f;
-      const int rr = w.row0 + r;
-      static_cast<T*>(a.o)[(((int64_t)w.b * a.T + rr / G) * a.H + w.kvh * G + rr % G) * hd + d] = from_f32<T>(y);
-      if (A::doubtful(y)) again[r] = 1;
+      finish(r, d, y, l);
     }
   }
-  if (nsplit > 1) return;
+  if (nsplit > 1) {
+    if (!last_of(counts + unit, nsplit, again + 16)) return;
+    const float* all = part + (int64_t)unit * nsplit * slots * ld;
+    for (int e = tid; e < nr * hd; e += W * 64) {
+      const int r = e / hd, d = e % hd;
+      const float* f = all + r * ld;
+      float top = -INFINITY, l = 0.f, y = 0.f;
+      // eight ranges at a time, their loads at once; a later, larger reference takes the sums so far down
+      for (int s0 = 0; s0 < nsplit; s0 += 8) {
+        float ref[8], sum[8], val[8], m = top;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t at = (int64_t)min(s0 + i, nsplit - 1) * slots * ld;
+          ref[i] = get_shared(f + at + hd);
+          sum[i] = get_shared(f + at + hd + 1);
+          val[i] = get_shared(f + at + d);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max_nan(m, ref[i]);
+        const float from = m == -INFINITY ? 0.f : m, down = __builtin_amdgcn_exp2f(top - from);
+        l *= down;
+        y *= down;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float by = s0 + i < nsplit ? __builtin_amdgcn_exp2f(ref[i] - from) : 0.f;
+          l = fmaf(sum[i], by, l);
+          y = fmaf(val[i], by, y);
+        }
+        top = m;
+      }
+      finish(r, d, y, l);
+    }
+  }
   __syncthreads();
   for (int r = wave; r < nr; r += W)
     if (again[r]) row_again<T, M, STEP>(a, w, r);
 }
 
-// Joins the key ranges of split rows: a workgroup per unit. The ranges' references and sums come first, all at once,
-// and become factors; the outputs are then read eight ranges at a time.
+// How a call is cut: tiles of 16 rows, and how many workgroups share a tile's keys.
 constexpr int kMaxSplits = 64;
-template <class T, class M, bool STEP>
-__global__ __launch_bounds__(256) void rows_join_kernel(RowsArgs a, int tiles, int nsplit, const float* part) {
-  __shared__ float by[32][kMaxSplits], inv[32];
-  __shared__ int again[32];
-  const int G = a.H / a.KV, hd = a.hd, ld = hd + 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Rows w;
-  if (!rows_of<STEP>(a, blockIdx.x, tiles, w)) return;
-  const float* unit0 = part + (int64_t)blockIdx.x * nsplit * 32 * ld;
-  for (int r = wave; r < w.rows; r += 4) {  // lane s: range s
-    float top = -INFINITY, l = 0.f;
-    if (lane < nsplit) {
-      top = unit0[((int64_t)lane * 32 + r) * ld + hd];
-      l = unit0[((int64_t)lane * 32 + r) * ld + hd + 1];
-    }
-    const float all = group_reduce<64>(top, max_nan), ref = all == -INFINITY ? 0.f : all;
-    const float f = __builtin_amdgcn_exp2f(top - ref);
-    const float sum = group_reduce<64>(l * f, Plus{});
-    if (lane < nsplit) by[r][lane] = f;
-    if (lane == 0) {
-      inv[r] = 1.f / sum;
-      again[r] = 0;
-    }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < w.rows * hd; e += 256) {
-    const int r = e / hd, d = e % hd;
-    float y = 0.f;
-    for (int s0 = 0; s0 < nsplit; s0 += 8) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = unit0[((int64_t)min(s0 + i, nsplit - 1) * 32 + r) * ld + d];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s0 + i < nsplit) y = fmaf(v[i], by[r][s0 + i], y);
-    }
-    y = w.n ? y * inv[r] : 0.f;
-    const int rr = w.row0 + r;
-    static_cast<T*>(a.o)[(((int64_t)w.b * a.T + rr / G) * a.H + w.kvh * G + rr % G) * hd + d] = from_f32<T>(y);
-    if (Attend<T, M, 8, false>::doubtful(y)) again[r] = 1;
-  }
-  __syncthreads();
-  for (int r = wave; r < w.rows; r += 4)
-    if (again[r]) row_again<T, M, STEP>(a, w, r);
-}
-
-// How a call is cut: tiles of 32 rows, and how many workgroups share a tile's keys.
 struct Plan {
   int tiles, nsplit;
   int64_t units;
 };
 Plan plan_of(const RowsArgs& a, int64_t keys, int cus) {
   Plan p;
-  p.tiles = (int)cdiv((int64_t)a.T * (a.H / a.KV), 32);
+  p.tiles = (int)cdiv((int64_t)a.T * (a.H / a.KV), 16);
   p.units = (int64_t)a.B * a.KV * p.tiles;
-  p.nsplit = keys < 640 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({keys / 256, cus / p.units, kMaxSplits}));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(keys + 255) / 256, cus / p.units, kMaxSplits}));
   return p;
 }
+int slots_of(const RowsArgs& a) { return (int)std::min<int64_t>(16, (int64_t)a.T * (a.H / a.KV)); }
 int64_t part_floats(const RowsArgs& a, const Plan& p) {
-  return p.nsplit == 1 ? 0 : p.units * p.nsplit * 32 * (a.hd + 2);
+  return p.nsplit == 1 ? 0 : p.units * p.nsplit * slots_of(a) * (a.hd + 2);
 }
 
 template <class T, class M, int KS, bool STEP>
-void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, float* part) {
+void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
   using Cfg = RowsCfg<T, M, KS>;
-  const int slots = (int)std::min<int64_t>(32, (int64_t)a.T * (a.H / a.KV));
-  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>, dim3((unsigned)(p.units * p.nsplit)),
-         dim3(64 * Cfg::W), (size_t)Cfg::lds(slots), a, p.tiles, p.nsplit, slots, part);
+  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>,
+         dim3((unsigned)(p.units * p.nsplit)), dim3(64 * Cfg::W), (size_t)Cfg::lds(slots_of(a)),
+         a, a.H / a.KV, p.tiles, p.nsplit, slots_of(a), join.part, join.counts);
 }
 template <class T, class M, bool STEP>
-void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, float* part) {
+void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
   MNN_REQUIRE(p.units * p.nsplit < (1 << 22), MNN_ERR_INVALID_CONFIGURATION,
               (STEP ? "WindowAttention" : "MemoryAttention") << ": too many sequences and tokens in one call");
-  MNN_REQUIRE(p.nsplit == 1 || part, MNN_ERR_INVALID_ARGUMENT, "rows of attention: split keys need a workspace");
-  switch ((a.hd + 15) / 16) {
-    case 1:
-    case 2: launch_ks<T, M, 2, STEP>(c, a, p, part); break;
-    case 3: launch_ks<T, M, 3, STEP>(c, a, p, part); break;
-    case 4: launch_ks<T, M, 4, STEP>(c, a, p, part); break;
-    case 5: launch_ks<T, M, 5, STEP>(c, a, p, part); break;
-    case 6: launch_ks<T, M, 6, STEP>(c, a, p, part); break;
-    default: launch_ks<T, M, 8, STEP>(c, a, p, part);
+  MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,
+              "rows of attention: split keys need a workspace");
+  switch ((a.hd + 31) / 32) {
+    case 1: return launch_ks<T, M, 1, STEP>(c, a, p, join);
+    case 2: return launch_ks<T, M, 2, STEP>(c, a, p, join);
+    case 3: return launch_ks<T, M, 3, STEP>(c, a, p, join);
+    default: return launch_ks<T, M, 4, STEP>(c, a, p, join);
   }
-  if (p.nsplit > 1)
-    launch(c, "rows_join", rows_join_kernel<T, M, STEP>, dim3((unsigned)p.units), dim3(256), 0, a, p.tiles, p.nsplit,
-           (const float*)part);
 }
 
 RowsArgs step_args(const WindowStepHeldArgs& s) {
@@ -480,7 +496,7 @@ RowsArgs step_args(const WindowStepHeldArgs& s) {
   return a;
 }
 int64_t step_keys(const WindowStepHeldArgs& a) {
-  return std::min<int64_t>((int64_t)a.left + a.sinks + std::min(a.T, 32), a.C);
+  return std::min<int64_t>((int64_t)a.left + a.sinks + std::min(a.T, 16), a.C);
 }
 RowsArgs memory_args(const MemoryArgs& m) {
   RowsArgs a{};
@@ -508,7 +524,7 @@ int64_t window_step_e4m3_part_floats(const LaunchCtx& c, const WindowStepHeldArg
   const RowsArgs a = step_args(s);
   return part_floats(a, plan_of(a, step_keys(s), c.dev->props.multiProcessorCount));
 }
-void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, float* part) {
+void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, const Join& part) {
   const RowsArgs a = step_args(s);
   const Plan p = plan_of(a, step_keys(s), c.dev->props.multiProcessorCount);
   if (s.type == MNN_F32)
@@ -521,7 +537,7 @@ int64_t memory_rows_part_floats(const LaunchCtx& c, const MemoryArgs& m) {
   const RowsArgs a = memory_args(m);
   return part_floats(a, plan_of(a, m.S, c.dev->props.multiProcessorCount));
 }
-void memory_rows(const LaunchCtx& c, const MemoryArgs& m, float* part) {
+void memory_rows(const LaunchCtx& c, const MemoryArgs& m, const Join& part) {
   const RowsArgs a = memory_args(m);
   const Plan p = plan_of(a, m.S, c.dev->props.multiProcessorCount);
   if (m.type == MNN_F32)

@@ -40,6 +40,26 @@ class Scratch {
   size_t size_ = 0;
 };
 
+// A layer's workspace for keys that workgroups share out. The counts are made with the layer, so that a call can be
+// captured into a graph.
+class JoinSpace {
+ public:
+  explicit JoinSpace(Device* d) {
+    d->make_current();
+    counts_.reserve(sizeof(int) * k::kJoinCounts);
+    HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * k::kJoinCounts));
+    HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
+  }
+  k::Join get(int64_t floats) {
+    if (!floats) return {};
+    return {static_cast<float*>(part_.get(sizeof(float) * floats)), counts_.as<int>()};
+  }
+
+ private:
+  DevBuf counts_;
+  Scratch part_;
+};
+
 // Layers without a one-input forward.
 class ManyInputLayer : public Layer {
  public:
@@ -413,7 +433,7 @@ class RotaryLayer : public ManyInputLayer {
 class WindowAttentionLayer : public ManyInputLayer {
  public:
   WindowAttentionLayer(Device* d, const mnn_window_attention_desc& desc)
-      : ManyInputLayer(d), d_(desc) {
+      : ManyInputLayer(d), d_(desc), join_(d) {
     MNN_REQUIRE(desc.num_heads > 0 && desc.num_kv_heads > 0 && desc.num_heads <= 65535 &&
                     desc.num_heads % desc.num_kv_heads == 0,
                 MNN_ERR_INVALID_CONFIGURATION,
@@ -516,9 +536,7 @@ class WindowAttentionLayer : public ManyInputLayer {
     if (ks) {
       a.ks = ks->f32();
       a.vs = vs->f32();
-      const int64_t part = k::window_step_e4m3_part_floats(ctx(s), a);
-      return k::window_step_e4m3(ctx(s), a,
-                                 part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
+      return k::window_step_e4m3(ctx(s), a, join_.get(k::window_step_e4m3_part_floats(ctx(s), a)));
     }
     const int64_t part = k::window_step_part_floats(ctx(s), a);
     k::window_step(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
@@ -551,6 +569,7 @@ class WindowAttentionLayer : public ManyInputLayer {
   }
   mnn_window_attention_desc d_;
   Scratch scratch_;
+  JoinSpace join_;  // of steps on 8-bit caches
 };
 
 // ------------------------------------------------------------------ rolling caches
@@ -629,7 +648,8 @@ class KVCacheLayer : public ManyInputLayer {
 // ------------------------------------------------------------------ attention to an encoder's states
 class MemoryAttentionLayer : public ManyInputLayer {
  public:
-  MemoryAttentionLayer(Device* d, const mnn_memory_attention_desc& desc) : ManyInputLayer(d), d_(desc) {
+  MemoryAttentionLayer(Device* d, const mnn_memory_attention_desc& desc)
+      : ManyInputLayer(d), d_(desc), join_(d) {
     MNN_REQUIRE(desc.num_heads > 0 && desc.num_kv_heads > 0 && desc.num_heads <= 65535 &&
                     desc.num_heads % desc.num_kv_heads == 0,
                 MNN_ERR_INVALID_CONFIGURATION,
@@ -689,13 +709,12 @@ class MemoryAttentionLayer : public ManyInputLayer {
     a.KV = d_.num_kv_heads;
     a.hd = d_.head_dim;
     a.scale = d_.scale;
-    const int64_t part = k::memory_part_floats(ctx(s), a);
-    k::memory_attention(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
+    k::memory_attention(ctx(s), a, join_.get(k::memory_part_floats(ctx(s), a)));
   }
 
  private:
   mnn_memory_attention_desc d_;
-  Scratch scratch_;
+  JoinSpace join_;
 };
 
 }  // namespace

@@ -100,13 +100,20 @@ struct WindowStepArgs {
 int64_t window_step_part_floats(const LaunchCtx& c, const WindowStepArgs& a);
 void window_step(const LaunchCtx& c, const WindowStepArgs& a, float* part);
 
+// Where workgroups that share out the keys of one unit meet: their results, and a count a unit, zeros between calls.
+constexpr int kJoinCounts = 1024;
+struct Join {
+  float* part = nullptr;
+  int* counts = nullptr;  // [kJoinCounts]
+};
+
 // The step on caches in 8 bits: kc and vc in e4m3, a scale for each head's row.
 struct WindowStepHeldArgs : WindowStepArgs {
   float* ks = nullptr;  // [B][C][KV]
   float* vs = nullptr;
 };
 int64_t window_step_e4m3_part_floats(const LaunchCtx& c, const WindowStepHeldArgs& a);
-void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& a, float* part);
+void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& a, const Join& join);
 
 // Rows of keys [0] and values [1] and the caches that they are written to or read from.
 struct KVCacheArgs {
@@ -135,7 +142,7 @@ struct MemoryArgs {
   float scale = 1.f;
 };
 int64_t memory_part_floats(const LaunchCtx& c, const MemoryArgs& a);
-void memory_attention(const LaunchCtx& c, const MemoryArgs& a, float* part);
+void memory_attention(const LaunchCtx& c, const MemoryArgs& a, const Join& join);
 
 }  // namespace k
 }  // namespace mnn
