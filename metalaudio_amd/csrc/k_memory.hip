@@ -39,19 +39,19 @@ struct MemoryCfg {
 };
 
 struct Unit {
-  int b, kvh, row0, rows, n, sp;  // rows: of the sequence's, n: its states
+  int b, kvh, tile, row0, rows, n, sp;  // rows: of the sequence's, n: its states
 };
-__device__ __forceinline__ Unit unit_of(const MemoryArgs& a, int id, int tiles, int nsplit, int bq) {
-  Unit u;
-  u.row0 = id % tiles * bq;
-  id /= tiles;
-  u.sp = id % nsplit;
-  id /= nsplit;
-  u.kvh = id % a.KV;
-  u.b = id / a.KV;
+// The tiles of a head that share a range of keys are a set.
+__device__ __forceinline__ bool unit_of(const MemoryArgs& a, const XcdGroups& sets, int nsplit, int bq, Unit& u) {
+  const int set = sets.set_of((int)blockIdx.x, u.tile), head = set / nsplit;
+  u.sp = set - head * nsplit;
+  u.b = head / a.KV;
+  u.kvh = head - u.b * a.KV;
+  if (u.b >= a.B || u.tile < 0) return false;
+  u.row0 = u.tile * bq;
   u.rows = (a.qlen ? min(max(a.qlen[u.b], 0), a.T) : a.T) * (a.H / a.KV);
   u.n = a.len ? min(max(a.len[u.b], 0), a.S) : a.S;
-  return u;
+  return u.row0 < u.rows;
 }
 // Where row r of a sequence's head group lies in q and o.
 __device__ __forceinline__ int64_t row_at(const MemoryArgs& a, const Unit& u, int r) {
@@ -81,7 +81,7 @@ __device__ __forceinline__ void memory_row_again(const MemoryArgs& a, const Unit
 
 template <class T, class M, int KS, int NW>
 __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M, KS, NW>::OCC)) void memory_kernel(
-    MemoryArgs a, int tiles, int nsplit, float* part, int* counts) {
+    MemoryArgs a, XcdGroups sets, int nsplit, float* part, int* counts) {
   using Cfg = MemoryCfg<T, M, KS, NW>;
   using A = typename Cfg::A;
   constexpr int BKV = Cfg::BKV, NT = Cfg::NT, PM = A::PM, PLANE = Cfg::PLANE, SLOT = Cfg::SLOT, PER = Cfg::PER;
@@ -90,10 +90,8 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
   __shared__ __attribute__((aligned(16))) char smem[Cfg::LDS];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // consecutive units, the rows that share keys first, run on one XCD and share its L2
-  const int id = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
-  const Unit u = unit_of(a, id, tiles, nsplit, Cfg::BQ);
-  if (u.row0 >= u.rows) return;
+  Unit u;
+  if (!unit_of(a, sets, nsplit, Cfg::BQ, u)) return;
   const int nb = (u.n + BKV - 1) / BKV;
   const int b0 = (int)((int64_t)nb * u.sp / nsplit), b1 = (int)((int64_t)nb * (u.sp + 1) / nsplit);
   const int hd = a.hd, kvw = a.KV * hd;
@@ -216,8 +214,9 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
     // O^T, reference and sum to the workspace, a register of all lanes beside each other; the last of the unit's
     // workgroups joins them, in the keys' order
     constexpr int REGS = 16 * A::DT + 2;
-    const int64_t step = (int64_t)tiles * NW * REGS * 64;  // from one range to the next
-    float* first = part + ((int64_t)(id - u.sp * tiles) * NW + wave) * REGS * 64 + lane;
+    const int64_t step = (int64_t)NW * REGS * 64;  // from one range to the next
+    const int unit = (u.b * a.KV + u.kvh) * sets.size + u.tile;
+    float* first = part + ((int64_t)unit * nsplit * NW + wave) * REGS * 64 + lane;
     float* to = first + u.sp * step;
     if (any) {
 #pragma unroll
@@ -228,7 +227,6 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
       put_shared(to + 64 * (REGS - 2), at.begun || !(l == 0.f) ? at.ref * (A::RAW ? at.cs : 1.f) : -INFINITY);
       put_shared(to + 64 * (REGS - 1), l);
     }
-    const int unit = (u.b * a.KV + u.kvh) * tiles + u.row0 / Cfg::BQ;
     if (!last_of(counts + unit, nsplit, reinterpret_cast<int*>(smem)) || !any) return;
     float top = -INFINITY;
     for (int s = 0; s < nsplit; ++s) top = max_nan(top, get_shared(first + s * step + 64 * (REGS - 2)));
@@ -298,12 +296,14 @@ Plan plan_of(const MemoryArgs& a, int cus) {
 
 template <class T, class M, int KS>
 void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
-  launch(c, "memory", memory_kernel<T, M, KS, kWaves>, dim3((unsigned)(p.units * p.nsplit)), dim3(64 * kWaves), 0, a, p.tiles,
-         p.nsplit, join.part, join.counts);
+  const int64_t n = (int64_t)a.B * a.KV * p.nsplit;
+  const XcdGroups sets(n, p.tiles);
+  launch(c, "memory", memory_kernel<T, M, KS, kWaves>, dim3((unsigned)sets.grid(n)), dim3(64 * kWaves), 0, a, sets, p.nsplit,
+         join.part, join.counts);
 }
 template <class T, class M>
 void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
-  MNN_REQUIRE(p.units * p.nsplit < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
+  MNN_REQUIRE(p.units * p.nsplit < (1 << 23), MNN_ERR_INVALID_CONFIGURATION,
               "MemoryAttention: too many tokens in one call");
   MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,
               "memory attention: split keys need a workspace");

@@ -125,7 +125,7 @@ struct RowsCfg {
 
 template <class T, class M, int KS, bool STEP>
 __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OCC)) void rows_kernel(
-    RowsArgs a, int G, int tiles, int nsplit, int slots, float* part, int* counts) {
+    RowsArgs a, XcdGroups sets, int G, int tiles, int nsplit, int slots, float* part, int* counts) {
   using Cfg = RowsCfg<T, M, KS>;
   using A = typename Cfg::A;
   constexpr int W = Cfg::W, PM = A::PM, PLANE = A::PLANE;
@@ -133,14 +133,14 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // heads, key ranges, tiles, sequences: the heads of a sequence, whose rows share cache lines, run on one XCD at one time
-  const int hd = a.hd, id = xcd_logical_tile((int)blockIdx.x, (int)gridDim.x);
+  // the heads of a sequence, whose rows share cache lines, are a set; sets: key ranges, tiles, sequences
+  const int hd = a.hd;
   Rows w;
-  int rest = over(id, a.KV);
-  w.kvh = id - rest * a.KV;
+  int rest = sets.set_of((int)blockIdx.x, w.kvh);
   const int sp = rest - over(rest, nsplit) * nsplit;
   rest = over(rest, nsplit);
   w.b = over(rest, tiles);
+  if (w.b >= a.B || w.kvh < 0) return;
   const int tile = rest - w.b * tiles;
   w.row0 = 16 * tile;
   // the queries' loads go out before the sequence's lengths have come; rows that are no tokens are not used
@@ -454,9 +454,11 @@ int64_t part_floats(const RowsArgs& a, const Plan& p) {
 template <class T, class M, int KS, bool STEP>
 void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
   using Cfg = RowsCfg<T, M, KS>;
+  const int64_t n = (int64_t)a.B * p.tiles * p.nsplit;
+  const XcdGroups sets(n, a.KV);
   launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>,
-         dim3((unsigned)(p.units * p.nsplit)), dim3(64 * Cfg::W), (size_t)Cfg::lds(slots_of(a)),
-         a, a.H / a.KV, p.tiles, p.nsplit, slots_of(a), join.part, join.counts);
+         dim3((unsigned)sets.grid(n)), dim3(64 * Cfg::W), (size_t)Cfg::lds(slots_of(a)),
+         a, sets, a.H / a.KV, p.tiles, p.nsplit, slots_of(a), join.part, join.counts);
 }
 template <class T, class M, bool STEP>
 void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
