@@ -34,8 +34,10 @@ struct MemoryCfg {
   // K planes, V planes, scales; V's fragments of the last 32 dimensions may reach 32 bytes past its rows
   static constexpr int SLOT = 2 * A::PM * PLANE + 64 + (A::HELD ? 2 * BKV * 4 : 0);
   static constexpr int LDS = 2 * SLOT;
-  // workgroups a CU, as the registers allow without spilling
-  static constexpr int OCC = A::F32 ? (A::PM == 3 ? (KS > 6 ? 1 : 2) : (KS > 4 ? 1 : 2)) : (KS > 6 ? 2 : KS > 4 ? 3 : 4);
+  // waves a SIMD, as the registers allow without spilling
+  static constexpr int OCC = A::F32    ? (A::PM == 3 ? (KS > 6 ? 1 : 2) : (KS > 4 ? 1 : 2))
+                             : A::HELD ? (KS > 4 ? 2 : KS > 2 ? 3 : 4)
+                                       : (KS > 5 ? 2 : KS > 4 ? 3 : 4);
 };
 
 struct Unit {
@@ -277,29 +279,39 @@ __global__ __launch_bounds__((MemoryCfg<T, M, KS, NW>::THREADS), (MemoryCfg<T, M
 }
 
 constexpr int kMaxSplits = 16;
-constexpr int kWaves = 4;
 struct Plan {
   bool few;  // rows so few that the other kernel takes them
-  int tiles, nsplit;
+  int waves, tiles, nsplit;
   int64_t units;
 };
 Plan plan_of(const MemoryArgs& a, int cus) {
   Plan p;
-  const int64_t rows = (int64_t)a.T * (a.H / a.KV);
+  const int64_t rows = (int64_t)a.T * (a.H / a.KV), heads = (int64_t)a.B * a.KV;
   p.few = rows <= 64;
-  p.tiles = (int)cdiv(rows, 32 * kWaves);
-  p.units = (int64_t)a.B * a.KV * p.tiles;
-  // ranges of 256 keys and more, while all workgroups run at once, three a compute unit
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({a.S / 256, 3 * cus / p.units, kMaxSplits}));
+  // bf16: 256 rows by 8 waves where that leaves a workgroup for each compute unit (blocks are staged for twice the rows):
+  // us at 128 / 256 rows, 8 / 2 heads of 64: 8192 tokens on 16384 states 345 / 320, in 8 bits 571 / 369; 4 x 1344 on
+  // 2688, 8 heads of 48 51 / 57. f32 there 150 / 170
+  p.waves = a.type == MNN_BF16 && heads * cdiv(rows, 256) >= cus ? 8 : 4;
+  p.tiles = (int)cdiv(rows, 32 * p.waves);
+  p.units = heads * p.tiles;
+  // ranges of 256 keys and more, while all workgroups run at once, 12 or 16 waves a compute unit
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({a.S / 256, (p.waves == 8 ? 2 : 3) * cus / p.units, kMaxSplits}));
+  if (p.units > kJoinCounts) p.nsplit = 1;
   return p;
 }
 
-template <class T, class M, int KS>
-void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
+template <class T, class M, int KS, int NW>
+void launch_nw(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
   const int64_t n = (int64_t)a.B * a.KV * p.nsplit;
   const XcdGroups sets(n, p.tiles);
-  launch(c, "memory", memory_kernel<T, M, KS, kWaves>, dim3((unsigned)sets.grid(n)), dim3(64 * kWaves), 0, a, sets, p.nsplit,
-         join.part, join.counts);
+  launch(c, NW == 8 ? "memory_256" : "memory_128", memory_kernel<T, M, KS, NW>, dim3((unsigned)sets.grid(n)), dim3(64 * NW),
+         0, a, sets, p.nsplit, join.part, join.counts);
+}
+template <class T, class M, int KS>
+void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
+  if constexpr (sizeof(T) == 2)
+    if (p.waves == 8) return launch_nw<T, M, KS, 8>(c, a, p, join);
+  launch_nw<T, M, KS, 4>(c, a, p, join);
 }
 template <class T, class M>
 void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
@@ -324,7 +336,7 @@ int64_t memory_part_floats(const LaunchCtx& c, const MemoryArgs& a) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
   if (p.few) return memory_rows_part_floats(c, a);
   const int dt = a.hd > 96 ? 4 : (a.hd + 31) / 32;  // 32-row tiles of O^T, as AttendMany has them
-  return p.nsplit == 1 ? 0 : p.units * p.nsplit * kWaves * (16 * dt + 2) * 64;
+  return p.nsplit == 1 ? 0 : p.units * p.nsplit * p.waves * (16 * dt + 2) * 64;
 }
 void memory_attention(const LaunchCtx& c, const MemoryArgs& a, const Join& join) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);

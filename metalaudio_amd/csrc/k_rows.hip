@@ -35,6 +35,14 @@ struct RowsArgs {
   int left, sinks;      // of a step
   float scale;
 };
+// How the launch is cut.
+struct RowsCut {
+  XcdGroups sets;          // heads of a sequence's tile and key range
+  int G, tiles, nsplit, slots;
+  FastDiv by_G, by_tiles, by_split, by_hd;
+  float* part;
+  int* counts;
+};
 
 // What a workgroup answers: rows row0 .. row0 + 15 (row = token * G + head of the group) of sequence b, and the keys
 // that any of them sees, numbered from 0. A step's: the sinks before the window's first token, then the window;
@@ -44,18 +52,17 @@ struct Rows {
   int n;                       // keys
   int pos, nt, t0, t1, lo, ns, ring, wrapped;  // of a step; wrapped: place in the ring of token max(lo, sinks)
 };
-__device__ __forceinline__ int over(int x, int by) { return by == 1 ? x : (int)((unsigned)x / (unsigned)by); }
 template <bool STEP>
-__device__ __forceinline__ bool rows_of(const RowsArgs& a, int G, Rows& w) {
+__device__ __forceinline__ bool rows_of(const RowsArgs& a, const RowsCut& c, Rows& w) {
   if constexpr (STEP)
     w.nt = kv_rows(a.c0, a.c1, w.b, a.T, w.pos);
   else
     w.nt = a.c0 ? min(max(a.c0[w.b], 0), a.T) : a.T;
-  w.rows = min(16, w.nt * G - w.row0);
+  w.rows = min(16, w.nt * c.G - w.row0);
   if (w.rows <= 0) return false;
   if constexpr (STEP) {
-    w.t0 = over(w.row0, G);
-    w.t1 = over(w.row0 + w.rows - 1, G);
+    w.t0 = c.by_G(w.row0);
+    w.t1 = c.by_G(w.row0 + w.rows - 1);
     w.lo = max(0, w.pos + w.t0 - a.left);
     w.ns = min(a.sinks, w.lo);
     w.n = w.ns + (w.pos + w.t0 - w.lo) + (w.t1 - w.t0) + 1;
@@ -113,19 +120,18 @@ struct RowsCfg {
   using A = AttendFew<T, M, KS>;
   static constexpr int W = A::PM == 3 && KS > 2 ? 4 : 8;               // waves
   static constexpr int WAVE = A::PM * A::PLANE + (A::HELD ? 256 : 0);  // V's block, and the scales
-  static constexpr int REGS = 4 * A::OT + 1;
   // waves a SIMD, as the registers allow
   static constexpr int OCC = KS == 1   ? (A::PM == 3 ? 3 : 4)
                              : A::PM == 3 ? (KS == 2 ? 2 : 1)
                              : KS == 2    ? (A::HELD && !A::F32 ? 4 : 3)
                                           : (KS == 3 && A::HELD && !A::F32 ? 3 : 2);
-  // bytes: the waves' blocks, or at the end their results (lanes of rows that there are), references and sums
-  static int lds(int slots) { return std::max(W * WAVE, W * 4 * (REGS * 4 * slots + slots)) + 4 * 17; }
+  // bytes: the waves' blocks, or at the end their references and sums and results (lanes of rows that there are)
+  static int lds(int slots) { return std::max(W * WAVE, 4 * (W * 32 + 16 + 64 + W * 4 * A::OT * 4 * slots)); }
 };
 
 template <class T, class M, int KS, bool STEP>
 __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OCC)) void rows_kernel(
-    RowsArgs a, XcdGroups sets, int G, int tiles, int nsplit, int slots, float* part, int* counts) {
+    RowsArgs a, RowsCut c) {
   using Cfg = RowsCfg<T, M, KS>;
   using A = typename Cfg::A;
   constexpr int W = Cfg::W, PM = A::PM, PLANE = A::PLANE;
@@ -136,18 +142,17 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
   // the heads of a sequence, whose rows share cache lines, are a set; sets: key ranges, tiles, sequences
   const int hd = a.hd;
   Rows w;
-  int rest = sets.set_of((int)blockIdx.x, w.kvh);
-  const int sp = rest - over(rest, nsplit) * nsplit;
-  rest = over(rest, nsplit);
-  w.b = over(rest, tiles);
+  int set = c.sets.set_of((int)blockIdx.x, w.kvh), rest = c.by_split(set);
+  const int sp = set - rest * c.nsplit, G = c.G, slots = c.slots;
+  w.b = c.by_tiles(rest);
   if (w.b >= a.B || w.kvh < 0) return;
-  const int tile = rest - w.b * tiles;
+  const int tile = rest - w.b * c.tiles;
   w.row0 = 16 * tile;
   // the queries' loads go out before the sequence's lengths have come; rows that are no tokens are not used
-  const int row = w.row0 + l16, t = over(row, G);
+  const int row = w.row0 + l16, t = c.by_G(row);
   Eight<T> q[KS];
   A::fetch_q(static_cast<const T*>(a.q) + (((int64_t)w.b * a.T + t) * a.H + w.kvh * G + (row - t * G)) * hd, t < a.T, hd, q);
-  if (!rows_of<STEP>(a, G, w)) return;
+  if (!rows_of<STEP>(a, c, w)) return;
 
   A at;
   at.begin();
@@ -161,7 +166,7 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
     first_last = w.ns + (max(0, w.pos + w.t1 - a.left) - w.lo);
   }
 
-  const int nb = (w.n + 31) / 32, each = over(nb + nsplit - 1, nsplit), b0 = sp * each, b1 = min(nb, b0 + each);
+  const int nb = (w.n + 31) / 32, each = c.by_split(nb + c.nsplit - 1), b0 = sp * each, b1 = min(nb, b0 + each);
   struct Block {
     Eight<M> k[2][KS], v[2][KS];  // of keys l16 and 16 + l16
     float scale;                  // of lanes below 32: the scale of key lane, of the others: of value lane - 32
@@ -225,17 +230,18 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
   };
   // keys behind the last: the last one again (their scores are masked, their values cleared); a step's own keys,
   // which the cache does not hold yet: the slot that they will have first, then the rows themselves
+  const int kvw = a.KV * hd;
   auto fetch = [&](int blk, Block& x) {
-    int idx[2];
-    int64_t slot[2];
+    int idx[2], slot[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       idx[j] = min(blk * 32 + 16 * j + l16, w.n - 1);
-      slot[j] = (int64_t)(STEP ? slot_of(a, w, token_of(w, idx[j])) : idx[j]) * a.KV;
-      load(kb + slot[j] * hd, x.k[j]);
-      load(vb + slot[j] * hd, x.v[j]);
+      slot[j] = STEP ? slot_of(a, w, token_of(w, idx[j])) : idx[j];
+      const int64_t at = (int64_t)slot[j] * kvw;
+      load(kb + at, x.k[j]);
+      load(vb + at, x.v[j]);
     }
-    if constexpr (HELD) x.scale = sb[g & 1 ? slot[1] : slot[0]];
+    if constexpr (HELD) x.scale = sb[(int64_t)(g & 1 ? slot[1] : slot[0]) * a.KV];
     if constexpr (STEP)
       if (token_of(w, min(blk * 32 + 31, w.n - 1)) >= w.pos) own_rows(idx, x);
   };
@@ -341,85 +347,88 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
     }
   }
 
-  // the waves' results through LDS, only the rows' lanes
+  // the waves' references, then their results times what these make of them, through LDS, only the rows' lanes
   const int nr = w.rows;
-  constexpr int REGS = Cfg::REGS;
-  float* res = reinterpret_cast<float*>(smem);              // [W][REGS][4][slots]
-  float* refs = res + W * REGS * 4 * slots;                 // [W][slots]
-  int* again = reinterpret_cast<int*>(refs + W * slots);    // [16], and one for last_of
+  constexpr int N = 4 * A::OT;
+  float* refs = reinterpret_cast<float*>(smem);  // [W][16]
+  float* sums = refs + W * 16;                   // [W][16]
+  float* tops = sums + W * 16;                   // [16]
+  int* again = reinterpret_cast<int*>(tops + 16);  // [16], and one for last_of
+  float* res = tops + 64;                        // [W][N][4][slots]
+  // NaN scores leave no reference and a sum of NaN, which stays one times 0
+  const float ref = at.begun ? at.ref : -INFINITY, l = other_half(other_row(at.sum, Plus{}), Plus{});
   __syncthreads();
+  if (lane < 16) refs[wave * 16 + lane] = ref;
+  if (tid < 16) again[tid] = 0;
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < W; ++i) top = max_nan(top, refs[i * 16 + l16]);
+  const float by = __builtin_amdgcn_exp2f(ref - (top == -INFINITY ? 0.f : top));
+  if (lane < 16) {
+    sums[wave * 16 + lane] = l * by;
+    tops[lane] = top;  // the same from every wave
+  }
   if (l16 < nr) {
-    float* to = res + wave * REGS * 4 * slots + g * slots + l16;
+    float* to = res + (wave * N * 4 + g) * slots + l16;
 #pragma unroll
     for (int i = 0; i < A::OT; ++i)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) to[(4 * i + v) * 4 * slots] = at.o[i][v];
-    to[4 * A::OT * 4 * slots] = at.sum;
-    // NaN scores leave the reference at 0 and a sum of NaN
-    if (g == 0) refs[wave * slots + l16] = at.begun ? at.ref : -INFINITY;
+      for (int v = 0; v < 4; ++v) to[(4 * i + v) * 4 * slots] = at.o[i][v] * by;
   }
-  if (tid < 16) again[tid] = 0;
   __syncthreads();
-  // joins n results of a row: references, sums and the output's value of each
   auto finish = [&](int r, int d, float y, float l) {
     y = w.n ? y / l : 0.f;
-    const int rr = w.row0 + r, t = over(rr, G);
+    const int rr = w.row0 + r, t = c.by_G(rr);
     static_cast<T*>(a.o)[(((int64_t)w.b * a.T + t) * a.H + w.kvh * G + (rr - t * G)) * hd + d] = from_f32<T>(y);
     if (A::doubtful(y)) again[r] = 1;
   };
-  const int ld = hd + 2, unit = (w.b * a.KV + w.kvh) * tiles + tile;
-  float* mine = part + ((int64_t)unit * nsplit + sp) * slots * ld;
+  const int ld = hd + 2, unit = (w.b * a.KV + w.kvh) * c.tiles + tile;
+  float* mine = c.part + ((int64_t)unit * c.nsplit + sp) * slots * ld;
   for (int e = tid; e < nr * hd; e += W * 64) {
-    const int r = e / hd, d = e % hd;
-    const int at0 = ((4 * (d / 16) + d % 4) * 4 + d % 16 / 4) * slots;  // register, lane group
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < W; ++i) top = max_nan(top, refs[i * slots + r]);
-    const float from = top == -INFINITY ? 0.f : top;
+    const int r = c.by_hd(e), d = e - r * hd;
+    const float* f = res + ((4 * (d / 16) + d % 4) * 4 + d % 16 / 4) * slots + r;  // register, lane group
     float l = 0.f, y = 0.f;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const float by = __builtin_amdgcn_exp2f(refs[i * slots + r] - from);
-      const float* f = res + i * REGS * 4 * slots + r;
-      const float* sums = f + 4 * A::OT * 4 * slots;
-      l = fmaf((sums[0] + sums[slots]) + (sums[2 * slots] + sums[3 * slots]), by, l);
-      y = fmaf(f[at0], by, y);
+      l += sums[i * 16 + r];
+      y += f[i * N * 4 * slots];
     }
-    if (nsplit > 1) {
+    if (c.nsplit > 1) {
       put_shared(mine + r * ld + d, y);
       if (d == 0) {
-        put_shared(mine + r * ld + hd, top);
+        put_shared(mine + r * ld + hd, tops[r]);
         put_shared(mine + r * ld + hd + 1, l);
       }
     } else {
       finish(r, d, y, l);
     }
   }
-  if (nsplit > 1) {
-    if (!last_of(counts + unit, nsplit, again + 16)) return;
-    const float* all = part + (int64_t)unit * nsplit * slots * ld;
+  if (c.nsplit > 1) {
+    if (!last_of(c.counts + unit, c.nsplit, again + 16)) return;
+    const float* all = c.part + (int64_t)unit * c.nsplit * slots * ld;
     for (int e = tid; e < nr * hd; e += W * 64) {
-      const int r = e / hd, d = e % hd;
+      const int r = c.by_hd(e), d = e - r * hd;
       const float* f = all + r * ld;
       float top = -INFINITY, l = 0.f, y = 0.f;
-      // eight ranges at a time, their loads at once; a later, larger reference takes the sums so far down
-      for (int s0 = 0; s0 < nsplit; s0 += 8) {
-        float ref[8], sum[8], val[8], m = top;
+      // four ranges at a time, their loads at once; a later, larger reference takes the sums so far down
+      for (int s0 = 0; s0 < c.nsplit; s0 += 4) {
+        float ref[4], sum[4], val[4], m = top;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t at = (int64_t)min(s0 + i, nsplit - 1) * slots * ld;
-          ref[i] = get_shared(f + at + hd);
-          sum[i] = get_shared(f + at + hd + 1);
-          val[i] = get_shared(f + at + d);
+        for (int i = 0; i < 4; ++i) {
+          const float* p = f + (int64_t)min(s0 + i, c.nsplit - 1) * slots * ld;
+          ref[i] = get_shared(p + hd);
+          sum[i] = get_shared(p + hd + 1);
+          val[i] = get_shared(p + d);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max_nan(m, ref[i]);
+        for (int i = 0; i < 4; ++i) m = max_nan(m, ref[i]);
         const float from = m == -INFINITY ? 0.f : m, down = __builtin_amdgcn_exp2f(top - from);
         l *= down;
         y *= down;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float by = s0 + i < nsplit ? __builtin_amdgcn_exp2f(ref[i] - from) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const float by = s0 + i < c.nsplit ? __builtin_amdgcn_exp2f(ref[i] - from) : 0.f;
           l = fmaf(sum[i], by, l);
           y = fmaf(val[i], by, y);
         }
@@ -456,13 +465,16 @@ void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join&
   using Cfg = RowsCfg<T, M, KS>;
   const int64_t n = (int64_t)a.B * p.tiles * p.nsplit;
   const XcdGroups sets(n, a.KV);
-  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>,
-         dim3((unsigned)sets.grid(n)), dim3(64 * Cfg::W), (size_t)Cfg::lds(slots_of(a)),
-         a, sets, a.H / a.KV, p.tiles, p.nsplit, slots_of(a), join.part, join.counts);
+  const int G = a.H / a.KV;
+  const RowsCut cut{sets, G, p.tiles, p.nsplit, slots_of(a), FastDiv(G), FastDiv(p.tiles), FastDiv(p.nsplit), FastDiv(a.hd), join.part,
+                    join.counts};
+  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>, dim3((unsigned)sets.grid(n)), dim3(64 * Cfg::W),
+         (size_t)Cfg::lds(slots_of(a)), a, cut);
 }
 template <class T, class M, bool STEP>
 void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
-  MNN_REQUIRE(p.units * p.nsplit < (1 << 22), MNN_ERR_INVALID_CONFIGURATION,
+  // what the kernel's divisions by FastDiv hold for, and a grid of 2^32 lanes
+  MNN_REQUIRE((int64_t)a.T * (a.H / a.KV) < (1 << 24) && p.units * p.nsplit < (1 << 20), MNN_ERR_INVALID_CONFIGURATION,
               (STEP ? "WindowAttention" : "MemoryAttention") << ": too many sequences and tokens in one call");
   MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,
               "rows of attention: split keys need a workspace");

@@ -80,21 +80,33 @@ __device__ __forceinline__ int xcd_logical_tile(int lin, int total) {
   return xcd < r ? xcd * (q + 1) + slot : r * (q + 1) + (xcd - r) * q + slot;
 }
 
+// Division by a number that the host knows, of x with x * by < 2^40: a few instructions, where the compiler's own takes
+// some 25, which a kernel of a few microseconds fetches once for each use.
+struct FastDiv {
+  unsigned long long m;
+  explicit FastDiv(int by) : m(((1ull << 40) + by - 1) / by) {}
+  __device__ __forceinline__ int operator()(int x) const { return (int)((unsigned)x * m >> 40); }
+};
+
 // Sets of `size` workgroups that share what they read, `sets` of them: each set is cut into groups of `inner`, which are dealt
 // round robin over the XCDs, so that the members of a group run on one XCD, and sets of unlike work, which follow each
 // other, on all of them. A set is cut smaller while there are fewer than 4 groups an XCD. Workgroups of sets behind the
 // last, and of members behind a set's last, are left out by the kernel.
 struct XcdGroups {
-  int size, inner, cuts;
-  XcdGroups(int64_t sets, int size_) : size(size_), inner(size_) {
+  int size, inner;
+  FastDiv by_inner, by_cuts;
+  int cuts;
+  XcdGroups(int64_t sets, int size_) : size(size_), inner(cut(sets, size_)), by_inner(inner), by_cuts((size_ + inner - 1) / inner),
+                                       cuts((size_ + inner - 1) / inner) {}
+  static int cut(int64_t sets, int size) {
+    int inner = size;
     while (inner > 1 && sets * ((size + inner - 1) / inner) < 32) inner = (inner + 1) / 2;
-    cuts = (size + inner - 1) / inner;
+    return inner;
   }
   int64_t grid(int64_t sets) const { return (sets * cuts + 7) / 8 * 8 * inner; }
-  // the set, and the workgroup's member of it (-1: none)
+  // the set, and the workgroup's member of it (-1: none); for grids below 2^24, sets below 2^16
   __device__ __forceinline__ int set_of(int lin, int& member) const {
-    const auto over = [](int x, int by) { return by == 1 ? x : (int)((unsigned)x / (unsigned)by); };
-    const int xcd = lin & 7, slot = lin >> 3, q = over(slot, inner), group = q * 8 + xcd, set = over(group, cuts);
+    const int xcd = lin & 7, slot = lin >> 3, q = by_inner(slot), group = q * 8 + xcd, set = by_cuts(group);
     member = (group - set * cuts) * inner + (slot - q * inner);
     if (member >= size) member = -1;
     return set;
