@@ -132,6 +132,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;
   static_assert(SLOT % (1024 * NW) == 0, "whole loads a wave");
   constexpr int FM = WM / 32, FN = WN / 32;
+  // blocks: a depth step's sums are kept apart until its end, where registers allow, else until its middle
+  constexpr bool KEEP = BLK && FM * FN <= 4;
   constexpr int OP = WN + 4;  // floats a row of the results in LDS
   constexpr int BYTES = 2 * SLOT > NW * 32 * OP * 4 ? 2 * SLOT : NW * 32 * OP * 4;
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
@@ -220,11 +222,12 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     }
     if (k + 1 < nk) issue(k + 1, slot ^ 1);
     const char* p = smem + slot * SLOT;
+    floatx16 t[KEEP ? FN : 1][KEEP ? FM : 1];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int c0 = at(4 * s + 2 * g), c1 = at(4 * s + 2 * g + 1);
       Operand x[FM], w[FN];
-      if constexpr (BLK) {
+      if constexpr (BLK && !KEEP) {
 #pragma unroll
         for (int i = 0; i < FN; ++i)
           w[i].set(*reinterpret_cast<const intx4*>(p + wa + 4096 * i + c0),
@@ -249,7 +252,22 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = mul(w[i], x[j], acc[i][j]);
+        for (int j = 0; j < FM; ++j) {
+          if constexpr (KEEP) {
+            if (s == 0) t[i][j] = floatx16{0.f};
+            t[i][j] = mul(w[i], x[j], t[i][j]);
+          } else {
+            acc[i][j] = mul(w[i], x[j], acc[i][j]);
+          }
+        }
+    }
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[i][j][v] = fmaf(t[i][j][v], by[j], acc[i][j][v]);
     }
   }
 

@@ -115,26 +115,28 @@ __device__ void row_again(const RowsArgs& a, const Rows& w, int r) {
   if (lane + 64 < a.hd) o[lane + 64] = from_f32<T>(o1);
 }
 
-template <class T, class M, int KS>
+// W: waves of a workgroup.
+template <class T, class M, int KS, int W>
 struct RowsCfg {
   using A = AttendFew<T, M, KS>;
-  static constexpr int W = A::PM == 3 && KS > 2 ? 4 : 8;               // waves
   static constexpr int WAVE = A::PM * A::PLANE + (A::HELD ? 256 : 0);  // V's block, and the scales
   // waves a SIMD, as the registers allow
-  static constexpr int OCC = KS == 1   ? (A::PM == 3 ? 3 : 4)
-                             : A::PM == 3 ? (KS == 2 ? 2 : 1)
-                             : KS == 2    ? (A::HELD && !A::F32 ? 4 : 3)
-                                          : (KS == 3 && A::HELD && !A::F32 ? 3 : 2);
+  static constexpr int OCC = W == 16 || KS == 1 ? 4
+                             : A::PM == 3       ? (KS == 2 ? 2 : 1)
+                             : A::F32           ? (KS == 2 ? 3 : 2)
+                             : KS == 4          ? 2
+                             : KS == 3          ? 3
+                                                : 4;
   // bytes: the waves' blocks, or at the end their references and sums and results (lanes of rows that there are)
   static int lds(int slots) { return std::max(W * WAVE, 4 * (W * 32 + 16 + 64 + W * 4 * A::OT * 4 * slots)); }
 };
 
-template <class T, class M, int KS, bool STEP>
-__global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OCC)) void rows_kernel(
+template <class T, class M, int KS, int W, bool STEP>
+__global__ __launch_bounds__((W * 64), (RowsCfg<T, M, KS, W>::OCC)) void rows_kernel(
     RowsArgs a, RowsCut c) {
-  using Cfg = RowsCfg<T, M, KS>;
+  using Cfg = RowsCfg<T, M, KS, W>;
   using A = typename Cfg::A;
-  constexpr int W = Cfg::W, PM = A::PM, PLANE = A::PLANE;
+  constexpr int PM = A::PM, PLANE = A::PLANE;
   constexpr bool HELD = A::HELD;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, l16 = lane & 15;
@@ -192,38 +194,42 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
       x[s].load(row + (A::may_end(s) ? min(d, hd - 8) : d));
     }
   };
-  // a step's own keys and values, rounded as the cache will hold them
+  // a step's own keys and values, rounded as the cache will hold them: lanes of other keys read the call's first row
+  // and leave it
   auto own_rows = [&](const int (&idx)[2], Block& x) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int p = token_of(w, idx[j]);
-      const bool mine = p >= w.pos;
-      const int64_t from = (((int64_t)w.b * a.T + (mine ? p - w.pos : 0)) * a.KV + w.kvh) * hd;
+      const int p = token_of(w, idx[j]) - w.pos;
+      const bool mine = p >= 0;
+      if (!__any(mine)) continue;
+      const int64_t from = (((int64_t)w.b * a.T + max(p, 0)) * a.KV + w.kvh) * hd;
+      Eight<T> e[2][KS];
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const T* src = static_cast<const T*>(kv ? a.vn : a.kn) + from;
-        Eight<T> e[KS];
-        float top = 0.f;
+      for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int d = A::dim_of(s, g);
-          e[s].clear();
-          if (mine && d < hd) e[s].load(src + d);
+          e[kv][s].load(static_cast<const T*>(kv ? a.vn : a.kn) + from + (A::may_end(s) ? min(d, hd - 8) : d));
         }
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        float top = 0.f;  // of the row; a chunk behind its end is one of it again
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(e[s][i]));
+          for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(e[kv][s][i]));
         const RowScale rs = row_scale(other_half(other_row(top, max_nan), max_nan));
         if constexpr (HELD) {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            const uint2 r = make_uint2(
-                pack_e4m3(e[s][0] * rs.inv, e[s][1] * rs.inv, e[s][2] * rs.inv, e[s][3] * rs.inv),
-                pack_e4m3(e[s][4] * rs.inv, e[s][5] * rs.inv, e[s][6] * rs.inv, e[s][7] * rs.inv));
-            if (mine) (kv ? x.v[j][s] : x.k[j][s]).x = r;
+            const Eight<T>& t = e[kv][s];
+            const uint2 r = make_uint2(pack_e4m3(t[0] * rs.inv, t[1] * rs.inv, t[2] * rs.inv, t[3] * rs.inv),
+                                       pack_e4m3(t[4] * rs.inv, t[5] * rs.inv, t[6] * rs.inv, t[7] * rs.inv));
+            uint2& to = (kv ? x.v[j][s] : x.k[j][s]).x;
+            to.x = mine ? r.x : to.x;
+            to.y = mine ? r.y : to.y;
           }
-          if (mine && g == 2 * kv + j) x.scale = rs.scale;
+          x.scale = mine && g == 2 * kv + j ? rs.scale : x.scale;
         }
       }
     }
@@ -312,16 +318,17 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
     __builtin_amdgcn_wave_barrier();
   };
 
-  Block x[2];
-  int blk = b0 + wave;
-  if (blk < b1) fetch(blk, x[0]);
+  // one copy of the code: a launch fetches all that it executes once, some 100 ns for 64 bytes, which is most of a short
+  // call's time (two copies, for blocks that alternate: 17 keys a wave more 1.9 us more)
   at.take_q(q, a.scale);
-  for (; blk < b1; blk += 2 * W) {
-    if (blk + W < b1) fetch(blk + W, x[1]);
-    compute(blk, x[0]);
-    if (blk + W >= b1) break;
-    if (blk + 2 * W < b1) fetch(blk + 2 * W, x[0]);
-    compute(blk + W, x[1]);
+  Block x, next;
+  const int mine0 = b0 + wave;
+#pragma unroll 1
+  for (int blk = mine0;; blk += W) {
+    if (blk < b1) fetch(blk, next);
+    if (blk != mine0) compute(blk - W, x);
+    if (blk >= b1) break;
+    x = next;
   }
 
   // the step's own rows to their slots: no key that is still seen lies there
@@ -442,17 +449,24 @@ __global__ __launch_bounds__((RowsCfg<T, M, KS>::W * 64), (RowsCfg<T, M, KS>::OC
     if (again[r]) row_again<T, M, STEP>(a, w, r);
 }
 
-// How a call is cut: tiles of 16 rows, and how many workgroups share a tile's keys.
+// How a call is cut: tiles of 16 rows, the waves of a workgroup, and how many workgroups share a tile's keys.
 constexpr int kMaxSplits = 64;
 struct Plan {
-  int tiles, nsplit;
+  int tiles, waves, nsplit;
   int64_t units;
 };
-Plan plan_of(const RowsArgs& a, int64_t keys, int cus) {
+Plan plan_of(const RowsArgs& a, mnn_dtype type, int64_t keys, int cus) {
   Plan p;
   p.tiles = (int)cdiv((int64_t)a.T * (a.H / a.KV), 16);
   p.units = (int64_t)a.B * a.KV * p.tiles;
-  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(keys + 255) / 256, cus / p.units, kMaxSplits}));
+  // 16 waves where 8-bit keys come to that many blocks a compute unit (and the registers allow four waves a SIMD): us with 8 /
+  // 16, 16 / 4 heads of 64: 64 streams on 4096 keys 37 / 28, on 2688 states 24 / 19; 8 heads, 16 streams on 2048 17 / 15; 8 / 2
+  // heads, 8 streams' 16 tokens on 1024 13.5 / 15.2. Keys of 16 bits are bound by memory (33 / 33). 4 where f32 keys of
+  // more than 64 dimensions take a SIMD's registers for one wave
+  const bool held = a.ks != nullptr, fits = a.hd <= (type == MNN_BF16 ? 64 : 32);
+  p.waves = held && fits && p.units * keys >= (int64_t)16 * 32 * cus ? 16 : !held && type == MNN_F32 && a.hd > 64 ? 4 : 8;
+  // a block for each wave, while that leaves no more workgroups than compute units: one that waits for others costs 2 us
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(keys, 32 * p.waves), cus / p.units, kMaxSplits}));
   return p;
 }
 int slots_of(const RowsArgs& a) { return (int)std::min<int64_t>(16, (int64_t)a.T * (a.H / a.KV)); }
@@ -460,16 +474,21 @@ int64_t part_floats(const RowsArgs& a, const Plan& p) {
   return p.nsplit == 1 ? 0 : p.units * p.nsplit * slots_of(a) * (a.hd + 2);
 }
 
-template <class T, class M, int KS, bool STEP>
-void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
-  using Cfg = RowsCfg<T, M, KS>;
+template <class T, class M, int KS, int W, bool STEP>
+void launch_w(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
   const int64_t n = (int64_t)a.B * p.tiles * p.nsplit;
   const XcdGroups sets(n, a.KV);
   const int G = a.H / a.KV;
-  const RowsCut cut{sets, G, p.tiles, p.nsplit, slots_of(a), FastDiv(G), FastDiv(p.tiles), FastDiv(p.nsplit), FastDiv(a.hd), join.part,
-                    join.counts};
-  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, STEP>, dim3((unsigned)sets.grid(n)), dim3(64 * Cfg::W),
-         (size_t)Cfg::lds(slots_of(a)), a, cut);
+  const RowsCut cut{sets,          G,          p.tiles, p.nsplit, slots_of(a), FastDiv(G), FastDiv(p.tiles), FastDiv(p.nsplit),
+                    FastDiv(a.hd), join.part, join.counts};
+  launch(c, STEP ? "rows_step" : "rows_memory", rows_kernel<T, M, KS, W, STEP>, dim3((unsigned)sets.grid(n)), dim3(64 * W),
+         (size_t)RowsCfg<T, M, KS, W>::lds(slots_of(a)), a, cut);
+}
+template <class T, class M, int KS, bool STEP>
+void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
+  if constexpr (sizeof(M) == 1 && KS <= (sizeof(T) == 2 ? 2 : 1))
+    if (p.waves == 16) return launch_w<T, M, KS, 16, STEP>(c, a, p, join);
+  launch_w<T, M, KS, (sizeof(M) == 4 && KS > 2 ? 4 : 8), STEP>(c, a, p, join);
 }
 template <class T, class M, bool STEP>
 void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
@@ -536,11 +555,11 @@ RowsArgs memory_args(const MemoryArgs& m) {
 
 int64_t window_step_e4m3_part_floats(const LaunchCtx& c, const WindowStepHeldArgs& s) {
   const RowsArgs a = step_args(s);
-  return part_floats(a, plan_of(a, step_keys(s), c.dev->props.multiProcessorCount));
+  return part_floats(a, plan_of(a, s.type, step_keys(s), c.dev->props.multiProcessorCount));
 }
 void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, const Join& part) {
   const RowsArgs a = step_args(s);
-  const Plan p = plan_of(a, step_keys(s), c.dev->props.multiProcessorCount);
+  const Plan p = plan_of(a, s.type, step_keys(s), c.dev->props.multiProcessorCount);
   if (s.type == MNN_F32)
     launch_rows<float, E4m3, true>(c, a, p, part);
   else
@@ -549,11 +568,11 @@ void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, const Joi
 
 int64_t memory_rows_part_floats(const LaunchCtx& c, const MemoryArgs& m) {
   const RowsArgs a = memory_args(m);
-  return part_floats(a, plan_of(a, m.S, c.dev->props.multiProcessorCount));
+  return part_floats(a, plan_of(a, m.type, m.S, c.dev->props.multiProcessorCount));
 }
 void memory_rows(const LaunchCtx& c, const MemoryArgs& m, const Join& part) {
   const RowsArgs a = memory_args(m);
-  const Plan p = plan_of(a, m.S, c.dev->props.multiProcessorCount);
+  const Plan p = plan_of(a, m.type, m.S, c.dev->props.multiProcessorCount);
   if (m.type == MNN_F32)
     m.ks ? launch_rows<float, E4m3, false>(c, a, p, part) : launch_rows<float, float, false>(c, a, p, part);
   else
