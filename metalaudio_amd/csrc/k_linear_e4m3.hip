@@ -387,13 +387,18 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
   }
 }
 
-__global__ __launch_bounds__(256) void pad_rows_u8_kernel(const uint8_t* x, int64_t rows, int n,
-                                                          uint8_t* y, int ld) {
-  const int64_t total = rows * ld;
+// V: bytes a lane, which divide n, and ld
+template <class V>
+__global__ __launch_bounds__(256) void pad_rows_u8_kernel(const uint8_t* x, int64_t rows, int n, uint8_t* y, int ld) {
+  constexpr int B = sizeof(V);
+  const int per = ld / B;
+  const int64_t total = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / ld;
-    const int col = (int)(i - row * ld);
-    y[i] = col < n ? x[row * n + col] : 0;
+    const int64_t row = i / per;
+    const int col = (int)(i - row * per) * B;
+    V v{};
+    if (col < n) v = *reinterpret_cast<const V*>(x + row * n + col);
+    *reinterpret_cast<V*>(y + row * ld + col) = v;
   }
 }
 
@@ -434,8 +439,17 @@ void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y
 }
 
 void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint8_t* y, int ld) {
-  const dim3 grid((unsigned)std::min<int64_t>((rows * ld + 255) / 256, 1 << 20));
-  launch(c, "pad_rows_u8", pad_rows_u8_kernel, grid, dim3(256), 0, x, rows, n, y, ld);
+  auto go = [&](auto v) {
+    using V = decltype(v);
+    const int64_t units = rows * (ld / (int)sizeof(V));
+    launch(c, "pad_rows_u8", pad_rows_u8_kernel<V>, dim3((unsigned)std::min<int64_t>((units + 255) / 256, 1 << 20)),
+           dim3(256), 0, x, rows, n, y, ld);
+  };
+  MNN_REQUIRE(ld % 16 == 0, MNN_ERR_INVALID_ARGUMENT, "pad_rows_u8: rows of whole 16 bytes");
+  if (n % 16 == 0) return go(uint4{});
+  if (n % 8 == 0) return go(uint2{});
+  if (n % 4 == 0) return go(0u);
+  go((uint8_t)0);
 }
 
 namespace {
@@ -472,7 +486,9 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   const int64_t cus = c.dev->props.multiProcessorCount;
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
-    return launch_tile<T, BLK, 256, 256, 128, 64>(c, a, tile_name(BLK, 3, F32));
+    // blocks: by 128 x 256, whose waves of 64 x 64 have the registers to keep a depth step's sums apart (8192 x 4096 x 4096
+    // 291 -> 276 us; 256 x 128 281)
+    return launch_tile<T, BLK, BLK ? 128 : 256, 256, BLK ? 64 : 128, 64>(c, a, tile_name(BLK, 3, F32));
   // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
   // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9
   if (4 * tiles(128) >= 3 * cus)
