@@ -287,7 +287,11 @@ struct Plan {
 Plan plan_of(const MemoryArgs& a, int cus) {
   Plan p;
   const int64_t rows = (int64_t)a.T * (a.H / a.KV), heads = (int64_t)a.B * a.KV;
-  p.few = rows <= 64;
+  // Tiles of 16 rows (k_rows.hip) up to a workgroup for four compute units, or where one holds all rows of a head: their
+  // workgroups share out the keys in finer ranges, but each reads all of them for its 16 rows. us there / here, 4 heads of
+  // 64, bf16: one sequence of 128 rows on 16384 states 26 / 33, on 1344 13.4 / 15.2 (f32 15.5 / 25.9), of 512 rows on
+  // 16384 39 / 35, on 4096 17 / 24; 16 sequences of 32 rows on 1344 17 / 15, of 16 rows 12 / 15.
+  p.few = rows <= 16 || heads * cdiv(rows, 16) <= cus / 4;
   // bf16: 256 rows by 8 waves where that leaves a workgroup for each compute unit (blocks are staged for twice the rows):
   // us at 128 / 256 rows, 8 / 2 heads of 64: 8192 tokens on 16384 states 345 / 320, in 8 bits 571 / 369; 4 x 1344 on
   // 2688, 8 heads of 48 51 / 57. f32 there 150 / 170
@@ -315,7 +319,7 @@ void launch_ks(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Joi
 }
 template <class T, class M>
 void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
-  MNN_REQUIRE(p.units * p.nsplit < (1 << 23), MNN_ERR_INVALID_CONFIGURATION,
+  MNN_REQUIRE(p.units * p.nsplit < (1 << 23) && (int64_t)a.T * (a.H / a.KV) <= (1 << 30), MNN_ERR_INVALID_CONFIGURATION,
               "MemoryAttention: too many tokens in one call");
   MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,
               "memory attention: split keys need a workspace");

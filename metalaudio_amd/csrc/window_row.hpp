@@ -9,16 +9,7 @@
 namespace mnn {
 namespace dev {
 
-// A row of 8-bit values and its scale, read as what they stand for.
-struct E4m3Row {
-  const uint8_t* p;
-  float scale;
-  __device__ __forceinline__ float operator[](int d) const {
-    return __builtin_amdgcn_cvt_f32_fp8((int)p[d], 0) * scale;
-  }
-};
-
-// key_at(t) / value_at(t): rows of the t-th of n visible keys, as pointers or E4m3Row. Returns the outputs of dimensions
+// key_at(t) / value_at(t): row pointers of the t-th of n visible keys. Returns the outputs of dimensions
 // lane and lane + 64 (HD <= 128).
 template <class T, class K, class V>
 __device__ __forceinline__ void window_row(const T* __restrict__ q, int hd, float scale, int64_t n,
@@ -31,7 +22,7 @@ __device__ __forceinline__ void window_row(const T* __restrict__ q, int hd, floa
     const int cnt = (int)(n - t0 < 64 ? n - t0 : 64);
     float s = -INFINITY;
     if (lane < cnt) {
-      const auto kp = key_at(t0 + lane);
+      const T* kp = key_at(t0 + lane);
       float dot = 0.f;
       for (int d = 0; d < hd; ++d) dot = fmaf(to_f32(q[d]), to_f32(kp[d]), dot);
       s = dot * qs;
@@ -53,7 +44,7 @@ __device__ __forceinline__ void window_row(const T* __restrict__ q, int hd, floa
     o1 *= alpha;
     for (int j = 0; j < cnt; ++j) {
       const float pj = __shfl(p, j, 64);
-      const auto vp = value_at(t0 + j);
+      const T* vp = value_at(t0 + j);
       if (lane < hd) o0 = fmaf(pj, to_f32(vp[lane]), o0);
       if (lane + 64 < hd) o1 = fmaf(pj, to_f32(vp[lane + 64]), o1);
     }

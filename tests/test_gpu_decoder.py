@@ -676,7 +676,20 @@ def test_memory_attention(dev, stream, B, T, S, H, KV, hd, kw, dtype, held):
 
 @pytest.mark.parametrize("held", [False, True])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("T,S", [(1, 900), (40, 333), (300, 200)])
+@pytest.mark.parametrize("B,T,S,kw", [
+    (3, 150, 700, {"lengths": [700, 1, 513]}), (6, 70, 100, {"queries": [70, 69, 0, 1, 33, 64]}),
+    (8, 900, 90, {"lengths": [90, 0, 64, 65, 1, 31, 33, 90], "queries": [900, 769, 768, 513, 900, 1, 0, 257]}),
+    (8, 800, 520, {"lengths": [520, 300, 520, 257, 10, 512, 511, 260]})])
+@pytest.mark.parametrize("hd", [16, 40, 48, 64, 72, 96, 128])
+def test_memory_attention_many_rows(dev, stream, B, T, S, kw, hd, dtype, held):
+    say(f"memory rows {B}x{T} on {S} hd {hd} {kw} {dtype} held {held}")
+    KV = 4 if B < 8 else 8
+    memory_case(dev, stream, B, T, S, KV, KV, hd, dtype, held, **kw)
+
+
+@pytest.mark.parametrize("held", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,S", [(1, 900), (40, 333), (300, 200), (600, 200)])
 def test_memory_attention_sizes(dev, stream, T, S, dtype, held):
     """Scores from tiny to hundreds, rising along the keys, and values of all sizes."""
     say(f"memory sizes {T} on {S} {dtype} held {held}")
@@ -690,7 +703,7 @@ def test_memory_attention_sizes(dev, stream, T, S, dtype, held):
         memory_case(dev, stream, 1, T, S, H, H, hd, dtype, held, v=rng.standard_normal((1, S, H * hd)) * size)
 
 
-@pytest.mark.parametrize("T", [1, 50, 300])
+@pytest.mark.parametrize("T", [1, 50, 300, 8192])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_memory_attention_not_finite(dev, stream, T, dtype):
     """A NaN or an infinity among the values reaches its head and dimension, a NaN key its head; other
