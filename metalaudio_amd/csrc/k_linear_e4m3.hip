@@ -132,8 +132,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;
   static_assert(SLOT % (1024 * NW) == 0, "whole loads a wave");
   constexpr int FM = WM / 32, FN = WN / 32;
-  // blocks: a depth step's sums are kept apart until its end, where registers allow, else until its middle
-  constexpr bool KEEP = BLK && FM * FN <= 4;
+  // blocks: a depth step's sums are kept apart until its end; tiles larger than 64 x 64 have no registers for that
+  static_assert(!BLK || FM * FN <= 4, "registers");
   constexpr int OP = WN + 4;  // floats a row of the results in LDS
   constexpr int BYTES = 2 * SLOT > NW * 32 * OP * 4 ? 2 * SLOT : NW * 32 * OP * 4;
   __shared__ __attribute__((aligned(1024))) char smem[BYTES];
@@ -222,25 +222,11 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     }
     if (k + 1 < nk) issue(k + 1, slot ^ 1);
     const char* p = smem + slot * SLOT;
-    floatx16 t[KEEP ? FN : 1][KEEP ? FM : 1];
+    floatx16 t[BLK ? FN : 1][BLK ? FM : 1];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int c0 = at(4 * s + 2 * g), c1 = at(4 * s + 2 * g + 1);
       Operand x[FM], w[FN];
-      if constexpr (BLK && !KEEP) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-          w[i].set(*reinterpret_cast<const intx4*>(p + wa + 4096 * i + c0),
-                   *reinterpret_cast<const intx4*>(p + wa + 4096 * i + c1));
-#pragma unroll
-        for (int j = 0; j < FM; ++j) {
-          x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
-                   *reinterpret_cast<const intx4*>(p + xa + 4096 * j + c1));
-#pragma unroll
-          for (int i = 0; i < FN; ++i) mul_scaled(w[i], x[j], by[j], acc[i][j]);
-        }
-        continue;
-      }
 #pragma unroll
       for (int j = 0; j < FM; ++j)
         x[j].set(*reinterpret_cast<const intx4*>(p + xa + 4096 * j + c0),
@@ -253,7 +239,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
       for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
-          if constexpr (KEEP) {
+          if constexpr (BLK) {
             if (s == 0) t[i][j] = floatx16{0.f};
             t[i][j] = mul(w[i], x[j], t[i][j]);
           } else {
@@ -261,7 +247,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
           }
         }
     }
-    if constexpr (KEEP) {
+    if constexpr (BLK) {
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
