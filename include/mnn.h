@@ -308,7 +308,8 @@ mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k
  * num_kv_heads * head_dim], k_scales and v_scales MNN_F32 [B, C, num_kv_heads]; q, k, v and output
  * MNN_F32 or MNN_BF16. Every key is seen as the cache holds it, the call's own among them, so that T
  * tokens in one call and one after the other see the same keys. With f32 the products are exact in the 8-bit values and
- * take fp32 queries and probabilities; with bf16 the probabilities (times the value's scale) are rounded to bf16. */
+ * take fp32 queries and probabilities; with bf16 the probabilities (times the value's scale) are rounded to bf16. Calls
+ * of 2^20 rows (B * T * H) and more may be refused, with MNN_ERR_INVALID_CONFIGURATION. */
 mnn_status mnn_window_attention_step_e4m3(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
                                           mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
                                           mnn_tensor k_scales, mnn_tensor v_cache, mnn_tensor v_scales,
@@ -327,7 +328,9 @@ mnn_status mnn_kv_cache_create(mnn_device dev, int num_kv_heads, int head_dim, i
  * x * (448 * (1 / max|x|)) rounded to nearest even, scale = max|x| * (1 / 448), a maximum below 2^-100
  * counting as 2^-100 (a row that holds a NaN or an infinity is read back as NaN or infinities). positions
  * and steps (may be NULL) as for mnn_window_attention_step; T may be larger than the cache: of tokens that
- * share a slot the last one stays. Other slots keep what they hold. No tensor may be two arguments. */
+ * share a slot the last one stays. Other slots keep what they hold. No tensor
+ * that is written may be another argument. Calls of more than 2^27 heads' rows (B * T * num_kv_heads) may be refused,
+ * with MNN_ERR_INVALID_CONFIGURATION. */
 mnn_status mnn_kv_cache_write(mnn_layer layer, mnn_tensor k, mnn_tensor v, mnn_tensor positions,
                               mnn_tensor steps, mnn_tensor k_cache, mnn_tensor k_scales,
                               mnn_tensor v_cache, mnn_tensor v_scales, mnn_stream s);
@@ -355,7 +358,8 @@ mnn_status mnn_memory_attention_create(mnn_device dev, const mnn_memory_attentio
  * nearer of the two): states behind a sequence's end are not read, output rows behind its last token are
  * left as they were. Tokens of a sequence without states get zeros. Softmax and sums run in fp32; f32
  * tensors keep fp32 products (8-bit values are exact in them), with bf16 ones the probabilities are rounded
- * to bf16. output may not be an input. */
+ * to bf16. output may not be an input. Calls of more than 2^24 tokens or 2^30 states a sequence, and of 2^20
+ * rows (B * T * H) and more, may be refused, with MNN_ERR_INVALID_CONFIGURATION. */
 mnn_status mnn_memory_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor k_scales,
                                         mnn_tensor v, mnn_tensor v_scales, mnn_tensor query_lengths,
                                         mnn_tensor lengths, mnn_tensor output, mnn_stream s);

@@ -90,8 +90,7 @@ __global__ __launch_bounds__(256) void kv_cache_kernel(KVCacheArgs a, FastDiv by
 template <class T, int L, bool HELD, bool WRITE>
 void launch_l(const LaunchCtx& c, const KVCacheArgs& a) {
   const int64_t units = (int64_t)a.T * a.KV, wgs = (units + 256 / L - 1) / (256 / L);
-  // FastDiv, and 2^32 lanes
-  MNN_REQUIRE(units <= (1 << 30) && (units + 256) * a.KV < ((int64_t)1 << 40) && wgs * a.B < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,
+  MNN_REQUIRE(units <= (1 << 30) && wgs * a.B < (1 << 24), MNN_ERR_INVALID_CONFIGURATION,  // 2^32 lanes
               "KVCache: too many tokens in one call");
   launch(c, WRITE ? "kv_cache_write" : "kv_cache_read", kv_cache_kernel<T, L, HELD, WRITE>,
          dim3((unsigned)wgs, (unsigned)a.B), dim3(256), 0, a, FastDiv(a.KV));

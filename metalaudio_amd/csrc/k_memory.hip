@@ -308,6 +308,8 @@ template <class T, class M, int KS, int NW>
 void launch_nw(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Join& join) {
   const int64_t n = (int64_t)a.B * a.KV * p.nsplit;
   const XcdGroups sets(n, p.tiles);
+  MNN_REQUIRE(sets.grid(n) * 64 * NW < ((int64_t)1 << 32), MNN_ERR_INVALID_CONFIGURATION,
+              "MemoryAttention: too many tokens in one call");
   launch(c, NW == 8 ? "memory_256" : "memory_128", memory_kernel<T, M, KS, NW>, dim3((unsigned)sets.grid(n)), dim3(64 * NW),
          0, a, sets, p.nsplit, join.part, join.counts);
 }

@@ -492,7 +492,7 @@ void launch_ks(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join&
 }
 template <class T, class M, bool STEP>
 void launch_rows(const LaunchCtx& c, const RowsArgs& a, const Plan& p, const Join& join) {
-  // what the kernel's divisions by FastDiv hold for, and a grid of 2^32 lanes
+  // rows are numbered by ints, up to the last tile's end; a grid of 2^32 lanes
   MNN_REQUIRE((int64_t)a.T * (a.H / a.KV) < (1 << 24) && p.units * p.nsplit < (1 << 20), MNN_ERR_INVALID_CONFIGURATION,
               (STEP ? "WindowAttention" : "MemoryAttention") << ": too many sequences and tokens in one call");
   MNN_REQUIRE(p.nsplit == 1 || (join.part && join.counts && p.units <= kJoinCounts), MNN_ERR_INVALID_ARGUMENT,

@@ -80,12 +80,18 @@ __device__ __forceinline__ int xcd_logical_tile(int lin, int total) {
   return xcd < r ? xcd * (q + 1) + slot : r * (q + 1) + (xcd - r) * q + slot;
 }
 
-// Division by a number that the host knows, of x with x * by < 2^40: a few instructions, where the compiler's own takes
-// some 25, which a kernel of a few microseconds fetches once for each use.
+// Division of 0 <= x < 2^31 by a number that the host knows: a few instructions, where the compiler's own takes some 25,
+// which a kernel of a few microseconds fetches once for each use. m = ceil(2^shift / by) with 2^(shift - 32) >= by: m is at
+// below 2^33 (x m < 2^64), and m by exceeds 2^shift by e < by <= 2^(shift - 32), so that x m / 2^shift exceeds x / by by
+// x e / (by 2^shift) < 1 / by, too little to reach the next whole number.
 struct FastDiv {
   unsigned long long m;
-  explicit FastDiv(int by) : m(((1ull << 40) + by - 1) / by) {}
-  __device__ __forceinline__ int operator()(int x) const { return (int)((unsigned)x * m >> 40); }
+  int shift;
+  explicit FastDiv(int by) : shift(32) {
+    while ((1ll << (shift - 32)) < by) ++shift;
+    m = ((1ull << shift) + by - 1) / by;
+  }
+  __device__ __forceinline__ int operator()(int x) const { return (int)((unsigned)x * m >> shift); }
 };
 
 // Sets of `size` workgroups that share what they read, `sets` of them: each set is cut into groups of `inner`, which are dealt
@@ -104,7 +110,7 @@ struct XcdGroups {
     return inner;
   }
   int64_t grid(int64_t sets) const { return (sets * cuts + 7) / 8 * 8 * inner; }
-  // the set, and the workgroup's member of it (-1: none); for grids below 2^24, sets below 2^16
+  // the set, and the workgroup's member of it (-1: none)
   __device__ __forceinline__ int set_of(int lin, int& member) const {
     const int xcd = lin & 7, slot = lin >> 3, q = by_inner(slot), group = q * 8 + xcd, set = by_cuts(group);
     member = (group - set * cuts) * inner + (slot - q * inner);

@@ -388,6 +388,25 @@ def test_cache_slots_beyond_32_bit_offsets(dev, stream):
         np.testing.assert_array_equal(o.to_numpy(), want.reshape(v.shape))
 
 
+def test_cache_of_more_rows_than_24_bits(dev, stream):
+    """2^24 + 70 rows of one head: each is found again, unrounded."""
+    T, hd = (1 << 24) + 70, 8
+    say(f"cache rows {T}")
+    step = rounded(np.random.default_rng(5).standard_normal((4099, hd)), "bf16")
+    k = np.tile(step.astype(np.float32), (-(-T // 4099), 1))[:T].reshape(1, T, hd)
+    k[0, :, 0] = np.arange(T) % 251  # whole numbers that bf16 holds; 251 and 4099 share no factor
+    layer, pos = nn.KVCache(dev, 1, hd, 3), tensor(dev, np.array([0]), "i32")
+    rows, kc, vc = tensor(dev, k, "bf16"), *(nn.Tensor(dev, (1, T + 1, hd), dtype="bf16") for _ in "kv")
+    layer.write(rows, rows, pos, kc, vc, stream=stream)
+    outs = [nn.Tensor(dev, k.shape, dtype="bf16") for _ in "kv"]
+    layer.read(kc, vc, pos, *outs, stream=stream)
+    stream.sync(60000)
+    for out in outs:
+        np.testing.assert_array_equal(out.to_numpy(), k)
+    for c in (kc, vc):
+        np.testing.assert_array_equal(c.to_numpy()[:, :T], k)
+
+
 def test_cache_refusals(dev, stream):
     say("cache refusals")
     T = lambda shape, dtype="f32": nn.Tensor(dev, shape, dtype=dtype)  # noqa: E731
