@@ -473,7 +473,7 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
     // blocks: by 128 x 256, whose waves of 64 x 64 have the registers to keep a depth step's sums apart (8192 x 4096 x 4096
-    // 291 -> 276 us; 256 x 128 281)
+    // 291 -> 266 us; 256 x 128 281)
     return launch_tile<T, BLK, BLK ? 128 : 256, 256, BLK ? 64 : 128, 64>(c, a, tile_name(BLK, 3, F32));
   // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
   // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9
