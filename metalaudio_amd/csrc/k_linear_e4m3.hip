@@ -126,6 +126,10 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 // loads and results: 8192 x 4096 x 4096 to bf16 200 to 214 us (1.3 PFLOP/s), 8192 x 8192 x 8192 750 us (1.5), 10752 x
 // 1536 x 384 to f32 with residual 19 us. The widening spread between the products by hand changes nothing, nor do
 // waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
+//
+// Blocks: the sums' scaling (one fma a result and depth step) comes to the widening, and its registers make the waves'
+// tiles smaller, so that more is widened for each product: 8192 x 4096 x 4096 to bf16 257 us, 8192 x 8192 x 8192 949 us, 10752 x 1536 x 384
+// to f32 with residual 25 us.
 template <class T, bool BLK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
@@ -211,16 +215,81 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 >> 1 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
   int slot = 0;
-  for (int k = 0; k < nk; ++k, slot ^= 1) {
+  // a step's slot whole, and the other one free to be filled again
+  auto turn = [&](int k, int to) {
     wait_lgkmcnt0();
     wait_vmcnt<0>();
     stage_barrier();
+    if (k + 1 < nk) issue(k + 1, to ^ 1);
+  };
+  auto join = [&](const floatx16& t, float by, floatx16& acc) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = fmaf(t[v], by, acc[v]);
+  };
+  if constexpr (BLK && FM * FN == 4) {
+    // sixteen values of depth at a time: while their products run, the next sixteen are widened and those behind
+    // them read, across the step's end as well. us with / without, (M, K, N): 8192 x 4096 x 4096 bf16 255 / 265, 8192 x 8192 x
+    // 8192 965 / 1018. Waves of 64 x 32 in 128 square, whose registers it takes, lose: 4096 x 2048 x 2048 47.5 / 44.3
+    intx4 raw[2][FM + FN];
+    bf16x8 op[2][FM + FN];
+    auto read = [&](const char* p, int pair) {
+      const int c = at(4 * (pair / 2) + 2 * g + pair % 2);
+#pragma unroll
+      for (int f = 0; f < FM + FN; ++f)
+        raw[pair % 2][f] = *reinterpret_cast<const intx4*>(p + (f < FM ? xa + 4096 * f : wa + 4096 * (f - FM)) + c);
+    };
+    auto widen = [&](int q) {
+#pragma unroll
+      for (int f = 0; f < FM + FN; ++f) {
+        const intx4& r = raw[q / 2 % 2][f];
+        op[q % 2][f] = q % 2 ? widen8(r[2], r[3]) : widen8(r[0], r[1]);
+      }
+    };
+    turn(0, 0);
+    read(smem, 0);
+    widen(0);
+    for (int k = 0; k < nk; ++k) {
+      const char* p = smem + slot * SLOT;
+      slot ^= 1;
+      floatx16 t[FN][FM];
+#pragma unroll
+      for (int j = 0; j < FM; ++j) by[j] = xnext[j] * wnext;
+      if (k + 1 < nk) next_scales(k + 1);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (q % 2 == 0 && q < 6) read(p, q / 2 + 1);
+        if (q == 7 && k + 1 < nk) {
+          turn(k + 1, slot);
+          read(smem + slot * SLOT, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+          for (int j = 0; j < FM; ++j) {
+            if (q == 0) t[i][j] = floatx16{0.f};
+            t[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[q % 2][FM + i], op[q % 2][j], t[i][j], 0, 0, 0);
+          }
+        widen((q + 1) % 8);
+#pragma unroll
+        for (int i = 0; i < FM * FN; ++i) {  // a product, then its share of the widening
+          __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(2, 4 * (FM + FN) / (FM * FN), 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) join(t[i][j], by[j], acc[i][j]);
+    }
+  }
+  for (int k = BLK && FM * FN == 4 ? nk : 0; k < nk; ++k, slot ^= 1) {
+    turn(k, slot);
     if constexpr (BLK) {
 #pragma unroll
       for (int j = 0; j < FM; ++j) by[j] = xnext[j] * wnext;
       if (k + 1 < nk) next_scales(k + 1);
     }
-    if (k + 1 < nk) issue(k + 1, slot ^ 1);
     const char* p = smem + slot * SLOT;
     floatx16 t[BLK ? FN : 1][BLK ? FM : 1];
 #pragma unroll
@@ -252,8 +321,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
       for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[i][j][v] = fmaf(t[i][j][v], by[j], acc[i][j][v]);
+          join(t[i][j], by[j], acc[i][j]);
     }
   }
 

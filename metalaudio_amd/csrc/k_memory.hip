@@ -7,8 +7,10 @@
 // (attend.hpp), and the next one is split or widened and stored to the other slot. Of workgroups that share out the keys
 // of the same rows the last one to finish joins the results of all of them.
 //
-// Bound by the vector units' issue beside the matrix instructions in bf16 (a quarter of it, 256 of 470 cycles for 32 x 32
-// scores, are exponentials), by the six products' matrix instructions in f32.
+// Bound by the vector units' issue beside the matrix instructions in bf16 (0.69 and 0.45 of the time; of the issue for 32 x 32
+// scores 256 of some 470 clocks are exponentials): 8192 tokens on 16384 states, 8 / 2 heads of 64 300 to 320 us, 0.9 PFLOP/s, on
+// e4m3 states 343 to 363. In f32 by the six products' matrix instructions beside the split of P (0.52 and 0.51): 4 x 1344
+// tokens on 2688 ragged states, 8 heads of 48, 91 to 97 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -92,6 +92,15 @@ def test_linear_blocks(dev, stream, M, K, N, kw):
     blocks_case(dev, stream, M, K, N, **kw)
 
 
+@pytest.mark.parametrize("M,K,N,kw", [
+    (4000, 100, 4090, {"out": "bf16"}), (4096, 300, 3842, {"residual": True}), (3841, 640, 4096, {"act": "gelu", "out": "bf16"}),
+    (3900, 256, 3970, {"residual": True, "out": "bf16"})])
+def test_linear_blocks_tiles_of_128_by_256(dev, stream, M, K, N, kw):
+    """One, two, three and five depth steps."""
+    say(f"linear blocks 128 x 256 {M}x{K}x{N} {kw}")
+    blocks_case(dev, stream, M, K, N, **kw)
+
+
 @pytest.mark.parametrize("M,K,N,inp,out", [(1, 384, 96, "f32", "f32"), (9, 257, 64, "bf16", "bf16"),
                                            (300, 512, 300, "bf16", "f32"), (45, 1000, 33, "f32", "bf16"),
                                            (2, 20000, 24, "bf16", "f32"), (700, 136, 60, "bf16", "f32"),
