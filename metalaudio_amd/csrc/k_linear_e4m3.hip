@@ -108,7 +108,7 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
     const int c = min(n + i, a.N - 1);
-    ws[i] = BLK ? a.unit : a.ws[c];
+    ws[i] = BLK ? *a.unit : a.ws[c];
     bias[i] = a.bias ? a.bias[c] : 0.f;
   }
 }

@@ -35,8 +35,8 @@ struct LinearE4m3Args {
   bool blocks = false;         // scales for blocks
   const float* xs = nullptr;   // [M], or [M][K / 128]
   const uint8_t* w = nullptr;  // [N][K]
-  const float* ws = nullptr;   // [N], or [scale_blocks(N)][K / 128] in units of `unit`
-  float unit = 1.f;            // a power of two
+  const float* ws = nullptr;   // [N], or [scale_blocks(N)][K / 128] in units of *unit
+  const float* unit = nullptr; // [1], a power of two, on the device: a captured call sees that of weights loaded later
   const float* bias = nullptr; // [N] or null
   const void* r = nullptr;     // [M][N] of the output's type, or null; may be y
   void* y = nullptr;           // [M][N]

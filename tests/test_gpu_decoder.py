@@ -196,6 +196,29 @@ def test_linear_blocks_many_calls_share_the_layer(dev, stream):
         np.testing.assert_array_equal(first.setdefault(M, y), y)
 
 
+def test_linear_blocks_weights_loaded_under_a_graph(dev):
+    """A captured call sees weights that are loaded between its replays, whatever their size."""
+    say("linear blocks loaded under a graph")
+    s = nn.Stream(dev)
+    rng = np.random.default_rng(17)
+    for M in (3, 200):
+        K, N = 256, 300
+        layer, fresh = (nn.Linear(dev, K, N, precision="e4m3_block") for _ in range(2))
+        w, b = rng.standard_normal((N, K)), rng.standard_normal(N)
+        x, y, z = tensor(dev, rng.standard_normal((M, K)), "f32"), nn.Tensor(dev, (M, N)), nn.Tensor(dev, (M, N))
+        layer.load_weights(w, b)
+        layer.forward_scaled(x, None, y, stream=s)
+        s.sync(60000)
+        graph = Graph(s, lambda: layer.forward_scaled(x, None, y, stream=s))
+        for size in (1.0, 5000.0, 1e30, 2.0):
+            for m in (layer, fresh):
+                m.load_weights(w * size, b)
+            graph.replay()
+            fresh.forward_scaled(x, None, z, stream=s)
+            s.sync(60000)
+            np.testing.assert_array_equal(y.to_numpy(), z.to_numpy())
+
+
 def test_linear_blocks_hold_outliers_that_rows_do_not(dev, stream):
     """What blocks are for: one value of 10^6 costs a row's other blocks nothing."""
     say("linear blocks outlier")
