@@ -381,7 +381,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
   }
 }
 
-// Few rows (up to 32): the weights are all the traffic. A workgroup takes 32 rows of w, its eight waves an
+// Few rows (up to 32; in blocks also more, 32 a workgroup): the weights are all the traffic. A workgroup takes 32 rows of w, its eight waves an
 // eighth of the depth each, operands straight from memory (a wave reads 64 bytes of 32 rows at a time, four
 // such steps in flight); their sums meet in LDS. Rows of x may be of any length: what a lane would read past
 // a row's end is 0.
@@ -390,14 +390,15 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
   __shared__ float sum[8][32][33];  // [wave][m][n]
   const int lane = threadIdx.x & 63, g = lane >> 5, l32 = lane & 31, wave = threadIdx.x >> 6;
   const int n0 = blockIdx.x * 32;
-  const uint8_t* x = a.x + min((int64_t)l32, a.M - 1) * a.ldx + 32 * g;
+  const int64_t m0 = (int64_t)blockIdx.y * 32, mine = min(m0 + l32, a.M - 1);
+  const uint8_t* x = a.x + mine * a.ldx + 32 * g;
   const uint8_t* w = a.w + (int64_t)min(n0 + l32, a.N - 1) * a.K + 32 * g;
   const int steps = a.K / 64, s0 = steps * wave / 8, s1 = steps * (wave + 1) / 8;
   floatx16 acc;
 #pragma unroll
   for (int v = 0; v < 16; ++v) acc[v] = 0.f;
   const int nk = a.K / kScaleBlock;
-  const float* xsp = a.xs + (BLK ? min((int64_t)l32, a.M - 1) * nk : 0);
+  const float* xsp = a.xs + (BLK ? mine * nk : 0);
   const float* wsp = a.ws + (BLK ? (int64_t)(n0 / kScaleBlock) * nk : 0);
   auto step = [&](int s, auto whole) {
     const intx4* q = reinterpret_cast<const intx4*>(w + 64 * s);
@@ -426,16 +427,16 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
 #pragma unroll
   for (int v = 0; v < 16; ++v) sum[wave][l32][8 * (v / 4) + 4 * g + v % 4] = acc[v];
   __syncthreads();
-  for (int e = threadIdx.x; e < 32 * a.M; e += 512) {
+  for (int e = threadIdx.x; e < 32 * min((int64_t)32, a.M - m0); e += 512) {
     const int m = e / 32, n = n0 + e % 32;
     if (n >= a.N) continue;
     float v[1] = {0.f}, ws, bias;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[0] += sum[i][m][e % 32];
     columns<1, BLK>(a, n, &ws, &bias);
-    v[0] = fmaf(v[0] * (BLK ? 1.f : a.xs[m]), ws, bias);
+    v[0] = fmaf(v[0] * (BLK ? 1.f : a.xs[m0 + m]), ws, bias);
     activate(v, a.act, a.alpha);
-    const int64_t at = (int64_t)m * a.N + n;
+    const int64_t at = (m0 + m) * a.N + n;
     if (a.r) v[0] += to_f32(static_cast<const T*>(a.r)[at]);
     static_cast<T*>(a.y)[at] = from_f32<T>(v[0]);
   }
@@ -530,14 +531,17 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   constexpr bool F32 = sizeof(T) == 4;
   MNN_REQUIRE(a.K % 128 == 0 && (a.ldx == a.K || a.M <= kLinearFew), MNN_ERR_INVALID_ARGUMENT,
               "linear_e4m3: rows of x are not padded");
-  if (a.M <= kLinearFew)
+  const int64_t cus = c.dev->props.multiProcessorCount;
+  // blocks: also more rows, 32 a workgroup, up to one a compute unit: the depth is split where tiles of 64 square leave most of
+  // the GPU idle. us at (M, K, N), such / 64 square: 64 x 384 x 384 4.4 / 6.1, 512 x 2048 x 512 (256 of them) 8.0 / 11.6, 128 x 512 x
+  // 2048 (256) 4.5 / 6.3; 1024 x 384 x 384 (384) 6.2 / 6.2; 256 x 2048 x 2048 (512) 13.4 / 11.7
+  if (a.M <= kLinearFew || (BLK && (a.M + 31) / 32 * ((a.N + 31) / 32) <= cus))
     return launch(c, tile_name(BLK, 0, F32), linear_e4m3_few_kernel<T, BLK>,
-                  dim3((unsigned)((a.N + 31) / 32)), dim3(512), 0, a);
+                  dim3((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 31) / 32)), dim3(512), 0, a);
   // 256 square where the rounds of one tile a compute unit are 7/8 full: a third less widening a product, but one
   // workgroup a compute unit, whose last round costs a whole one. us at (M, K, N), 256 / 128 / 64 square: 8192 x 4096 x
   // 4096 bf16 203 / 227 / 281, f32 215 / 235 / 285; 10752 x 384 x 1536 bf16 (252 tiles) 19.2 / 20.2 / 23.6; 8192 x
   // 1024 x 1536 bf16 (192 tiles) 32 / 29 / 35; 12800 x 1024 x 1536 bf16 (300 tiles) 58 / 44 / 52.
-  const int64_t cus = c.dev->props.multiProcessorCount;
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
     // blocks: by 128 x 256, whose waves of 64 x 64 have the registers to keep a depth step's sums apart (8192 x 4096 x 4096

@@ -101,6 +101,16 @@ def test_linear_blocks_tiles_of_128_by_256(dev, stream, M, K, N, kw):
     blocks_case(dev, stream, M, K, N, **kw)
 
 
+@pytest.mark.parametrize("M,K,N,kw", [
+    (600, 130, 500, {"out": "bf16"}), (900, 100, 300, {"residual": True}), (513, 1536, 520, {"act": "relu"}),
+    (33, 2048, 512, {"out": "bf16"}), (500, 129, 511, {"residual": True, "in_place": True}), (512, 2048, 512, {"act": "gelu"}),
+    (64, 100, 4096, {"out": "bf16"}), (257, 384, 900, {"residual": True, "out": "bf16"})])
+def test_linear_blocks_between_few_and_many_rows(dev, stream, M, K, N, kw):
+    """Tiles of 64 square, and 32 rows a workgroup where those are few."""
+    say(f"linear blocks {M}x{K}x{N} {kw}")
+    blocks_case(dev, stream, M, K, N, **kw)
+
+
 @pytest.mark.parametrize("M,K,N,inp,out", [(1, 384, 96, "f32", "f32"), (9, 257, 64, "bf16", "bf16"),
                                            (300, 512, 300, "bf16", "f32"), (45, 1000, 33, "f32", "bf16"),
                                            (2, 20000, 24, "bf16", "f32"), (700, 136, 60, "bf16", "f32"),
