@@ -278,7 +278,7 @@ typedef struct mnn_window_attention_desc {
  * reference). The query of token i sees the keys j <= i + window_right with j >= i - window_left or j <
  * sinks. Softmax and sums run in fp32; f32 tensors keep fp32 products, bf16 ones take bf16 products with
  * fp32 accumulation: over whole sequences the probabilities are rounded to bf16 for theirs, in steps they
- * stay in fp32. No weights: q, k and v are projected (and turned) before. */
+ * stay in fp32 (on 8-bit caches in 16 bits). No weights: q, k and v are projected (and turned) before. */
 mnn_status mnn_window_attention_create(mnn_device dev, const mnn_window_attention_desc* desc,
                                        mnn_layer* out);
 /* Whole sequences: q and output [S, H * head_dim] or [B, S, H * head_dim], k and v the same of
@@ -308,7 +308,7 @@ mnn_status mnn_window_attention_step(mnn_layer layer, mnn_tensor q, mnn_tensor k
  * num_kv_heads * head_dim], k_scales and v_scales MNN_F32 [B, C, num_kv_heads]; q, k, v and output
  * MNN_F32 or MNN_BF16. Every key is seen as the cache holds it, the call's own among them, so that T
  * tokens in one call and one after the other see the same keys. With f32 the products are exact in the 8-bit values and
- * take fp32 queries and probabilities; with bf16 the probabilities (times the value's scale) are rounded to bf16. Calls
+ * take fp32 queries and probabilities; with bf16 the probabilities (times the value's scale) keep 16 bits. Calls
  * of 2^20 rows (B * T * H) and more may be refused, with MNN_ERR_INVALID_CONFIGURATION. */
 mnn_status mnn_window_attention_step_e4m3(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor v,
                                           mnn_tensor positions, mnn_tensor steps, mnn_tensor k_cache,
@@ -357,8 +357,8 @@ mnn_status mnn_memory_attention_create(mnn_device dev, const mnn_memory_attentio
  * MNN_I32 [B], the tokens and states of each padded sequence (values outside 0..T and 0..S count as the
  * nearer of the two): states behind a sequence's end are not read, output rows behind its last token are
  * left as they were. Tokens of a sequence without states get zeros. Softmax and sums run in fp32; f32
- * tensors keep fp32 products (8-bit values are exact in them), with bf16 ones the probabilities are rounded
- * to bf16. output may not be an input. Calls of more than 2^24 tokens or 2^30 states a sequence, and of 2^20
+ * tensors keep fp32 products (8-bit values are exact in them), with bf16 ones the probabilities keep 16 bits
+ * for up to 16 rows (T * num_heads / num_kv_heads) of a key/value head, and may be rounded to bf16 for more. output may not be an input. Calls of more than 2^24 tokens or 2^30 states a sequence, and of 2^20
  * rows (B * T * H) and more, may be refused, with MNN_ERR_INVALID_CONFIGURATION. */
 mnn_status mnn_memory_attention_forward(mnn_layer layer, mnn_tensor q, mnn_tensor k, mnn_tensor k_scales,
                                         mnn_tensor v, mnn_tensor v_scales, mnn_tensor query_lengths,

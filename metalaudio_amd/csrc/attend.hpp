@@ -116,8 +116,9 @@ struct AttendTypes {
     st = mfma(k.p[0], q[0], st);
   }
   // Eight probabilities (e4m3: times their values' scales) to the second product; v(part, tile): fragments of V^T.
-  // Returns their sum, where it is that of the rounded ones.
-  template <int TILES, class Acc, class V, class Mfma>
+  // PP: the bf16 parts that a probability beside bf16 values is taken in, one (off by 2^-8 of itself at most) or two
+  // (2^-16). Returns the sum of the rounded ones, of one part, without scales; else 0.
+  template <int PP, int TILES, class Acc, class V, class Mfma>
   static __device__ __forceinline__ float values(const float (&p)[8], V v, Acc (&o)[TILES], Mfma mfma) {
     typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
     float ps = 0.f;
@@ -139,16 +140,27 @@ struct AttendTypes {
         o[i] = mfma(h, px.h, o[i]);
       }
     } else {
-      // probabilities to bf16, to nearest (each is off by 2^-9 of itself at most): what the second product takes.
-      // Without scales the sum is that of the rounded ones, two an instruction
       const uintx4 pb{cvt_pk_bf16(p[0], p[1]), cvt_pk_bf16(p[2], p[3]), cvt_pk_bf16(p[4], p[5]), cvt_pk_bf16(p[6], p[7])};
       const bf16x8 px = __builtin_bit_cast(bf16x8, pb);
-      if (!HELD) {
+      if constexpr (PP == 2) {
+        uintx4 rb;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ps = add_pair(pb[e], ps);
+        for (int e = 0; e < 4; ++e) rb[e] = cvt_pk_bf16(p[2 * e] - bf16_lo(pb[e]), p[2 * e + 1] - bf16_hi(pb[e]));
+        const bf16x8 rx = __builtin_bit_cast(bf16x8, rb);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const bf16x8 f = v(0, i);
+          o[i] = mfma(f, rx, o[i]);
+          o[i] = mfma(f, px, o[i]);
+        }
+      } else {
+        if (!HELD) {  // two an instruction
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ps = add_pair(pb[e], ps);
+        }
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) o[i] = mfma(v(0, i), px, o[i]);
       }
-#pragma unroll
-      for (int i = 0; i < TILES; ++i) o[i] = mfma(v(0, i), px, o[i]);
     }
     return ps;
   }
@@ -274,7 +286,7 @@ struct AttendMany : AttendTypes<T, M> {
         if (!RAW) ps += p[e];
         if (HELD) p[e] *= vs(8 * ks + e);
       }
-      ps += A::values(p, [&](int part, int t) { return v(part, t, ks); }, o, mfma);
+      ps += A::template values<1>(p, [&](int part, int t) { return v(part, t, ks); }, o, mfma);
     }
     sum += ps;
   }
@@ -374,10 +386,12 @@ struct AttendFew : AttendTypes<T, M> {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       p[e] = __builtin_amdgcn_exp2f(st[e / 4][e % 4] - ref);
-      if (F32 || HELD) ps += p[e];
+      ps += p[e];
       if (HELD) p[e] *= vs[e];
     }
-    ps += A::values(p, v, o, mfma);
+    // bf16 calls: two parts, so that their results keep a rounding's distance, as the step on unrounded caches does (2-norm
+    // 1.7e-3 against 2.4e-3 with one part), where memory or one block's chain bounds the call
+    A::template values<2>(p, v, o, mfma);
     sum += ps;
   }
   // Where the lane's fragments of V^T begin in a block of V in LDS.

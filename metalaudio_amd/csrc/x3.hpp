@@ -43,21 +43,21 @@ __device__ __forceinline__ unsigned cvt_pk_bf16(float a, float b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(unsigned, __builtin_convertvector((float2v){a, b}, bf16x2));
 }
+__device__ __forceinline__ float bf16_lo(unsigned p) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_perm(0u, p, 0x01000c0cu));
+}
+__device__ __forceinline__ float bf16_hi(unsigned p) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_perm(0u, p, 0x03020c0cu));
+}
 __device__ __forceinline__ Split8 split8(const float* x) {
   unsigned h[4], m[4], l[4];
   auto bits = [](float v) { return __builtin_bit_cast(unsigned, v); };
-  auto lo = [](unsigned p) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_perm(0u, p, 0x01000c0cu));
-  };
-  auto hi = [](unsigned p) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_perm(0u, p, 0x03020c0cu));
-  };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     h[i] = cvt_pk_bf16(x[2 * i], x[2 * i + 1]);
-    const float r0 = x[2 * i] - lo(h[i]), r1 = x[2 * i + 1] - hi(h[i]);
+    const float r0 = x[2 * i] - bf16_lo(h[i]), r1 = x[2 * i + 1] - bf16_hi(h[i]);
     m[i] = cvt_pk_bf16(r0, r1);
-    l[i] = __builtin_amdgcn_perm(bits(r1 - hi(m[i])), bits(r0 - lo(m[i])), 0x07060302u);
+    l[i] = __builtin_amdgcn_perm(bits(r1 - bf16_hi(m[i])), bits(r0 - bf16_lo(m[i])), 0x07060302u);
   }
   typedef unsigned uint4v __attribute__((ext_vector_type(4)));
   Split8 s;
