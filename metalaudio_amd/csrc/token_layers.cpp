@@ -40,19 +40,19 @@ class Scratch {
   size_t size_ = 0;
 };
 
-// A layer's workspace for keys that workgroups share out. The counts are made with the layer, so that a call can be
-// captured into a graph.
+// A layer's workspace for keys that workgroups share out, made by the first call that needs one: making the layer takes
+// nothing of the device, and a call of that size can be captured into a graph.
 class JoinSpace {
  public:
-  explicit JoinSpace(Device* d) {
-    d->make_current();
-    counts_.reserve(sizeof(int) * k::kJoinCounts);
-    HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * k::kJoinCounts));
-    HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
-  }
   k::Join get(int64_t floats) {
     if (!floats) return {};
-    return {static_cast<float*>(part_.get(sizeof(float) * floats)), counts_.as<int>()};
+    float* part = static_cast<float*>(part_.get(sizeof(float) * floats));
+    if (!counts_.ptr) {
+      counts_.reserve(sizeof(int) * k::kJoinCounts);
+      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * k::kJoinCounts));
+      HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
+    }
+    return {part, counts_.as<int>()};
   }
 
  private:
@@ -434,7 +434,7 @@ class RotaryLayer : public ManyInputLayer {
 class WindowAttentionLayer : public ManyInputLayer {
  public:
   WindowAttentionLayer(Device* d, const mnn_window_attention_desc& desc)
-      : ManyInputLayer(d), d_(desc), join_(d) {
+      : ManyInputLayer(d), d_(desc) {
     MNN_REQUIRE(desc.num_heads > 0 && desc.num_kv_heads > 0 && desc.num_heads <= 65535 &&
                     desc.num_heads % desc.num_kv_heads == 0,
                 MNN_ERR_INVALID_CONFIGURATION,
@@ -650,7 +650,7 @@ class KVCacheLayer : public ManyInputLayer {
 class MemoryAttentionLayer : public ManyInputLayer {
  public:
   MemoryAttentionLayer(Device* d, const mnn_memory_attention_desc& desc)
-      : ManyInputLayer(d), d_(desc), join_(d) {
+      : ManyInputLayer(d), d_(desc) {
     MNN_REQUIRE(desc.num_heads > 0 && desc.num_kv_heads > 0 && desc.num_heads <= 65535 &&
                     desc.num_heads % desc.num_kv_heads == 0,
                 MNN_ERR_INVALID_CONFIGURATION,
