@@ -340,11 +340,12 @@ void memory_tm(const LaunchCtx& c, const MemoryArgs& a, const Plan& p, const Joi
 
 }  // namespace
 
-int64_t memory_part_floats(const LaunchCtx& c, const MemoryArgs& a) {
+JoinSize memory_join(const LaunchCtx& c, const MemoryArgs& a) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);
-  if (p.few) return memory_rows_part_floats(c, a);
+  if (p.few) return memory_rows_join(c, a);
+  if (p.nsplit == 1) return {};
   const int dt = a.hd > 96 ? 4 : (a.hd + 31) / 32;  // 32-row tiles of O^T, as AttendMany has them
-  return p.nsplit == 1 ? 0 : p.units * p.nsplit * p.waves * (16 * dt + 2) * 64;
+  return {p.units * p.nsplit * p.waves * (16 * dt + 2) * 64, (int)p.units};
 }
 void memory_attention(const LaunchCtx& c, const MemoryArgs& a, const Join& join) {
   const Plan p = plan_of(a, c.dev->props.multiProcessorCount);

@@ -476,8 +476,9 @@ Plan plan_of(const RowsArgs& a, mnn_dtype type, int64_t keys, int cus) {
   return p;
 }
 int slots_of(const RowsArgs& a) { return (int)std::min<int64_t>(16, (int64_t)a.T * (a.H / a.KV)); }
-int64_t part_floats(const RowsArgs& a, const Plan& p) {
-  return p.nsplit == 1 ? 0 : p.units * p.nsplit * slots_of(a) * (a.hd + 2);
+JoinSize join_of(const RowsArgs& a, const Plan& p) {
+  if (p.nsplit == 1) return {};
+  return {p.units * p.nsplit * slots_of(a) * (a.hd + 2), (int)p.units};
 }
 
 template <class T, class M, int KS, int W, bool STEP>
@@ -559,9 +560,9 @@ RowsArgs memory_args(const MemoryArgs& m) {
 
 }  // namespace
 
-int64_t window_step_e4m3_part_floats(const LaunchCtx& c, const WindowStepHeldArgs& s) {
+JoinSize window_step_e4m3_join(const LaunchCtx& c, const WindowStepHeldArgs& s) {
   const RowsArgs a = step_args(s);
-  return part_floats(a, plan_of(a, s.type, step_keys(s), c.dev->props.multiProcessorCount));
+  return join_of(a, plan_of(a, s.type, step_keys(s), c.dev->props.multiProcessorCount));
 }
 void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, const Join& part) {
   const RowsArgs a = step_args(s);
@@ -572,9 +573,9 @@ void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& s, const Joi
     launch_rows<__bf16, E4m3, true>(c, a, p, part);
 }
 
-int64_t memory_rows_part_floats(const LaunchCtx& c, const MemoryArgs& m) {
+JoinSize memory_rows_join(const LaunchCtx& c, const MemoryArgs& m) {
   const RowsArgs a = memory_args(m);
-  return part_floats(a, plan_of(a, m.type, m.S, c.dev->props.multiProcessorCount));
+  return join_of(a, plan_of(a, m.type, m.S, c.dev->props.multiProcessorCount));
 }
 void memory_rows(const LaunchCtx& c, const MemoryArgs& m, const Join& part) {
   const RowsArgs a = memory_args(m);

@@ -7,8 +7,7 @@
 namespace mnn {
 namespace k {
 
-// floats of workspace that a call needs (0: none), the same on every call of the same sizes
-int64_t memory_rows_part_floats(const LaunchCtx& c, const MemoryArgs& a);
+JoinSize memory_rows_join(const LaunchCtx& c, const MemoryArgs& a);
 void memory_rows(const LaunchCtx& c, const MemoryArgs& a, const Join& join);
 
 }  // namespace k

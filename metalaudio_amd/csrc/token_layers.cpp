@@ -7,6 +7,7 @@
 #include <cmath>
 #include <initializer_list>
 
+#include "kernels.hpp"
 #include "token_ops.hpp"
 
 namespace mnn {
@@ -42,21 +43,47 @@ class Scratch {
 
 // A layer's workspace for keys that workgroups share out, made by the first call that needs one: making the layer takes
 // nothing of the device, and a call of that size can be captured into a graph.
+//
+// Counts are zeros before and after a call, whose last workgroups find themselves by them. One that two calls passed at the
+// same time would be wrong for all later ones, so no two calls that could overlap have the same: each stream has its
+// own, and each captured call, which no replay of its graph overlaps. Calls for which none are left share some
+// that a launch of their own clears first.
 class JoinSpace {
  public:
-  k::Join get(int64_t floats) {
-    if (!floats) return {};
-    float* part = static_cast<float*>(part_.get(sizeof(float) * floats));
-    if (!counts_.ptr) {
-      counts_.reserve(sizeof(int) * k::kJoinCounts);
-      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * k::kJoinCounts));
+  k::Join get(const LaunchCtx& c, k::JoinSize n) {
+    if (!n.floats) return {};
+    float* part = static_cast<float*>(part_.get(sizeof(float) * n.floats));
+    if (!zeros_) {
+      counts_.reserve(sizeof(int) * kCounts);
+      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * kCounts));
       HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
+      zeros_ = true;
     }
-    return {part, counts_.as<int>()};
+    return {part, counts(c, n.units)};
   }
 
  private:
+  static constexpr int kCounts = 1 << 15;  // the first kJoinCounts of them the ones that are shared
+  int* counts(const LaunchCtx& c, int units) {
+    hipStreamCaptureStatus status;
+    HIP_CHECK(hipStreamIsCapturing(c.stream, &status));
+    const bool captured = status != hipStreamCaptureStatusNone;
+    auto mine = captured ? streams_.end() : streams_.find(c.stream);
+    if (mine != streams_.end()) return counts_.as<int>() + mine->second;
+    const int n = captured ? (units + 31) / 32 * 32 : k::kJoinCounts, at = next_;
+    if (n > kCounts - at) {
+      k::zero_u32(c, counts_.as<unsigned>(), units);
+      return counts_.as<int>();
+    }
+    next_ += n;
+    if (!captured) streams_[c.stream] = at;
+    return counts_.as<int>() + at;
+  }
+
   DevBuf counts_;
+  bool zeros_ = false;
+  int next_ = k::kJoinCounts;
+  std::map<hipStream_t, int> streams_;
   Scratch part_;
 };
 
@@ -537,7 +564,7 @@ class WindowAttentionLayer : public ManyInputLayer {
     if (ks) {
       a.ks = ks->f32();
       a.vs = vs->f32();
-      return k::window_step_e4m3(ctx(s), a, join_.get(k::window_step_e4m3_part_floats(ctx(s), a)));
+      return k::window_step_e4m3(ctx(s), a, join_.get(ctx(s), k::window_step_e4m3_join(ctx(s), a)));
     }
     const int64_t part = k::window_step_part_floats(ctx(s), a);
     k::window_step(ctx(s), a, part ? static_cast<float*>(scratch_.get(sizeof(float) * part)) : nullptr);
@@ -710,7 +737,7 @@ class MemoryAttentionLayer : public ManyInputLayer {
     a.KV = d_.num_kv_heads;
     a.hd = d_.head_dim;
     a.scale = d_.scale;
-    k::memory_attention(ctx(s), a, join_.get(k::memory_part_floats(ctx(s), a)));
+    k::memory_attention(ctx(s), a, join_.get(ctx(s), k::memory_join(ctx(s), a)));
   }
 
  private:

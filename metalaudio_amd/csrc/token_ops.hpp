@@ -101,10 +101,15 @@ int64_t window_step_part_floats(const LaunchCtx& c, const WindowStepArgs& a);
 void window_step(const LaunchCtx& c, const WindowStepArgs& a, float* part);
 
 // Where workgroups that share out the keys of one unit meet: their results, and a count a unit, zeros between calls.
-constexpr int kJoinCounts = 1024;
+constexpr int kJoinCounts = 1024;  // the most units of a call
 struct Join {
   float* part = nullptr;
-  int* counts = nullptr;  // [kJoinCounts]
+  int* counts = nullptr;
+};
+// What a call needs of it (0 floats: nothing), the same on every call of the same sizes.
+struct JoinSize {
+  int64_t floats = 0;
+  int units = 0;
 };
 
 // The step on caches in 8 bits: kc and vc in e4m3, a scale for each head's row.
@@ -112,7 +117,7 @@ struct WindowStepHeldArgs : WindowStepArgs {
   float* ks = nullptr;  // [B][C][KV]
   float* vs = nullptr;
 };
-int64_t window_step_e4m3_part_floats(const LaunchCtx& c, const WindowStepHeldArgs& a);
+JoinSize window_step_e4m3_join(const LaunchCtx& c, const WindowStepHeldArgs& a);
 void window_step_e4m3(const LaunchCtx& c, const WindowStepHeldArgs& a, const Join& join);
 
 // Rows of keys [0] and values [1] and the caches that they are written to or read from.
@@ -141,7 +146,7 @@ struct MemoryArgs {
   int B = 0, T = 0, S = 0, H = 0, KV = 0, hd = 0;
   float scale = 1.f;
 };
-int64_t memory_part_floats(const LaunchCtx& c, const MemoryArgs& a);
+JoinSize memory_join(const LaunchCtx& c, const MemoryArgs& a);
 void memory_attention(const LaunchCtx& c, const MemoryArgs& a, const Join& join);
 
 }  // namespace k
