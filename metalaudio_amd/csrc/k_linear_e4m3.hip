@@ -50,14 +50,19 @@ __device__ __forceinline__ floatx16 mul(const Operand& a, const Operand& b, floa
   return c;
 }
 
-// Blocks: a product of 64 of them begins at 0, and joins the running sums times its two scales.
-__device__ __forceinline__ void mul_scaled(const Operand& a, const Operand& b, float by, floatx16& c) {
+// Blocks: a product of 64 of them begins at 0, and joins the running sums times its two scales, by their product where that
+// is a normal number. Where it leaves fp32's range the sums may be in it all the same (small rows on small weights; large rows
+// on small weights beside large ones): they take one scale after the other then.
+__device__ __forceinline__ void mul_scaled(const Operand& a, const Operand& b, float xs, float ws, floatx16& c) {
   floatx16 t;
 #pragma unroll
   for (int v = 0; v < 16; ++v) t[v] = 0.f;
   t = mul(a, b, t);
+  const float both = xs * ws;
+  const bool apart = !__builtin_isnormal(both);
+  const float first = apart ? xs : 1.f, last = apart ? ws : both;
 #pragma unroll
-  for (int v = 0; v < 16; ++v) c[v] = fmaf(t[v], by, c[v]);
+  for (int v = 0; v < 16; ++v) c[v] = fmaf(t[v] * first, last, c[v]);
 }
 
 // The activation of CNT values; its choice is made once for all of them (a branch an element, the same for
@@ -101,14 +106,13 @@ __device__ __forceinline__ void store_some(T* p, const float* v, bool vec, int c
 }
 
 // Scales and biases of CNT consecutive columns, those behind the last column as the last; the scales of
-// blocks are in the sums already, but for their unit: the weights' scales are kept as 1 at most, or in units of the
-// largest, so that their products with those of x overflow only where results do.
+// blocks are in the sums already.
 template <int CNT, bool BLK>
 __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* ws, float* bias) {
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
     const int c = min(n + i, a.N - 1);
-    ws[i] = BLK ? *a.unit : a.ws[c];
+    ws[i] = BLK ? 1.f : a.ws[c];
     bias[i] = a.bias ? a.bias[c] : 0.f;
   }
 }
@@ -128,8 +132,8 @@ __device__ __forceinline__ void columns(const LinearE4m3Args& a, int n, float* w
 // waves of 128 x 128 (a third less of it, one wave a SIMD: 225 us).
 //
 // Blocks: the sums' scaling (one fma a result and depth step) comes to the widening, and its registers make the waves'
-// tiles smaller, so that more is widened for each product: 8192 x 4096 x 4096 to bf16 257 us, 8192 x 8192 x 8192 949 us, 10752 x 1536 x 384
-// to f32 with residual 25 us.
+// tiles smaller, so that more is widened for each product: 8192 x 4096 x 4096 to bf16 264 us, 8192 x 8192 x 8192 985 us, 10752 x 1536 x 384
+// to f32 with residual 26.5 us (of these 2 %, 1 % and 1.5 us for the look at the scales' products).
 template <class T, bool BLK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(LinearE4m3Args a) {
   constexpr int NW = BM / WM * (BN / WN);
@@ -211,6 +215,17 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     for (int j = 0; j < FM; ++j) xsp[j] = a.xs + min(m0 + wm * WM + 32 * j + l32, a.M - 1) * nk;
     next_scales(0);
   }
+  bool any_apart = false;  // a product of a step's scales that is no normal number
+  auto take_scales = [&](int k) {
+    bool apart = false;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      by[j] = xnext[j] * wnext;
+      apart |= !__builtin_isnormal(by[j]);
+    }
+    any_apart = __any(apart);
+    if (k + 1 < nk) next_scales(k + 1);
+  };
   // chunk c of a row that is l32 modulo 32
   auto at = [&](int c) { return l32 * 128 + ((c ^ (l32 >> 1 & 7)) << 4); };
   const int xa = wm * WM * 128, wa = (BM + wn * WN) * 128;
@@ -222,14 +237,30 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
     stage_barrier();
     if (k + 1 < nk) issue(k + 1, to ^ 1);
   };
-  auto join = [&](const floatx16& t, float by, floatx16& acc) {
+  // a step's sums t to the running ones: as in mul_scaled, in a branch, since it is rare
+  auto join = [&](int k, floatx16 (&t)[BLK ? FN : 1][BLK ? FM : 1]) {
+    if constexpr (BLK) {
+      if (any_apart) {
 #pragma unroll
-    for (int v = 0; v < 16; ++v) acc[v] = fmaf(t[v], by, acc[v]);
+        for (int j = 0; j < FM; ++j) {
+          const bool apart = !__builtin_isnormal(by[j]);
+          const float first = apart ? xsp[j][k] : 1.f;
+          by[j] = apart ? wsp[k] : by[j];
+#pragma unroll
+          for (int i = 0; i < FN; ++i) t[i][j] *= first;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[i][j][v] = fmaf(t[i][j][v], by[j], acc[i][j][v]);
+    }
   };
   if constexpr (BLK && FM * FN == 4) {
     // sixteen values of depth at a time: while their products run, the next sixteen are widened and those behind
-    // them read, across the step's end as well. us with / without, (M, K, N): 8192 x 4096 x 4096 bf16 255 / 265, 8192 x 8192 x
-    // 8192 965 / 1018. Waves of 64 x 32 in 128 square, whose registers it takes, lose: 4096 x 2048 x 2048 47.5 / 44.3
+    // them read, across the step's end as well: 4 to 5 % of 8192 x 4096 x 4096 and of 8192 x 8192 x 8192. Waves of 64 x 32 in 128 square, whose registers it takes, lose: 4096 x 2048 x 2048 47.5 / 44.3
     intx4 raw[2][FM + FN];
     bf16x8 op[2][FM + FN];
     auto read = [&](const char* p, int pair) {
@@ -252,9 +283,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
       const char* p = smem + slot * SLOT;
       slot ^= 1;
       floatx16 t[FN][FM];
-#pragma unroll
-      for (int j = 0; j < FM; ++j) by[j] = xnext[j] * wnext;
-      if (k + 1 < nk) next_scales(k + 1);
+      take_scales(k);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         if (q % 2 == 0 && q < 6) read(p, q / 2 + 1);
@@ -277,18 +306,13 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) join(t[i][j], by[j], acc[i][j]);
+      join(k, t);
     }
   }
   for (int k = BLK && FM * FN == 4 ? nk : 0; k < nk; ++k, slot ^= 1) {
     turn(k, slot);
     if constexpr (BLK) {
-#pragma unroll
-      for (int j = 0; j < FM; ++j) by[j] = xnext[j] * wnext;
-      if (k + 1 < nk) next_scales(k + 1);
+      take_scales(k);
     }
     const char* p = smem + slot * SLOT;
     floatx16 t[BLK ? FN : 1][BLK ? FM : 1];
@@ -316,13 +340,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void linear_e4m3_kernel(L
           }
         }
     }
-    if constexpr (BLK) {
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-          join(t[i][j], by[j], acc[i][j]);
-    }
+    if constexpr (BLK) join(k, t);
   }
 
   // 32 rows of results at a time, through a part of LDS that is this wave's; the residual's rows are on
@@ -416,7 +434,7 @@ __global__ __launch_bounds__(512) void linear_e4m3_few_kernel(LinearE4m3Args a) 
     }
     xo.set(lo, hi);
     if constexpr (BLK)
-      mul_scaled(wo, xo, xsp[s / 2] * wsp[s / 2], acc);
+      mul_scaled(wo, xo, xsp[s / 2], wsp[s / 2], acc);
     else
       acc = mul(wo, xo, acc);
   };
@@ -459,7 +477,7 @@ __global__ __launch_bounds__(256) void pad_rows_u8_kernel(const uint8_t* x, int6
 
 // Weights in blocks of 128 square: a workgroup a block, a row a wave's pass, two values a lane.
 __global__ __launch_bounds__(256) void quantise_tiles_kernel(const float* w, int N, int n, uint8_t* y, int ld,
-                                                             float* scales, float inv_unit) {
+                                                             float* scales) {
   __shared__ float sh[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r0 = blockIdx.y * kScaleBlock, c0 = blockIdx.x * kScaleBlock;
@@ -476,20 +494,19 @@ __global__ __launch_bounds__(256) void quantise_tiles_kernel(const float* w, int
 #pragma unroll
     for (int c = c0 + lane; c < c0 + kScaleBlock; c += 64)
       y[(int64_t)r * ld + c] = (uint8_t)pack_e4m3(at(r, c) * rs.inv, 0.f, 0.f, 0.f);
-  if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = rs.scale * inv_unit;
+  if (threadIdx.x == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = rs.scale;
 }
 
 }  // namespace
 
-void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y, int ld, float* scales,
-                    float unit) {
+void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y, int ld, float* scales) {
   MNN_REQUIRE(ld == scale_blocks(n) * kScaleBlock, MNN_ERR_INVALID_ARGUMENT, "quantise_tiles: rows of whole blocks");
   // up to 2^17 rows of blocks (N <= 2^24), 2^13 in a launch's y
   for (int r0 = 0; r0 < N; r0 += kScaleBlock << 13) {
     const int rows = std::min(N - r0, kScaleBlock << 13);
     const dim3 grid((unsigned)scale_blocks(n), (unsigned)scale_blocks(rows));
     launch(c, "quantise_tiles", quantise_tiles_kernel, grid, dim3(256), 0, w + (int64_t)r0 * n, rows, n,
-           y + (int64_t)r0 * ld, ld, scales + (int64_t)(r0 / kScaleBlock) * scale_blocks(n), 1.f / unit);
+           y + (int64_t)r0 * ld, ld, scales + (int64_t)(r0 / kScaleBlock) * scale_blocks(n));
   }
 }
 
@@ -544,8 +561,8 @@ void linear_e4m3_t(const LaunchCtx& c, const LinearE4m3Args& a) {
   // 1024 x 1536 bf16 (192 tiles) 32 / 29 / 35; 12800 x 1024 x 1536 bf16 (300 tiles) 58 / 44 / 52.
   auto tiles = [&](int b) { return (a.M + b - 1) / b * ((a.N + b - 1) / b); };
   if (7 * ((tiles(256) + cus - 1) / cus * cus) <= 8 * tiles(256))
-    // blocks: by 128 x 256, whose waves of 64 x 64 have the registers to keep a depth step's sums apart (8192 x 4096 x 4096
-    // 291 -> 266 us; 256 x 128 281)
+    // blocks: by 128 x 256, whose waves of 64 x 64 have the registers to keep a depth step's sums apart (a tenth of 8192 x
+    // 4096 x 4096, 256 x 128 half of that)
     return launch_tile<T, BLK, BLK ? 128 : 256, 256, BLK ? 64 : 128, 64>(c, a, tile_name(BLK, 3, F32));
   // 128 square from three quarters of the compute units on, 128 / 64 square: 10752 x 1536 x 384 (252 tiles) f32 19.3 /
   // 19.5, bf16 17.1 / 19.2; 2688 x 384 x 1152 bf16 (189) 7.8 / 7.8; 5376 x 1536 x 384 f32 (126) 16.3 / 12.9

@@ -233,7 +233,7 @@ class LinearE4m3Layer : public Layer {
     kp_ = (in + 127) / 128 * 128;
     dev_->make_current();
     wq_.reserve((size_t)out * kp_);
-    const size_t scales = blocks ? (size_t)k::scale_blocks(out) * kb_ + 1 : out;  // blocks: their unit behind them
+    const size_t scales = blocks ? (size_t)k::scale_blocks(out) * kb_ : out;
     ws_.reserve(sizeof(float) * scales);
     HIP_CHECK(hipMemset(wq_.ptr, 0, (size_t)out * kp_));  // zero until loaded
     HIP_CHECK(hipMemset(ws_.ptr, 0, sizeof(float) * scales));
@@ -293,7 +293,6 @@ class LinearE4m3Layer : public Layer {
     if (rows == 0) return;
     k::LinearE4m3Args g;
     g.blocks = blocks_;
-    g.unit = blocks_ ? ws_.f32() + (size_t)k::scale_blocks(out_) * kb_ : nullptr;
     g.x = static_cast<const uint8_t*>(in.data);
     g.xs = scales ? scales->f32() : nullptr;
     if (!scales) {  // rows rounded to 8 bits first, their scales behind them
@@ -341,12 +340,7 @@ class LinearE4m3Layer : public Layer {
     HIP_CHECK(hipMemcpy(w.ptr, data, sizeof(float) * in_ * out_, hipMemcpyHostToDevice));
     const LaunchCtx c{dev_, dev_->default_stream};
     if (blocks_) {
-      float top = 512.f;
-      for (size_t i = 0; i < (size_t)in_ * out_; ++i) top = std::max(top, std::fabs(data[i]));
-      const float unit = std::ldexp(1.f, std::ilogb(top) - 9);  // about the largest scale, where that is above 1
-      k::quantise_tiles(c, w.f32(), out_, in_, wq_.as<uint8_t>(), kp_, ws_.f32(), unit);
-      HIP_CHECK(hipMemcpyAsync(ws_.f32() + (size_t)k::scale_blocks(out_) * kb_, &unit, sizeof unit, hipMemcpyHostToDevice,
-                               c.stream));
+      k::quantise_tiles(c, w.f32(), out_, in_, wq_.as<uint8_t>(), kp_, ws_.f32());
       HIP_CHECK(hipStreamSynchronize(c.stream));
       return;
     }

@@ -35,8 +35,7 @@ struct LinearE4m3Args {
   bool blocks = false;         // scales for blocks
   const float* xs = nullptr;   // [M], or [M][K / 128]
   const uint8_t* w = nullptr;  // [N][K]
-  const float* ws = nullptr;   // [N], or [scale_blocks(N)][K / 128] in units of *unit
-  const float* unit = nullptr; // [1], a power of two, on the device: a captured call sees that of weights loaded later
+  const float* ws = nullptr;   // [N], or [scale_blocks(N)][K / 128]
   const float* bias = nullptr; // [N] or null
   const void* r = nullptr;     // [M][N] of the output's type, or null; may be y
   void* y = nullptr;           // [M][N]
@@ -48,9 +47,8 @@ struct LinearE4m3Args {
 };
 constexpr int kLinearFew = 32;
 void linear_e4m3(const LaunchCtx& c, const LinearE4m3Args& a);
-// weights w [N][n] in blocks of kScaleBlock square: values y [N][ld], zeros behind n, and their
-// scales in units of `unit`, a power of two
-void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y, int ld, float* scales, float unit);
+// weights w [N][n] in blocks of kScaleBlock square: values y [N][ld], zeros behind n, and their scales
+void quantise_tiles(const LaunchCtx& c, const float* w, int N, int n, uint8_t* y, int ld, float* scales);
 // rows of `n` bytes copied to rows of `ld` >= n, the rest zero
 void pad_rows_u8(const LaunchCtx& c, const uint8_t* x, int64_t rows, int n, uint8_t* y, int ld);
 

@@ -5,9 +5,10 @@ import pytest
 
 from metalaudio_amd import nn
 from tests import token_bits as bits
-from tests.decoder_refs import held_rows, held_tolerance, memory, values_of
+from tests.decoder_refs import (blocks_of, held_rows, held_tolerance, linear_blocks, memory, quantise_blocks,
+                                quantise_tiles, values_of)
 from tests.test_gpu_tokens import check, tensor
-from tests.token_refs import HALF, attend, rounded, slot_of
+from tests.token_refs import EPS, HALF, attend, rounded, slot_of
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +86,55 @@ def test_memory_of_few_rows_probabilities(dev, stream, B, T, S, H, KV, hd, held)
         wants[b], spread, size = memory(q[b], kv[0][b], kv[1][b], H, KV, hd ** -0.5)
         check_probabilities(got[b], wants[b], spread, size, hd, S + 8, f"sequence {b}")
     assert bits.distance(got, wants) <= bits.STEP_BF16
+
+
+# ------------------------------------------------------------------ the linear layer, in blocks
+# (rows, outputs) of each of the kernel's forms: few rows, few and more, tiles of 64 and 128 square, of 128 x 256
+LINEARS = [(5, 96), (64, 320), (1000, 400), (2500, 1240), (4000, 4090)]
+
+
+def linear_blocks_of(dev, stream, x, w, out="f32"):
+    layer = nn.Linear(dev, w.shape[1], w.shape[0], use_bias=False, precision="e4m3_block")
+    layer.load_weights(w)
+    y = nn.Tensor(dev, (x.shape[0], w.shape[0]), dtype=out)
+    layer.forward_scaled(tensor(dev, x, "f32"), None, y, stream=stream)
+    stream.sync(60000)
+    return y.to_numpy()
+
+
+def check_linear(got, x, w, what):
+    """As for ordinary sizes (1.5 half steps of the running sum an addition, a few a block for its scales), and half of
+    fp32's smallest step a block where sums are that small."""
+    K = x.shape[1]
+    want, mass = linear_blocks(*quantise_blocks(x), *quantise_tiles(w), None)
+    check(got, want, (1.5 * K + 4 * blocks_of(K) + 8) * EPS * mass + blocks_of(K) * 2.0 ** -150, what)
+
+
+@pytest.mark.parametrize("xsize,wsize", [(1e-20, 1e-17), (2e-17, 1e-20), (1e-19, 1e-19), (1e-28, 1e-9), (1e-7, 1e-30),
+                                         (1e18, 1e-18), (1e16, 1e15)])
+@pytest.mark.parametrize("M,N", LINEARS)
+def test_linear_blocks_scales_of_one_sign(dev, stream, M, N, xsize, wsize):
+    """Rows and weights that are both small: their scales' product is no normal number, the results are. And both large."""
+    say(f"linear blocks {M} rows {N} outputs sizes {xsize} {wsize}")
+    rng = np.random.default_rng(M)
+    x = (rng.standard_normal((M, 300)) * np.exp(rng.standard_normal((M, 1)))).astype(np.float32) * np.float32(xsize)
+    x[1::3] /= np.float32(xsize)  # ordinary rows between them, whose scales' products are normal numbers
+    w = rng.standard_normal((N, 300)).astype(np.float32) * np.float32(wsize)
+    check_linear(linear_blocks_of(dev, stream, x, w), x, w, "both small or large")
+
+
+@pytest.mark.parametrize("M,N", LINEARS)
+def test_linear_blocks_beside_a_huge_weight(dev, stream, M, N):
+    """One weight near fp32's largest: it takes the bits of its own 128 x 128 values and of no others, however small what they are
+    multiplied by. A row of zeros gives zeros, also where the product of its weights' scale and the rows' is infinite."""
+    say(f"linear blocks {M} rows {N} outputs, one weight of 1e38")
+    rng = np.random.default_rng(M + 1)
+    x = (rng.standard_normal((M, 400)) * 1e-6).astype(np.float32)
+    w = (rng.standard_normal((N, 400)) / 20).astype(np.float32)
+    w[N - 3, 140] = 1e38
+    w[N - 2] = 0
+    x[2] = 1e30
+    x[2, 140] = 0
+    got = linear_blocks_of(dev, stream, x, w)
+    assert (got[:, N - 2] == 0).all()
+    check_linear(got, x, w, "beside 1e38")
