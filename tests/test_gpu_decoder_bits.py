@@ -138,3 +138,34 @@ def test_linear_blocks_beside_a_huge_weight(dev, stream, M, N):
     got = linear_blocks_of(dev, stream, x, w)
     assert (got[:, N - 2] == 0).all()
     check_linear(got, x, w, "beside 1e38")
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [128, 384])
+@pytest.mark.parametrize("M,N", LINEARS)
+def test_linear_blocks_sums_that_cancel_within_a_block(dev, stream, M, N, K, out):
+    """Two products of 448 x 448 cancel beside small ones of the same block. All products are multiples of 1/16 and no sum of
+    some of them reaches 2^19, so no block's sum is rounded; times the block's scale, within some half steps of 1, it is by a
+    half step, and so is each addition of another block's, which is no larger than the sums of the magnitudes."""
+    say(f"linear blocks that cancel in a block {M}x{K}x{N} {out}")
+    rng = np.random.default_rng(M + K + N)
+    for gap in (1, 7, 40, 100):
+        x = rng.integers(-4, 5, (M, K)).astype(np.float32) / 4
+        w = rng.integers(-4, 5, (N, K)).astype(np.float32) / 4
+        at = int(rng.integers(0, K // 128)) * 128 + int(rng.integers(0, 128 - gap))
+        w[::128, ::128] = 448  # every block's largest value
+        x[:, ::128] = 0
+        x[:, [at, at + gap]] = 448
+        w[:, at], w[:, at + gap] = 448, -448
+        wq, ws = quantise_tiles(w)
+        np.testing.assert_array_equal(wq, w)
+        assert (ws == ws[0, 0]).all()
+        layer = nn.Linear(dev, K, N, use_bias=False, precision="e4m3_block")
+        layer.load_weights(w)
+        y = nn.Tensor(dev, (M, N), dtype=out)
+        layer.forward_scaled(tensor(dev, x, "e4m3"), tensor(dev, np.ones((M, K // 128)), "f32"), y, stream=stream)
+        stream.sync(60000)
+        sums = [x[:, i:i + 128].astype(np.float64) @ w[:, i:i + 128].astype(np.float64).T for i in range(0, K, 128)]
+        want = sum(sums) * float(ws[0, 0])
+        tol = 2 * EPS * sum(np.abs(s) for s in sums) * (2 if K > 128 else 1)
+        check(y.to_numpy(), want, tol + HALF[out] * (out == "bf16") * (np.abs(want) + tol), f"gap {gap}")
