@@ -46,19 +46,14 @@ class Scratch {
 //
 // Counts are zeros before and after a call, whose last workgroups find themselves by them. One that two calls passed at the
 // same time would be wrong for all later ones, so no two calls that could overlap have the same: each stream has its
-// own, and each captured call, which no replay of its graph overlaps. Calls for which none are left share some
-// that a launch of their own clears first.
+// own, and each captured call, which no replay of its graph overlaps. Calls for which none are left, and captured ones before
+// the first that is not, share some that a launch of their own clears first.
 class JoinSpace {
  public:
   k::Join get(const LaunchCtx& c, k::JoinSize n) {
     if (!n.floats) return {};
     float* part = static_cast<float*>(part_.get(sizeof(float) * n.floats));
-    if (!zeros_) {
-      counts_.reserve(sizeof(int) * kCounts);
-      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * kCounts));
-      HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
-      zeros_ = true;
-    }
+    counts_.reserve(sizeof(int) * kCounts);
     return {part, counts(c, n.units)};
   }
 
@@ -68,10 +63,15 @@ class JoinSpace {
     hipStreamCaptureStatus status;
     HIP_CHECK(hipStreamIsCapturing(c.stream, &status));
     const bool captured = status != hipStreamCaptureStatusNone;
+    if (!zeros_ && !captured) {
+      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * kCounts));
+      HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
+      zeros_ = true;
+    }
     auto mine = captured ? streams_.end() : streams_.find(c.stream);
     if (mine != streams_.end()) return counts_.as<int>() + mine->second;
     const int n = captured ? (units + 31) / 32 * 32 : k::kJoinCounts, at = next_;
-    if (n > kCounts - at) {
+    if (!zeros_ || n > kCounts - at) {
       k::zero_u32(c, counts_.as<unsigned>(), units);
       return counts_.as<int>();
     }

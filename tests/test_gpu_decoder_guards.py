@@ -120,3 +120,23 @@ def test_more_captured_calls_than_counts(dev):
         for c, w in zip(calls, want):
             np.testing.assert_array_equal(c.out.to_numpy(), w)
             np.testing.assert_array_equal(c.result(layer, s), w)
+
+
+def test_calls_captured_before_any_other(dev):
+    """Where the capture's mode lets a call allocate, a layer's first call may be a captured one."""
+    say("memory captured first")
+    H, hd, dtype = 2, 64, "bf16"
+    s = nn.Stream(dev)
+    calls = [MemoryCall(dev, 1, T, S, H, hd, dtype, T) for T, S in ((1, 3000), (300, 1100))]
+    want = [c.result(nn.MemoryAttention(dev, H, hd), s) for c in calls]
+    layer = nn.MemoryAttention(dev, H, hd)
+    graph = Graph(s, lambda: [c.run(layer, s) for c in calls] and None)
+    for i in range(4):
+        for c in calls:
+            c.out.copy_from(np.full(c.out.shape, -7, np.float32))
+        graph.replay()
+        s.sync(60000)
+        for c, w in zip(calls, want):
+            np.testing.assert_array_equal(c.out.to_numpy(), w)
+            if i > 1:
+                np.testing.assert_array_equal(c.result(layer, s), w)
