@@ -30,16 +30,6 @@ struct E4m3 {
   uint8_t x;
 };
 
-// Eight e4m3 values to bf16, exactly.
-__device__ __forceinline__ bf16x8 widen8(uint2 q) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.x, 1.f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)q.y, 1.f, true);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
 // Eight values of a row as they come: split in three for f32, else one part.
 template <class M>
 struct Parts {
@@ -70,7 +60,7 @@ struct Eight<E4m3> {
 };
 __device__ __forceinline__ Parts<E4m3> parts_of(const Eight<E4m3>& x) {
   Parts<E4m3> r;
-  r.p[0] = widen8(x.x);
+  r.p[0] = widen8((int)x.x.x, (int)x.x.y);
   return r;
 }
 

@@ -23,16 +23,6 @@ namespace {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
 
-// Eight e4m3 values to bf16, exactly.
-__device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
 // 64 products a row: lane (g, r) holds 32 bytes of row r of both operands (which k they are does not matter
 // as long as both sides agree). The result: b's row l % 32, a's rows 8 (v / 4) + 4 (l / 32) + v % 4.
 struct Operand {

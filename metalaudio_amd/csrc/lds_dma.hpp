@@ -81,8 +81,8 @@ __device__ __forceinline__ int xcd_logical_tile(int lin, int total) {
 }
 
 // Division of 0 <= x < 2^31 by a number that the host knows: a few instructions, where the compiler's own takes some 25,
-// which a kernel of a few microseconds fetches once for each use. m = ceil(2^shift / by) with 2^(shift - 32) >= by: m is at
-// below 2^33 (x m < 2^64), and m by exceeds 2^shift by e < by <= 2^(shift - 32), so that x m / 2^shift exceeds x / by by
+// which a kernel of a few microseconds fetches once for each use. m = ceil(2^shift / by) with 2^(shift - 32) >= by, the least
+// such: m is at most 2^33 (x m < 2^64), and m by exceeds 2^shift by e < by <= 2^(shift - 32), so that x m / 2^shift exceeds x / by by
 // x e / (by 2^shift) < 1 / by, too little to reach the next whole number.
 struct FastDiv {
   unsigned long long m;

@@ -8,11 +8,11 @@
 namespace mnn {
 namespace k {
 
-// A row of values that a kernel reads or writes, f32 or bf16 (or e4m3 where stated).
 // 8-bit values in blocks have a scale for each kScaleBlock of a row (of weights: kScaleBlock square).
 constexpr int kScaleBlock = 128;
 constexpr int scale_blocks(int64_t n) { return (int)((n + kScaleBlock - 1) / kScaleBlock); }
 
+// Rows of values that a kernel reads or writes, f32 or bf16 (or e4m3 where stated).
 struct RmsNormArgs {
   const void* x = nullptr;
   const void* r = nullptr;     // residual, may be null
