@@ -1,4 +1,5 @@
-"""What the decoder's layers hold of the device, and keep from call to call."""
+"""What the decoder's layers hold of the device and keep from call to call, and calls near the ends of what they take, through
+the C ABI. Tolerances count roundings (token_refs.py, decoder_refs.py) and were fixed before the first run."""
 import ctypes as C
 
 import numpy as np
@@ -7,7 +8,10 @@ import pytest
 from metalaudio_amd import nn
 from metalaudio_amd._lib import check as ok
 from metalaudio_amd._lib import lib
-from tests.test_gpu_tokens import Graph, tensor
+from tests.decoder_refs import (blocks_of, held_rows, held_tolerance, linear_blocks, memory, quantise_blocks,
+                                quantise_tiles, values_of)
+from tests.test_gpu_tokens import Graph, check, tensor
+from tests.token_refs import EPS, rounded, slot_of
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +144,81 @@ def test_calls_captured_before_any_other(dev):
             np.testing.assert_array_equal(c.out.to_numpy(), w)
             if i > 1:
                 np.testing.assert_array_equal(c.result(layer, s), w)
+
+
+# ----------------------------------------------------------------- sizes near the ends of what calls take
+def rows_of(rng, n, heads, hd):
+    return rounded(rng.standard_normal((n, heads * hd)), "bf16")
+
+
+@pytest.mark.parametrize("B,T,S,H,KV,hd", [(60001, 1, 3, 8, 8, 8), (1, 1, 5, 60003, 60003, 8), (65535, 1, 1, 1, 1, 16),
+                                           (1, 300007, 5, 1, 1, 8), (7, 9001, 70, 16, 16, 8), (1, 1, 200003, 1, 1, 8)])
+@pytest.mark.parametrize("held", [False, True])
+def test_memory_attention_of_many_rows_heads_and_sequences(dev, B, T, S, H, KV, hd, held):
+    say(f"memory many {B}x{T} on {S} heads {H}/{KV} hd {hd} held {held}")
+    rng = np.random.default_rng(T)
+    s = nn.Stream(dev)
+    q, k, v = (rows_of(rng, B * n, w, hd).reshape(B, n, w * hd) for n, w in ((T, H), (S, KV), (S, KV)))
+    kv, scales = [tensor(dev, x, "bf16") for x in (k, v)], [None, None]
+    if held:
+        (k8, ks), (v8, vs) = held_rows(k, KV), held_rows(v, KV)
+        kv, scales = [tensor(dev, x, "e4m3") for x in (k8, v8)], [tensor(dev, x, "f32") for x in (ks, vs)]
+        k, v = values_of(k8, ks), values_of(v8, vs)
+    out = nn.Tensor(dev, q.shape, dtype="bf16")
+    nn.MemoryAttention(dev, H, hd, KV).forward(tensor(dev, q, "bf16"), *kv, out, None, None, *scales, stream=s)
+    s.sync(60000)
+    got = out.to_numpy()
+    for b in sorted({0, 1, B // 2, B - 2, B - 1} & set(range(B))):
+        t = np.unique(np.r_[0:min(T, 40), T // 2:min(T, T // 2 + 40), max(0, T - 40):T])
+        h = np.unique(np.r_[0:min(H, 3), H // 2:min(H, H // 2 + 3), H - min(H, 3):H])
+        cols = (h[:, None] * hd + np.arange(hd)).ravel()
+        want, spread, size = memory(q[b][t][:, cols], k[b][:, cols], v[b][:, cols], len(h), len(h), hd ** -0.5)
+        check(got[b][t][:, cols], want, held_tolerance(spread, size, hd, S, "bf16"), f"sequence {b}")
+
+
+@pytest.mark.parametrize("B,T,KV,hd,left,sinks", [(1, 65535, 1, 8, 10, 2), (30001, 1, 4, 8, 3, 1), (1, 2, 40009, 8, 3, 0)])
+def test_window_step_held_of_many_rows_heads_and_streams(dev, B, T, KV, hd, left, sinks):
+    say(f"8-bit step many {B}x{T} heads {KV} hd {hd}")
+    rng = np.random.default_rng(B)
+    s = nn.Stream(dev)
+    slots, p0 = sinks + left + T, 7 * left
+    q, k, v = (rows_of(rng, B * T, KV, hd).reshape(B, T, KV * hd) for _ in range(3))
+    old = [held_rows(rng.standard_normal((B, slots, KV * hd)), KV) for _ in "kv"]
+    out = nn.Tensor(dev, q.shape, dtype="bf16")
+    c, sc = [tensor(dev, x, "e4m3") for x, _ in old], [tensor(dev, x, "f32") for _, x in old]
+    nn.WindowAttention(dev, KV, hd, KV, left, 0, sinks).step(
+        *(tensor(dev, x, "bf16") for x in (q, k, v)), tensor(dev, np.full(B, p0), "i32"), *c, out, None, s, *sc)
+    s.sync(60000)
+    got, cache, scales = out.to_numpy(), [x.to_numpy() for x in c], [x.to_numpy() for x in sc]
+    new = [held_rows(x, KV) for x in (k, v)]
+    at = [slot_of(p0 + i, sinks, slots) for i in range(T)]
+    for i in (0, 1):
+        np.testing.assert_array_equal(cache[i][:, at], new[i][0])
+        np.testing.assert_array_equal(scales[i][:, at], new[i][1])
+    h = np.unique(np.r_[0:min(KV, 3), KV // 2, KV - 1])
+    cols = (h[:, None] * hd + np.arange(hd)).ravel()
+    for b in sorted({0, B // 2, B - 1}):
+        for t in sorted({0, min(1, T - 1), T // 2, T - 1}):
+            told = [p for p in range(p0 + t + 1) if p < sinks or p >= p0 + t - left]
+            rows = [np.stack([values_of(n[0][b, p - p0], n[1][b, p - p0]) if p >= p0 else
+                              values_of(o[0][b, slot_of(p, sinks, slots)], o[1][b, slot_of(p, sinks, slots)])
+                              for p in told])[:, cols] for n, o in zip(new, old)]
+            want, spread, size = memory(q[b, t:t + 1][:, cols], *rows, len(h), len(h), hd ** -0.5)
+            check(got[b, t:t + 1][:, cols], want, held_tolerance(spread, size, hd, len(told), "bf16"), f"{b} {t}")
+
+
+@pytest.mark.parametrize("M,K,N", [(300007, 100, 8), (2, 16, (1 << 20) + 200), (70001, 130, 33), (1, 100003, 5)])
+def test_linear_blocks_of_many_rows_and_outputs(dev, M, K, N):
+    say(f"linear blocks many {M}x{K}x{N}")
+    rng = np.random.default_rng(N)
+    s = nn.Stream(dev)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    w = (rng.standard_normal((N, K)) / np.sqrt(K)).astype(np.float32)
+    layer = nn.Linear(dev, K, N, use_bias=False, precision="e4m3_block")
+    layer.load_weights(w)
+    y = nn.Tensor(dev, (M, N))
+    layer.forward_scaled(tensor(dev, x, "f32"), None, y, stream=s)
+    s.sync(60000)
+    rows = np.unique(np.r_[0:min(M, 70), M // 2:min(M, M // 2 + 70), max(0, M - 70):M])
+    want, mass = linear_blocks(*quantise_blocks(x[rows]), *quantise_tiles(w), None)
+    check(y.to_numpy()[rows], want, (1.5 * K + 4 * blocks_of(K) + 8) * EPS * mass + 1e-37, "rows")
