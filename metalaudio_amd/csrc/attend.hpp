@@ -107,7 +107,7 @@ struct AttendTypes {
   }
   // Eight probabilities (e4m3: times their values' scales) to the second product; v(part, tile): fragments of V^T.
   // PP: the bf16 parts that a probability beside bf16 values is taken in, one (off by 2^-8 of itself at most) or two
-  // (2^-16). Returns the sum of the rounded ones, of one part, without scales; else 0.
+  // (2^-16); v_exp_f32 and the sums are fp32's. Returns the sum of the rounded ones, of one part, without scales; else 0.
   template <int PP, int TILES, class Acc, class V, class Mfma>
   static __device__ __forceinline__ float values(const float (&p)[8], V v, Acc (&o)[TILES], Mfma mfma) {
     typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
@@ -276,6 +276,8 @@ struct AttendMany : AttendTypes<T, M> {
         if (!RAW) ps += p[e];
         if (HELD) p[e] *= vs(8 * ks + e);
       }
+      // one part: results of 1.8e-3 (2-norm, e4m3 2.4e-3) where two give 1.66e-3, for 319 us against 437 (8192 tokens on
+      // 16384 states; e4m3 364 against 537), since the instructions beside the exponentials bound these calls
       ps += A::template values<1>(p, [&](int part, int t) { return v(part, t, ks); }, o, mfma);
     }
     sum += ps;

@@ -12,10 +12,10 @@
 // waves a SIMD instead of four); rows on the vector units, eight lanes a key, cost as much for each.
 //
 // Bound by the loads where there are many streams, each lane group reading short rows: 64 streams on 4096 keys in 8 bits, 16 / 4 heads
-// of 64, bf16 (142 MB) 28 us with the 256 MB cache warm, 5.1 TB/s, 35 us from memory; on 2688 ragged states (70 MB) 18 to 20 us.
-// Lines touched a block or two ahead lose (36 and 41 us), as do loads around the caches. By the chain of one block and
-// the code's first fetch where there are few: one stream on 516 keys in 8 bits, 8 heads of 48, f32 8.7 us, one token on 1344 states
-// 11.7 (bf16 8.1), 8 streams' 16 tokens on 1043 keys 12 us.
+// of 64, bf16 (142 MB) 28.8 us with the 256 MB cache warm, 4.9 TB/s, 35 us from memory; on 2688 ragged states (70 MB) 18 to 20 us.
+// Lines touched a block or two ahead lose (36 and 41 us), as do loads around the caches. By the length of this form
+// (V through LDS, two joins) and its code's first fetch where there are few: one stream on 516 keys in 8 bits, 8 heads of 48, f32 8.7 us, one token on 1344 states
+// 11.7 (bf16 8.1), 8 streams' 16 tokens on 1043 keys 12 us; one stream on 516 f32 keys by k_window_step.hip, its row on the vector units, 7 to 8.
 #include <algorithm>
 #include <type_traits>
 
