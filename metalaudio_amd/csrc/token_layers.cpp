@@ -64,8 +64,10 @@ class JoinSpace {
     HIP_CHECK(hipStreamIsCapturing(c.stream, &status));
     const bool captured = status != hipStreamCaptureStatusNone;
     if (!zeros_ && !captured) {
-      HIP_CHECK(hipMemset(counts_.ptr, 0, sizeof(int) * kCounts));
-      HIP_CHECK(hipStreamSynchronize(nullptr));  // streams that do not wait for the null stream use them
+      // on the call's own stream (the null stream may not be touched while another one is captured), and waited for, since
+      // others use them too
+      k::zero_u32(c, counts_.as<unsigned>(), kCounts);
+      HIP_CHECK(hipStreamSynchronize(c.stream));
       zeros_ = true;
     }
     auto mine = captured ? streams_.end() : streams_.find(c.stream);

@@ -146,6 +146,24 @@ def test_calls_captured_before_any_other(dev):
                 np.testing.assert_array_equal(c.result(layer, s), w)
 
 
+def test_first_call_while_another_stream_is_captured(dev):
+    say("memory first call beside a capture")
+    a, b, graph = nn.Stream(dev), nn.Stream(dev), C.c_void_p()
+    call = MemoryCall(dev, 1, 1, 3000, 2, 64, "bf16", 9)
+    want = call.result(nn.MemoryAttention(dev, 2, 64), b)
+    layer = nn.MemoryAttention(dev, 2, 64)
+    handle = C.c_void_p(C.cast(a.handle, C.POINTER(C.c_void_p))[1])
+    assert hip().hipStreamBeginCapture(handle, 2) == 0
+    try:
+        call.run(layer, b)
+    finally:
+        ended = hip().hipStreamEndCapture(handle, C.byref(graph))
+    b.sync(60000)
+    assert ended == 0
+    np.testing.assert_array_equal(call.out.to_numpy(), want)
+    np.testing.assert_array_equal(call.result(layer, a), want)
+
+
 # ----------------------------------------------------------------- sizes near the ends of what calls take
 def rows_of(rng, n, heads, hd):
     return rounded(rng.standard_normal((n, heads * hd)), "bf16")
